@@ -353,6 +353,117 @@ int mi_squareplus_clamp(const float* x, float* y, int64_t n, float lo, float hi,
 int mi_ste_clamp(const float* x, float* y, int64_t n, float lo, float hi, void* stream);
 int mi_sigmoid_gate(const float* y, const float* z, float* out, int64_t n, void* stream);
 
+/*
+ * Float Mamba layer: the operators of a layer with exponential decays, for
+ * training (with their backward passes), prompts and single tokens.  No
+ * counterpart on the reference's dyadic path; they stand beside mi_ssm_scan /
+ * mi_ssm_step, mi_conv_act_quant / mi_conv_step and mi_rowprep.
+ *
+ * Activations are fp32, bf16 or fp16 (`dtype`, one for all of a call); all
+ * arithmetic, states, statistics and parameters are fp32, and a result is
+ * rounded to its type once.  [batch, L, *] operands have unit last stride and
+ * the given batch and row strides in elements; outputs are contiguous.
+ * lengths (optional, int32 [batch]): sequence b ends before position
+ * lengths[b] (clamped to [0, L]); what the inputs hold from there on is not
+ * used, outputs and gradients there are 0, and the final state is the one at
+ * the length.
+ */
+#define MI_DT_F32 0
+#define MI_DT_BF16 1
+#define MI_DT_F16 2
+
+/*
+ * Selective scan: dt = delta + delta_bias[d], softplus of it if `softplus`;
+ *   h[t] = exp(dt A[d,n]) h[t-1] + dt B[t,n] u[t,d],  h[-1] = h0 (0 if NULL)
+ *   y[t,d] = (sum_n C[t,n] h[t,d,n] + D[d] u[t,d]) * z sigmoid(z)
+ * u, delta, z, y [batch, L, Dm]; B, C [batch, L, N]; A [Dm, N]; D, delta_bias
+ * [Dm]; h0, h_out [batch, Dm, N]; D, z, delta_bias, h0, lengths, h_out may be
+ * NULL.  checkpoints (NULL without a backward pass): the states that
+ * mi_selective_scan_backward starts from, mi_selective_scan_checkpoints()
+ * floats.  workspace: mi_selective_scan_workspace(.., 0) bytes.  L >= 1,
+ * 1 <= N <= 64; A, h0, h_out, checkpoints, workspace 16-byte aligned.
+ */
+int mi_selective_scan(const void* u, int64_t u_batch, int64_t u_row, const void* delta, int64_t delta_batch,
+                      int64_t delta_row, const float* A, const void* B, int64_t B_batch, int64_t B_row, const void* C,
+                      int64_t C_batch, int64_t C_row, const float* D, const void* z, int64_t z_batch, int64_t z_row,
+                      const float* delta_bias, const float* h0, const int32_t* lengths, void* y, float* h_out,
+                      float* checkpoints, void* workspace, int batch, int L, int Dm, int N, int softplus, int dtype,
+                      void* stream);
+int64_t mi_selective_scan_checkpoints(int batch, int L, int Dm, int N);
+int64_t mi_selective_scan_workspace(int batch, int L, int Dm, int N, int backward);
+
+/*
+ * Its gradients, from dy [batch, L, Dm] and dh_out (NULL: 0): du, ddelta, dz
+ * [batch, L, Dm] (dz with z); dB, dC [batch, L, N]; dA [Dm, N]; dD,
+ * ddelta_bias [Dm]; dh0 [batch, Dm, N].  All but du, ddelta and dz may be
+ * NULL.  Sums over channels and positions are taken in a fixed order: the
+ * same inputs give the same bits.
+ */
+int mi_selective_scan_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const float* dh_out, const void* u,
+                               int64_t u_batch, int64_t u_row, const void* delta, int64_t delta_batch,
+                               int64_t delta_row, const float* A, const void* B, int64_t B_batch, int64_t B_row,
+                               const void* C, int64_t C_batch, int64_t C_row, const float* D, const void* z,
+                               int64_t z_batch, int64_t z_row, const float* delta_bias, const int32_t* lengths,
+                               const float* checkpoints, void* du, void* ddelta, float* dA, void* dB, void* dC,
+                               float* dD, void* dz, float* ddelta_bias, float* dh0, void* workspace, int batch, int L,
+                               int Dm, int N, int softplus, int dtype, void* stream);
+
+/* One new token a stream: u, delta, z, y [batch, Dm], B, C [batch, N] with the
+ * given batch strides; h [batch, Dm, N] is advanced in place. */
+int mi_selective_scan_step(const void* u, int64_t u_batch, const void* delta, int64_t delta_batch, const float* A,
+                           const void* B, int64_t B_batch, const void* C, int64_t C_batch, const float* D,
+                           const void* z, int64_t z_batch, const float* delta_bias, float* h, void* y, int batch,
+                           int Dm, int N, int softplus, int dtype, void* stream);
+
+/*
+ * Causal depthwise convolution: c[t] = bias + sum_k w[d,k] x[t - W + 1 + k],
+ * y = c sigmoid(c) if `silu`, else c.  x, y [batch, L, D]; w [D, W],
+ * 2 <= W <= 4; bias [D] or NULL; win [batch, W - 1, D] (x's type): the inputs
+ * before position 0 (NULL: zeros); win_out (or NULL): the last W - 1 inputs,
+ * those of win among them where the sequence is shorter.
+ */
+int mi_causal_conv1d(const void* x, int64_t x_batch, int64_t x_row, const float* w, const float* bias, const void* win,
+                     const int32_t* lengths, void* y, void* win_out, int batch, int L, int D, int W, int silu,
+                     int dtype, void* stream);
+
+/* Its gradients, from dy and dwin_out (NULL: 0): dx [batch, L, D]; dw [D, W];
+ * dbias [D]; dwin [batch, W - 1, D]; each may be NULL.  workspace (for dw or
+ * dbias): mi_causal_conv1d_backward_workspace() bytes.  L >= 1. */
+int mi_causal_conv1d_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* dwin_out, const void* x,
+                              int64_t x_batch, int64_t x_row, const float* w, const float* bias, const void* win,
+                              const int32_t* lengths, void* dx, float* dw, float* dbias, void* dwin, void* workspace,
+                              int batch, int L, int D, int W, int silu, int dtype, void* stream);
+int64_t mi_causal_conv1d_backward_workspace(int batch, int L, int D, int W);
+
+/* One new token a stream: x, y [batch, D]; win [batch, W - 1, D] is advanced
+ * in place. */
+int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const float* bias, void* win, void* y,
+                          int batch, int D, int W, int silu, int dtype, void* stream);
+
+/*
+ * RMS norm with the residual's addition: s = x + residual (s = x with residual
+ * NULL), kept in the residual's type (`rdtype`: dtype, or MI_DT_F32) as `sum`;
+ * rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight.  The norm is of s
+ * as it is kept.  x, residual [T, D] with row strides ldx, ldr; y, sum [T, D];
+ * rstd [T] (may be NULL) for the backward pass.  D <= 16384.
+ */
+int mi_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight, void* y, void* sum,
+                float* rstd, int T, int D, float eps, int dtype, int rdtype, void* stream);
+
+/* The same with y quantised as mi_quantize_rows does: xq [T, D], xscale [T]
+ * feed the ternary GEMMs. */
+int mi_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight, int8_t* xq,
+                      float* xscale, void* sum, int T, int D, float eps, int dtype, int rdtype, void* stream);
+
+/* Gradients of mi_rms_norm from dy (dtype) and dsum (rdtype, or NULL), with
+ * s [T, D] of row stride lds in rdtype: dx (dtype) and dresidual (rdtype), the
+ * same values, and dweight [D]; each may be NULL.  workspace (for dweight):
+ * mi_rms_norm_backward_workspace() bytes. */
+int mi_rms_norm_backward(const void* dy, const void* dsum, const void* s, int64_t lds, const float* weight,
+                         const float* rstd, void* dx, void* dresidual, float* dweight, void* workspace, int T, int D,
+                         int dtype, int rdtype, void* stream);
+int64_t mi_rms_norm_backward_workspace(int T, int D);
+
 #ifdef __cplusplus
 }
 #endif

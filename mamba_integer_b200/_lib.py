@@ -17,11 +17,15 @@ MI_EPI_F32_SCALED = 1
 MI_DEV_OVERFLOW = 0x1
 MI_DEV_TIMEOUT = 0x2
 MI_DEV_PRECOND = 0x4
+MI_DT_F32 = 0
+MI_DT_BF16 = 1
+MI_DT_F16 = 2
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
+_s = (_p, _i64, _i64)  # a [batch, L, *] operand: pointer, batch stride, row stride
 
 # name -> argument types (all return int status unless listed in _RESTYPE)
 SIGNATURES = {
@@ -52,8 +56,25 @@ SIGNATURES = {
     "mi_squareplus_clamp": [_p, _p, _i64, _f, _f, _p],
     "mi_ste_clamp": [_p, _p, _i64, _f, _f, _p],
     "mi_sigmoid_gate": [_p, _p, _p, _i64, _p],
+    "mi_selective_scan": [*_s, *_s, _p, *_s, *_s, _p, *_s, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+    "mi_selective_scan_checkpoints": [_i, _i, _i, _i],
+    "mi_selective_scan_workspace": [_i, _i, _i, _i, _i],
+    "mi_selective_scan_backward": [*_s, _p, *_s, *_s, _p, *_s, *_s, _p, *_s, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p,
+                                   _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+    "mi_selective_scan_step": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _i, _i, _i, _i,
+                               _i, _p],
+    "mi_causal_conv1d": [*_s, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+    "mi_causal_conv1d_backward": [*_s, _p, *_s, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
+    "mi_causal_conv1d_backward_workspace": [_i, _i, _i, _i],
+    "mi_causal_conv1d_step": [_p, _i64, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p],
+    "mi_rms_norm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
+    "mi_rms_norm_quant": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
+    "mi_rms_norm_backward": [_p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
+    "mi_rms_norm_backward_workspace": [_i, _i],
 }
-_RESTYPE = {"mi_status_string": ctypes.c_char_p}
+_RESTYPE = {"mi_status_string": ctypes.c_char_p, "mi_selective_scan_checkpoints": _i64,
+            "mi_selective_scan_workspace": _i64, "mi_causal_conv1d_backward_workspace": _i64,
+            "mi_rms_norm_backward_workspace": _i64}
 
 _lib = None
 

@@ -9,3 +9,6 @@
 #include "decode.cu"
 #include "train.cu"
 #include "noalloc.cu"
+#include "selective.cu"
+#include "conv1d.cu"
+#include "rmsnorm.cu"

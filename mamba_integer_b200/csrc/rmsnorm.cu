@@ -1,0 +1,395 @@
+// rmsnorm.cu -- RMS norm with the residual's addition in front of it, and an
+// int8 output with row scales; its backward pass.
+//
+//   s = x + r                     (kept in r's type; s = x without a residual)
+//   rstd = 1 / sqrt(mean(s^2) + eps)
+//   y = s * rstd * w
+//   int8: m = max(max|y|, 1e-8); q = rne(y * 127 / m); scale = m / 127, the
+//         rows quantise_rows gives, ready for the ternary GEMMs
+//   ds = rstd * (w dy - xhat * mean(w dy xhat)) + dsum,  xhat = s * rstd
+//   dw = sum over rows of dy * xhat
+//
+// Every row is read once and held in registers between the reduction and the
+// output, so the bound is HBM: x and r in, s and y out.  A row belongs to TPR
+// threads (a warp up to 1024 columns of 16 bits); rows that need more than a
+// warp reduce through shared memory.
+#include "mi_elem.cuh"
+
+namespace mi {
+namespace rms {
+
+constexpr int THREADS = 256;
+
+struct Args {
+    const void* x;
+    const void* r;
+    const float* w;
+    void* y;       // forward: y (NULL with xq)
+    void* sum;     // s, in r's type (NULL without a residual)
+    int8_t* xq;
+    float* xscale;
+    float* rstd;   // forward out (may be NULL), backward in
+    const void* dy;
+    const void* dsum;  // may be NULL
+    void* dx;          // may be NULL
+    void* dr;          // in r's type, may be NULL
+    float* dw_part;    // [gridDim.x, D], may be NULL
+    int64_t ldx, ldr;  // row strides of x and r in elements
+    int T, D;
+    float eps;
+    int vec;           // every row starts on the packs' alignment
+};
+
+// Sum (or maximum) of one value over the TPR threads of a row, in a fixed order.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* red) {
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+        const float o = __shfl_xor_sync(0xffffffffu, v, m);
+        v = MAX ? max_nan(v, o) : __fadd_rn(v, o);
+    }
+    if (TPR > 32) {
+        constexpr int W = TPR / 32;
+        const int warp = threadIdx.x >> 5, row = threadIdx.x / TPR;
+        __syncthreads();  // the last round's reads of red are done
+        if ((threadIdx.x & 31) == 0) red[warp] = v;
+        __syncthreads();
+        v = red[row * W];
+#pragma unroll
+        for (int i = 1; i < W; i++) v = MAX ? max_nan(v, red[row * W + i]) : __fadd_rn(v, red[row * W + i]);
+    }
+    return v;
+}
+
+// T: element type of x and y; R: of the residual and s.  A thread holds NV
+// packs of K elements, TPR * K apart.
+template <typename T, typename R, int K, int NV, int TPR, bool QUANT>
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(const Args a) {
+    __shared__ float red[32];
+    constexpr int ROWS = (TPR > THREADS ? TPR : THREADS) / TPR;
+    const int lane = threadIdx.x % TPR;
+    grid_dependency_sync();
+    const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+    // the threads of a row that does not exist still take part in the barriers
+    const bool live = t < a.T;
+    const T* x = static_cast<const T*>(a.x) + t * a.ldx;
+    const R* r = static_cast<const R*>(a.r) + t * a.ldr;
+    const bool vec = a.vec != 0;
+    float s[NV][K];
+    float acc = 0.0f;
+    Pack<T, K> px[NV];
+    Pack<R, K> pr[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + lane) * K;
+        const int valid = live ? a.D - c : 0;
+        px[j] = load_pack<K>(x + c, valid, vec);
+        if (a.r) pr[j] = load_pack<K>(r + c, valid, vec);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + lane) * K;
+        const int valid = live ? a.D - c : 0;
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            s[j][i] = to_f(px[j].v[i]);
+            // the norm is of the sum as it is kept, so that a backward pass finds the same one
+            if (a.r) s[j][i] = to_f(from_f<R>(__fadd_rn(s[j][i], to_f(pr[j].v[i]))));
+        }
+        if (a.r && valid > 0) store_pack<K>(static_cast<R*>(a.sum) + t * a.D + c, s[j], valid, vec);
+#pragma unroll
+        for (int i = 0; i < K; i++) acc = __fmaf_rn(s[j][i], s[j][i], acc);
+    }
+    acc = row_reduce<TPR, false>(acc, red);
+    const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(acc, (float)a.D), a.eps)));
+    if (live && lane == 0 && a.rstd) a.rstd[t] = rstd;
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + lane) * K;
+        const Pack<float, K> w = load_pack<K>(a.w + c, a.D - c, vec);
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            s[j][i] = __fmul_rn(__fmul_rn(s[j][i], rstd), w.v[i]);
+            if (QUANT) amax = max_nan(amax, fabsf(s[j][i]));
+        }
+        if (!QUANT && live && c < a.D) store_pack<K>(static_cast<T*>(a.y) + t * a.D + c, s[j], a.D - c, vec);
+    }
+    if (QUANT) {
+        amax = row_reduce<TPR, true>(amax, red);
+        float scale;
+        const float inv = quant_inv_scale(amax, scale);
+        if (live && lane == 0) a.xscale[t] = scale;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (j * TPR + lane) * K;
+            if (!live || c >= a.D) continue;
+            int8_t* o = a.xq + t * a.D + c;
+            Pack<int8_t, K> q;
+#pragma unroll
+            for (int i = 0; i < K; i++) q.v[i] = (int8_t)quant_i8(__fmul_rn(s[j][i], inv));
+            if (vec && a.D - c >= K) {
+                *reinterpret_cast<Pack<int8_t, K>*>(o) = q;
+            } else {
+#pragma unroll
+                for (int i = 0; i < K; i++)
+                    if (i < a.D - c) o[i] = q.v[i];
+            }
+        }
+    }
+}
+
+// Rows are dealt to the CTAs in a fixed order; each thread keeps the sums of
+// its columns' dy * xhat over its rows in registers, a CTA adds its row groups
+// through shared memory and writes one row of partial sums, and
+// column_sum_kernel adds those.
+template <typename T, typename R, int K, int NV, int TPR>
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) bwd_kernel(const Args a) {
+    __shared__ float red[32];
+    extern __shared__ float dw_sh[];  // [D] for ROWS > 1
+    constexpr int ROWS = (TPR > THREADS ? TPR : THREADS) / TPR;
+    const int lane = threadIdx.x % TPR, row = threadIdx.x / TPR;
+    const bool vec = a.vec != 0;
+    float dw[NV][K];
+    Pack<float, K> w[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int c = (j * TPR + lane) * K;
+        w[j] = load_pack<K>(a.w + c, a.D - c, vec);
+#pragma unroll
+        for (int i = 0; i < K; i++) dw[j][i] = 0.0f;
+    }
+    for (int64_t t0 = (int64_t)blockIdx.x * ROWS; t0 < a.T; t0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t t = t0 + row;
+        const bool live = t < a.T;
+        Pack<R, K> ps[NV];
+        Pack<T, K> pg[NV];
+        Pack<R, K> pd[NV];
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (j * TPR + lane) * K;
+            const int valid = live ? a.D - c : 0;
+            ps[j] = load_pack<K>(static_cast<const R*>(a.sum) + t * a.ldr + c, valid, vec);
+            pg[j] = load_pack<K>(static_cast<const T*>(a.dy) + t * a.D + c, valid, vec);
+            if (a.dsum) pd[j] = load_pack<K>(static_cast<const R*>(a.dsum) + t * a.D + c, valid, vec);
+        }
+        const float rstd = live ? a.rstd[t] : 0.0f;
+        float dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                const float xh = __fmul_rn(to_f(ps[j].v[i]), rstd);
+                const float g = to_f(pg[j].v[i]);
+                dot = __fmaf_rn(__fmul_rn(w[j].v[i], g), xh, dot);
+                dw[j][i] = __fmaf_rn(g, xh, dw[j][i]);
+            }
+        dot = row_reduce<TPR, false>(dot, red);
+        const float mean = __fdiv_rn(dot, (float)a.D);
+        if (a.dx || a.dr) {
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int c = (j * TPR + lane) * K;
+                if (!live || c >= a.D) continue;
+                float o[K];
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    const float xh = __fmul_rn(to_f(ps[j].v[i]), rstd);
+                    const float g = __fmul_rn(w[j].v[i], to_f(pg[j].v[i]));
+                    o[i] = __fmul_rn(rstd, __fmaf_rn(-xh, mean, g));
+                    if (a.dsum) o[i] = __fadd_rn(o[i], to_f(pd[j].v[i]));
+                }
+                if (a.dx) store_pack<K>(static_cast<T*>(a.dx) + t * a.D + c, o, a.D - c, vec);
+                if (a.dr) store_pack<K>(static_cast<R*>(a.dr) + t * a.D + c, o, a.D - c, vec);
+            }
+        }
+    }
+    if (!a.dw_part) return;
+    float* part = a.dw_part + (int64_t)blockIdx.x * a.D;
+    for (int g = 0; g < ROWS; g++) {
+        if (row == g) {
+#pragma unroll
+            for (int j = 0; j < NV; j++)
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    const int c = (j * TPR + lane) * K + i;
+                    if (c >= a.D) continue;
+                    const float v = g ? __fadd_rn(dw_sh[c], dw[j][i]) : dw[j][i];
+                    if (g == ROWS - 1)
+                        part[c] = v;
+                    else
+                        dw_sh[c] = v;
+                }
+        }
+        if (ROWS > 1) __syncthreads();
+    }
+}
+
+// out[c] = sum over p of part[p, c], in the order of p within four strands
+__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int P,
+                                                         int64_t D) {
+    __shared__ float sh[8][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c < D) {
+        int p = g;
+        for (; p + 24 < P; p += 32)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[j] = __fadd_rn(s[j], part[(int64_t)(p + 8 * j) * D + c]);
+        for (; p < P; p += 8) s[0] = __fadd_rn(s[0], part[(int64_t)p * D + c]);
+    }
+    sh[g][threadIdx.x & 31] = __fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3]));
+    __syncthreads();
+    if (g == 0 && c < D) {
+        float v = sh[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 8; i++) v = __fadd_rn(v, sh[i][threadIdx.x]);
+        out[c] = v;
+    }
+}
+
+// Threads of a row: the fewest that hold it in at most 4 packs of 8 (2 of 4
+// for fp32 rows), and a whole CTA's where there are too few rows to fill the
+// GPU with warps.
+static inline int threads_per_row(int T, int D, int K) {
+    const int packs = cdiv(D, K);
+    int tpr = 32;
+    while (tpr * 4 < packs) tpr *= 2;
+    while (tpr < 256 && tpr < packs && (int64_t)T * tpr < 148 * 256) tpr *= 2;
+    return tpr;
+}
+
+constexpr int MAX_D = 16384;  // 512 threads of 4 packs
+constexpr int BWD_CTAS = 148 * 4;
+
+template <typename T, typename R, int K, int TPR, bool BWD, bool QUANT>
+static int launch_nv(const Args& a, int grid, int block, cudaStream_t s) {
+    const int nv = cdiv(cdiv(a.D, K), TPR);
+    const size_t smem = BWD && block > TPR ? sizeof(float) * a.D : 0;
+#define MI_RMS_CASE(NV)                                                                     \
+    do {                                                                                    \
+        if constexpr (BWD)                                                                  \
+            bwd_kernel<T, R, K, NV, TPR><<<grid, block, smem, s>>>(a);                      \
+        else                                                                                \
+            MI_LAUNCH_DEPENDENT(fwd_kernel<T, R, K, NV, TPR, QUANT>, grid, block, 0, s, a); \
+    } while (0)
+    if (nv <= 1)
+        MI_RMS_CASE(1);
+    else if (nv <= 2)
+        MI_RMS_CASE(2);
+    else
+        MI_RMS_CASE(4);
+#undef MI_RMS_CASE
+    MI_CHECK_LAUNCH();
+    return MI_OK;
+}
+
+template <typename T, typename R, bool BWD, bool QUANT>
+static int launch(const Args& a, int grid_cap, cudaStream_t s) {
+    constexpr int K = 8;
+    const int tpr = threads_per_row(a.T, a.D, K);
+    const int block = tpr > THREADS ? tpr : THREADS;
+    int grid = cdiv(a.T, block / tpr);
+    if (grid_cap && grid > grid_cap) grid = grid_cap;
+    switch (tpr) {
+        case 32: return launch_nv<T, R, K, 32, BWD, QUANT>(a, grid, block, s);
+        case 64: return launch_nv<T, R, K, 64, BWD, QUANT>(a, grid, block, s);
+        case 128: return launch_nv<T, R, K, 128, BWD, QUANT>(a, grid, block, s);
+        case 256: return launch_nv<T, R, K, 256, BWD, QUANT>(a, grid, block, s);
+        default: return launch_nv<T, R, K, 512, BWD, QUANT>(a, grid, block, s);
+    }
+}
+
+static int grid_of(int T, int D) {
+    const int tpr = threads_per_row(T, D, 8);
+    const int block = tpr > THREADS ? tpr : THREADS;
+    const int grid = cdiv(T, block / tpr);
+    return grid < BWD_CTAS ? grid : BWD_CTAS;
+}
+
+template <bool BWD, bool QUANT>
+static int dispatch(const Args& a, int dtype, int rdtype, int grid_cap, cudaStream_t s) {
+    MI_DISPATCH_DTYPE(dtype, T, {
+        if (rdtype == dtype) return launch<T, T, BWD, QUANT>(a, grid_cap, s);
+        if (rdtype == MI_DT_F32) return launch<T, float, BWD, QUANT>(a, grid_cap, s);
+        return MI_ERR_INVALID;
+    });
+    return MI_ERR_INVALID;
+}
+
+}  // namespace rms
+}  // namespace mi
+
+static int mi_rms_check(int T, int D) {
+    if (T < 0 || D <= 0) return MI_ERR_INVALID;
+    if (D > mi::rms::MAX_D) return MI_ERR_UNSUPPORTED;
+    return MI_OK;
+}
+
+static int mi_rms_forward(const void* x, int64_t ldx, const void* r, int64_t ldr, const float* w, void* y, void* sum,
+                          int8_t* xq, float* xscale, float* rstd, int T, int D, float eps, int dtype, int rdtype,
+                          void* stream) {
+    if (!x || !w || (r && !sum)) return MI_ERR_INVALID;
+    const int rc = mi_rms_check(T, D);
+    if (rc != MI_OK) return rc;
+    if (ldx < 0 || (r && ldr < 0)) return MI_ERR_INVALID;
+    if (T == 0) return MI_OK;
+    mi::rms::Args a = {};
+    a.x = x, a.r = r, a.w = w, a.y = y, a.sum = sum, a.xq = xq, a.xscale = xscale, a.rstd = rstd;
+    a.ldx = ldx, a.ldr = ldr, a.T = T, a.D = D, a.eps = eps;
+    bool vec = D % 8 == 0 && ldx % 8 == 0 && mi::aligned16(x) && mi::aligned16(w);
+    if (r) vec = vec && ldr % 8 == 0 && mi::aligned16(r) && mi::aligned16(sum);
+    vec = vec && (xq ? (reinterpret_cast<uintptr_t>(xq) & 7) == 0 : mi::aligned16(y));
+    a.vec = vec;
+    if (xq) return mi::rms::dispatch<false, true>(a, dtype, r ? rdtype : dtype, 0, (cudaStream_t)stream);
+    return mi::rms::dispatch<false, false>(a, dtype, r ? rdtype : dtype, 0, (cudaStream_t)stream);
+}
+
+extern "C" int mi_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight, void* y,
+                           void* sum, float* rstd, int T, int D, float eps, int dtype, int rdtype, void* stream) {
+    if (!y) return MI_ERR_INVALID;
+    return mi_rms_forward(x, ldx, residual, ldr, weight, y, sum, nullptr, nullptr, rstd, T, D, eps, dtype, rdtype,
+                          stream);
+}
+
+extern "C" int mi_rms_norm_quant(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight,
+                                 int8_t* xq, float* xscale, void* sum, int T, int D, float eps, int dtype, int rdtype,
+                                 void* stream) {
+    if (!xq || !xscale) return MI_ERR_INVALID;
+    return mi_rms_forward(x, ldx, residual, ldr, weight, nullptr, sum, xq, xscale, nullptr, T, D, eps, dtype, rdtype,
+                          stream);
+}
+
+extern "C" int64_t mi_rms_norm_backward_workspace(int T, int D) {
+    if (T <= 0 || D <= 0 || D > mi::rms::MAX_D) return 0;
+    return (int64_t)sizeof(float) * mi::rms::grid_of(T, D) * D;
+}
+
+extern "C" int mi_rms_norm_backward(const void* dy, const void* dsum, const void* s, int64_t lds, const float* weight,
+                                    const float* rstd, void* dx, void* dresidual, float* dweight, void* workspace,
+                                    int T, int D, int dtype, int rdtype, void* stream) {
+    if (!dy || !s || !weight || !rstd || (!dx && !dresidual && !dweight)) return MI_ERR_INVALID;
+    if (dweight && !workspace) return MI_ERR_INVALID;
+    const int rc = mi_rms_check(T, D);
+    if (rc != MI_OK) return rc;
+    if (lds < 0) return MI_ERR_INVALID;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T == 0) {
+        if (dweight && cudaMemsetAsync(dweight, 0, sizeof(float) * D, st) != cudaSuccess) return MI_ERR_CUDA;
+        return MI_OK;
+    }
+    mi::rms::Args a = {};
+    a.dy = dy, a.dsum = dsum, a.sum = const_cast<void*>(s), a.ldr = lds, a.w = weight;
+    a.rstd = const_cast<float*>(rstd), a.dx = dx, a.dr = dresidual;
+    a.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
+    a.T = T, a.D = D;
+    a.vec = D % 8 == 0 && lds % 8 == 0 && mi::aligned16(dy) && mi::aligned16(s) && mi::aligned16(weight) &&
+            (!dsum || mi::aligned16(dsum)) && (!dx || mi::aligned16(dx)) && (!dresidual || mi::aligned16(dresidual));
+    const int grid = mi::rms::grid_of(T, D);
+    const int rc2 = mi::rms::dispatch<true, false>(a, dtype, rdtype, grid, st);
+    if (rc2 != MI_OK || !dweight) return rc2;
+    mi::rms::column_sum_kernel<<<mi::cdiv(D, 32), 256, 0, st>>>(a.dw_part, dweight, grid, D);
+    MI_CHECK_LAUNCH();
+    return MI_OK;
+}

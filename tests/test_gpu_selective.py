@@ -1,0 +1,640 @@
+"""The float Mamba operators against their 64-bit formulas (tests/selective_ref.py).
+
+Tolerances.  A result is a sum of terms; each term meets a number of fp32 roundings (2^-24 of the term each) on its way.
+Scan: a state passes at most L positions.  A position costs it at most 8: the decay a = 2^x, x = dt A log2(e), is off by
+x times the 8 roundings behind x (softplus 5, two products, the constant) plus 4 for ex2 itself, and a (4 + 8 |x|) =
+e^-v (4 + 8 v / ln 2 ln 2) <= 4 + 8 / e < 7; the multiply-add is one more.  Around it the inputs, gates and sums over
+states and channels cost less than 64, so 8 L + 64 for y and h.  A gradient meets the recurrence twice, and its sums
+over batch and positions add at most batch * L roundings: 16 L + 128 + batch * L.
+Convolution: 4 taps, bias, SiLU's sigmoid and products: 32; its parameters' sums batch * L more.
+Norm: a row's squares are added at most 32 in a thread, then over at most 16 warps and 5 + 15 steps: 64, and 16 around.
+"""
+import pytest
+import torch
+
+import selective_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def sel(cuda_dev):
+    from mamba_integer_b200 import selective
+    return selective
+
+
+def scan_inputs(dev, dtype, b, n, d, k, seed=0, D=True, z=True, bias=True, softplus=True, h0=False, lengths=None):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(u=r(b, n, d).to(dtype), A=-(0.2 * r(d, k)).exp() * torch.arange(1, k + 1), B=r(b, n, k).to(dtype),
+             C=r(b, n, k).to(dtype), D=r(d) if D else None, z=r(b, n, d).to(dtype) if z else None,
+             h0=r(b, d, k) if h0 else None, softplus=softplus)
+    if softplus:
+        a["delta"] = (r(b, n, d) - (0 if bias else 3)).to(dtype)
+        a["bias"] = r(d) - 4 if bias else None
+    else:
+        a["delta"] = (0.05 * r(b, n, d).exp()).to(dtype)
+        a["bias"] = None if not bias else 0.01 * r(d).exp()
+    a["lengths"] = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    return {key: t.to(dev) if isinstance(t, torch.Tensor) else t for key, t in a.items()}
+
+
+def call_scan(sel, a, **over):
+    a = {**a, **over}
+    return sel.selective_scan(a["u"], a["delta"], a["A"], a["B"], a["C"], D=a["D"], z=a["z"], delta_bias=a["bias"],
+                              delta_softplus=a["softplus"], h0=a["h0"], lengths=a["lengths"], return_state=True)
+
+
+def check_scan(y, h, a):
+    want, mag = ref.scan(a), ref.scan(a, mag=True)
+    units = 8 * a["u"].shape[1] + 64
+    ref.check(y, want["y"], mag["y"], units, "y")
+    ref.check(h, want["h"], mag["h"], units, "h")
+
+
+SCAN_SIZES = [
+    # batch, L, channels, states: tiles of 16 and 32 positions, blocks of 32 and 64 channels, lanes of 4 states
+    (1, 1, 1, 1), (2, 1, 64, 16), (1, 2, 33, 3), (3, 15, 31, 8), (2, 16, 32, 16), (2, 17, 65, 17), (1, 31, 100, 5),
+    (2, 33, 64, 24), (1, 64, 40, 32), (2, 65, 24, 33), (1, 40, 17, 64), (2, 127, 8, 16), (1, 128, 96, 16),
+    (2, 200, 72, 16), (1, 333, 40, 64), (1, 161, 130, 8),
+]
+
+
+@pytest.mark.parametrize("size", SCAN_SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_prompt(sel, cuda_dev, size, dtype):
+    a = scan_inputs(cuda_dev, dtype, *size, h0=size[1] % 2 == 1)
+    check_scan(*call_scan(sel, a), a)
+
+
+@pytest.mark.parametrize("D,z,bias,softplus,h0", [(False, False, False, False, False), (True, False, False, True, True),
+                                                  (False, True, True, False, True), (False, False, True, True, False)])
+def test_scan_options(sel, cuda_dev, D, z, bias, softplus, h0):
+    a = scan_inputs(cuda_dev, F32, 2, 37, 48, 16, D=D, z=z, bias=bias, softplus=softplus, h0=h0)
+    check_scan(*call_scan(sel, a), a)
+
+
+@pytest.mark.parametrize("n", [37, 260])
+def test_scan_lengths(sel, cuda_dev, n):
+    # 0, 1, inside and at a tile's border, past the end (clamped), negative (clamped)
+    lens = [0, 1, 16, 20, n, n + 5, -3]
+    a = scan_inputs(cuda_dev, BF16, len(lens), n, 40, 16, h0=True, lengths=lens)
+    clamped = dict(a, lengths=torch.tensor([min(max(v, 0), n) for v in lens], dtype=torch.int32))
+    for name in ("u", "delta", "B", "C", "z"):
+        for i, v in enumerate(clamped["lengths"].tolist()):
+            a[name][i, v:] = float("nan")  # what lies behind a length is not used
+    y, h = call_scan(sel, a)
+    check_scan(y, h, clamped)
+    for i, v in enumerate(clamped["lengths"].tolist()):
+        assert not y[i, v:].any()
+    assert torch.equal(h[0], a["h0"][0])
+
+
+def test_scan_strides_slices_and_broadcasts(sel, cuda_dev):
+    b, n, d, k = 3, 70, 48, 16
+    a = scan_inputs(cuda_dev, BF16, b, n, d, k)
+    want = call_scan(sel, a)
+    # columns of wider rows, aligned and not; every other row; sequences expanded from one
+    for pad in (8, 3):
+        wide = torch.randn(b, 2 * n, 2 * d + pad, device=cuda_dev).to(BF16)
+        z = wide[:, ::2, pad:pad + d]
+        z.copy_(a["z"])
+        rows = torch.randn(b, n, pad + 2 * k, device=cuda_dev).to(BF16)
+        B, C = rows[..., pad:pad + k], rows[..., pad + k:]
+        B.copy_(a["B"]), C.copy_(a["C"])
+        got = call_scan(sel, a, z=z, B=B, C=C)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = {key: a[key][:1] for key in ("u", "delta", "B", "C", "z")}
+    spread = call_scan(sel, a, **{key: t.expand(b, -1, -1) for key, t in one.items()})
+    copied = call_scan(sel, a, **{key: t.repeat(b, 1, 1) for key, t in one.items()})
+    assert torch.equal(spread[0], copied[0]) and torch.equal(spread[1], copied[1])
+    # parameters off the 16-byte boundary, and transposed
+    flat = torch.empty(d * k + 1, device=cuda_dev)
+    A = flat[1:].view(d, k)
+    A.copy_(a["A"])
+    got = call_scan(sel, a, A=A)
+    assert torch.equal(got[0], want[0])
+    got = call_scan(sel, a, A=a["A"].t().contiguous().t())
+    assert torch.equal(got[0], want[0])
+
+
+def test_scan_offsets_past_32_bits(sel, cuda_dev):
+    n, d, k = 20, 32, 16
+    a = scan_inputs(cuda_dev, BF16, 2, n, d, k)
+    want = call_scan(sel, a)
+    big = torch.empty(2 ** 31 + 64 * n, dtype=BF16, device=cuda_dev)
+    far = {}
+    for i, key in enumerate(("u", "delta", "z")):
+        far[key] = big[i * 8 * d:].as_strided((2, n, d), (2 ** 31 + 3 * d - 2 ** 10, d, 1))
+        far[key].copy_(a[key])
+        got = call_scan(sel, a, **{key: far[key]})
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_scan_extreme_steps(sel, cuda_dev):
+    """A step that forgets the state at once, one that keeps it exactly, softplus far on both sides."""
+    a = scan_inputs(cuda_dev, F32, 1, 40, 32, 16, h0=True, bias=False)
+    a["delta"][0, ::3] = 60.0
+    a["delta"][0, 1::3] = -80.0
+    check_scan(*call_scan(sel, a), a)
+    a["delta"][0, 5] = float("nan")
+    y, h = call_scan(sel, a)
+    assert not y[0, :5].isnan().any() and y[0, 5:].isnan().all() and h.isnan().all()
+
+
+def scan_grads(sel, a, dy, dh):
+    names = [k for k in ("u", "delta", "A", "B", "C", "D", "z", "bias", "h0") if a[k] is not None]
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in names}
+    y, h = call_scan(sel, a, **leaves)
+    outs = [(o, g) for o, g in ((y, dy), (h, dh)) if g is not None]
+    got = torch.autograd.grad([o for o, _ in outs], list(leaves.values()), [g for _, g in outs], allow_unused=True)
+    return y, h, dict(zip(names, got))
+
+
+def check_scan_grads(got, a, dy, dh):
+    args = dict(a, dy=dy, dh=dh)
+    want, mag = ref.scan(args), ref.scan(args, mag=True)
+    b, n, _ = a["u"].shape
+    for name, t in got.items():
+        assert t.dtype == a[name].dtype
+        ref.check(t, want["d" + name], mag["d" + name], 16 * n + 128 + b * n, "d" + name)
+
+
+@pytest.mark.parametrize("size", SCAN_SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_gradients(sel, cuda_dev, size, dtype):
+    b, n, d, k = size
+    a = scan_inputs(cuda_dev, dtype, *size, h0=True)
+    g = torch.Generator().manual_seed(5)
+    dy = torch.randn(b, n, d, generator=g).to(cuda_dev, dtype)
+    dh = torch.randn(b, d, k, generator=g).to(cuda_dev)
+    y, h, got = scan_grads(sel, a, dy, dh)
+    check_scan(y, h, a)
+    check_scan_grads(got, a, dy, dh)
+
+
+@pytest.mark.parametrize("D,z,bias,softplus", [(False, False, False, False), (True, False, False, True),
+                                               (False, True, True, False)])
+@pytest.mark.parametrize("only", ["y", "h"])
+def test_scan_gradients_of_options(sel, cuda_dev, D, z, bias, softplus, only):
+    a = scan_inputs(cuda_dev, F32, 2, 37, 72, 16, D=D, z=z, bias=bias, softplus=softplus)
+    dy = torch.randn(2, 37, 72, device=cuda_dev) if only == "y" else None
+    dh = torch.randn(2, 72, 16, device=cuda_dev) if only == "h" else None
+    _, _, got = scan_grads(sel, a, dy, dh)
+    check_scan_grads(got, a, dy, dh)
+
+
+@pytest.mark.parametrize("n", [37, 260])
+def test_scan_gradients_with_lengths(sel, cuda_dev, n):
+    lens = [0, 1, 16, 20, n]
+    a = scan_inputs(cuda_dev, BF16, len(lens), n, 40, 16, h0=True, lengths=lens)
+    dy = torch.randn(len(lens), n, 40, device=cuda_dev).to(BF16)
+    dh = torch.randn(len(lens), 40, 16, device=cuda_dev)
+    dirty = dict(a)
+    for name in ("u", "delta", "B", "C", "z"):
+        dirty[name] = a[name].clone()
+        for i, v in enumerate(lens):
+            dirty[name][i, v:] = float("inf")
+    dirty_dy = dy.clone()
+    for i, v in enumerate(lens):
+        dirty_dy[i, v:] = float("nan")
+    _, _, got = scan_grads(sel, dirty, dirty_dy, dh)
+    check_scan_grads(got, a, dy, dh)
+    for name in ("u", "delta", "B", "C", "z"):
+        for i, v in enumerate(lens):
+            assert not got[name][i, v:].any()
+
+
+def test_scan_gradients_follow_differences(sel, cuda_dev):
+    """<gradient, v> against a central difference of the operator itself along v."""
+    a = scan_inputs(cuda_dev, F32, 2, 24, 32, 16, h0=True)
+    dy = torch.randn(2, 24, 32, device=cuda_dev)
+    _, _, got = scan_grads(sel, a, dy, torch.zeros(2, 32, 16, device=cuda_dev))
+    g = torch.Generator(device=cuda_dev).manual_seed(3)
+    # a step of 2^-7 of each value: the curvature gives ~(2^-7)^2 of the slope's terms, rounding 2^-24 * 2^7 of y's
+    for name in got:
+        v = torch.randn(a[name].shape, generator=g, device=cuda_dev) * a[name].abs()
+        up, down = (call_scan(sel, a, **{name: a[name] + s * 2 ** -7 * v})[0].double() for s in (1, -1))
+        terms = (up - down) * 2 ** 6 * dy
+        assert abs(float((got[name].double() * v).sum() - terms.sum())) <= 2e-2 * float(terms.norm()) + 1e-3, name
+
+
+def test_scan_gradients_of_shared_inputs(sel, cuda_dev):
+    """One leaf for every sequence (expanded), and the same leaf as two inputs: their gradients add up."""
+    a = scan_inputs(cuda_dev, F32, 3, 20, 32, 16)
+    B = a["B"][:1].clone().requires_grad_(True)
+    y, _ = call_scan(sel, a, B=B.expand(3, -1, -1), C=B.expand(3, -1, -1))
+    (got,) = torch.autograd.grad(y.sum(), B)  # the gradient of a sum is expanded too
+    full = dict(a, B=B.detach().expand(3, -1, -1), C=B.detach().expand(3, -1, -1), dy=torch.ones_like(y))
+    want, mag = ref.scan(full), ref.scan(full, mag=True)
+    ref.check(got, (want["dB"] + want["dC"]).sum(0, keepdim=True), (mag["dB"] + mag["dC"]).sum(0, keepdim=True),
+              16 * 20 + 128 + 60, "shared")
+
+
+def test_scan_repeats_its_bits(sel, cuda_dev):
+    a = scan_inputs(cuda_dev, BF16, 2, 300, 96, 16, h0=True)
+    dy = torch.randn(2, 300, 96, device=cuda_dev).to(BF16)
+    dh = torch.randn(2, 96, 16, device=cuda_dev)
+    one, two = (scan_grads(sel, a, dy, dh) for _ in range(2))
+    assert torch.equal(one[0], two[0]) and all(torch.equal(one[2][k], two[2][k]) for k in one[2])
+    y, h = call_scan(sel, a)  # the form without a backward pass gives the training form's bits
+    assert torch.equal(y, one[0]) and torch.equal(h, one[1])
+
+
+@pytest.mark.parametrize("size", [(1, 1, 1), (3, 33, 5), (5, 64, 16), (2, 100, 24), (4, 32, 64), (70, 17, 33)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_step(sel, cuda_dev, size, dtype):
+    b, d, k = size
+    a = scan_inputs(cuda_dev, dtype, b, 3, d, k, h0=True)
+    h = a["h0"].clone()
+    rows = torch.empty(b, 3, 2 * d + 1, dtype=dtype, device=cuda_dev)
+    z = rows[..., 1:d + 1]
+    z.copy_(a["z"])
+    ys = [sel.selective_scan_step(h, a["u"][:, t], a["delta"][:, t], a["A"], a["B"][:, t], a["C"][:, t], D=a["D"],
+                                  z=z[:, t], delta_bias=a["bias"], delta_softplus=True) for t in range(3)]
+    check_scan(torch.stack(ys, 1), h, a)
+
+
+def test_empty_calls(sel, cuda_dev):
+    z = lambda *s, dtype=F32: torch.randn(*s, device=cuda_dev).to(dtype)  # noqa: E731
+    for b, n in ((0, 5), (2, 0)):
+        h0 = z(b, 8, 4).requires_grad_(True)
+        y, h = sel.selective_scan(z(b, n, 8), z(b, n, 8), z(8, 4), z(b, n, 4), z(b, n, 4), h0=h0, return_state=True)
+        assert y.shape == (b, n, 8) and torch.equal(h, h0)
+        (g,) = torch.autograd.grad(h.sum(), h0)
+        assert torch.equal(g, torch.ones_like(h0))
+        win = z(b, 3, 8)
+        y, out = sel.causal_conv1d(z(b, n, 8), z(8, 4), win=win, return_window=True)
+        assert y.shape == (b, n, 8) and torch.equal(out, win)
+    assert sel.selective_scan_step(z(0, 8, 4), z(0, 8), z(0, 8), z(8, 4), z(0, 4), z(0, 4)).shape == (0, 8)
+    assert sel.causal_conv1d_step(z(0, 8), z(8, 4), z(0, 3, 8)).shape == (0, 8)
+    y, s = sel.rms_norm(z(0, 8), z(8), residual=z(0, 8))
+    assert y.shape == s.shape == (0, 8)
+    q, scale, s = sel.rms_norm_quant(z(2, 0, 8), z(8))
+    assert q.shape == (2, 0, 8) and scale.shape == (2, 0) and s is None
+
+
+# ---------------------------------------------------------------------------
+# convolution
+# ---------------------------------------------------------------------------
+def conv_inputs(dev, dtype, b, n, d, k, bias=True, silu=True, win=False, lengths=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(x=r(b, n, d).to(dtype), w=r(d, k), bias=r(d) if bias else None, silu=silu,
+             win=r(b, k - 1, d).to(dtype) if win else None,
+             lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32))
+    return {key: t.to(dev) if isinstance(t, torch.Tensor) else t for key, t in a.items()}
+
+
+def call_conv(sel, a, **over):
+    a = {**a, **over}
+    return sel.causal_conv1d(a["x"], a["w"], bias=a["bias"], silu=a["silu"], win=a["win"], lengths=a["lengths"],
+                             return_window=True)
+
+
+CONV_SIZES = [(1, 1, 1, 4), (2, 2, 5, 4), (3, 3, 64, 4), (1, 16, 8, 2), (2, 17, 33, 3), (2, 19, 128, 4), (1, 130, 36, 4),
+              (2, 257, 20, 3), (1, 128, 260, 2)]
+
+
+@pytest.mark.parametrize("size", CONV_SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bias,silu,win", [(True, True, True), (False, False, False), (True, False, True)])
+def test_conv(sel, cuda_dev, size, dtype, bias, silu, win):
+    b, n, d, k = size
+    a = conv_inputs(cuda_dev, dtype, *size, bias=bias, silu=silu, win=win)
+    g = torch.Generator().manual_seed(9)
+    dy = torch.randn(b, n, d, generator=g).to(cuda_dev, dtype)
+    dwin = torch.randn(b, k - 1, d, generator=g).to(cuda_dev, dtype) if win else None
+    y, out = call_conv(sel, a)
+    args = dict(a, dy=dy, dwin=dwin)
+    want, mag = ref.conv(args), ref.conv(args, mag=True)
+    ref.check(y, want["y"], mag["y"], 32, "y")
+    assert torch.equal(out.cpu().double(), want["win"])
+    names = [m for m in ("x", "w", "bias", "win") if a[m] is not None]
+    leaves = {m: a[m].clone().requires_grad_(True) for m in names}
+    y2, out2 = call_conv(sel, a, **leaves)
+    assert torch.equal(y2, y)
+    got = torch.autograd.grad([y2, out2] if win else [y2], list(leaves.values()), [dy, dwin] if win else [dy])
+    for m, t in zip(names, got):
+        ref.check(t, want["d" + m], mag["d" + m], 64 + (b * n if m in ("w", "bias") else 0), "d" + m)
+
+
+@pytest.mark.parametrize("n", [5, 40, 150])
+def test_conv_lengths(sel, cuda_dev, n):
+    lens = [0, 1, 2, n - 1, n, n + 7, -1]
+    a = conv_inputs(cuda_dev, BF16, len(lens), n, 24, 4, win=True, lengths=lens)
+    clamped = [min(max(v, 0), n) for v in lens]
+    dy = torch.randn(len(lens), n, 24, device=cuda_dev).to(BF16)
+    dwin = torch.randn(len(lens), 3, 24, device=cuda_dev).to(BF16)
+    clean = dict(a, lengths=torch.tensor(clamped, dtype=torch.int32), dy=dy.clone(), dwin=dwin)
+    want, mag = ref.conv(clean), ref.conv(clean, mag=True)
+    a["x"] = a["x"].clone()
+    for i, v in enumerate(clamped):
+        a["x"][i, v:] = float("nan")
+        dy[i, v:] = float("nan")
+    leaves = {m: a[m].clone().requires_grad_(True) for m in ("x", "w", "bias", "win")}
+    y, out = call_conv(sel, a, **leaves)
+    got = torch.autograd.grad([y, out], list(leaves.values()), [dy, dwin])
+    ref.check(y, want["y"], mag["y"], 32, "y")
+    assert torch.equal(out.cpu().double(), want["win"])
+    for m, t in zip(leaves, got):
+        ref.check(t, want["d" + m], mag["d" + m], 64 + (len(lens) * n if m in ("w", "bias") else 0), "d" + m)
+
+
+def test_conv_strides_and_weight_forms(sel, cuda_dev):
+    a = conv_inputs(cuda_dev, BF16, 2, 50, 40, 4)
+    want, win = call_conv(sel, a)
+    for pad in (8, 1):
+        wide = torch.zeros(2, 100, 80 + pad, dtype=BF16, device=cuda_dev)
+        x = wide[:, ::2, pad:pad + 40]
+        x.copy_(a["x"])
+        got = call_conv(sel, a, x=x)
+        assert torch.equal(got[0], want) and torch.equal(got[1], win)
+    got = call_conv(sel, a, w=a["w"].unsqueeze(1))
+    assert torch.equal(got[0], want)
+    big = torch.empty(2 ** 31 + 4096, dtype=BF16, device=cuda_dev)
+    far = big.as_strided((2, 50, 40), (2 ** 31 - 1024, 40, 1))
+    far.copy_(a["x"])
+    got = call_conv(sel, a, x=far)
+    assert torch.equal(got[0], want)
+    x = a["x"][:1].clone().requires_grad_(True)  # one sequence for both, and an expanded gradient
+    (g,) = torch.autograd.grad(call_conv(sel, a, x=x.expand(2, -1, -1))[0].sum(), x)
+    one = dict(a, x=x.detach(), dy=torch.ones(1, 50, 40, device=cuda_dev))
+    r, m = ref.conv(one), ref.conv(one, mag=True)
+    # two rounded halves and their rounded sum
+    assert ((g.cpu().double() - 2 * r["dx"]).abs() <= 2 ** -8 * 4 * r["dx"].abs() + 2 ** -24 * 200 * m["dx"]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("d,k,silu", [(1, 2, True), (33, 3, False), (64, 4, True), (1030, 4, True)])
+def test_conv_step(sel, cuda_dev, dtype, d, k, silu):
+    a = conv_inputs(cuda_dev, dtype, 3, 5, d, k, silu=silu, win=True)
+    win = a["win"].clone()
+    ys = [sel.causal_conv1d_step(a["x"][:, t], a["w"], win, bias=a["bias"], silu=silu) for t in range(5)]
+    y, out = call_conv(sel, a)
+    assert torch.equal(torch.stack(ys, 1), y) and torch.equal(win, out)
+
+
+# ---------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------
+NORM_SIZES = [(1, 1), (3, 7), (2, 32), (5, 100), (9, 256), (4, 768), (3, 1000), (2, 1025), (1, 2048), (2, 4096), (3, 8191),
+              (1, 16384), (700, 264)]
+
+
+@pytest.mark.parametrize("size", NORM_SIZES)
+@pytest.mark.parametrize("dtype,rdtype", [(F32, None), (F32, F32), (BF16, None), (BF16, BF16), (BF16, F32), (F16, F16),
+                                          (F16, F32)])
+def test_norm(sel, cuda_dev, size, dtype, rdtype):
+    T, d = size
+    g = torch.Generator().manual_seed(T + d)
+    r = lambda *s: torch.randn(*s, generator=g).to(cuda_dev)  # noqa: E731
+    x, w = r(T, d).to(dtype).requires_grad_(True), (1 + 0.3 * r(d)).requires_grad_(True)
+    res = None if rdtype is None else (2 * r(T, d)).to(rdtype).requires_grad_(True)
+    dy, ds = r(T, d).to(dtype), None if rdtype is None else r(T, d).to(rdtype)
+    y, s = sel.rms_norm(x, w, eps=1e-5, residual=res)
+    kept = x.detach() if res is None else (x.detach().float() + res.detach().float()).to(rdtype)
+    assert s is None if res is None else torch.equal(s, kept)
+    want = ref.norm(kept, w, 1e-5, dy, ds)
+    ref.check(y, want["y"], want["y"].abs(), 80, "y")
+    outs = ([y], [dy]) if res is None else ([y, s], [dy, ds])
+    got = torch.autograd.grad(outs[0], [x, w] + ([] if res is None else [res]), outs[1])
+    assert all(t.dtype == o.dtype for t, o in zip(got, [x, w, res]))
+    ref.check(got[0], want["ds"], want["ds_mag"], 200, "dx")
+    ref.check(got[1], want["dw"], want["dw_mag"], 100 + T, "dw")
+    if res is not None:
+        ref.check(got[2], want["ds"], want["ds_mag"], 200, "dresidual")
+    with torch.no_grad():
+        y2, s2 = sel.rms_norm(x, w, eps=1e-5, residual=res)
+        assert torch.equal(y, y2)
+        # the int8 form: the scale is max|y| / 127, a value half a step off at most
+        q, scale, s3 = sel.rms_norm_quant(x, w, eps=1e-5, residual=res)
+    assert s3 is None if res is None else torch.equal(s3, kept)
+    most = want["y"].abs().amax(1)
+    assert ((scale.cpu().double() - most.clamp(min=1e-8) / 127).abs() <= 82 * 2 ** -24 * most / 127 + 1e-12).all()
+    off = (q.cpu().double() * scale.cpu().double()[:, None] - want["y"]).abs()
+    assert (off <= scale.cpu().double()[:, None] * (0.5 + 127 * 90 * 2 ** -24)).all()
+    assert int(q.abs().max()) <= 127
+
+
+def test_norm_strides_zeros_and_infinities(sel, cuda_dev):
+    wide = torch.randn(6, 2, 300, device=cuda_dev).to(BF16)
+    w = torch.randn(96, device=cuda_dev)
+    for x in (wide[:, 0, :96], wide[:, 1, 3:99], wide[:1, 0, :96].expand(4, -1), wide[..., 8:104]):
+        y, _ = sel.rms_norm(x, w)
+        y2, _ = sel.rms_norm(x.contiguous(), w)
+        assert y.shape == x.shape and torch.equal(y, y2)
+    lead = torch.randn(96, device=cuda_dev)
+    y, s = sel.rms_norm(lead, w, residual=lead)
+    assert y.shape == (96,) and torch.equal(s, 2 * lead)
+    x = torch.zeros(3, 96, device=cuda_dev)
+    x[1] = 1e30  # its square is infinite: the norm is 0, as the formula says in 32 bits
+    x[2, 5] = float("nan")
+    y, _ = sel.rms_norm(x, w)
+    assert not y[0].any() and not y[1].any() and y[2].isnan().all()
+    q, scale, _ = sel.rms_norm_quant(x[:2], w)
+    assert not q.any() and torch.equal(scale.cpu(), torch.full((2,), 1e-8) / 127)  # a true division
+    x2 = wide[:, 0, :96].float().requires_grad_(True)  # a strided row, an expanded gradient, one gradient of two
+    _, s = sel.rms_norm(x2, w, residual=x2)
+    (g,) = torch.autograd.grad(s.sum(), x2)
+    assert torch.equal(g, torch.full_like(x2, 2))
+
+
+def test_norm_quant_feeds_the_ternary_product(sel, cuda_dev):
+    from mamba_integer_b200 import kernels, synth
+    from mamba_integer_b200.rational_bitnet import BitLinear
+    g = torch.Generator().manual_seed(0)
+    lin = BitLinear(256, 128)
+    lin.weight.data.copy_(synth.ternary_weight(128, 256, g))
+    lin = lin.to(cuda_dev)
+    x, r = (torch.randn(37, 256, generator=g).to(cuda_dev) for _ in range(2))
+    w = torch.ones(256, device=cuda_dev)
+    q, scale, s = sel.rms_norm_quant(x, w, residual=r)
+    tw = lin.device_weights(cuda_dev)
+    got = kernels.bitlinear_packed(q, tw.w2, scale, tw.scale)
+    with torch.no_grad():
+        y, _ = sel.rms_norm(x, w, residual=r)
+        assert torch.equal(got, lin(y))  # quantising the fp32 rows apart gives the same int8 rows
+
+
+# ---------------------------------------------------------------------------
+# together, on other streams, in graphs
+# ---------------------------------------------------------------------------
+class FloatLayer(torch.nn.Module):
+    """norm, input projection, convolution, scan, output projection: a float Mamba layer as a user writes it."""
+
+    def __init__(self, d=48, k=16, R=6, taps=4, seed=0):
+        super().__init__()
+        g = torch.Generator().manual_seed(seed)
+        p = lambda *s, scale=1.0: torch.nn.Parameter(torch.randn(*s, generator=g) * scale)  # noqa: E731
+        di = 2 * d
+        self.di, self.k, self.R = di, k, R
+        self.norm_w = torch.nn.Parameter(torch.ones(d))
+        self.w_in, self.w_x = p(2 * di, d, scale=d ** -0.5), p(R + 2 * k, di, scale=di ** -0.5)
+        self.w_dt, self.w_out = p(di, R, scale=R ** -0.5), p(d, di, scale=di ** -0.5)
+        self.conv_w, self.conv_b = p(di, taps, scale=0.5), p(di, scale=0.1)
+        self.A = torch.nn.Parameter(-torch.arange(1, k + 1).float().repeat(di, 1))
+        self.D, self.dt_bias = torch.nn.Parameter(torch.ones(di)), torch.nn.Parameter(torch.full((di,), -3.0))
+
+    def forward(self, sel, x, residual, win=None, h0=None):
+        F = torch.nn.functional
+        y, residual = sel.rms_norm(x, self.norm_w, residual=residual)
+        xz = F.linear(y, self.w_in)
+        c, win = sel.causal_conv1d(xz[..., :self.di], self.conv_w, bias=self.conv_b, silu=True, win=win,
+                                   return_window=True)
+        xp = F.linear(c, self.w_x)
+        delta = F.linear(xp[..., :self.R], self.w_dt)
+        s, h = sel.selective_scan(c, delta, self.A, xp[..., self.R:self.R + self.k], xp[..., self.R + self.k:], D=self.D,
+                                  z=xz[..., self.di:], delta_bias=self.dt_bias, delta_softplus=True, h0=h0,
+                                  return_state=True)
+        return F.linear(s, self.w_out), residual, win, h
+
+    def step(self, sel, x, residual, win, h):
+        F = torch.nn.functional
+        y, residual = sel.rms_norm(x, self.norm_w, residual=residual)
+        xz = F.linear(y, self.w_in)
+        c = sel.causal_conv1d_step(xz[:, :self.di], self.conv_w, win, bias=self.conv_b, silu=True)
+        xp = F.linear(c, self.w_x)
+        delta = F.linear(xp[:, :self.R], self.w_dt)
+        s = sel.selective_scan_step(h, c, delta, self.A, xp[:, self.R:self.R + self.k], xp[:, self.R + self.k:], D=self.D,
+                                    z=xz[:, self.di:], delta_bias=self.dt_bias, delta_softplus=True)
+        return F.linear(s, self.w_out), residual
+
+    def plain(self, x, residual):
+        """the same in torch, for 64 bits"""
+        F = torch.nn.functional
+        residual = residual + x
+        y = residual / torch.sqrt((residual ** 2).mean(-1, keepdim=True) + 1e-6) * self.norm_w
+        xz = F.linear(y, self.w_in)
+        n, taps = x.shape[1], self.conv_w.shape[1]
+        rows = F.pad(xz[..., :self.di], (0, 0, taps - 1, 0))
+        c = F.silu(sum(rows[:, i:i + n] * self.conv_w[:, i] for i in range(taps)) + self.conv_b)
+        xp = F.linear(c, self.w_x)
+        dt = F.softplus(F.linear(xp[..., :self.R], self.w_dt) + self.dt_bias)
+        B, C = xp[..., self.R:self.R + self.k], xp[..., self.R + self.k:]
+        h, out = torch.zeros(x.shape[0], self.di, self.k, dtype=x.dtype, device=x.device), []
+        for t in range(n):
+            h = torch.exp(dt[:, t, :, None] * self.A) * h + (dt[:, t] * c[:, t])[..., None] * B[:, t, None]
+            out.append((h * C[:, t, None]).sum(-1) + self.D * c[:, t])
+        return F.linear(torch.stack(out, 1) * F.silu(xz[..., self.di:]), self.w_out), residual
+
+
+@pytest.fixture
+def exact_products(cuda_dev):
+    kept = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    yield
+    torch.backends.cuda.matmul.allow_tf32 = kept
+
+
+def test_layer_forward_and_gradients(sel, cuda_dev, exact_products):
+    layer = FloatLayer().to(cuda_dev)
+    x, r = (torch.randn(2, 45, 48, device=cuda_dev).requires_grad_(True) for _ in range(2))
+    y, res, _, _ = layer(sel, x, r)
+    g, gr = torch.randn_like(y), torch.randn_like(res)
+    leaves = [x, r, *layer.parameters()]
+    got = torch.autograd.grad([y, res], leaves, [g, gr])
+    exact = FloatLayer().double().to(cuda_dev)
+    xd, rd = (t.detach().double().requires_grad_(True) for t in (x, r))
+    yd, resd = exact.plain(xd, rd)
+    want = torch.autograd.grad([yd, resd], [xd, rd, *exact.parameters()], [g.double(), gr.double()])
+    # five products and three operators in a row, each within 1e-6 of what enters it in the 2-norm, gains of order 10
+    for a, b in [(y.detach(), yd.detach()), (res.detach(), resd.detach()), *zip(got, want)]:
+        assert float((a.double() - b).norm()) <= 1e-4 * float(b.norm())
+
+
+def test_layer_prompt_then_tokens(sel, cuda_dev, exact_products):
+    layer = FloatLayer().to(cuda_dev)
+    x, r = (torch.randn(3, 24, 48, device=cuda_dev) for _ in range(2))
+    with torch.no_grad():
+        whole, res, win_w, h_w = layer(sel, x, r)
+        y, _, win, h = layer(sel, x[:, :17], r[:, :17])
+        parts = [y]
+        y, _, win, h = layer(sel, x[:, 17:20], r[:, 17:20], win=win, h0=h)
+        parts.append(y)
+        for t in range(20, 24):
+            y, _ = layer.step(sel, x[:, t], r[:, t], win, h)
+            parts.append(y.unsqueeze(1))
+    got = torch.cat(parts, 1)
+    # the products of other shapes round differently: 1e-6 of the rows' norm through three operators
+    assert float((got - whole).norm()) <= 2e-5 * float(whole.norm())
+    assert float((h - h_w).norm()) <= 2e-5 * float(h_w.norm())
+    assert float((win - win_w).norm()) <= 2e-5 * float(win_w.norm())
+
+
+def test_other_stream(sel, cuda_dev):
+    a = scan_inputs(cuda_dev, BF16, 2, 300, 64, 16)
+    dy = torch.randn(2, 300, 64, device=cuda_dev).to(BF16)
+    want = scan_grads(sel, a, dy, None)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = scan_grads(sel, a, dy, None)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(got[2][k], want[2][k]) for k in want[2])
+
+
+def _capture(fn):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fn()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = fn()
+    return g, out
+
+
+def test_graphs_of_prompts_and_training_steps(sel, cuda_dev):
+    """Two graphs of different sizes, replayed in turn on new values: each keeps its own workspaces."""
+    made = []
+    for seed, size in ((0, (1, 320, 64, 16)), (1, (2, 150, 40, 24))):
+        a = scan_inputs(cuda_dev, F32, *size, seed=seed, h0=True)
+        dy = torch.randn(*a["u"].shape, device=cuda_dev)
+        leaves = {k: a[k].requires_grad_(True) for k in ("u", "A", "B", "h0")}
+
+        def train(a=a, dy=dy, leaves=leaves):
+            y, h = call_scan(sel, a)
+            grads = torch.autograd.grad(y, list(leaves.values()), dy)
+            return y.detach(), grads  # no autograd graph outlives the call
+        made.append((a, dy, train, *_capture(train)))
+    for round_ in range(2):
+        for a, dy, train, graph, out in made:
+            with torch.no_grad():
+                a["u"].copy_(torch.randn_like(a["u"]))
+                a["h0"].mul_(0.5)
+        for a, dy, train, graph, out in made:
+            graph.replay()
+        torch.cuda.synchronize()
+        for a, dy, train, graph, out in made:
+            y, grads = train()
+            assert torch.equal(y, out[0]) and all(torch.equal(p, q) for p, q in zip(grads, out[1]))
+
+
+def test_graph_of_decode_steps(sel, cuda_dev):
+    a = scan_inputs(cuda_dev, BF16, 5, 6, 64, 16, h0=True)
+    c = conv_inputs(cuda_dev, BF16, 5, 6, 64, 4, win=True)
+    w = torch.randn(64, device=cuda_dev)
+    x, h, win = a["u"][:, 0].clone(), a["h0"].clone(), c["win"].clone()
+
+    def token():
+        q, scale, _ = sel.rms_norm_quant(x, w, residual=x)
+        y = sel.causal_conv1d_step(x, c["w"], win, bias=c["bias"], silu=True)
+        return q, scale, y, sel.selective_scan_step(h, y, a["delta"][:, 0], a["A"], a["B"][:, 0], a["C"][:, 0], D=a["D"],
+                                                    delta_bias=a["bias"], delta_softplus=True)
+    graph, out = _capture(token)
+    h.copy_(a["h0"]), win.copy_(c["win"])
+    got = []
+    for t in range(6):
+        x.copy_(a["u"][:, t])
+        graph.replay()
+        got.append([o.clone() for o in out])
+    h2, win2 = h.clone(), win.clone()
+    h.copy_(a["h0"]), win.copy_(c["win"])
+    for t in range(6):
+        x.copy_(a["u"][:, t])
+        assert all(torch.equal(p, q) for p, q in zip(token(), got[t]))
+    assert torch.equal(h, h2) and torch.equal(win, win2)
