@@ -57,6 +57,40 @@ __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&f)[K
     }
 }
 
+// Asynchronous copies into shared memory: `src` of BYTES bytes exist, the rest are zeros.
+template <int BYTES>
+__device__ __forceinline__ void cp_async(void* to, const void* from, int src) {
+    const uint32_t s = (uint32_t)__cvta_generic_to_shared(to);
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(s), "l"(from), "r"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(s), "l"(from), "n"(BYTES), "r"(src)
+                     : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+
+// Starts the copy of K elements at p, of which `valid` exist, into this
+// thread's own slot; the others become zeros.  `vec`: p is aligned to the pack
+// (16 bytes at most); elements one by one otherwise.  `any` is an address that
+// can be named where nothing is read.
+template <int K, typename T>
+__device__ __forceinline__ void fetch_pack(T* slot, const T* p, const void* any, int valid, bool vec) {
+    constexpr int BYTES = K * sizeof(T) < 16 ? K * sizeof(T) : 16, N = K * sizeof(T) / BYTES;
+    if (vec) {
+        const int have = valid <= 0 ? 0 : (valid < K ? valid : K) * (int)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int src = have - i * BYTES < 0 ? 0 : (have - i * BYTES < BYTES ? have - i * BYTES : BYTES);
+            cp_async<BYTES>(reinterpret_cast<char*>(slot) + i * BYTES,
+                            src ? reinterpret_cast<const char*>(p) + i * BYTES : reinterpret_cast<const char*>(any), src);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < K; i++) slot[i] = i < valid ? p[i] : from_f<T>(0.0f);
+    }
+}
+
 // 2^x to 2 ulp; results below the normal range are zero.
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;

@@ -60,6 +60,7 @@ struct Args {
     int softplus;
     int chunks, span;  // positions a chunk (a multiple of 32)
     int ovec;          // outputs' rows start on 8 elements' alignment
+    int pvec;          // D and delta_bias start on 16 bytes
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
@@ -100,18 +101,61 @@ struct St {  // 4 states in two f32x2 pairs
 __device__ __forceinline__ St st(float4 v) { return {make_float2(v.x, v.y), make_float2(v.z, v.w)}; }
 __device__ __forceinline__ float4 f4(St s) { return make_float4(s.a.x, s.a.y, s.b.x, s.b.y); }
 __device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
 __device__ __forceinline__ St mul(St x, float v) { return {__fmul2_rn(x.a, dup(v)), __fmul2_rn(x.b, dup(v))}; }
 __device__ __forceinline__ St mul(St x, St y) { return {__fmul2_rn(x.a, y.a), __fmul2_rn(x.b, y.b)}; }
 __device__ __forceinline__ St fma(St x, St y, St z) { return {__ffma2_rn(x.a, y.a, z.a), __ffma2_rn(x.b, y.b, z.b)}; }
-__device__ __forceinline__ St fma(St x, float v, St z) {
-    return {__ffma2_rn(x.a, dup(v), z.a), __ffma2_rn(x.b, dup(v), z.b)};
-}
+__device__ __forceinline__ St mul(St x, float2 v) { return {__fmul2_rn(x.a, v), __fmul2_rn(x.b, v)}; }
+__device__ __forceinline__ St fma(St x, float2 v, St z) { return {__ffma2_rn(x.a, v, z.a), __ffma2_rn(x.b, v, z.b)}; }
 __device__ __forceinline__ float dot(St x, St y) {
     const float2 p = __ffma2_rn(x.b, y.b, __fmul2_rn(x.a, y.a));
     return __fadd_rn(p.x, p.y);
 }
 __device__ __forceinline__ St exp2s(St x) {
     return {make_float2(exp2_fast(x.a.x), exp2_fast(x.a.y)), make_float2(exp2_fast(x.b.x), exp2_fast(x.b.y))};
+}
+
+// 2^x of two values on the FMA pipe: n = x rounded, 2^x = 2^n 2^r with r = x - n in [-1/2, 1/2] and 2^r = 1 + r q(r), q of
+// degree 5 with the least relative error (2^-27.9, by Remez's exchange).  x below -126 counts as -126, above 128 as 128
+// (inf); a NaN is not kept.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x = make_float2(fminf(fmaxf(x.x, -126.0f), 128.0f), fminf(fmaxf(x.y, -126.0f), 128.0f));
+    const float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers and leaves them in the low bits
+    const float2 t = __fadd2_rn(x, dup(magic));
+    const float2 r = __fadd2_rn(x, neg(__fadd2_rn(t, dup(-magic))));
+    float2 p = __ffma2_rn(dup(1.5469732170458883e-4f), r, dup(1.3410000829026103e-3f));
+    p = __ffma2_rn(p, r, dup(9.618030861020088e-3f));
+    p = __ffma2_rn(p, r, dup(5.550297349691391e-2f));
+    p = __ffma2_rn(p, r, dup(2.4022650718688965e-1f));
+    p = __ffma2_rn(p, r, dup(6.931472420692444e-1f));
+    p = __ffma2_rn(p, r, dup(1.0f));
+    return make_float2(__int_as_float((__float_as_int(t.x) << 23) + __float_as_int(p.x)),
+                       __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
+}
+
+// The decays of 4 positions.  One state of a lane's four goes through the FMA
+// pipe, the others through the special-function unit, so that neither waits
+// for the other.  The polynomial is the exacter of the two near 1, where a
+// decay's error adds up over the longest memory; A usually begins with its
+// slowest state, so it is the first of the four.
+template <bool EXACT>
+__device__ __forceinline__ void decays(const St& A2, const float (&dt)[4], St (&e)[4]) {
+    if constexpr (!EXACT) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) e[k] = exp2s(mul(A2, dup(dt[k])));
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            const float2 p = exp2_poly(__fmul2_rn(dup(A2.a.x), make_float2(dt[k], dt[k + 1])));
+            e[k].a.x = p.x, e[k + 1].a.x = p.y;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 x = __fmul2_rn(A2.b, dup(dt[k]));
+            e[k].a.y = exp2_fast(__fmul_rn(A2.a.y, dt[k]));
+            e[k].b = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+        }
+    }
 }
 
 // v[0 .. M): after the call the first M / 2 hold the sums over lanes that
@@ -128,24 +172,118 @@ __device__ __forceinline__ void halve(float* v, int mask) {
     }
 }
 
+// Sums of 4 positions' values over a channel's LN lanes: lane nl keeps position
+// nl % 4 (LN = 2: positions 2 nl and 2 nl + 1).
 template <int LN>
+__device__ __forceinline__ void over_states(float (&y)[4]) {
+    if constexpr (LN == 2) {
+        halve<4>(y, 1);
+    } else {
+        halve<4>(y, 2);
+        halve<2>(y, 1);
+#pragma unroll
+        for (int m = 4; m < LN; m *= 2) y[0] = __fadd_rn(y[0], __shfl_xor_sync(0xffffffffu, y[0], m));
+    }
+}
+template <int LN, int STRIDE>
+__device__ __forceinline__ void store_positions(float* col, const float* y, int nl) {
+    if constexpr (LN == 2) {
+        col[(2 * nl) * STRIDE] = y[0];
+        col[(2 * nl + 1) * STRIDE] = y[1];
+    } else {
+        if (nl < 4) col[nl * STRIDE] = y[0];
+    }
+}
+
+// Where the channels 2 u and 2 u + 1 of position t lie in its row of staged
+// (dt, dt u): a thread stages 4 such pairs, 16 bytes each, and the rotation
+// puts what 8 threads store at once into 8 different bank groups.
+__device__ __forceinline__ int place(int u, int t) { return u ^ (((u >> 3) ^ ((t & 1) << 1)) & 3); }
+
+// (dt, dt u) of a lane's channels c .. c + CPL - 1 at a position
+template <int CPL>
+__device__ __forceinline__ void staged(const float4* row, int c, int t, float (&dt)[CPL], float (&v)[CPL]) {
+    if constexpr (CPL == 1) {
+        const float2 x = reinterpret_cast<const float2*>(row + place(c >> 1, t))[c & 1];
+        dt[0] = x.x, v[0] = x.y;
+    } else {
+#pragma unroll
+        for (int j = 0; j < CPL; j += 2) {
+            const float4 x = row[place((c + j) >> 1, t)];
+            dt[j] = x.x, v[j] = x.y, dt[j + 1] = x.z, v[j + 1] = x.w;
+        }
+    }
+}
+// a thread's 8 (K) channels from c on
+template <int K>
+__device__ __forceinline__ void stage_steps(float4* row, int c, int t, const float (&dt)[K], const float (&v)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k += 2) row[place((c + k) >> 1, t)] = make_float4(dt[k], v[k], dt[k + 1], v[k + 1]);
+}
+
+// A NaN in A, which the polynomial would lose, is put into the state.
+__device__ __forceinline__ St keep_nan(St h, St A) {
+    if (isnan(A.a.x)) h.a.x = A.a.x;
+    return h;
+}
+
+template <typename T, int LN>
 struct Cfg {
     static constexpr int NP = 4 * LN;                    // padded states
     static constexpr int CL = 32 / LN;                   // channel lanes of a warp
-    static constexpr int CPL = LN <= 4 ? 1 : LN / 4;     // channels a lane, forward
-    static constexpr int CB = 4 * CL * CPL;              // channels a CTA: 64 (LN = 2) or 32
-    static constexpr int TT = 8 * THREADS / CB;          // positions a tile: 16 or 32
+    static constexpr int CPL = LN == 2 ? 1 : LN == 16 ? 4 : 2;  // channels a lane
+    static constexpr int CB = 4 * CL * CPL;              // channels a CTA: 64 (LN = 2, 4) or 32
+    static constexpr int TT = 8 * THREADS / CB;             // positions a tile: 16 or 32
     static constexpr int VPR = CB / 8;                   // packs of 8 channels a row
     static constexpr int QUADS = (TT * LN + THREADS - 1) / THREADS;  // packs of 4 states a thread, of each of B and C
+    static constexpr int YS = CB + 8;  // the 4 positions that a step of the loop stores lie in different banks
+    struct Smem {
+        float4 sd[TT][CB / 2];  // (dt, dt u) of two channels
+        float B[TT][NP], C[TT][NP];
+        float y[TT][YS];
+        float bias[CB], skip[CB];
+        alignas(16) T raw[2][3][THREADS * 8];       // by thread: u, delta and z as they come, of this tile and the next
+        alignas(16) T raw_bc[2][QUADS][THREADS * 4];  // B and C
+    };
+    struct ChunkSmem {
+        float4 sd[TT][CB / 2];  // (dt, dt u) or (dt, ds) of two channels
+        float B[TT][NP];    // B or C
+        float bias[CB];
+        alignas(16) T raw[3][THREADS * 8];  // by thread: delta, u or dy, and z as they come
+        alignas(16) T raw_bc[QUADS][THREADS * 4];
+    };
 };
 
-// One thread's part of a tile's loads: 8 channels of one position of u, delta
-// and z (or dy), and QUADS packs of B and C.
-template <typename T, int QUADS>
-struct Raw {
-    Pack<T, 8> u, d, z;
-    Pack<T, 4> B[QUADS], C[QUADS];
-};
+template <int K, typename T>
+__device__ __forceinline__ Pack<T, K> slot_pack(const T* slot) {
+    return *reinterpret_cast<const Pack<T, K>*>(slot);
+}
+
+// The CTA's channels of a parameter (zeros without one, and beyond the last channel)
+template <int CB>
+__device__ __forceinline__ void stage_param(float (&to)[CB], const float* p, int d0, int D) {
+    for (int c = threadIdx.x; c < CB; c += THREADS) to[c] = p && d0 + c < D ? p[d0 + c] : 0.0f;
+}
+
+template <int K>
+__device__ __forceinline__ void getk(const float* p, float (&v)[K]) {
+    const Pack<float, K> r = *reinterpret_cast<const Pack<float, K>*>(p);
+#pragma unroll
+    for (int i = 0; i < K; i++) v[i] = r.v[i];
+}
+template <int K>
+__device__ __forceinline__ void setk(float* p, const float (&v)[K]) {
+    Pack<float, K> r;
+#pragma unroll
+    for (int i = 0; i < K; i++) r.v[i] = v[i];
+    *reinterpret_cast<Pack<float, K>*>(p) = r;
+}
+
+__device__ __forceinline__ float4 quad(const Pack<float, 4>& p) { return make_float4(p.v[0], p.v[1], p.v[2], p.v[3]); }
+template <typename T>
+__device__ __forceinline__ float4 quad(const Pack<T, 4>& p) {
+    return make_float4(to_f(p.v[0]), to_f(p.v[1]), to_f(p.v[2]), to_f(p.v[3]));
+}
 
 // ---------------------------------------------------------------------------
 // A chunk's own end state, from a zero start (forward: REV = false), or the
@@ -153,87 +291,122 @@ struct Raw {
 // (REV = true; dy, z and C in the place of u, delta and B), and the sum of its
 // dt.  Only chunks > 1 need it: one more exponential for each state.
 template <typename T, int LN, bool REV>
-__global__ void __launch_bounds__(THREADS) chunk_kernel(const Args a) {
-    using F = Cfg<LN>;
-    __shared__ __align__(16) float2 sd[F::TT][F::CB];  // (dt, dt u) or (dt, ds)
-    __shared__ __align__(16) float sm[F::TT][F::NP];   // B or C
+__global__ void __launch_bounds__(THREADS, 3) chunk_kernel(const Args a) {
+    using F = Cfg<T, LN>;
+    constexpr int CB = F::CB, TT = F::TT, CPL = F::CPL;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    typename F::ChunkSmem& sm = *reinterpret_cast<typename F::ChunkSmem*>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
-    const int d0 = blockIdx.x * F::CB, b = blockIdx.y, ck = blockIdx.z + (REV ? 1 : 0);
+    const int d0 = blockIdx.x * CB, b = blockIdx.y, ck = blockIdx.z + (REV ? 1 : 0);
     const int len = length_of(a, b);
     const int tb = ck * a.span, te = tb + a.span < a.L ? tb + a.span : a.L;
     const int end = te < len ? te : len;  // past it nothing changes the state
-    const int lt = tid / F::VPR, lv = tid % F::VPR;  // this thread's row and pack of the loads
-    const int ldd = d0 + 8 * lv;
-    int ch[F::CPL];
-    St A2[F::CPL], h[F::CPL];
-    float sum[F::CPL];
-#pragma unroll
-    for (int j = 0; j < F::CPL; j++) {
-        ch[j] = warp * F::CL * F::CPL + cl * F::CPL + j;
-        const int d = d0 + ch[j];
-        A2[j] = st(d < a.D ? load4(a.A + (int64_t)d * a.N, n0, a.N) : make_float4(0, 0, 0, 0));
-        A2[j] = mul(A2[j], LOG2E);
-        h[j] = st(make_float4(0, 0, 0, 0));
-        sum[j] = 0.0f;
-    }
-    const int tiles = end > tb ? cdiv(end - tb, F::TT) : 0;
-    for (int i = 0; i < tiles; i++) {
-        const int t0 = tb + (REV ? tiles - 1 - i : i) * F::TT;
-        const int t = t0 + lt;
-        const bool in = t < end;
-        {
-            const int valid = in ? a.D - ldd : 0;
-            const Pack<T, 8> pd = load_pack<8>(row_of<T>(a.delta, b, t) + ldd, valid, a.delta.vec);
-            const Pack<T, 8> pu = REV ? load_pack<8>(row_of<T>(a.dy, b, t) + ldd, valid, a.dy.vec)
-                                      : load_pack<8>(row_of<T>(a.u, b, t) + ldd, valid, a.u.vec);
-            Pack<T, 8> pz;
-            if (REV && a.z.p) pz = load_pack<8>(row_of<T>(a.z, b, t) + ldd, valid, a.z.vec);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                float dt = to_f(pd.v[k]);
-                if (a.bias && ldd + k < a.D) dt = __fadd_rn(dt, a.bias[ldd + k]);
-                if (a.softplus) dt = softplus(dt);
-                if (!in || ldd + k >= a.D) dt = 0.0f;
-                float v = to_f(pu.v[k]);
-                if (!REV)
-                    v = __fmul_rn(dt, v);
-                else if (a.z.p) {
-                    const float z = to_f(pz.v[k]);
-                    v = __fmul_rn(v, __fmul_rn(z, sigmoid(z)));
-                }
-                sd[lt][8 * lv + k] = make_float2(dt, in ? v : 0.0f);
-            }
-        }
+    const int tiles = end > tb ? cdiv(end - tb, TT) : 0;
+    const int lt = tid / F::VPR, lv = tid % F::VPR, d = d0 + 8 * lv;
+    const int first = tb + (REV ? (tiles - 1) * TT : 0), rows = REV ? -TT : TT;
+    const Seq &su = REV ? a.dy : a.u, &sB = REV ? a.C : a.B;
+    const int have = a.D - d;
+    const int nq = 4 * (tid % LN), tq = tid / LN;
+    stage_param(sm.bias, a.bias, d0, a.D);
+    __syncthreads();
+    const T *wd = row_of<T>(a.delta, b, first + lt) + d, *wu = row_of<T>(su, b, first + lt) + d;
+    const T *wz = row_of<T>(a.z, b, first + lt) + d, *wB = row_of<T>(sB, b, first + tq) + nq;
+    auto load = [&](int i) {
+        const int t0 = first + i * rows, valid = t0 + lt < end ? have : 0;
+        fetch_pack<8>(&sm.raw[0][8 * tid], wd, a.delta.p, valid, a.delta.vec);
+        fetch_pack<8>(&sm.raw[1][8 * tid], wu, su.p, valid, su.vec);
+        if (REV && a.z.p) fetch_pack<8>(&sm.raw[2][8 * tid], wz, a.z.p, valid, a.z.vec);
 #pragma unroll
         for (int q = 0; q < F::QUADS; q++) {
-            const int e = tid + q * THREADS, tq = t0 + e / LN, nq = 4 * (e % LN);
-            if (e >= F::TT * LN) break;
-            const Seq& s = REV ? a.C : a.B;
-            const Pack<T, 4> p = load_pack<4>(row_of<T>(s, b, tq) + nq, tq < end ? a.N - nq : 0, s.vec);
-            *reinterpret_cast<float4*>(&sm[e / LN][nq]) =
-                make_float4(to_f(p.v[0]), to_f(p.v[1]), to_f(p.v[2]), to_f(p.v[3]));
+            const int r = tq + q * (THREADS / LN);
+            if (r < TT)
+                fetch_pack<4>(&sm.raw_bc[q][4 * tid], wB + q * (THREADS / LN) * sB.sl, sB.p, t0 + r < end ? a.N - nq : 0,
+                              sB.vec);
         }
-        __syncthreads();
-#pragma unroll 4
-        for (int k = 0; k < F::TT; k++) {
-            const int r = REV ? F::TT - 1 - k : k;
-            const St m = st(*reinterpret_cast<const float4*>(&sm[r][n0]));
+        cp_async_commit();
+        wd += rows * a.delta.sl, wu += rows * su.sl, wz += rows * a.z.sl, wB += rows * sB.sl;
+    };
+    auto stage = [&](int i) {
+        cp_async_wait();
+        if (first + i * rows + lt < end) {
+            const Pack<T, 8> pd = slot_pack<8>(&sm.raw[0][8 * tid]), pu = slot_pack<8>(&sm.raw[1][8 * tid]);
+            Pack<T, 8> pz;
+            if (REV && a.z.p) pz = slot_pack<8>(&sm.raw[2][8 * tid]);
+            float dt[8];
+            getk<8>(&sm.bias[8 * lv], dt);
 #pragma unroll
-            for (int j = 0; j < F::CPL; j++) {
-                const float2 dd = sd[r][ch[j]];
-                const St e = exp2s(mul(A2[j], dd.x));
-                h[j] = REV ? mul(e, fma(m, dd.y, h[j])) : fma(e, h[j], mul(m, dd.y));
-                sum[j] = __fadd_rn(sum[j], dd.x);
+            for (int k = 0; k < 8; k++) {
+                dt[k] = __fadd_rn(to_f(pd.v[k]), dt[k]);
+                if (a.softplus) dt[k] = softplus(dt[k]);
+            }
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                v[k] = to_f(pu.v[k]);
+                if (!REV)
+                    v[k] = __fmul_rn(dt[k], v[k]);
+                else if (a.z.p) {
+                    const float z = to_f(pz.v[k]);
+                    v[k] = __fmul_rn(v[k], __fmul_rn(z, sigmoid(z)));
+                }
+            }
+            stage_steps<8>(sm.sd[lt], 8 * lv, lt, dt, v);
+        } else {
+            const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            stage_steps<8>(sm.sd[lt], 8 * lv, lt, zero, zero);
+        }
+#pragma unroll
+        for (int q = 0; q < F::QUADS; q++)
+            if (tq + q * (THREADS / LN) < TT)
+                *reinterpret_cast<float4*>(&sm.B[tq + q * (THREADS / LN)][nq]) = quad(slot_pack<4>(&sm.raw_bc[q][4 * tid]));
+    };
+    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
+    int ch[CPL];
+    St A2[CPL], h[CPL];
+    float sum[CPL];
+#pragma unroll
+    for (int j = 0; j < CPL; j++) {
+        ch[j] = warp * F::CL * CPL + cl * CPL + j;
+        const int c = d0 + ch[j];
+        A2[j] = mul(st(c < a.D ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
+        h[j] = keep_nan(st(make_float4(0, 0, 0, 0)), A2[j]);
+        sum[j] = 0.0f;
+    }
+    if (tiles > 0) load(0);
+    for (int i = 0; i < tiles; i++) {
+        stage(i);
+        __syncthreads();
+        if (i + 1 < tiles) load(i + 1);
+#pragma unroll 2
+        for (int q4 = 0; q4 < TT; q4 += 4) {
+            const int r4 = REV ? TT - 4 - q4 : q4;
+            St m[4];
+            float dt[4][CPL], v[4][CPL];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                m[k] = st(*reinterpret_cast<const float4*>(&sm.B[r4 + k][n0]));
+                staged<CPL>(sm.sd[r4 + k], ch[0], k, dt[k], v[k]);
+            }
+#pragma unroll
+            for (int j = 0; j < CPL; j++) {
+                const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                St e[4];
+                decays<true>(A2[j], dj, e);
+                sum[j] = __fadd_rn(sum[j], __fadd_rn(__fadd_rn(dj[0], dj[1]), __fadd_rn(dj[2], dj[3])));
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int r = REV ? 3 - k : k;
+                    h[j] = REV ? mul(e[r], fma(m[r], dup(v[r][j]), h[j])) : fma(e[r], h[j], mul(m[r], dup(v[r][j])));
+                }
             }
         }
         __syncthreads();
     }
 #pragma unroll
-    for (int j = 0; j < F::CPL; j++) {
-        const int d = d0 + ch[j];
-        if (d >= a.D) continue;
-        const int64_t row = ((int64_t)b * a.chunks + ck) * a.D + d;
+    for (int j = 0; j < CPL; j++) {
+        const int c = d0 + ch[j];
+        if (c >= a.D) continue;
+        const int64_t row = ((int64_t)b * a.chunks + ck) * a.D + c;
         *reinterpret_cast<float4*>(a.cst + row * F::NP + n0) = f4(h[j]);
         if (nl == 0) a.cdt[row] = sum[j];
     }
@@ -266,137 +439,173 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// The scan of one chunk (the whole sequence with chunks = 1).
+// The scan of one chunk (the whole sequence with chunks = 1).  A tile's loads
+// are issued before the tile in front of it is worked on, and wait in
+// registers; its outputs are gated and stored while the next one is staged.
 template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(const Args a) {
-    using F = Cfg<LN>;
+__global__ void __launch_bounds__(THREADS, 3) scan_kernel(const Args a) {
+    using F = Cfg<T, LN>;
     constexpr int NP = F::NP, CB = F::CB, TT = F::TT, CPL = F::CPL;
-    constexpr int YS = CB + 8;  // the 4 positions that a step of the loop stores lie in different banks
-    __shared__ __align__(16) float2 sd[TT][CB];
-    __shared__ __align__(16) float sB[TT][NP], sC[TT][NP];
-    __shared__ __align__(16) float sy[TT][YS];
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    typename F::Smem& sm = *reinterpret_cast<typename F::Smem*>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
     const int d0 = blockIdx.x * CB, b = blockIdx.y, ck = blockIdx.z;
     const int len = length_of(a, b);
     const int tb = ck * a.span, te = tb + a.span < a.L ? tb + a.span : a.L;
     const int end = te < len ? te : len;
-    const int lt = tid / F::VPR, lv = tid % F::VPR, ldd = d0 + 8 * lv;
+    const int tiles = end > tb ? cdiv(end - tb, TT) : 0;  // tiles behind the length only get their zeros
+    const int lt = tid / F::VPR, lv = tid % F::VPR, d = d0 + 8 * lv;
+    T* yp = static_cast<T*>(a.y) + ((int64_t)b * a.L + tb + lt) * a.D + d;
+    const int have = a.D - d;
+    const int nq = 4 * (tid % LN), tq = tid / LN;
+    const T *wu = row_of<T>(a.u, b, tb + lt) + d, *wd = row_of<T>(a.delta, b, tb + lt) + d;
+    const T *wz = row_of<T>(a.z, b, tb + lt) + d;
+    const T *wB = row_of<T>(a.B, b, tb + tq) + nq, *wC = row_of<T>(a.C, b, tb + tq) + nq;
+    stage_param(sm.bias, a.bias, d0, a.D);
+    stage_param(sm.skip, a.Dskip, d0, a.D);
+    __syncthreads();
+    auto load = [&](int i) {
+        const int t0 = tb + i * TT, valid = t0 + lt < end ? have : 0;
+        fetch_pack<8>(&sm.raw[i & 1][0][8 * tid], wu, a.u.p, valid, a.u.vec);
+        fetch_pack<8>(&sm.raw[i & 1][1][8 * tid], wd, a.delta.p, valid, a.delta.vec);
+        if (a.z.p) fetch_pack<8>(&sm.raw[i & 1][2][8 * tid], wz, a.z.p, valid, a.z.vec);
+#pragma unroll
+        for (int q = 0; q < F::QUADS; q++) {
+            const int r = tq + q * (THREADS / LN), valid4 = t0 + r < end ? a.N - nq : 0;
+            if (r >= TT) break;
+            fetch_pack<4>(&sm.raw_bc[0][q][4 * tid], wB + q * (THREADS / LN) * a.B.sl, a.B.p, valid4, a.B.vec);
+            fetch_pack<4>(&sm.raw_bc[1][q][4 * tid], wC + q * (THREADS / LN) * a.C.sl, a.C.p, valid4, a.C.vec);
+        }
+        cp_async_commit();
+        wu += TT * a.u.sl, wd += TT * a.delta.sl, wz += TT * a.z.sl, wB += TT * a.B.sl, wC += TT * a.C.sl;
+    };
+    auto stage = [&](int i) {
+        cp_async_wait();
+        float dt[8], v[8];
+        if (tb + i * TT + lt < end) {
+            const Pack<T, 8> pu = slot_pack<8>(&sm.raw[i & 1][0][8 * tid]), pd = slot_pack<8>(&sm.raw[i & 1][1][8 * tid]);
+            getk<8>(&sm.bias[8 * lv], dt);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                dt[k] = __fadd_rn(to_f(pd.v[k]), dt[k]);
+                if (a.softplus) dt[k] = softplus(dt[k]);
+                v[k] = __fmul_rn(dt[k], to_f(pu.v[k]));
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++) dt[k] = v[k] = 0.0f;
+        }
+        stage_steps<8>(sm.sd[lt], 8 * lv, lt, dt, v);
+#pragma unroll
+        for (int q = 0; q < F::QUADS; q++) {
+            const int r = tq + q * (THREADS / LN);
+            if (r >= TT) break;
+            *reinterpret_cast<float4*>(&sm.B[r][nq]) = quad(slot_pack<4>(&sm.raw_bc[0][q][4 * tid]));
+            *reinterpret_cast<float4*>(&sm.C[r][nq]) = quad(slot_pack<4>(&sm.raw_bc[1][q][4 * tid]));
+        }
+    };
+    auto finish = [&](int i) {
+        const int t = tb + i * TT + lt;
+        if (t < te && d < a.D) {
+            float o[8];
+            getk<8>(&sm.y[lt][8 * lv], o);
+            if (a.Dskip) {
+                const Pack<T, 8> eu = slot_pack<8>(&sm.raw[i & 1][0][8 * tid]);
+                float skip[8];
+                getk<8>(&sm.skip[8 * lv], skip);
+#pragma unroll
+                for (int k = 0; k < 8; k++) o[k] = __fmaf_rn(skip[k], to_f(eu.v[k]), o[k]);
+            }
+            if (a.z.p) {
+                const Pack<T, 8> ez = slot_pack<8>(&sm.raw[i & 1][2][8 * tid]);
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float z = to_f(ez.v[k]);
+                    o[k] = __fmul_rn(o[k], __fmul_rn(z, sigmoid(z)));
+                }
+            }
+            if (t >= end) {
+#pragma unroll
+                for (int k = 0; k < 8; k++) o[k] = 0.0f;
+            }
+            store_pack<8>(yp, o, a.D - d, a.ovec);
+        }
+        yp += (int64_t)TT * a.D;
+    };
+    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
     int ch[CPL];
     St A2[CPL], h[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
         ch[j] = warp * F::CL * CPL + cl * CPL + j;
-        const int d = d0 + ch[j];
-        const bool in = d < a.D;
-        A2[j] = mul(st(in ? load4(a.A + (int64_t)d * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
+        const int c = d0 + ch[j];
+        const bool in = c < a.D;
+        A2[j] = mul(st(in ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
         float4 v = make_float4(0, 0, 0, 0);
         if (in && a.chunks > 1)
-            v = *reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + d) * NP + n0);
+            v = *reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + c) * NP + n0);
         else if (in && a.h0)
-            v = load4(a.h0 + ((int64_t)b * a.D + d) * a.N, n0, a.N);
-        h[j] = st(v);
+            v = load4(a.h0 + ((int64_t)b * a.D + c) * a.N, n0, a.N);
+        h[j] = tiles > 0 ? keep_nan(st(v), A2[j]) : st(v);
     }
-    float bias[8], skip[8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        bias[k] = a.bias && ldd + k < a.D ? a.bias[ldd + k] : 0.0f;
-        skip[k] = a.Dskip && ldd + k < a.D ? a.Dskip[ldd + k] : 0.0f;
-    }
-    const int tiles = te > tb ? cdiv(te - tb, TT) : 0;
-    Raw<T, F::QUADS> raw;
-    auto load = [&](int t0) {
-        const int t = t0 + lt;
-        const int valid = t < end ? a.D - ldd : 0;
-        raw.u = load_pack<8>(row_of<T>(a.u, b, t) + ldd, valid, a.u.vec);
-        raw.d = load_pack<8>(row_of<T>(a.delta, b, t) + ldd, valid, a.delta.vec);
-        if (a.z.p) raw.z = load_pack<8>(row_of<T>(a.z, b, t) + ldd, valid, a.z.vec);
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++) {
-            const int e = tid + q * THREADS, tq = t0 + e / LN, nq = 4 * (e % LN);
-            const int have = tq < end && e < TT * LN ? a.N - nq : 0;
-            raw.B[q] = load_pack<4>(row_of<T>(a.B, b, tq) + nq, have, a.B.vec);
-            raw.C[q] = load_pack<4>(row_of<T>(a.C, b, tq) + nq, have, a.C.vec);
-        }
-    };
-    load(tb);
+    float* keep = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK) * a.D + d0 + ch[0]) * NP + n0;
+    if (tiles > 0) load(0);
     for (int i = 0; i < tiles; i++) {
-        const int t0 = tb + i * TT, t = t0 + lt;
-        const bool in = t < end;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            float dt = __fadd_rn(to_f(raw.d.v[k]), bias[k]);
-            if (a.softplus) dt = softplus(dt);
-            if (!in || ldd + k >= a.D) dt = 0.0f;
-            sd[lt][8 * lv + k] = make_float2(dt, __fmul_rn(dt, to_f(raw.u.v[k])));
-        }
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++) {
-            const int e = tid + q * THREADS;
-            if (e >= TT * LN) break;
-            float4 v = make_float4(to_f(raw.B[q].v[0]), to_f(raw.B[q].v[1]), to_f(raw.B[q].v[2]), to_f(raw.B[q].v[3]));
-            *reinterpret_cast<float4*>(&sB[e / LN][4 * (e % LN)]) = v;
-            v = make_float4(to_f(raw.C[q].v[0]), to_f(raw.C[q].v[1]), to_f(raw.C[q].v[2]), to_f(raw.C[q].v[3]));
-            *reinterpret_cast<float4*>(&sC[e / LN][4 * (e % LN)]) = v;
-        }
+        const int t0 = tb + i * TT;
+        if (i > 0) finish(i - 1);
+        stage(i);
         __syncthreads();
-        const Pack<T, 8> ru = raw.u, rz = raw.z;
-        if (i + 1 < tiles) load(t0 + TT);
-        if (t0 < end) {
+        if (i + 1 < tiles) load(i + 1);
 #pragma unroll 1
-            for (int r4 = 0; r4 < TT; r4 += 4) {
-                if (a.ckpt && (t0 + r4) % CK == 0 && t0 + r4 < a.L) {
+        for (int r16 = 0; r16 < TT; r16 += CK) {
+            if (a.ckpt && t0 + r16 < a.L) {
 #pragma unroll
-                    for (int j = 0; j < CPL; j++)
-                        if (d0 + ch[j] < a.D)
-                            *reinterpret_cast<float4*>(
-                                a.ckpt + (((int64_t)b * cdiv(a.L, CK) + (t0 + r4) / CK) * a.D + d0 + ch[j]) * NP + n0) =
-                                f4(h[j]);
-                }
-                float y[CPL][4];
+                for (int j = 0; j < CPL; j++)
+                    if (d0 + ch[j] < a.D) *reinterpret_cast<float4*>(keep + j * NP) = f4(h[j]);
+                keep += (int64_t)a.D * NP;
+            }
+            // 16 positions without a store in between, which would hold back the loads behind it
+            constexpr int KEEP = LN == 2 ? 2 : 1;
+            float out[CPL][4][KEEP];
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int r4 = r16 + 4 * g;
+                St Bv[4], Cv[4];
+                float dt[4][CPL], v[4][CPL];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const St Bv = st(*reinterpret_cast<const float4*>(&sB[r4 + k][n0]));
-                    const St Cv = st(*reinterpret_cast<const float4*>(&sC[r4 + k][n0]));
-#pragma unroll
-                    for (int j = 0; j < CPL; j++) {
-                        const float2 dd = sd[r4 + k][ch[j]];
-                        h[j] = fma(exp2s(mul(A2[j], dd.x)), h[j], mul(Bv, dd.y));
-                        y[j][k] = dot(h[j], Cv);
-                    }
+                    Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[r4 + k][n0]));
+                    Cv[k] = st(*reinterpret_cast<const float4*>(&sm.C[r4 + k][n0]));
+                    staged<CPL>(sm.sd[r4 + k], ch[0], k, dt[k], v[k]);
                 }
-                // sums over the channel's lanes: of 4 positions, each lane keeps one (LN = 2: two)
 #pragma unroll
                 for (int j = 0; j < CPL; j++) {
-                    if constexpr (LN == 2) {
-                        halve<4>(y[j], 1);
-                        sy[r4 + 2 * nl][ch[j]] = y[j][0];
-                        sy[r4 + 2 * nl + 1][ch[j]] = y[j][1];
-                    } else {
-                        halve<4>(y[j], 2);
-                        halve<2>(y[j], 1);
+                    const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                    St e[4];
+                    float y[4];
+                    decays<true>(A2[j], dj, e);
 #pragma unroll
-                        for (int m = 4; m < LN; m *= 2)
-                            y[j][0] = __fadd_rn(y[j][0], __shfl_xor_sync(0xffffffffu, y[j][0], m));
-                        if (nl < 4) sy[r4 + nl][ch[j]] = y[j][0];
+                    for (int k = 0; k < 4; k++) {
+                        h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
+                        y[k] = dot(h[j], Cv[k]);
                     }
+                    over_states<LN>(y);
+#pragma unroll
+                    for (int m = 0; m < KEEP; m++) out[j][g][m] = y[m];
                 }
             }
+#pragma unroll
+            for (int j = 0; j < CPL; j++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) store_positions<LN, F::YS>(&sm.y[r16 + 4 * g][ch[j]], out[j][g], nl);
         }
         __syncthreads();
-        if (t < te && ldd < a.D) {
-            float o[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                float v = __fmaf_rn(skip[k], to_f(ru.v[k]), sy[lt][8 * lv + k]);
-                if (a.z.p) {
-                    const float z = to_f(rz.v[k]);
-                    v = __fmul_rn(v, __fmul_rn(z, sigmoid(z)));
-                }
-                o[k] = in ? v : 0.0f;
-            }
-            store_pack<8>(static_cast<T*>(a.y) + ((int64_t)b * a.L + t) * a.D + ldd, o, a.D - ldd, a.ovec);
-        }
+    }
+    if (tiles > 0) finish(tiles - 1);
+    if (d < a.D) {
+        const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        for (int t = tb + tiles * TT + lt; t < te; t += TT, yp += (int64_t)TT * a.D)
+            store_pack<8>(yp, zero, a.D - d, a.ovec);
     }
     if (a.hT && ck == a.chunks - 1) {
 #pragma unroll
@@ -407,267 +616,365 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(const Args a) {
 
 // ---------------------------------------------------------------------------
 // Backward of one chunk.  Tiles of 16 positions, from the last to the first.
-// From the state that the forward pass kept at a tile's start, each half of 8
-// positions is run again (the first half twice: once on the way to the
-// second), with its decays and states held in registers, and then walked
-// backwards.  A lane goes through its CPL channels one after the other, so
-// that the terms of dB and dC add up over them in registers before they are
-// added across the lanes, and once a tile across the warps; sum_bc_kernel adds
-// the channel blocks.
-template <int LN>
+// From the state that the forward pass kept at a tile's start, 12 positions
+// are run to find the states at positions 4, 8 and 12; then each block of 4,
+// from the last, is run again with its decays and states held in registers,
+// and walked backwards.  dB and dC are added over a lane's channels (where it
+// has more than one), across the warp's channel lanes, and once a tile across
+// the warps; sum_bc_kernel adds the channel blocks.
+//
+// Across the channel lanes, a lane sends the half of its states that it does
+// not keep.  Lanes hold their 4 states in an order of their own (state
+// i ^ perm), so that what is kept always lies in the first registers and
+// nothing has to be selected; B and C are staged once for each order.
+template <typename T, int LN>
 struct BCfg {
     static constexpr int NP = 4 * LN, CL = 32 / LN;
-    static constexpr int CB = 64, CPL = CB / (4 * CL);  // channels a CTA, a lane
-    static constexpr int TT = CK, VPR = CB / 8;
+    static constexpr int CPL = LN == 2 ? 1 : LN == 16 ? 4 : 2, CB = 4 * CL * CPL;  // channels a lane, a CTA
+    static constexpr int TT = CK, E = TT * CB / THREADS, VPR = CB / E;  // positions a tile; a thread stages E channels
     static constexpr int QUADS = (TT * LN + THREADS - 1) / THREADS;
-    static constexpr int OS = CB + 8;
+    static constexpr int PERMS = CL < 4 ? CL : 4;  // orders of the states
+    static constexpr int OS = CB + 8, BS = 2 * NP + 8;
     struct Smem {
-        float2 sd[TT][CB];             // dt, dt u
-        float ds[TT][CB];              // dy z sigmoid(z)
-        float B[TT][NP], C[TT][NP];
-        float S[3][TT][OS];            // sum_n g B, sum_n w A log2(e), sum_n C h
-        float4 own[4][CPL][3][32];     // by lane: A log2(e), the gradient's carry, dA
-        float bc[4][TT][2 * NP];       // a warp's dB | dC
-        float acc[2][TT][CB];          // dD and dbias, by position of the tile
+        float4 sd[TT][CB / 2];                   // (dt, dt u) of two channels
+        float ds[TT][CB];                        // dy z sigmoid(z)
+        float B[PERMS][TT][NP], C[PERMS][TT][NP];
+        float S[3][TT][OS];                      // sum_n g B, sum_n w A log2(e), sum_n C h
+        float4 mid[4][CPL][3][32];               // by lane: the states at positions 4, 8 and 12
+        float bc[4][TT][BS];                     // a warp's dB | dC
+        float bias[CB], skip[CB];
+        float4 kept[CPL][THREADS];               // by thread: the kept states of the next tile
+        alignas(16) T raw[4][THREADS * E];       // by thread: u, delta, dy and z as they come
+        alignas(16) T raw_bc[2][QUADS][THREADS * 4];
     };
 };
 
+__device__ __forceinline__ float2 swap(float2 v) { return make_float2(v.y, v.x); }
+template <int PERMS>
+__device__ __forceinline__ St permute(St s, int p) {
+    if (p & 1) s.a = swap(s.a), s.b = swap(s.b);
+    if (PERMS == 4 && (p & 2)) {
+        const float2 t = s.a;
+        s.a = s.b, s.b = t;
+    }
+    return s;
+}
+__device__ __forceinline__ float take(float keep, float send, int mask) {
+    return __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, send, mask));
+}
+
 template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS) bwd_kernel(const Args a) {
-    using F = BCfg<LN>;
-    constexpr int NP = F::NP, CB = F::CB, CPL = F::CPL, TT = F::TT, CL = F::CL;
+__global__ void __launch_bounds__(THREADS, 3) bwd_kernel(const Args a) {
+    using F = BCfg<T, LN>;
+    constexpr int NP = F::NP, CB = F::CB, CPL = F::CPL, TT = F::TT, CL = F::CL, PERMS = F::PERMS, E = F::E;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     typename F::Smem& sm = *reinterpret_cast<typename F::Smem*>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
+    const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl, perm = cl & (PERMS - 1);
     const int d0 = blockIdx.x * CB, b = blockIdx.y, ck = blockIdx.z;
     const int len = length_of(a, b);
     const int tb = ck * a.span, te = tb + a.span < a.L ? tb + a.span : a.L;
     const int end = te < len ? te : len;
-    const int lt = tid / F::VPR, lv = tid % F::VPR, ldd = d0 + 8 * lv;
-    const int nck = cdiv(a.L, CK);
-    for (int j = 0; j < CPL; j++) {
-        const int d = d0 + warp * CL * CPL + cl * CPL + j;
-        const bool in = d < a.D;
-        float4 A = make_float4(0, 0, 0, 0), g = A;
-        if (in) {
-            A = f4(mul(st(load4(a.A + (int64_t)d * a.N, n0, a.N)), LOG2E));
-            if (a.chunks > 1)
-                g = *reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + d) * NP + n0);
-            else if (a.dhT)
-                g = load4(a.dhT + ((int64_t)b * a.D + d) * a.N, n0, a.N);
-        }
-        sm.own[warp][j][0][lane] = A;
-        sm.own[warp][j][1][lane] = g;
-        sm.own[warp][j][2][lane] = make_float4(0, 0, 0, 0);
-    }
-    float bias[8], skip[8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        bias[k] = a.bias && ldd + k < a.D ? a.bias[ldd + k] : 0.0f;
-        skip[k] = a.Dskip && ldd + k < a.D ? a.Dskip[ldd + k] : 0.0f;
-        sm.acc[0][lt][8 * lv + k] = 0.0f;
-        sm.acc[1][lt][8 * lv + k] = 0.0f;
-    }
     const int tiles = te > tb ? cdiv(te - tb, TT) : 0;
-    for (int i = tiles - 1; i >= 0; i--) {
+    const int active = end > tb ? cdiv(end - tb, TT) : 0;  // tiles behind the length change nothing
+    const int lt = tid / F::VPR, lc = E * (tid % F::VPR), d = d0 + lc, have = a.D - d;
+    const int c0 = warp * CL * CPL + cl * CPL;  // this lane's first channel in the CTA
+
+    St A2[CPL], gc[CPL], dA[CPL];
+#pragma unroll
+    for (int j = 0; j < CPL; j++) {
+        const int c = d0 + c0 + j;
+        A2[j] = gc[j] = dA[j] = st(make_float4(0, 0, 0, 0));
+        if (c < a.D) {
+            A2[j] = permute<PERMS>(mul(st(load4(a.A + (int64_t)c * a.N, n0, a.N)), LOG2E), perm);
+            if (a.chunks > 1)
+                gc[j] = st(*reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + c) * NP + n0));
+            else if (a.dhT)
+                gc[j] = st(load4(a.dhT + ((int64_t)b * a.D + c) * a.N, n0, a.N));
+            gc[j] = permute<PERMS>(gc[j], perm);
+        }
+    }
+    constexpr int AK = E / 4;  // dD and dbias of a quarter of this thread's channels, over 4 positions of each tile
+    float accD[AK], accb[AK];
+#pragma unroll
+    for (int k = 0; k < AK; k++) accD[k] = accb[k] = 0.0f;
+
+    // this thread's packs of 4 of a tile's dB | dC
+    constexpr int PACKS = TT * 2 * NP / 4, PER = (PACKS + THREADS - 1) / THREADS, ROW4 = 2 * NP / 4;
+    auto put_bc = [&](int t0, bool zero) {
+        float* p = a.part_bc + (((int64_t)blockIdx.x * a.batch + b) * a.L + t0) * (2 * NP) + 4 * tid;
+#pragma unroll
+        for (int m = 0; m < PER; m++) {
+            const int e = tid + m * THREADS, r = e / ROW4, k = 4 * (e % ROW4);
+            if (e >= PACKS || t0 + r >= te) break;
+            float4 x = make_float4(0, 0, 0, 0);
+            if (!zero && t0 + r < end) {
+                const float4 v0 = *reinterpret_cast<const float4*>(&sm.bc[0][r][k]);
+                const float4 v1 = *reinterpret_cast<const float4*>(&sm.bc[1][r][k]);
+                const float4 v2 = *reinterpret_cast<const float4*>(&sm.bc[2][r][k]);
+                const float4 v3 = *reinterpret_cast<const float4*>(&sm.bc[3][r][k]);
+                x.x = __fadd_rn(__fadd_rn(v0.x, v1.x), __fadd_rn(v2.x, v3.x));
+                x.y = __fadd_rn(__fadd_rn(v0.y, v1.y), __fadd_rn(v2.y, v3.y));
+                x.z = __fadd_rn(__fadd_rn(v0.z, v1.z), __fadd_rn(v2.z, v3.z));
+                x.w = __fadd_rn(__fadd_rn(v0.w, v1.w), __fadd_rn(v2.w, v3.w));
+            }
+            *reinterpret_cast<float4*>(p + m * (4 * THREADS)) = x;
+        }
+    };
+    auto put = [&](int t, const float (&du)[E], const float (&dd)[E], const float (&dz)[E]) {
+        const int64_t o = ((int64_t)b * a.L + t) * a.D + d;
+        store_pack<E>(static_cast<T*>(a.du) + o, du, have, a.ovec);
+        store_pack<E>(static_cast<T*>(a.ddelta) + o, dd, have, a.ovec);
+        if (a.z.p) store_pack<E>(static_cast<T*>(a.dz) + o, dz, have, a.ovec);
+    };
+    for (int i = active; i < tiles; i++) {
+        float zero[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) zero[k] = 0.0f;
+        if (tb + i * TT + lt < te && have > 0) put(tb + i * TT + lt, zero, zero, zero);
+        put_bc(tb + i * TT, true);
+    }
+
+    const int nq = 4 * (tid % LN), tq = tid / LN;
+    stage_param(sm.bias, a.bias, d0, a.D);
+    stage_param(sm.skip, a.Dskip, d0, a.D);
+    __syncthreads();
+    const int first = tb + (active - 1) * TT;
+    const T *wu = row_of<T>(a.u, b, first + lt) + d, *wd = row_of<T>(a.delta, b, first + lt) + d;
+    const T *wg = row_of<T>(a.dy, b, first + lt) + d, *wz = row_of<T>(a.z, b, first + lt) + d;
+    const T *wB = row_of<T>(a.B, b, first + tq) + nq, *wC = row_of<T>(a.C, b, first + tq) + nq;
+    const float* kp = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK + active - 1) * a.D + d0 + c0) * NP + n0;
+    // a tile's inputs, into the slots that the tile behind it has left
+    auto load = [&](int i) {
+        const int t0 = tb + i * TT, valid = t0 + lt < end ? have : 0;
+        fetch_pack<E>(&sm.raw[0][E * tid], wu, a.u.p, valid, a.u.vec);
+        fetch_pack<E>(&sm.raw[1][E * tid], wd, a.delta.p, valid, a.delta.vec);
+        fetch_pack<E>(&sm.raw[2][E * tid], wg, a.dy.p, valid, a.dy.vec);
+        if (a.z.p) fetch_pack<E>(&sm.raw[3][E * tid], wz, a.z.p, valid, a.z.vec);
+#pragma unroll
+        for (int q = 0; q < F::QUADS; q++) {
+            const int r = tq + q * (THREADS / LN), valid4 = t0 + r < end ? a.N - nq : 0;
+            if (r >= TT) break;
+            fetch_pack<4>(&sm.raw_bc[0][q][4 * tid], wB + q * (THREADS / LN) * a.B.sl, a.B.p, valid4, a.B.vec);
+            fetch_pack<4>(&sm.raw_bc[1][q][4 * tid], wC + q * (THREADS / LN) * a.C.sl, a.C.p, valid4, a.C.vec);
+        }
+#pragma unroll
+        for (int j = 0; j < CPL; j++) {
+            const bool exists = d0 + c0 + j < a.D;
+            cp_async<16>(&sm.kept[j][tid], exists ? kp + j * NP : a.ckpt, exists ? 16 : 0);
+        }
+        cp_async_commit();
+        wu -= TT * a.u.sl, wd -= TT * a.delta.sl, wg -= TT * a.dy.sl, wz -= TT * a.z.sl;
+        wB -= TT * a.B.sl, wC -= TT * a.C.sl, kp -= (int64_t)a.D * NP;
+    };
+    if (active > 0) load(active - 1);
+    for (int i = active - 1; i >= 0; i--) {
         const int t0 = tb + i * TT, t = t0 + lt;
         const bool in = t < end;
-        const int valid = in ? a.D - ldd : 0;
-        float u[8], sg[8], dyz[8], dsk[8];  // u; d dt / d delta; dy (z sigmoid(z))'; ds
+        cp_async_wait();
         {
-            const Pack<T, 8> pu = load_pack<8>(row_of<T>(a.u, b, t) + ldd, valid, a.u.vec);
-            const Pack<T, 8> pd = load_pack<8>(row_of<T>(a.delta, b, t) + ldd, valid, a.delta.vec);
-            const Pack<T, 8> pg = load_pack<8>(row_of<T>(a.dy, b, t) + ldd, valid, a.dy.vec);
-            Pack<T, 8> pz;
-            if (a.z.p) pz = load_pack<8>(row_of<T>(a.z, b, t) + ldd, valid, a.z.vec);
+            const Pack<T, E> eu = slot_pack<E>(&sm.raw[0][E * tid]), ed = slot_pack<E>(&sm.raw[1][E * tid]);
+            const Pack<T, E> eg = slot_pack<E>(&sm.raw[2][E * tid]), ez = slot_pack<E>(&sm.raw[3][E * tid]);
+            float dt[E], v[E], g[E];
+            getk<E>(&sm.bias[lc], dt);
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                u[k] = to_f(pu.v[k]);
-                const float x = __fadd_rn(to_f(pd.v[k]), bias[k]);
-                float dt = x;
-                sg[k] = 1.0f;
-                if (a.softplus) dt = softplus(x), sg[k] = sigmoid(x);
-                if (!in || ldd + k >= a.D) dt = 0.0f;
-                sm.sd[lt][8 * lv + k] = make_float2(dt, __fmul_rn(dt, u[k]));
-                const float dy = to_f(pg.v[k]);
-                dsk[k] = dy, dyz[k] = 0.0f;
+            for (int k = 0; k < E; k++) {
+                dt[k] = __fadd_rn(to_f(ed.v[k]), dt[k]);
+                if (a.softplus) dt[k] = softplus(dt[k]);
+                if (!in) dt[k] = 0.0f;
+                v[k] = __fmul_rn(dt[k], to_f(eu.v[k]));
+                g[k] = to_f(eg.v[k]);
                 if (a.z.p) {
-                    const float z = to_f(pz.v[k]), s = sigmoid(z);
-                    dsk[k] = __fmul_rn(dy, __fmul_rn(z, s));
-                    dyz[k] = __fmul_rn(dy, __fmul_rn(s, __fmaf_rn(z, __fsub_rn(1.0f, s), 1.0f)));
+                    const float z = to_f(ez.v[k]);
+                    g[k] = __fmul_rn(g[k], __fmul_rn(z, sigmoid(z)));
                 }
-                sm.ds[lt][8 * lv + k] = dsk[k];
             }
+            stage_steps<E>(sm.sd[lt], lc, lt, dt, v);
+            setk<E>(&sm.ds[lt][lc], g);
         }
 #pragma unroll
         for (int q = 0; q < F::QUADS; q++) {
-            const int e = tid + q * THREADS, tq = t0 + e / LN, nq = 4 * (e % LN);
-            if (e < TT * LN) {
-                const int have = tq < end ? a.N - nq : 0;
-                const Pack<T, 4> pB = load_pack<4>(row_of<T>(a.B, b, tq) + nq, have, a.B.vec);
-                const Pack<T, 4> pC = load_pack<4>(row_of<T>(a.C, b, tq) + nq, have, a.C.vec);
-                *reinterpret_cast<float4*>(&sm.B[e / LN][nq]) =
-                    make_float4(to_f(pB.v[0]), to_f(pB.v[1]), to_f(pB.v[2]), to_f(pB.v[3]));
-                *reinterpret_cast<float4*>(&sm.C[e / LN][nq]) =
-                    make_float4(to_f(pC.v[0]), to_f(pC.v[1]), to_f(pC.v[2]), to_f(pC.v[3]));
+            const int r = tq + q * (THREADS / LN);
+            if (r >= TT) break;
+            const St sB = st(quad(slot_pack<4>(&sm.raw_bc[0][q][4 * tid])));
+            const St sC = st(quad(slot_pack<4>(&sm.raw_bc[1][q][4 * tid])));
+#pragma unroll
+            for (int p = 0; p < PERMS; p++) {
+                *reinterpret_cast<float4*>(&sm.B[p][r][nq]) = f4(permute<PERMS>(sB, p));
+                *reinterpret_cast<float4*>(&sm.C[p][r][nq]) = f4(permute<PERMS>(sC, p));
             }
         }
         __syncthreads();
-        if (t0 < end) {  // a tile behind the length changes nothing
-#pragma unroll 1
-            for (int half = 1; half >= 0; half--) {
-                float v[8][8];  // by position: 4 states' dB and dC
+        {
+            St h[CPL], mid[3][CPL];
 #pragma unroll
-                for (int k = 0; k < 8; k++)
+            for (int j = 0; j < CPL; j++) h[j] = permute<PERMS>(st(sm.kept[j][tid]), perm);
 #pragma unroll
-                    for (int m = 0; m < 8; m++) v[k][m] = 0.0f;
-#pragma unroll 1
+            for (int q = 0; q < 3; q++) {
+                St Bv[4];
+                float dt[4][CPL], v[4][CPL];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[perm][4 * q + k][n0]));
+                    staged<CPL>(sm.sd[4 * q + k], c0, k, dt[k], v[k]);
+                }
+#pragma unroll
                 for (int j = 0; j < CPL; j++) {
-                    const int c = warp * CL * CPL + cl * CPL + j;
-                    float4* mine = &sm.own[warp][j][0][lane];
-                    const St A2 = st(mine[0]);
-                    St h0 = st(make_float4(0, 0, 0, 0));
-                    if (d0 + c < a.D)
-                        h0 = st(*reinterpret_cast<const float4*>(
-                            a.ckpt + (((int64_t)b * nck + t0 / CK) * a.D + d0 + c) * NP + n0));
-                    if (half == 1) {
+                    const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                    St e[4];
+                    decays<false>(A2[j], dj, e);
 #pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const float2 dd = sm.sd[k][c];
-                            const St Bv = st(*reinterpret_cast<const float4*>(&sm.B[k][n0]));
-                            h0 = fma(exp2s(mul(A2, dd.x)), h0, mul(Bv, dd.y));
-                        }
-                    }
-                    St e[8], h[8];
-                    {
-                        St x = h0;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const float2 dd = sm.sd[8 * half + k][c];
-                            const St Bv = st(*reinterpret_cast<const float4*>(&sm.B[8 * half + k][n0]));
-                            e[k] = exp2s(mul(A2, dd.x));
-                            x = fma(e[k], x, mul(Bv, dd.y));
-                            h[k] = x;
-                        }
-                    }
-                    St gc = st(mine[32]), dA = st(mine[64]);
-                    float s[3][8];
-#pragma unroll
-                    for (int k = 7; k >= 0; k--) {
-                        const int r = 8 * half + k;
-                        const float2 dd = sm.sd[r][c];
-                        const float ds = sm.ds[r][c];
-                        const St Bv = st(*reinterpret_cast<const float4*>(&sm.B[r][n0]));
-                        const St Cv = st(*reinterpret_cast<const float4*>(&sm.C[r][n0]));
-                        const St g = fma(Cv, ds, gc);
-                        const float4 fg = f4(g), fh = f4(h[k]);
-                        v[k][0] = __fmaf_rn(fg.x, dd.y, v[k][0]);
-                        v[k][1] = __fmaf_rn(fg.y, dd.y, v[k][1]);
-                        v[k][2] = __fmaf_rn(fg.z, dd.y, v[k][2]);
-                        v[k][3] = __fmaf_rn(fg.w, dd.y, v[k][3]);
-                        v[k][4] = __fmaf_rn(fh.x, ds, v[k][4]);
-                        v[k][5] = __fmaf_rn(fh.y, ds, v[k][5]);
-                        v[k][6] = __fmaf_rn(fh.z, ds, v[k][6]);
-                        v[k][7] = __fmaf_rn(fh.w, ds, v[k][7]);
-                        s[0][k] = dot(g, Bv);
-                        gc = mul(e[k], g);
-                        const St w = mul(gc, k ? h[k ? k - 1 : 0] : h0);
-                        s[1][k] = dot(w, A2);
-                        s[2][k] = dot(h[k], Cv);
-                        dA = fma(w, dd.x, dA);
-                    }
-                    mine[32] = f4(gc);
-                    mine[64] = f4(dA);
-                    // over the channel's lanes; each keeps 8 / LN of the 8 positions
-#pragma unroll
-                    for (int m = 0; m < 3; m++) {
-                        constexpr int KEEP = LN >= 8 ? 1 : 8 / LN;
-                        int pos = 0;
-                        if constexpr (LN >= 8) {
-                            halve<8>(s[m], 4), halve<4>(s[m], 2), halve<2>(s[m], 1);
-                            pos = nl & 7;
-                            if constexpr (LN == 16)
-                                s[m][0] = __fadd_rn(s[m][0], __shfl_xor_sync(0xffffffffu, s[m][0], 8));
-                        } else if constexpr (LN == 4) {
-                            halve<8>(s[m], 2), halve<4>(s[m], 1);
-                            pos = 2 * nl;
-                        } else {
-                            halve<8>(s[m], 1);
-                            pos = 4 * nl;
-                        }
-                        if (LN < 16 || nl < 8) {
-#pragma unroll
-                            for (int k = 0; k < KEEP; k++) sm.S[m][8 * half + pos + k][c] = s[m][k];
-                        }
-                    }
+                    for (int k = 0; k < 4; k++) h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
+                    mid[q][j] = h[j];
                 }
-                // over the warp's channel lanes: first by position, then dB from dC
-                float* f = &v[0][0];
-                int pos = 0, cnt = 8;
-                if constexpr (CL >= 2) halve<64>(f, LN), pos = (cl & 1) * 4, cnt = 4;
-                if constexpr (CL >= 4) halve<32>(f, 2 * LN), pos += ((cl >> 1) & 1) * 2, cnt = 2;
-                if constexpr (CL >= 8) halve<16>(f, 4 * LN), pos += (cl >> 2) & 1, cnt = 1;
-                if constexpr (CL == 16) {
-                    halve<8>(f, 8 * LN);
-                    *reinterpret_cast<float4*>(&sm.bc[warp][8 * half + pos][((cl >> 3) & 1) * NP + n0]) =
-                        make_float4(f[0], f[1], f[2], f[3]);
-                } else {
+            }
 #pragma unroll
-                    for (int k = 0; k < (CL >= 8 ? 1 : 8 / CL); k++) {
-                        float* row = sm.bc[warp][8 * half + pos + k];
-                        *reinterpret_cast<float4*>(row + n0) = make_float4(f[8 * k], f[8 * k + 1], f[8 * k + 2], f[8 * k + 3]);
-                        *reinterpret_cast<float4*>(row + NP + n0) =
-                            make_float4(f[8 * k + 4], f[8 * k + 5], f[8 * k + 6], f[8 * k + 7]);
-                    }
+            for (int q = 0; q < 3; q++)
+#pragma unroll
+                for (int j = 0; j < CPL; j++) sm.mid[warp][j][q][lane] = f4(mid[q][j]);
+        }
+#pragma unroll 1
+        for (int q = 3; q >= 0; q--) {
+            St Bv[4], Cv[4], vB[4], vC[4];
+            float dt[4][CPL], v[4][CPL], ds[4][CPL];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[perm][4 * q + k][n0]));
+                Cv[k] = st(*reinterpret_cast<const float4*>(&sm.C[perm][4 * q + k][n0]));
+                staged<CPL>(sm.sd[4 * q + k], c0, k, dt[k], v[k]);
+                getk<CPL>(&sm.ds[4 * q + k][c0], ds[k]);
+            }
+            float out[3][CPL][4];
+#pragma unroll
+            for (int j = 0; j < CPL; j++) {
+                const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                const St h0 = q ? st(sm.mid[warp][j][q ? q - 1 : 0][lane]) : permute<PERMS>(st(sm.kept[j][tid]), perm);
+                St e[4], h[4];
+                decays<false>(A2[j], dj, e);
+#pragma unroll
+                for (int k = 0; k < 4; k++) h[k] = fma(e[k], k ? h[k ? k - 1 : 0] : h0, mul(Bv[k], dup(v[k][j])));
+#pragma unroll
+                for (int k = 3; k >= 0; k--) {
+                    const float2 dsk = dup(ds[k][j]);
+                    const St g = fma(Cv[k], dsk, gc[j]);
+                    vB[k] = j ? fma(g, dup(v[k][j]), vB[k]) : mul(g, dup(v[k][j]));
+                    vC[k] = j ? fma(h[k], dsk, vC[k]) : mul(h[k], dsk);
+                    out[0][j][k] = dot(g, Bv[k]);
+                    gc[j] = mul(e[k], g);
+                    const St w = mul(gc[j], k ? h[k ? k - 1 : 0] : h0);
+                    out[1][j][k] = dot(w, A2[j]);
+                    out[2][j][k] = dot(h[k], Cv[k]);
+                    dA[j] = fma(w, dup(dj[k]), dA[j]);
+                }
+#pragma unroll
+                for (int m = 0; m < 3; m++) over_states<LN>(out[m][j]);
+            }
+            // over the warp's channel lanes
+            float f[16];
+            int pos = 0;
+            if constexpr (PERMS == 4) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    f[2 * k] = take(take(vB[k].a.x, vB[k].b.x, 2 * LN), take(vB[k].a.y, vB[k].b.y, 2 * LN), LN);
+                    f[2 * k + 1] = take(take(vC[k].a.x, vC[k].b.x, 2 * LN), take(vC[k].a.y, vC[k].b.y, 2 * LN), LN);
+                }
+                if constexpr (CL >= 8) halve<8>(f, 4 * LN), pos = ((cl >> 2) & 1) * 2;
+                if constexpr (CL == 16) halve<4>(f, 8 * LN), pos += (cl >> 3) & 1;
+            } else {  // two channel lanes: each keeps two states
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    f[4 * k] = take(vB[k].a.x, vB[k].a.y, LN), f[4 * k + 1] = take(vB[k].b.x, vB[k].b.y, LN);
+                    f[4 * k + 2] = take(vC[k].a.x, vC[k].a.y, LN), f[4 * k + 3] = take(vC[k].b.x, vC[k].b.y, LN);
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 3; m++)
+#pragma unroll
+                for (int j = 0; j < CPL; j++) store_positions<LN, F::OS>(&sm.S[m][4 * q][c0 + j], out[m][j], nl);
+            if constexpr (PERMS == 4) {
+#pragma unroll
+                for (int k = 0; k < 16 / CL && k < 4; k++) {
+                    sm.bc[warp][4 * q + pos + k][n0 + perm] = f[2 * k];
+                    sm.bc[warp][4 * q + pos + k][NP + n0 + perm] = f[2 * k + 1];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    float* row = sm.bc[warp][4 * q + k] + n0 + perm;
+                    row[0] = f[4 * k], row[2] = f[4 * k + 1], row[NP] = f[4 * k + 2], row[NP + 2] = f[4 * k + 3];
                 }
             }
         }
         __syncthreads();
-        for (int e = tid; e < TT * 2 * NP; e += THREADS) {
-            const int r = e / (2 * NP), k = e % (2 * NP);
-            if (t0 + r >= te) break;
-            float x = 0.0f;
-            if (t0 + r < end)
-                x = __fadd_rn(__fadd_rn(sm.bc[0][r][k], sm.bc[1][r][k]), __fadd_rn(sm.bc[2][r][k], sm.bc[3][r][k]));
-            a.part_bc[(((int64_t)blockIdx.x * a.batch + b) * a.L + t0 + r) * (2 * NP) + k] = x;
-        }
-        if (t < te && ldd < a.D) {
-            float du[8], dd[8], dz[8];
+        float pD[E], pb[E];  // this position's terms of dD and dbias
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const int c = 8 * lv + k;
-                const float dt = sm.sd[lt][c].x;
-                const float s1 = sm.S[0][lt][c], s2 = __fmul_rn(sm.S[1][lt][c], LN2);
-                const float sc = __fmaf_rn(skip[k], u[k], sm.S[2][lt][c]);
-                du[k] = in ? __fmaf_rn(dt, s1, __fmul_rn(skip[k], dsk[k])) : 0.0f;
-                dd[k] = in ? __fmul_rn(__fmaf_rn(u[k], s1, s2), sg[k]) : 0.0f;
-                dz[k] = in ? __fmul_rn(dyz[k], sc) : 0.0f;
-                if (in) {
-                    sm.acc[0][lt][c] = __fmaf_rn(dsk[k], u[k], sm.acc[0][lt][c]);
-                    sm.acc[1][lt][c] = __fadd_rn(sm.acc[1][lt][c], dd[k]);
-                }
+        for (int k = 0; k < E; k++) pD[k] = pb[k] = 0.0f;
+        if (t < te && have > 0) {
+            const Pack<T, E> eu = slot_pack<E>(&sm.raw[0][E * tid]), ed = slot_pack<E>(&sm.raw[1][E * tid]);
+            const Pack<T, E> eg = slot_pack<E>(&sm.raw[2][E * tid]), ez = slot_pack<E>(&sm.raw[3][E * tid]);
+            float du[E], dd[E], dz[E], s1[E], ds[E], sc[E], skip[E], bias[E];
+            getk<E>(&sm.S[0][lt][lc], s1);
+            getk<E>(&sm.S[1][lt][lc], dd);
+            getk<E>(&sm.S[2][lt][lc], sc);
+            getk<E>(&sm.ds[lt][lc], ds);
+            getk<E>(&sm.skip[lc], skip);
+            getk<E>(&sm.bias[lc], bias);
+#pragma unroll
+            for (int k = 0; k < E; k += 2) {
+                const float4 x = sm.sd[lt][place((lc + k) >> 1, lt)];
+                du[k] = __fmul_rn(x.x, s1[k]), du[k + 1] = __fmul_rn(x.z, s1[k + 1]);
             }
-            const int64_t o = ((int64_t)b * a.L + t) * a.D + ldd;
-            store_pack<8>(static_cast<T*>(a.du) + o, du, a.D - ldd, a.ovec);
-            store_pack<8>(static_cast<T*>(a.ddelta) + o, dd, a.D - ldd, a.ovec);
-            if (a.z.p) store_pack<8>(static_cast<T*>(a.dz) + o, dz, a.D - ldd, a.ovec);
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const float u = to_f(eu.v[k]);
+                dd[k] = __fmaf_rn(u, s1[k], __fmul_rn(dd[k], LN2));
+                if (a.Dskip) {
+                    du[k] = __fmaf_rn(skip[k], ds[k], du[k]);
+                    sc[k] = __fmaf_rn(skip[k], u, sc[k]);
+                }
+                if (a.softplus) dd[k] = __fmul_rn(dd[k], sigmoid(__fadd_rn(to_f(ed.v[k]), bias[k])));
+                dz[k] = 0.0f;
+                if (a.z.p) {
+                    const float z = to_f(ez.v[k]), sg = sigmoid(z);
+                    dz[k] = __fmul_rn(__fmul_rn(to_f(eg.v[k]), sc[k]),
+                                      __fmul_rn(sg, __fmaf_rn(z, __fsub_rn(1.0f, sg), 1.0f)));
+                }
+                if (!in) du[k] = dd[k] = dz[k] = 0.0f;
+                pD[k] = in ? __fmul_rn(ds[k], u) : 0.0f;
+                pb[k] = dd[k];
+            }
+            put(t, du, dd, dz);
         }
+        if (i > 0) load(i - 1);
+        put_bc(t0, false);
+        // over the warp's positions: lanes VPR (and 2 VPR) apart
+        static_assert(F::VPR == 8, "4 positions a warp");
+        halve<E>(pD, 8), halve<E>(pb, 8);
+        halve<E / 2>(pD, 16), halve<E / 2>(pb, 16);
+#pragma unroll
+        for (int k = 0; k < AK; k++) accD[k] = __fadd_rn(accD[k], pD[k]), accb[k] = __fadd_rn(accb[k], pb[k]);
         __syncthreads();
     }
     const int64_t bk = (int64_t)b * a.chunks + ck;
+#pragma unroll
     for (int j = 0; j < CPL; j++) {
-        const int d = d0 + warp * CL * CPL + cl * CPL + j;
-        if (d >= a.D) continue;
-        *reinterpret_cast<float4*>(a.part_a + (bk * a.D + d) * NP + n0) = sm.own[warp][j][2][lane];
-        if (ck == 0 && a.dh0) store4(a.dh0 + ((int64_t)b * a.D + d) * a.N, n0, a.N, sm.own[warp][j][1][lane]);
+        const int c = d0 + c0 + j;
+        if (c >= a.D) break;
+        *reinterpret_cast<float4*>(a.part_a + (bk * a.D + c) * NP + n0) = f4(permute<PERMS>(dA[j], perm));
+        if (ck == 0 && a.dh0)
+            store4(a.dh0 + ((int64_t)b * a.D + c) * a.N, n0, a.N, f4(permute<PERMS>(gc[j], perm)));
     }
+    // what the halvings left with this thread
+    const int off = ((lane >> 3) & 1) * (E / 2) + (lane >> 4) * (E / 4);
+#pragma unroll
+    for (int k = 0; k < AK; k++) sm.S[0][warp][lc + off + k] = accD[k], sm.S[1][warp][lc + off + k] = accb[k];
     __syncthreads();
     for (int e = tid; e < 2 * CB; e += THREADS) {
         const int c = e % CB, k = e / CB;
         if (d0 + c >= a.D) continue;
         float x = 0.0f;
-        for (int r = 0; r < TT; r++) x = __fadd_rn(x, sm.acc[k][r][c]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) x = __fadd_rn(x, sm.S[k][r][c]);
         a.part_d[(bk * 2 + k) * a.D + d0 + c] = x;
     }
 }
@@ -755,6 +1062,11 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 static inline int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
+static inline int fwd_channels(int N) { return lanes_of(N) <= 4 ? Cfg<float, 4>::CB : Cfg<float, 8>::CB; }
+static inline int bwd_channels(int N) { return lanes_of(N) <= 4 ? BCfg<float, 4>::CB : BCfg<float, 8>::CB; }
+static_assert(Cfg<float, 2>::CB == Cfg<float, 4>::CB && Cfg<float, 8>::CB == Cfg<float, 16>::CB, "fwd_channels");
+static_assert(BCfg<float, 2>::CB == BCfg<float, 4>::CB && BCfg<float, 8>::CB == BCfg<float, 16>::CB, "bwd_channels");
+
 // Chunks of the sequence: one where the channels alone give every SM 2 CTAs;
 // else as many as bring it there, of 64 positions at least (a chunked scan
 // makes each exponential twice).
@@ -780,7 +1092,7 @@ struct Ws {  // floats from the workspace's start
 };
 static inline Ws ws_of(int batch, int L, int D, int N, bool backward) {
     const int LN = lanes_of(N), NP = 4 * LN;
-    const Plan p = plan_of(batch, L, D, backward ? 64 : LN == 2 ? 64 : 32);
+    const Plan p = plan_of(batch, L, D, backward ? bwd_channels(N) : fwd_channels(N));
     Ws w = {};
     int64_t at = 0;
     auto take = [&](int64_t n) {
@@ -793,7 +1105,7 @@ static inline Ws ws_of(int batch, int L, int D, int N, bool backward) {
         w.cdt = take((int64_t)batch * p.chunks * D);
     }
     if (backward) {
-        w.part_bc = take((int64_t)cdiv(D, 64) * batch * L * 2 * NP);
+        w.part_bc = take((int64_t)cdiv(D, bwd_channels(N)) * batch * L * 2 * NP);
         w.part_a = take((int64_t)batch * p.chunks * D * NP);
         w.part_d = take((int64_t)batch * p.chunks * 2 * D);
     }
@@ -816,22 +1128,39 @@ static int check(int batch, int L, int D, int N, int dtype) {
     return MI_OK;
 }
 
+template <typename K>
+static bool allow_smem(K* kernel, size_t bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+}
+
+// the chunks' starting states (REV: what they receive from behind), in a.cst
+template <typename T, int LN, bool REV>
+static int start_chunks(const Args& a, cudaStream_t s) {
+    using F = Cfg<T, LN>;
+    constexpr size_t smem = sizeof(typename F::ChunkSmem);
+    if (!allow_smem(chunk_kernel<T, LN, REV>, smem)) return MI_ERR_CUDA;
+    chunk_kernel<T, LN, REV><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), THREADS, smem, s>>>(a);
+    MI_CHECK_LAUNCH();
+    const int64_t items = (int64_t)a.batch * a.D * LN;
+    join_kernel<LN, REV><<<(unsigned)((items + THREADS - 1) / THREADS), THREADS, 0, s>>>(a);
+    MI_CHECK_LAUNCH();
+    return MI_OK;
+}
+
 template <typename T, int LN>
 static int forward(Args& a, float* ws, cudaStream_t s) {
-    using F = Cfg<LN>;
+    using F = Cfg<T, LN>;
     const Plan p = plan_of(a.batch, a.L, a.D, F::CB);
     a.chunks = p.chunks, a.span = p.span;
-    const int blocks = cdiv(a.D, F::CB);
     if (p.chunks > 1) {
         const Ws w = ws_of(a.batch, a.L, a.D, a.N, false);
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        chunk_kernel<T, LN, false><<<dim3(blocks, a.batch, p.chunks - 1), THREADS, 0, s>>>(a);
-        MI_CHECK_LAUNCH();
-        const int64_t items = (int64_t)a.batch * a.D * LN;
-        join_kernel<LN, false><<<(unsigned)((items + THREADS - 1) / THREADS), THREADS, 0, s>>>(a);
-        MI_CHECK_LAUNCH();
+        const int rc = start_chunks<T, LN, false>(a, s);
+        if (rc != MI_OK) return rc;
     }
-    fwd_kernel<T, LN><<<dim3(blocks, a.batch, p.chunks), THREADS, 0, s>>>(a);
+    constexpr size_t smem = sizeof(typename F::Smem);
+    if (!allow_smem(scan_kernel<T, LN>, smem)) return MI_ERR_CUDA;
+    scan_kernel<T, LN><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }
@@ -845,22 +1174,18 @@ static int step(Args& a, float*, cudaStream_t s) {
 
 template <typename T, int LN>
 static int backward(Args& a, float* ws, cudaStream_t s) {
-    using F = BCfg<LN>;
+    using F = BCfg<T, LN>;
     const Plan p = plan_of(a.batch, a.L, a.D, F::CB);
     a.chunks = p.chunks, a.span = p.span;
     const Ws w = ws_of(a.batch, a.L, a.D, a.N, true);
     a.part_bc = ws + w.part_bc, a.part_a = ws + w.part_a, a.part_d = ws + w.part_d;
     if (p.chunks > 1) {
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        chunk_kernel<T, LN, true><<<dim3(cdiv(a.D, Cfg<LN>::CB), a.batch, p.chunks - 1), THREADS, 0, s>>>(a);
-        MI_CHECK_LAUNCH();
-        const int64_t items = (int64_t)a.batch * a.D * LN;
-        join_kernel<LN, true><<<(unsigned)((items + THREADS - 1) / THREADS), THREADS, 0, s>>>(a);
-        MI_CHECK_LAUNCH();
+        const int rc = start_chunks<T, LN, true>(a, s);
+        if (rc != MI_OK) return rc;
     }
-    constexpr int smem = (int)sizeof(typename F::Smem);
-    if (cudaFuncSetAttribute(bwd_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return MI_ERR_CUDA;
+    constexpr size_t smem = sizeof(typename F::Smem);
+    if (!allow_smem(bwd_kernel<T, LN>, smem)) return MI_ERR_CUDA;
     bwd_kernel<T, LN><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
@@ -917,6 +1242,7 @@ extern "C" int mi_selective_scan(const void* u, int64_t u_batch, int64_t u_row, 
     a.y = y, a.hT = h_out, a.ckpt = checkpoints;
     a.batch = batch, a.L = L, a.D = Dm, a.N = N, a.softplus = softplus;
     a.ovec = Dm % 8 == 0 && mi::aligned16(y);
+    a.pvec = mi::aligned16(D) && mi::aligned16(delta_bias);
     float* ws = static_cast<float*>(workspace);
     MI_DISPATCH_DTYPE(dtype, T, MI_SSCAN_STATES(N, forward, T, a, ws, (cudaStream_t)stream));
     return MI_ERR_INVALID;
@@ -969,12 +1295,13 @@ extern "C" int mi_selective_scan_backward(
     a.du = du, a.ddelta = ddelta, a.dz = dz, a.dh0 = dh0;
     a.batch = batch, a.L = L, a.D = Dm, a.N = N, a.softplus = softplus;
     a.ovec = Dm % 8 == 0 && mi::aligned16(du) && mi::aligned16(ddelta) && mi::aligned16(dz);
+    a.pvec = mi::aligned16(D) && mi::aligned16(delta_bias);
     float* ws = static_cast<float*>(workspace);
     cudaStream_t s = (cudaStream_t)stream;
     int rc2 = MI_OK;
     MI_DISPATCH_DTYPE(dtype, T, rc2 = mi_sscan_backward_states<T>(a, ws, s));
     if (rc2 != MI_OK) return rc2;
-    const int NP = 4 * lanes_of(N), blocks = mi::cdiv(Dm, 64);
+    const int NP = 4 * lanes_of(N), blocks = mi::cdiv(Dm, bwd_channels(N));
     const int64_t rows = (int64_t)batch * L;
     if (dB || dC) {
         const int64_t n = rows * 2 * NP;
