@@ -54,8 +54,36 @@ def build_bpe(force: bool = False) -> str:
     return BPE_SO
 
 
+TORCH_SO = os.path.join(HERE, "_mi_torch.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+
+
+def build_torch(force: bool = False) -> str:
+    """The float operators' calls from torch, _mi_torch.so (g++, C++17; no CUDA compiler)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    deps = [TORCH_SRC, os.path.join(ROOT, "include", "mi_b200.h")]
+    if not force and os.path.exists(TORCH_SO) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_SO) for d in deps):
+        return TORCH_SO
+    cxx = shutil.which("g++") or "g++"
+    cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
+    includes = [*cpp_extension.include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    subprocess.run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+                    "-DTORCH_EXTENSION_NAME=_mi_torch", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    *[arg for path in includes for arg in ("-isystem", path)], "-o", TORCH_SO + ".tmp", TORCH_SRC,
+                    "-L" + libs, "-Wl,-rpath," + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
+                   check=True)
+    os.replace(TORCH_SO + ".tmp", TORCH_SO)
+    return TORCH_SO
+
+
 def build(verbose: bool = False, force: bool = False) -> str:
     build_bpe(force=force)
+    build_torch(force=force)
     if not force and not needs_build():
         return SO
     nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"

@@ -233,6 +233,18 @@ def test_scan_gradients_of_shared_inputs(sel, cuda_dev):
               16 * 20 + 128 + 60, "shared")
 
 
+def test_gradients_are_of_first_order(sel, cuda_dev):
+    x = torch.randn(4, 8, device=cuda_dev, requires_grad=True)
+    w = torch.ones(8, device=cuda_dev, requires_grad=True)
+    y, _ = sel.rms_norm(x, w)
+    dy = torch.ones_like(y, requires_grad=True)
+    (g,) = torch.autograd.grad(y, x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(g.sum(), dy)
+    c = sel.causal_conv1d(x.unsqueeze(0), torch.ones(8, 4, device=cuda_dev), silu=True)
+    torch.autograd.grad(c.sum(), x, create_graph=True)  # one order is there, whatever the mode
+
+
 def test_scan_repeats_its_bits(sel, cuda_dev):
     a = scan_inputs(cuda_dev, BF16, 2, 300, 96, 16, h0=True)
     dy = torch.randn(2, 300, 96, device=cuda_dev).to(BF16)
