@@ -16,7 +16,6 @@
 namespace mi {
 namespace conv1d {
 
-constexpr int RUN = 16;   // positions a thread
 constexpr int MAXW = 4;
 
 struct Args {
@@ -37,6 +36,7 @@ struct Args {
     int batch, L, D;
     int silu;
     int vec;
+    int run;               // positions a thread, forward: 8, 16, 32 or 64
 };
 
 __device__ __forceinline__ int length_of(const int* lengths, int b, int L) {
@@ -60,6 +60,20 @@ __device__ __forceinline__ Pack<T, K> load_x(const Args& a, int b, int t, int c,
 
 template <int W, int K>
 __device__ __forceinline__ void load_w(const Args& a, int c, float (&w)[W][K], float (&bias)[K]) {
+    if (W == 4 && a.vec) {  // a channel's taps at once
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            const float4 t = reinterpret_cast<const float4*>(a.w)[c + i];
+            w[0][i] = t.x, w[1][i] = t.y, w[W - 2][i] = t.z, w[W - 1][i] = t.w;
+        }
+        Pack<float, K> t;
+#pragma unroll
+        for (int i = 0; i < K; i++) t.v[i] = 0.0f;
+        if (a.bias) t = *reinterpret_cast<const Pack<float, K>*>(a.bias + c);
+#pragma unroll
+        for (int i = 0; i < K; i++) bias[i] = t.v[i];
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < K; i++) {
         const bool in = c + i < a.D;
@@ -69,88 +83,122 @@ __device__ __forceinline__ void load_w(const Args& a, int c, float (&w)[W][K], f
     }
 }
 
-template <typename T, int W, int K>
-__global__ void __launch_bounds__(128) fwd_kernel(const Args a) {
+// K channels of a row that exists, as they lie: no branch and no conversion,
+// behind either of which a warp would wait for each load by itself.  Channels
+// beyond the last read the row's first ones; nothing comes of them.
+template <bool VEC, int K, typename T>
+__device__ __forceinline__ Pack<T, K> raw_row(const T* p, int have) {
+    if (VEC) return *reinterpret_cast<const Pack<T, K>*>(p);
+    Pack<T, K> r;
+#pragma unroll
+    for (int i = 0; i < K; i++) r.v[i] = p[i < have ? i : 0];
+    return r;
+}
+
+// The W - 1 inputs in front of position t0 (a run's first)
+template <int W, int K, bool VEC, typename T>
+__device__ __forceinline__ void rows_before(const Args& a, int b, int t0, int len, int c, float (&x)[W - 1][K]) {
+    const int have = a.D - c;
+    Pack<T, K> p[W - 1];
+    if (t0 > 0) {  // runs are longer than W - 1
+#pragma unroll
+        for (int k = 0; k < W - 1; k++)
+            p[k] = raw_row<VEC, K>(static_cast<const T*>(a.x) + b * a.xb + (t0 - (W - 1) + k) * a.xl + c, have);
+    } else if (a.win) {
+#pragma unroll
+        for (int k = 0; k < W - 1; k++)
+            p[k] = raw_row<VEC, K>(static_cast<const T*>(a.win) + ((int64_t)b * (W - 1) + k) * a.D + c, have);
+    }
+    const bool some = t0 > 0 || a.win;
+#pragma unroll
+    for (int k = 0; k < W - 1; k++)
+#pragma unroll
+        for (int i = 0; i < K; i++) x[k][i] = some && t0 - (W - 1) + k < len ? to_f(p[k].v[i]) : 0.0f;
+}
+
+// A thread's run, 4 positions at a time, with the next 4 rows on their way;
+// rows behind the sequence's length are named by its last one, and not used.
+template <typename T, int W, int K, bool VEC>
+__global__ void __launch_bounds__(128, 5) fwd_kernel(const Args a) {
+    using P = Pack<T, K>;
     const int vecs = cdiv(a.D, K);
-    const int runs = a.L > 0 ? cdiv(a.L, RUN) : 1;  // an empty sequence still passes its window on
+    const int runs = a.L > 0 ? cdiv(a.L, a.run) : 1;  // an empty sequence still passes its window on
     const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (item >= (int64_t)vecs * runs * a.batch) return;
-    const int c = (int)(item % vecs) * K;
+    const int c = (int)(item % vecs) * K, have = a.D - c;
     const int run = (int)(item / vecs % runs), b = (int)(item / vecs / runs);
-    const bool vec = a.vec != 0;
     const int len = length_of(a.lengths, b, a.L);
-    const int t0 = run * RUN, t1 = t0 + RUN < a.L ? t0 + RUN : a.L;
-    T* y = static_cast<T*>(a.y) + ((int64_t)b * a.L) * a.D + c;
-    float w[W][K], bias[K];
-    load_w<W, K>(a, c, w, bias);
-    float row[W][K];  // the inputs of the last W positions, oldest first
+    const int t0 = run * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
+    if (t0 < t1) {
+        const T* xb = static_cast<const T*>(a.x) + b * a.xb + c;
+        const int last = len > 0 ? len - 1 : 0;
+        P p[4];
+        auto fetch = [&](int t) {
 #pragma unroll
-    for (int k = 0; k < W - 1; k++) {
-        const int t = t0 - (W - 1) + k;
-        if (t < len) {
-            const Pack<T, K> p = load_x<W, K, T>(a, b, t, c, vec);
-#pragma unroll
-            for (int i = 0; i < K; i++) row[k + 1][i] = to_f(p.v[i]);
-        }
-    }
+            for (int j = 0; j < 4; j++) p[j] = raw_row<VEC, K>(xb + (int64_t)(t + j < last ? t + j : last) * a.xl, have);
+        };
+        fetch(t0);
+        float x[W + 3][K], w[W][K], bias[K];
+        rows_before<W, K, VEC, T>(a, b, t0, len, c, reinterpret_cast<float(&)[W - 1][K]>(x));
+        load_w<W, K>(a, c, w, bias);
+        T* y = static_cast<T*>(a.y) + ((int64_t)b * a.L + t0) * a.D + c;
 #pragma unroll 1
-    for (int t = t0; t < t1; t += 4) {
-        Pack<T, K> p[4];
+        for (int t = t0; t < t1; t += 4) {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (t + j < t1 && t + j < len) p[j] = load_x<W, K, T>(a, b, t + j, c, vec);
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (t + j >= t1) break;
-            float o[K];
-            if (t + j < len) {
+                for (int i = 0; i < K; i++) x[W - 1 + j][i] = to_f(p[j].v[i]);
+            fetch(t + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float o[K];
 #pragma unroll
                 for (int i = 0; i < K; i++) {
-#pragma unroll
-                    for (int k = 0; k < W - 1; k++) row[k][i] = row[k + 1][i];
-                    row[W - 1][i] = to_f(p[j].v[i]);
                     float s = bias[i];
 #pragma unroll
-                    for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], row[k][i], s);
-                    o[i] = a.silu ? __fmul_rn(s, sigmoid(s)) : s;
+                    for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], x[j + k][i], s);
+                    if (a.silu) s = __fmul_rn(s, sigmoid(s));
+                    o[i] = t + j < len ? s : 0.0f;
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < K; i++) o[i] = 0.0f;
+                if (t + j < t1) store_pack<K>(y, o, have, VEC);
+                y += a.D;
             }
-            store_pack<K>(y + (int64_t)(t + j) * a.D, o, a.D - c, vec);
+#pragma unroll
+            for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                for (int i = 0; i < K; i++) x[j][i] = x[j + 4][i];
         }
     }
     // the window that leaves: inputs len - W + 1 .. len - 1, by the first run
     if (run == 0 && a.win_out) {
 #pragma unroll
         for (int k = 0; k < W - 1; k++) {
-            const Pack<T, K> p = load_x<W, K, T>(a, b, len - (W - 1) + k, c, vec);
+            const P p = load_x<W, K, T>(a, b, len - (W - 1) + k, c, VEC);
             float o[K];
 #pragma unroll
             for (int i = 0; i < K; i++) o[i] = to_f(p.v[i]);
-            store_pack<K>(static_cast<T*>(a.win_out) + ((int64_t)b * (W - 1) + k) * a.D + c, o, a.D - c, vec);
+            store_pack<K>(static_cast<T*>(a.win_out) + ((int64_t)b * (W - 1) + k) * a.D + c, o, have, VEC);
         }
     }
 }
 
 // Backward.  A CTA is 32 channel packs by 8 runs of one sequence.  A thread
-// walks its run forward: dc[t] needs x up to t, dx[t] needs dc up to
-// t + W - 1, so it goes W - 1 positions past its run, and dx comes out W - 1
-// positions late.  Its own positions' terms of dw and dbias stay in registers;
+// walks its run forward, 4 positions at a time: dc[t] needs x up to t, dx[t]
+// needs dc up to t + W - 1, so it goes W - 1 positions past its run, and dx
+// comes out W - 1 positions late.  Its own positions' terms of dw and dbias stay in registers;
 // the CTA adds its 8 runs in shared memory, in order, and writes one partial
 // row, which sum_kernel adds.
-constexpr int BWD_RUNS = 8;
+constexpr int BWD_RUNS = 8;  // of a.run positions: 16 or 32
 
-template <typename T, int W, int K>
-__global__ void __launch_bounds__(256) bwd_kernel(const Args a) {
+template <typename T, int W, int K, bool VEC>
+__global__ void __launch_bounds__(256, 2) bwd_kernel(const Args a) {
+    using P = Pack<T, K>;
     constexpr int S = (W + 1) * K;
     __shared__ float sh[BWD_RUNS][32][S + 1];
     const int cx = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int c = (blockIdx.x * 32 + cx) * K;
+    const int c = (blockIdx.x * 32 + cx) * K, have = a.D - c;
     const int b = blockIdx.z;
-    const int t0 = (blockIdx.y * BWD_RUNS + g) * RUN, t1 = t0 + RUN < a.L ? t0 + RUN : a.L;
-    const bool vec = a.vec != 0;
+    const int t0 = (blockIdx.y * BWD_RUNS + g) * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
     const int len = length_of(a.lengths, b, a.L);
     float dw[W][K], db[K];
 #pragma unroll
@@ -159,98 +207,92 @@ __global__ void __launch_bounds__(256) bwd_kernel(const Args a) {
 #pragma unroll
         for (int k = 0; k < W; k++) dw[k][i] = 0.0f;
     }
-    if (c < a.D && t0 < a.L) {
-        float w[W][K], bias[K];
-        load_w<W, K>(a, c, w, bias);
-        const T* dyp = static_cast<const T*>(a.dy) + b * a.gb + c;
-        T* dxp = static_cast<T*>(a.dx) + (int64_t)b * a.L * a.D + c;
+    if (have > 0 && t0 < a.L) {
+        const T* xb = static_cast<const T*>(a.x) + b * a.xb + c;
+        const T* gb = static_cast<const T*>(a.dy) + b * a.gb + c;
         const T* gwin = static_cast<const T*>(a.dwin_out);
-        float row[W][K], dc[W][K];  // the last W inputs and the last W dc, oldest first
+        const int last = len > 0 ? len - 1 : 0;
+        P nx[4], ng[4];
+        auto fetch = [&](int t) {
 #pragma unroll
-        for (int i = 0; i < K; i++)
+            for (int j = 0; j < 4; j++) {
+                const int64_t r = t + j < last ? t + j : last;
+                nx[j] = raw_row<VEC, K>(xb + r * a.xl, have);
+                ng[j] = raw_row<VEC, K>(gb + r * a.gl, have);
+            }
+        };
+        fetch(t0);
+        float w[W][K], bias[K];
+        float x[W + 3][K], dc[W + 3][K];  // inputs and dc from W - 1 positions before a group to its end
+        rows_before<W, K, VEC, T>(a, b, t0, len, c, reinterpret_cast<float(&)[W - 1][K]>(x));
+        load_w<W, K>(a, c, w, bias);
 #pragma unroll
-            for (int k = 0; k < W; k++) row[k][i] = dc[k][i] = 0.0f;
-        // the run that begins the sequence also makes the window's gradients,
-        // dx at t = -(W-1) .. -1
+        for (int j = 0; j < W - 1; j++)
+#pragma unroll
+            for (int i = 0; i < K; i++) dc[j][i] = 0.0f;
+        // the run that begins the sequence also makes the window's gradients, dx at t = -(W-1) .. -1
         const int first = t0 == 0 ? -(W - 1) : t0;
-#pragma unroll
-        for (int k = 0; k < W - 1; k++) {
-            const int t = t0 - (W - 1) + k;
-            if (t < len) {
-                const Pack<T, K> p = load_x<W, K, T>(a, b, t, c, vec);
-#pragma unroll
-                for (int i = 0; i < K; i++) row[k + 1][i] = to_f(p.v[i]);
-            }
-        }
 #pragma unroll 1
-        for (int tb = t0; tb < t1 + W - 1; tb += 4) {
-            Pack<T, K> px[4], pg[4];
+        for (int t = t0; t < t1 + W - 1; t += 4) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int t = tb + j;
-                if (t < t1 + W - 1 && t < len) {
-                    px[j] = load_x<W, K, T>(a, b, t, c, vec);
-                    pg[j] = load_pack<K>(dyp + t * a.gl, a.D - c, vec);
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    x[W - 1 + j][i] = t + j < len ? to_f(nx[j].v[i]) : 0.0f;
+                    dc[W - 1 + j][i] = t + j < len ? to_f(ng[j].v[i]) : 0.0f;
                 }
-            }
+            fetch(t + 4);
+            if (a.silu) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int t = tb + j;
-                if (t >= t1 + W - 1) break;
-#pragma unroll
-                for (int i = 0; i < K; i++)
-#pragma unroll
-                    for (int k = 0; k < W - 1; k++) dc[k][i] = dc[k + 1][i];
-                if (t < len) {
+                for (int j = 0; j < 4; j++)
 #pragma unroll
                     for (int i = 0; i < K; i++) {
+                        float s = bias[i];
 #pragma unroll
-                        for (int k = 0; k < W - 1; k++) row[k][i] = row[k + 1][i];
-                        row[W - 1][i] = to_f(px[j].v[i]);
-                        float gr = to_f(pg[j].v[i]);
-                        if (a.silu) {
-                            float s = bias[i];
-#pragma unroll
-                            for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], row[k][i], s);
-                            const float sg = sigmoid(s);
-                            gr = __fmul_rn(gr, __fmul_rn(sg, __fmaf_rn(s, __fsub_rn(1.0f, sg), 1.0f)));
-                        }
-                        dc[W - 1][i] = gr;
-                        if (t < t1) {
-                            db[i] = __fadd_rn(db[i], gr);
-#pragma unroll
-                            for (int k = 0; k < W; k++) dw[k][i] = __fmaf_rn(gr, row[k][i], dw[k][i]);
-                        }
+                        for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], x[j + k][i], s);
+                        const float sg = sigmoid(s);
+                        const float f = __fmul_rn(sg, __fmaf_rn(s, __fsub_rn(1.0f, sg), 1.0f));
+                        dc[W - 1 + j][i] = t + j < len ? __fmul_rn(dc[W - 1 + j][i], f) : 0.0f;
                     }
-                } else {
+            }
 #pragma unroll
-                    for (int i = 0; i < K; i++) dc[W - 1][i] = 0.0f;
-                }
-                // dx at td = t - (W - 1), whose last reader is t; dc[j] is dc at td + j
-                const int td = t - (W - 1);
-                if (td >= first && td < t1 && (td < 0 ? a.dwin != nullptr : a.dx != nullptr)) {
-                    float o[K];
+            for (int j = 0; j < 4; j++)
+                if (t + j < t1) {  // the run's own positions
 #pragma unroll
                     for (int i = 0; i < K; i++) {
-                        float s = 0.0f;
+                        db[i] = __fadd_rn(db[i], dc[W - 1 + j][i]);
 #pragma unroll
-                        for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], dc[W - 1 - k][i], s);
-                        o[i] = s;
+                        for (int k = 0; k < W; k++) dw[k][i] = __fmaf_rn(dc[W - 1 + j][i], x[j + k][i], dw[k][i]);
                     }
-                    // this input's place in the window that leaves, if it has one
-                    const int kw = td - (len - (W - 1));
-                    if (gwin && kw >= 0 && kw < W - 1) {
-                        const Pack<T, K> p = load_pack<K>(gwin + ((int64_t)b * (W - 1) + kw) * a.D + c, a.D - c, vec);
-#pragma unroll
-                        for (int i = 0; i < K; i++) o[i] = __fadd_rn(o[i], to_f(p.v[i]));
-                    }
-                    if (td < 0)
-                        store_pack<K>(static_cast<T*>(a.dwin) + ((int64_t)b * (W - 1) + td + W - 1) * a.D + c, o,
-                                      a.D - c, vec);
-                    else
-                        store_pack<K>(dxp + (int64_t)td * a.D, o, a.D - c, vec);
                 }
+            // dx of the positions W - 1 earlier
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int td = t + j - (W - 1);
+                T* to = td >= 0 ? static_cast<T*>(a.dx) : static_cast<T*>(a.dwin);
+                if (td < first || td >= t1 || !to) continue;
+                float o[K];
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    float s = __fmul_rn(w[0][i], dc[j + W - 1][i]);
+#pragma unroll
+                    for (int k = 1; k < W; k++) s = __fmaf_rn(w[k][i], dc[j + W - 1 - k][i], s);
+                    o[i] = s;
+                }
+                // this input's place in the window that leaves, if it has one
+                const int kw = td - (len - (W - 1));
+                if (gwin && kw >= 0 && kw < W - 1) {
+                    const P p = raw_row<VEC, K>(gwin + ((int64_t)b * (W - 1) + kw) * a.D + c, have);
+#pragma unroll
+                    for (int i = 0; i < K; i++) o[i] = __fadd_rn(o[i], to_f(p.v[i]));
+                }
+                store_pack<K>(to + (td >= 0 ? (int64_t)b * a.L + td : (int64_t)b * (W - 1) + td + W - 1) * a.D + c, o, have,
+                              VEC);
             }
+#pragma unroll
+            for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                for (int i = 0; i < K; i++) x[j][i] = x[j + 4][i], dc[j][i] = dc[j + 4][i];
         }
     }
     if (!a.part) return;
@@ -338,12 +380,24 @@ __global__ void __launch_bounds__(128) step_kernel(const Args a) {
     for (int k = 0; k < W - 1; k++) store_pack<K>(win + (int64_t)k * a.D, row[k + 1], valid, vec);
 }
 
-constexpr int KF = 4;  // channels a thread: 16 bytes of fp32, 8 of 16-bit types
+// Channels a thread.  Wider packs need fewer loads, but what a thread holds for
+// each channel (4 taps, 7 inputs; backward 4 sums and 7 dc more) costs
+// registers, and occupancy is worth more than the loads: 8 x 2048 x 1536 bf16
+// took 41 us forward with 8 channels (209 registers) and 37 with 4.
+constexpr int KF = 4, KB = 2;
 
 template <typename T, int W>
-static int forward(const Args& a, cudaStream_t s) {
-    const int64_t items = (int64_t)cdiv(a.D, KF) * (a.L > 0 ? cdiv(a.L, RUN) : 1) * a.batch;
-    fwd_kernel<T, W, KF><<<(unsigned)((items + 127) / 128), 128, 0, s>>>(a);
+static int forward(Args& a, cudaStream_t s) {
+    // long runs read fewer rows twice and their taps once; short ones where they are what fills the GPU (148 x 768 threads)
+    const int64_t lanes = (int64_t)cdiv(a.D, KF) * a.batch;
+    a.run = 64;
+    while (a.run > 8 && lanes * cdiv(a.L, a.run) < 148 * 768) a.run /= 2;
+    const int64_t items = lanes * (a.L > 0 ? cdiv(a.L, a.run) : 1);
+    const unsigned grid = (unsigned)((items + 127) / 128);
+    if (a.vec)
+        fwd_kernel<T, W, KF, true><<<grid, 128, 0, s>>>(a);
+    else
+        fwd_kernel<T, W, KF, false><<<grid, 128, 0, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }
@@ -355,10 +409,22 @@ static int step(const Args& a, cudaStream_t s) {
     return MI_OK;
 }
 
+// positions a thread: 32 where that still gives every SM 4 CTAs
+static inline int bwd_run(int batch, int L, int D) {
+    return (int64_t)cdiv(D, 32 * KB) * cdiv(L, 32 * BWD_RUNS) * batch >= 148 * 4 ? 32 : 16;
+}
+static inline int64_t parts(int batch, int L, int D) {
+    return (int64_t)batch * cdiv(L, bwd_run(batch, L, D) * BWD_RUNS);
+}
+
 template <typename T, int W>
-static int backward(const Args& a, cudaStream_t s) {
-    const dim3 grid(cdiv(a.D, 32 * KF), cdiv(cdiv(a.L, RUN), BWD_RUNS), a.batch);
-    bwd_kernel<T, W, KF><<<grid, 256, 0, s>>>(a);
+static int backward(Args& a, cudaStream_t s) {
+    a.run = bwd_run(a.batch, a.L, a.D);
+    const dim3 grid(cdiv(a.D, 32 * KB), cdiv(a.L, a.run * BWD_RUNS), a.batch);
+    if (a.vec)
+        bwd_kernel<T, W, KB, true><<<grid, 256, 0, s>>>(a);
+    else
+        bwd_kernel<T, W, KB, false><<<grid, 256, 0, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }
@@ -366,11 +432,9 @@ static int backward(const Args& a, cudaStream_t s) {
 static int check(int batch, int L, int D, int W, int dtype) {
     if (batch < 0 || L < 0 || D <= 0) return MI_ERR_INVALID;
     if (dtype != MI_DT_F32 && dtype != MI_DT_BF16 && dtype != MI_DT_F16) return MI_ERR_INVALID;
-    if (W < 2 || W > MAXW || batch > 65535 || L > 65535 * RUN * BWD_RUNS) return MI_ERR_UNSUPPORTED;
+    if (W < 2 || W > MAXW || batch > 65535 || L > 65535 * 16 * BWD_RUNS) return MI_ERR_UNSUPPORTED;
     return MI_OK;
 }
-
-static inline int64_t parts(int batch, int L) { return (int64_t)batch * cdiv(cdiv(L, RUN), BWD_RUNS); }
 
 }  // namespace conv1d
 }  // namespace mi
@@ -394,7 +458,7 @@ extern "C" int mi_causal_conv1d(const void* x, int64_t x_batch, int64_t x_row, c
     a.x = x, a.xb = x_batch, a.xl = x_row, a.w = w, a.bias = bias, a.win = win, a.lengths = lengths;
     a.y = y, a.win_out = win_out, a.batch = batch, a.L = L, a.D = D, a.silu = silu;
     a.vec = D % KF == 0 && x_batch % KF == 0 && x_row % KF == 0 && mi::aligned16(x) && mi::aligned16(y) &&
-            mi::aligned16(win) && mi::aligned16(win_out);
+            mi::aligned16(win) && mi::aligned16(win_out) && mi::aligned16(w) && mi::aligned16(bias);
     MI_DISPATCH_DTYPE(dtype, T, MI_CONV_TAPS(W, forward, T, a, (cudaStream_t)stream));
     return MI_ERR_INVALID;
 }
@@ -409,14 +473,15 @@ extern "C" int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float
     Args a = {};
     a.x = x, a.xb = x_batch, a.w = w, a.bias = bias, a.win_out = win, a.y = y;
     a.batch = batch, a.L = 1, a.D = D, a.silu = silu;
-    a.vec = D % KF == 0 && x_batch % KF == 0 && mi::aligned16(x) && mi::aligned16(y) && mi::aligned16(win);
+    a.vec = D % KF == 0 && x_batch % KF == 0 && mi::aligned16(x) && mi::aligned16(y) && mi::aligned16(win) &&
+            mi::aligned16(w) && mi::aligned16(bias);
     MI_DISPATCH_DTYPE(dtype, T, MI_CONV_TAPS(W, step, T, a, (cudaStream_t)stream));
     return MI_ERR_INVALID;
 }
 
 extern "C" int64_t mi_causal_conv1d_backward_workspace(int batch, int L, int D, int W) {
     if (batch <= 0 || L <= 0 || D <= 0 || W < 2 || W > mi::conv1d::MAXW) return 0;
-    return (int64_t)sizeof(float) * mi::conv1d::parts(batch, L) * D * (W + 1);
+    return (int64_t)sizeof(float) * mi::conv1d::parts(batch, L, D) * D * (W + 1);
 }
 
 extern "C" int mi_causal_conv1d_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const void* dwin_out,
@@ -438,13 +503,13 @@ extern "C" int mi_causal_conv1d_backward(const void* dy, int64_t dy_batch, int64
     a.batch = batch, a.L = L, a.D = D, a.silu = silu;
     a.vec = D % KF == 0 && x_batch % KF == 0 && x_row % KF == 0 && dy_batch % KF == 0 && dy_row % KF == 0 &&
             mi::aligned16(x) && mi::aligned16(dy) && mi::aligned16(win) && mi::aligned16(dwin_out) &&
-            mi::aligned16(dx) && mi::aligned16(dwin);
-    int (*fn)(const Args&, cudaStream_t) = nullptr;
+            mi::aligned16(dx) && mi::aligned16(dwin) && mi::aligned16(w) && mi::aligned16(bias);
+    int (*fn)(Args&, cudaStream_t) = nullptr;
     MI_DISPATCH_DTYPE(dtype, T, fn = W == 2 ? backward<T, 2> : W == 3 ? backward<T, 3> : backward<T, 4>);
     const int rc2 = fn(a, s);
     if (rc2 != MI_OK || !a.part) return rc2;
     const int64_t cols = (int64_t)D * (W + 1);
-    sum_kernel<<<(unsigned)((cols + 31) / 32), 256, 0, s>>>(a.part, dw, dbias, (int)parts(batch, L), D, W);
+    sum_kernel<<<(unsigned)((cols + 31) / 32), 256, 0, s>>>(a.part, dw, dbias, (int)parts(batch, L, D), D, W);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }

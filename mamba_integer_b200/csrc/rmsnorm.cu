@@ -61,9 +61,26 @@ __device__ __forceinline__ float row_reduce(float v, float* red) {
     return v;
 }
 
+// K elements from p on, `valid` of which exist.  VEC: all of them or none, and
+// aligned, so that the load needs a predicate and no branch (behind a branch
+// the warp would wait for it).
+template <bool VEC, int K, typename T>
+__device__ __forceinline__ Pack<T, K> row_pack(const T* p, int valid) {
+    Pack<T, K> r;
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < K; i++) r.v[i] = from_f<T>(0.0f);
+        if (valid > 0) r = *reinterpret_cast<const Pack<T, K>*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < K; i++) r.v[i] = i < valid ? p[i] : from_f<T>(0.0f);
+    }
+    return r;
+}
+
 // T: element type of x and y; R: of the residual and s.  A thread holds NV
 // packs of K elements, TPR * K apart.
-template <typename T, typename R, int K, int NV, int TPR, bool QUANT>
+template <typename T, typename R, int K, int NV, int TPR, bool VEC, bool QUANT>
 __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(const Args a) {
     __shared__ float red[32];
     constexpr int ROWS = (TPR > THREADS ? TPR : THREADS) / TPR;
@@ -74,7 +91,6 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
     const bool live = t < a.T;
     const T* x = static_cast<const T*>(a.x) + t * a.ldx;
     const R* r = static_cast<const R*>(a.r) + t * a.ldr;
-    const bool vec = a.vec != 0;
     float s[NV][K];
     float acc = 0.0f;
     Pack<T, K> px[NV];
@@ -83,8 +99,8 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + lane) * K;
         const int valid = live ? a.D - c : 0;
-        px[j] = load_pack<K>(x + c, valid, vec);
-        if (a.r) pr[j] = load_pack<K>(r + c, valid, vec);
+        px[j] = row_pack<VEC, K>(x + c, valid);
+        if (a.r) pr[j] = row_pack<VEC, K>(r + c, valid);
     }
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -96,7 +112,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
             // the norm is of the sum as it is kept, so that a backward pass finds the same one
             if (a.r) s[j][i] = to_f(from_f<R>(__fadd_rn(s[j][i], to_f(pr[j].v[i]))));
         }
-        if (a.r && valid > 0) store_pack<K>(static_cast<R*>(a.sum) + t * a.D + c, s[j], valid, vec);
+        if (a.r && valid > 0) store_pack<K>(static_cast<R*>(a.sum) + t * a.D + c, s[j], valid, VEC);
 #pragma unroll
         for (int i = 0; i < K; i++) acc = __fmaf_rn(s[j][i], s[j][i], acc);
     }
@@ -107,13 +123,13 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + lane) * K;
-        const Pack<float, K> w = load_pack<K>(a.w + c, a.D - c, vec);
+        const Pack<float, K> w = row_pack<VEC, K>(a.w + c, a.D - c);
 #pragma unroll
         for (int i = 0; i < K; i++) {
             s[j][i] = __fmul_rn(__fmul_rn(s[j][i], rstd), w.v[i]);
             if (QUANT) amax = max_nan(amax, fabsf(s[j][i]));
         }
-        if (!QUANT && live && c < a.D) store_pack<K>(static_cast<T*>(a.y) + t * a.D + c, s[j], a.D - c, vec);
+        if (!QUANT && live && c < a.D) store_pack<K>(static_cast<T*>(a.y) + t * a.D + c, s[j], a.D - c, VEC);
     }
     if (QUANT) {
         amax = row_reduce<TPR, true>(amax, red);
@@ -128,7 +144,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
             Pack<int8_t, K> q;
 #pragma unroll
             for (int i = 0; i < K; i++) q.v[i] = (int8_t)quant_i8(__fmul_rn(s[j][i], inv));
-            if (vec && a.D - c >= K) {
+            if (VEC) {
                 *reinterpret_cast<Pack<int8_t, K>*>(o) = q;
             } else {
 #pragma unroll
@@ -143,19 +159,22 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
 // its columns' dy * xhat over its rows in registers, a CTA adds its row groups
 // through shared memory and writes one row of partial sums, and
 // column_sum_kernel adds those.
-template <typename T, typename R, int K, int NV, int TPR>
-__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) bwd_kernel(const Args a) {
+// registers that a thread of the backward pass holds for its packs, and the CTAs an SM that they leave room for
+template <typename T, typename R, int K, int NV>
+constexpr int held = (2 * K + (sizeof(T) + 2 * sizeof(R)) * K / 4) * NV;
+template <typename T, typename R, int K, int NV, int TPR, bool VEC>
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR <= THREADS && held<T, R, K, NV> <= 92 ? 2 : 1)
+    bwd_kernel(const Args a) {
     __shared__ float red[32];
     extern __shared__ float dw_sh[];  // [D] for ROWS > 1
     constexpr int ROWS = (TPR > THREADS ? TPR : THREADS) / TPR;
     const int lane = threadIdx.x % TPR, row = threadIdx.x / TPR;
-    const bool vec = a.vec != 0;
     float dw[NV][K];
     Pack<float, K> w[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int c = (j * TPR + lane) * K;
-        w[j] = load_pack<K>(a.w + c, a.D - c, vec);
+        w[j] = row_pack<VEC, K>(a.w + c, a.D - c);
 #pragma unroll
         for (int i = 0; i < K; i++) dw[j][i] = 0.0f;
     }
@@ -169,9 +188,9 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) bwd_kernel(cons
         for (int j = 0; j < NV; j++) {
             const int c = (j * TPR + lane) * K;
             const int valid = live ? a.D - c : 0;
-            ps[j] = load_pack<K>(static_cast<const R*>(a.sum) + t * a.ldr + c, valid, vec);
-            pg[j] = load_pack<K>(static_cast<const T*>(a.dy) + t * a.D + c, valid, vec);
-            if (a.dsum) pd[j] = load_pack<K>(static_cast<const R*>(a.dsum) + t * a.D + c, valid, vec);
+            ps[j] = row_pack<VEC, K>(static_cast<const R*>(a.sum) + t * a.ldr + c, valid);
+            pg[j] = row_pack<VEC, K>(static_cast<const T*>(a.dy) + t * a.D + c, valid);
+            if (a.dsum) pd[j] = row_pack<VEC, K>(static_cast<const R*>(a.dsum) + t * a.D + c, valid);
         }
         const float rstd = live ? a.rstd[t] : 0.0f;
         float dot = 0.0f;
@@ -199,8 +218,8 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) bwd_kernel(cons
                     o[i] = __fmul_rn(rstd, __fmaf_rn(-xh, mean, g));
                     if (a.dsum) o[i] = __fadd_rn(o[i], to_f(pd[j].v[i]));
                 }
-                if (a.dx) store_pack<K>(static_cast<T*>(a.dx) + t * a.D + c, o, a.D - c, vec);
-                if (a.dr) store_pack<K>(static_cast<R*>(a.dr) + t * a.D + c, o, a.D - c, vec);
+                if (a.dx) store_pack<K>(static_cast<T*>(a.dx) + t * a.D + c, o, a.D - c, VEC);
+                if (a.dr) store_pack<K>(static_cast<R*>(a.dr) + t * a.D + c, o, a.D - c, VEC);
             }
         }
     }
@@ -225,61 +244,65 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) bwd_kernel(cons
     }
 }
 
-// out[c] = sum over p of part[p, c], in the order of p within four strands
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int P,
-                                                         int64_t D) {
-    __shared__ float sh[8][33];
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int g = threadIdx.x >> 5;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+// out[c] = sum over p of part[p, c]: 32 strands of rows, then the strands in order
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int P,
+                                                          int D) {
+    __shared__ float sh[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+    float s = 0.0f;
     if (c < D) {
-        int p = g;
-        for (; p + 24 < P; p += 32)
-#pragma unroll
-            for (int j = 0; j < 4; j++) s[j] = __fadd_rn(s[j], part[(int64_t)(p + 8 * j) * D + c]);
-        for (; p < P; p += 8) s[0] = __fadd_rn(s[0], part[(int64_t)p * D + c]);
+#pragma unroll 8
+        for (int p = g; p < P; p += 32) s = __fadd_rn(s, part[(int64_t)p * D + c]);
     }
-    sh[g][threadIdx.x & 31] = __fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3]));
+    sh[g][threadIdx.x & 31] = s;
     __syncthreads();
     if (g == 0 && c < D) {
         float v = sh[0][threadIdx.x];
 #pragma unroll
-        for (int i = 1; i < 8; i++) v = __fadd_rn(v, sh[i][threadIdx.x]);
+        for (int i = 1; i < 32; i++) v = __fadd_rn(v, sh[i][threadIdx.x]);
         out[c] = v;
     }
 }
 
-// Threads of a row: the fewest that hold it in at most 4 packs of 8 (2 of 4
-// for fp32 rows), and a whole CTA's where there are too few rows to fill the
-// GPU with warps.
+constexpr int MAX_D = 16384;  // 512 threads of 4 packs
+
+// Threads of a row: a warp where 4 packs of 8 a thread hold it, 128 or 512
+// where they do not, and 128 too for the few rows of a decode batch, which
+// would leave most of the GPU without a warp.
 static inline int threads_per_row(int T, int D, int K) {
     const int packs = cdiv(D, K);
-    int tpr = 32;
-    while (tpr * 4 < packs) tpr *= 2;
-    while (tpr < 256 && tpr < packs && (int64_t)T * tpr < 148 * 256) tpr *= 2;
-    return tpr;
+    if (packs > 4 * 128) return 512;
+    return packs > 4 * 32 || (packs > 32 && T <= 148 * 4) ? 128 : 32;
 }
 
-constexpr int MAX_D = 16384;  // 512 threads of 4 packs
-constexpr int BWD_CTAS = 148 * 4;
+// two CTAs an SM, as many as the backward pass's registers allow: each keeps its sums of dw to the end
+static inline int grid_of(int T, int D) {
+    const int tpr = threads_per_row(T, D, 8);
+    const int grid = cdiv(T, (tpr > THREADS ? tpr : THREADS) / tpr);
+    return grid < 148 * 2 ? grid : 148 * 2;
+}
 
 template <typename T, typename R, int K, int TPR, bool BWD, bool QUANT>
 static int launch_nv(const Args& a, int grid, int block, cudaStream_t s) {
     const int nv = cdiv(cdiv(a.D, K), TPR);
     const size_t smem = BWD && block > TPR ? sizeof(float) * a.D : 0;
-#define MI_RMS_CASE(NV)                                                                     \
-    do {                                                                                    \
-        if constexpr (BWD)                                                                  \
-            bwd_kernel<T, R, K, NV, TPR><<<grid, block, smem, s>>>(a);                      \
-        else                                                                                \
-            MI_LAUNCH_DEPENDENT(fwd_kernel<T, R, K, NV, TPR, QUANT>, grid, block, 0, s, a); \
+#define MI_RMS_CASE(NV, VEC)                                                                     \
+    do {                                                                                         \
+        if constexpr (BWD)                                                                       \
+            bwd_kernel<T, R, K, NV, TPR, VEC><<<grid, block, smem, s>>>(a);                      \
+        else                                                                                     \
+            MI_LAUNCH_DEPENDENT(fwd_kernel<T, R, K, NV, TPR, VEC, QUANT>, grid, block, 0, s, a); \
     } while (0)
-    if (nv <= 1)
-        MI_RMS_CASE(1);
-    else if (nv <= 2)
-        MI_RMS_CASE(2);
+    if (!a.vec)
+        MI_RMS_CASE(4, false);
+    else if (nv <= 1)
+        MI_RMS_CASE(1, true);
+    else if (nv == 2)
+        MI_RMS_CASE(2, true);
+    else if (nv == 3)
+        MI_RMS_CASE(3, true);
     else
-        MI_RMS_CASE(4);
+        MI_RMS_CASE(4, true);
 #undef MI_RMS_CASE
     MI_CHECK_LAUNCH();
     return MI_OK;
@@ -294,18 +317,9 @@ static int launch(const Args& a, int grid_cap, cudaStream_t s) {
     if (grid_cap && grid > grid_cap) grid = grid_cap;
     switch (tpr) {
         case 32: return launch_nv<T, R, K, 32, BWD, QUANT>(a, grid, block, s);
-        case 64: return launch_nv<T, R, K, 64, BWD, QUANT>(a, grid, block, s);
         case 128: return launch_nv<T, R, K, 128, BWD, QUANT>(a, grid, block, s);
-        case 256: return launch_nv<T, R, K, 256, BWD, QUANT>(a, grid, block, s);
         default: return launch_nv<T, R, K, 512, BWD, QUANT>(a, grid, block, s);
     }
-}
-
-static int grid_of(int T, int D) {
-    const int tpr = threads_per_row(T, D, 8);
-    const int block = tpr > THREADS ? tpr : THREADS;
-    const int grid = cdiv(T, block / tpr);
-    return grid < BWD_CTAS ? grid : BWD_CTAS;
 }
 
 template <bool BWD, bool QUANT>
@@ -389,7 +403,7 @@ extern "C" int mi_rms_norm_backward(const void* dy, const void* dsum, const void
     const int grid = mi::rms::grid_of(T, D);
     const int rc2 = mi::rms::dispatch<true, false>(a, dtype, rdtype, grid, st);
     if (rc2 != MI_OK || !dweight) return rc2;
-    mi::rms::column_sum_kernel<<<mi::cdiv(D, 32), 256, 0, st>>>(a.dw_part, dweight, grid, D);
+    mi::rms::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, st>>>(a.dw_part, dweight, grid, D);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }

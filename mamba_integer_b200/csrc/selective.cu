@@ -1022,40 +1022,71 @@ __global__ void __launch_bounds__(256) sum_params_kernel(const float* __restrict
 
 // ---------------------------------------------------------------------------
 // One new token a stream: the state is read and written once, 8 bytes a state,
-// which bounds it.  LN lanes a channel as above.
-template <typename T, int LN>
+// which bounds it.  LN lanes a channel as above; a thread takes ROWS streams
+// of its channel, so that A and the channel's parameters are read once for
+// them and all their loads are on their way together.  VEC: N is a multiple
+// of 4 and B and C are aligned, so that nothing is loaded behind a branch.
+template <typename T, int LN, int ROWS, bool VEC>
 __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
     const int64_t item = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / LN;
     const int n0 = 4 * (threadIdx.x % LN);
     grid_dependency_sync();
-    const bool live = item < (int64_t)a.batch * a.D;
-    const int d = live ? (int)(item % a.D) : 0, b = live ? (int)(item / a.D) : 0;
-    float* hp = a.hT + ((int64_t)b * a.D + d) * a.N;
-    float y = 0.0f, u = 0.0f;
-    if (live) {
-        const float4 hv = load4(hp, n0, a.N), Av = load4(a.A + (int64_t)d * a.N, n0, a.N);
-        const Pack<T, 4> pB = load_pack<4>(row_of<T>(a.B, b, 0) + n0, a.N - n0, a.B.vec);
-        const Pack<T, 4> pC = load_pack<4>(row_of<T>(a.C, b, 0) + n0, a.N - n0, a.C.vec);
-        u = to_f(row_of<T>(a.u, b, 0)[d]);
-        float dt = to_f(row_of<T>(a.delta, b, 0)[d]);
-        if (a.bias) dt = __fadd_rn(dt, a.bias[d]);
-        if (a.softplus) dt = softplus(dt);
-        const St Bv = st(make_float4(to_f(pB.v[0]), to_f(pB.v[1]), to_f(pB.v[2]), to_f(pB.v[3])));
-        const St Cv = st(make_float4(to_f(pC.v[0]), to_f(pC.v[1]), to_f(pC.v[2]), to_f(pC.v[3])));
-        const St e = exp2s(mul(mul(st(Av), LOG2E), dt));
-        const St h = fma(e, st(hv), mul(Bv, __fmul_rn(dt, u)));
-        store4(hp, n0, a.N, f4(h));
-        y = dot(h, Cv);
-    }
+    const int d = (int)(item % a.D), b0 = (int)(item / a.D) * ROWS;
+    const bool quad_in = n0 < a.N;
+    const int nc = quad_in ? n0 : 0;
+    float4 hv[ROWS], Av;
+    Pack<T, 4> pB[ROWS], pC[ROWS];
+    T tu[ROWS], td[ROWS], tz[ROWS];
+    // streams beyond the last and states beyond the last quad read others' values, and use none
+    Av = VEC ? *reinterpret_cast<const float4*>(a.A + (int64_t)d * a.N + nc) : load4(a.A + (int64_t)d * a.N, n0, a.N);
 #pragma unroll
-    for (int m = 1; m < LN; m *= 2) y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, m));
-    if (live && n0 == 0) {
-        if (a.Dskip) y = __fmaf_rn(a.Dskip[d], u, y);
-        if (a.z.p) {
-            const float z = to_f(row_of<T>(a.z, b, 0)[d]);
-            y = __fmul_rn(y, __fmul_rn(z, sigmoid(z)));
+    for (int r = 0; r < ROWS; r++) {
+        const int b = b0 + r < a.batch ? b0 + r : a.batch - 1;
+        const float* hp = a.hT + ((int64_t)b * a.D + d) * a.N;
+        if (VEC) {
+            hv[r] = *reinterpret_cast<const float4*>(hp + nc);
+            pB[r] = *reinterpret_cast<const Pack<T, 4>*>(row_of<T>(a.B, b, 0) + nc);
+            pC[r] = *reinterpret_cast<const Pack<T, 4>*>(row_of<T>(a.C, b, 0) + nc);
+        } else {
+            hv[r] = load4(hp, n0, a.N);
+            pB[r] = load_pack<4>(row_of<T>(a.B, b, 0) + n0, a.N - n0, a.B.vec);
+            pC[r] = load_pack<4>(row_of<T>(a.C, b, 0) + n0, a.N - n0, a.C.vec);
         }
-        static_cast<T*>(a.y)[(int64_t)b * a.D + d] = from_f<T>(y);
+        tu[r] = row_of<T>(a.u, b, 0)[d];
+        td[r] = row_of<T>(a.delta, b, 0)[d];
+        tz[r] = (a.z.p ? row_of<T>(a.z, b, 0) : row_of<T>(a.u, b, 0))[d];
+    }
+    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
+    if (VEC && !quad_in) {
+        Av = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            hv[r] = Av;
+#pragma unroll
+            for (int i = 0; i < 4; i++) pB[r].v[i] = pC[r].v[i] = from_f<T>(0.0f);
+        }
+    }
+    const St A2 = mul(st(Av), LOG2E);
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+        const int b = b0 + r;
+        const bool live = b < a.batch;
+        const float u = to_f(tu[r]);
+        float t = __fadd_rn(to_f(td[r]), bias);
+        if (a.softplus) t = softplus(t);
+        const St h = fma(exp2s(mul(A2, dup(t))), st(hv[r]), mul(st(quad(pB[r])), dup(__fmul_rn(t, u))));
+        if (live) store4(a.hT + ((int64_t)b * a.D + d) * a.N, n0, a.N, f4(h));
+        float y = dot(h, st(quad(pC[r])));
+#pragma unroll
+        for (int m = 1; m < LN; m *= 2) y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, m));
+        if (live && n0 == 0) {
+            y = __fmaf_rn(skip, u, y);
+            if (a.z.p) {
+                const float z = to_f(tz[r]);
+                y = __fmul_rn(y, __fmul_rn(z, sigmoid(z)));
+            }
+            static_cast<T*>(a.y)[(int64_t)b * a.D + d] = from_f<T>(y);
+        }
     }
 }
 
@@ -1165,11 +1196,19 @@ static int forward(Args& a, float* ws, cudaStream_t s) {
     return MI_OK;
 }
 
+template <typename T, int LN, int ROWS, bool VEC>
+static int step_rows(Args& a, cudaStream_t s) {
+    const int64_t threads = (int64_t)cdiv(a.batch, ROWS) * a.D * LN;
+    MI_LAUNCH_DEPENDENT(step_kernel<T, LN, ROWS, VEC>, (unsigned)((threads + THREADS - 1) / THREADS), THREADS, 0, s, a);
+    return MI_OK;
+}
+
+// 4 streams a thread where that leaves every SM its 1024 threads; 1 elsewhere
 template <typename T, int LN>
 static int step(Args& a, float*, cudaStream_t s) {
-    const int64_t threads = (int64_t)a.batch * a.D * LN;
-    MI_LAUNCH_DEPENDENT(step_kernel<T, LN>, (unsigned)((threads + THREADS - 1) / THREADS), THREADS, 0, s, a);
-    return MI_OK;
+    if (a.N % 4 || !a.B.vec || !a.C.vec) return step_rows<T, LN, 1, false>(a, s);
+    if ((int64_t)a.batch * a.D * LN >= 148 * 1024 * 4) return step_rows<T, LN, 4, true>(a, s);
+    return step_rows<T, LN, 1, true>(a, s);
 }
 
 template <typename T, int LN>
