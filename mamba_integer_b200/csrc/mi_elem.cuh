@@ -68,7 +68,10 @@ __device__ __forceinline__ void cp_async(void* to, const void* from, int src) {
                      : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group 0;\n" ::: "memory"); }
+template <int PENDING = 0>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(PENDING) : "memory");
+}
 
 // Starts the copy of K elements at p, of which `valid` exist, into this
 // thread's own slot; the others become zeros.  `vec`: p is aligned to the pack

@@ -22,6 +22,8 @@
 // Tiles of TT positions by CB channels are staged in shared memory as
 // (dt, dt u); positions from the length on are staged with dt = 0, B = C = 0,
 // where the recurrence leaves the state as it is.
+#include <type_traits>
+
 #include "mi_elem.cuh"
 
 namespace mi {
@@ -115,14 +117,14 @@ __device__ __forceinline__ St exp2s(St x) {
     return {make_float2(exp2_fast(x.a.x), exp2_fast(x.a.y)), make_float2(exp2_fast(x.b.x), exp2_fast(x.b.y))};
 }
 
-// 2^x of two values on the FMA pipe: n = x rounded, 2^x = 2^n 2^r with r = x - n in [-1/2, 1/2] and 2^r = 1 + r q(r), q of
-// degree 5 with the least relative error (2^-27.9, by Remez's exchange).  x below -126 counts as -126, above 128 as 128
-// (inf); a NaN is not kept.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    x = make_float2(fminf(fmaxf(x.x, -126.0f), 128.0f), fminf(fmaxf(x.y, -126.0f), 128.0f));
+// 2^(A dt) of two positions on the FMA pipe: with x = A dt and n = x rounded,
+// 2^x = 2^n 2^r, r = x - n in [-1/2, 1/2], and 2^r = 1 + r q(r), q of degree 5
+// with the least relative error (2^-27.9, by Remez's exchange).  dt is from 0
+// to 126 / |A|, where the decay is 2^-126 and no more than rounding.
+__device__ __forceinline__ float2 exp2_poly(float A, float2 dt) {
     const float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers and leaves them in the low bits
-    const float2 t = __fadd2_rn(x, dup(magic));
-    const float2 r = __fadd2_rn(x, neg(__fadd2_rn(t, dup(-magic))));
+    const float2 t = __ffma2_rn(dup(A), dt, dup(magic));
+    const float2 r = __ffma2_rn(dup(A), dt, __ffma2_rn(t, dup(-1.0f), dup(magic)));
     float2 p = __ffma2_rn(dup(1.5469732170458883e-4f), r, dup(1.3410000829026103e-3f));
     p = __ffma2_rn(p, r, dup(9.618030861020088e-3f));
     p = __ffma2_rn(p, r, dup(5.550297349691391e-2f));
@@ -133,20 +135,23 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
                        __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
 }
 
-// The decays of 4 positions.  One state of a lane's four goes through the FMA
-// pipe, the others through the special-function unit, so that neither waits
-// for the other.  The polynomial is the exacter of the two near 1, where a
-// decay's error adds up over the longest memory; A usually begins with its
-// slowest state, so it is the first of the four.
+// The decays of 4 positions.  With EXACT (step sizes from softplus, which are
+// not negative) one state of a lane's four goes through the FMA pipe, the
+// others through the special-function unit.  The polynomial is the exacter of
+// the two near 1, where a decay's error adds up over the longest memory; A
+// usually begins with its slowest state, so it is the first of the four: dA's
+// error against 64 bits is 6e-7 with it and 1.6e-6 without (8 x 2048 x 1536),
+// and the special-function unit, the slower of the two, has a quarter less to
+// do.  `lim` is 126 / |A| of the first state.
 template <bool EXACT>
-__device__ __forceinline__ void decays(const St& A2, const float (&dt)[4], St (&e)[4]) {
+__device__ __forceinline__ void decays(const St& A2, float lim, const float (&dt)[4], St (&e)[4]) {
     if constexpr (!EXACT) {
 #pragma unroll
         for (int k = 0; k < 4; k++) e[k] = exp2s(mul(A2, dup(dt[k])));
     } else {
 #pragma unroll
         for (int k = 0; k < 4; k += 2) {
-            const float2 p = exp2_poly(__fmul2_rn(dup(A2.a.x), make_float2(dt[k], dt[k + 1])));
+            const float2 p = exp2_poly(A2.a.x, make_float2(fminf(dt[k], lim), fminf(dt[k + 1], lim)));
             e[k].a.x = p.x, e[k + 1].a.x = p.y;
         }
 #pragma unroll
@@ -221,38 +226,49 @@ __device__ __forceinline__ void stage_steps(float4* row, int c, int t, const flo
     for (int k = 0; k < K; k += 2) row[place((c + k) >> 1, t)] = make_float4(dt[k], v[k], dt[k + 1], v[k + 1]);
 }
 
-// A NaN in A, which the polynomial would lose, is put into the state.
-__device__ __forceinline__ St keep_nan(St h, St A) {
-    if (isnan(A.a.x)) h.a.x = A.a.x;
-    return h;
+// A NaN in the A of a lane's first state, which the polynomial would lose, is
+// put into the state; an infinite one becomes a large one.
+__device__ __forceinline__ float limit(St& A2, St& h) {
+    if (isnan(A2.a.x)) h.a.x = A2.a.x;
+    A2.a.x = fminf(fmaxf(A2.a.x, -1e30f), 1e30f);
+    return __fdiv_rn(126.0f, fmaxf(fabsf(A2.a.x), 1e-30f));
 }
 
-template <typename T, int LN>
+// The forward kernels' CTA: 4 warps that carry the recurrence, 4 that stage
+// its tiles and finish its outputs.  CPL: channels a lane.
+constexpr int WORKERS = 128, STAGERS = 128, CTA = WORKERS + STAGERS;
+template <typename T, int LN, int CPL_>
 struct Cfg {
     static constexpr int NP = 4 * LN;                    // padded states
     static constexpr int CL = 32 / LN;                   // channel lanes of a warp
-    static constexpr int CPL = LN == 2 ? 1 : LN == 16 ? 4 : 2;  // channels a lane
-    static constexpr int CB = 4 * CL * CPL;              // channels a CTA: 64 (LN = 2, 4) or 32
-    static constexpr int TT = 8 * THREADS / CB;             // positions a tile: 16 or 32
-    static constexpr int VPR = CB / 8;                   // packs of 8 channels a row
-    static constexpr int QUADS = (TT * LN + THREADS - 1) / THREADS;  // packs of 4 states a thread, of each of B and C
+    static constexpr int CPL = CPL_;
+    static constexpr int CB = 4 * CL * CPL;              // channels a CTA: 64 or 32
+    static constexpr int TT = 1024 / CB, E = TT * CB / STAGERS;  // positions a tile: 16 or 32; a stager's channels
+    static constexpr int VPR = CB / E;                   // stagers a row
+    static constexpr int QUADS = TT * LN;                // packs of 4 states of a tile, of each of B and C
     static constexpr int YS = CB + 8;  // the 4 positions that a step of the loop stores lie in different banks
+    template <bool SCAN>
     struct Smem {
-        float4 sd[TT][CB / 2];  // (dt, dt u) of two channels
-        float B[TT][NP], C[TT][NP];
-        float y[TT][YS];
+        float4 sd[2][TT][CB / 2];  // (dt, dt u) of two channels (chunk_kernel backwards: (dt, ds))
+        float B[2][TT][NP];        // B (C)
+        float C[SCAN ? 2 : 0][TT][NP];
+        float y[SCAN ? 2 : 0][TT][YS];
         float bias[CB], skip[CB];
-        alignas(16) T raw[2][3][THREADS * 8];       // by thread: u, delta and z as they come, of this tile and the next
-        alignas(16) T raw_bc[2][QUADS][THREADS * 4];  // B and C
-    };
-    struct ChunkSmem {
-        float4 sd[TT][CB / 2];  // (dt, dt u) or (dt, ds) of two channels
-        float B[TT][NP];    // B or C
-        float bias[CB];
-        alignas(16) T raw[3][THREADS * 8];  // by thread: delta, u or dy, and z as they come
-        alignas(16) T raw_bc[QUADS][THREADS * 4];
+        // by stager, as they come: u (dy) and z until a tile is finished, the rest until it is staged
+        alignas(16) T raw_u[4][STAGERS * E];
+        alignas(16) T raw_z[4][STAGERS * E];
+        alignas(16) T raw_d[2][STAGERS * E];
+        alignas(16) T raw_bc[2][SCAN ? 2 : 1][QUADS * 4];
     };
 };
+
+// setmaxnreg: the workers' registers come from what the stagers give up.  The
+// launch gives each of the 256 threads 128 (two CTAs an SM), 32768 in all:
+// 128 x 176 + 128 x 80.  Three CTAs with 96 and 64 measured 210 us against 229
+// at 8 x 2048 x 1536, but 62 against 53 for ragged prompts of 6 x 777 x 2048.
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n"); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n"); }
+__device__ __forceinline__ void cta_barrier() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
 
 template <int K, typename T>
 __device__ __forceinline__ Pack<T, K> slot_pack(const T* slot) {
@@ -262,7 +278,7 @@ __device__ __forceinline__ Pack<T, K> slot_pack(const T* slot) {
 // The CTA's channels of a parameter (zeros without one, and beyond the last channel)
 template <int CB>
 __device__ __forceinline__ void stage_param(float (&to)[CB], const float* p, int d0, int D) {
-    for (int c = threadIdx.x; c < CB; c += THREADS) to[c] = p && d0 + c < D ? p[d0 + c] : 0.0f;
+    for (int c = threadIdx.x; c < CB; c += blockDim.x) to[c] = p && d0 + c < D ? p[d0 + c] : 0.0f;
 }
 
 template <int K>
@@ -286,125 +302,207 @@ __device__ __forceinline__ float4 quad(const Pack<T, 4>& p) {
 }
 
 // ---------------------------------------------------------------------------
-// A chunk's own end state, from a zero start (forward: REV = false), or the
-// gradient that a chunk passes to the one before it, from a zero one behind it
-// (REV = true; dy, z and C in the place of u, delta and B), and the sum of its
-// dt.  Only chunks > 1 need it: one more exponential for each state.
-template <typename T, int LN, bool REV>
-__global__ void __launch_bounds__(THREADS, 3) chunk_kernel(const Args a) {
-    using F = Cfg<T, LN>;
-    constexpr int CB = F::CB, TT = F::TT, CPL = F::CPL;
+// What the stagers of a forward kernel do: while the workers are at tile i,
+// tile i + 2's inputs are on their way, tile i + 1 is staged and tile i - 1's
+// outputs are gated and stored.  MODE: SCAN, or a chunk's own end state
+// (CHUNK), or that of the gradient, backwards (RCHUNK: dy, z and C in the
+// place of u, delta's neighbour, and B).
+enum { SCAN, CHUNK, RCHUNK };
+template <typename T, int LN, int CPL, int MODE>
+__device__ __forceinline__ void stagers(const Args& a, typename Cfg<T, LN, CPL>::template Smem<MODE == SCAN>& sm, int d0, int b,
+                                        int tb, int te, int end, int tiles) {
+    using F = Cfg<T, LN, CPL>;
+    constexpr int TT = F::TT, E = F::E, PER = (F::QUADS + STAGERS - 1) / STAGERS;
+    constexpr bool REV = MODE == RCHUNK, GATED = MODE != CHUNK;
+    const int tid = threadIdx.x - WORKERS;
+    const int lt = tid / F::VPR, lc = E * (tid % F::VPR), d = d0 + lc, have = a.D - d;
+    const int first = tb + (REV ? (tiles - 1) * TT : 0), rows = REV ? -TT : TT;
+    const int nq = 4 * (tid % LN), tq = tid / LN;  // this thread's first pack of B and C
+    const Seq &su = REV ? a.dy : a.u, &sB = REV ? a.C : a.B;
+    const T *wu = row_of<T>(su, b, first + lt) + d, *wd = row_of<T>(a.delta, b, first + lt) + d;
+    const T* wz = row_of<T>(a.z, b, first + lt) + d;
+    const T *wB = row_of<T>(sB, b, first + tq) + nq, *wC = row_of<T>(a.C, b, first + tq) + nq;
+    T* yp = MODE == SCAN ? static_cast<T*>(a.y) + ((int64_t)b * a.L + tb + lt) * a.D + d : nullptr;
+    auto load = [&](int i) {
+        if (i < tiles) {
+            const int t0 = first + i * rows, valid = t0 + lt < end ? have : 0;
+            fetch_pack<E>(&sm.raw_u[i & 3][E * tid], wu, su.p, valid, su.vec);
+            fetch_pack<E>(&sm.raw_d[i & 1][E * tid], wd, a.delta.p, valid, a.delta.vec);
+            if (GATED && a.z.p) fetch_pack<E>(&sm.raw_z[i & 3][E * tid], wz, a.z.p, valid, a.z.vec);
+#pragma unroll
+            for (int q = 0; q < PER; q++) {
+                const int e = tid + q * STAGERS, r = tq + q * (STAGERS / LN), valid4 = t0 + r < end ? a.N - nq : 0;
+                if (e >= F::QUADS) break;
+                fetch_pack<4>(&sm.raw_bc[i & 1][0][4 * e], wB + q * (STAGERS / LN) * sB.sl, sB.p, valid4, sB.vec);
+                if (MODE == SCAN)
+                    fetch_pack<4>(&sm.raw_bc[i & 1][MODE == SCAN][4 * e], wC + q * (STAGERS / LN) * a.C.sl, a.C.p, valid4,
+                                  a.C.vec);
+            }
+            wu += rows * su.sl, wd += rows * a.delta.sl, wz += rows * a.z.sl, wB += rows * sB.sl, wC += rows * a.C.sl;
+        }
+        cp_async_commit();
+    };
+    auto stage = [&](int i) {
+        float dt[E], v[E];
+        if (first + i * rows + lt < end) {
+            const Pack<T, E> pu = slot_pack<E>(&sm.raw_u[i & 3][E * tid]), pd = slot_pack<E>(&sm.raw_d[i & 1][E * tid]);
+            getk<E>(&sm.bias[lc], dt);
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                dt[k] = __fadd_rn(to_f(pd.v[k]), dt[k]);
+                if (a.softplus) dt[k] = softplus(dt[k]);
+                v[k] = to_f(pu.v[k]);
+                if (!REV) v[k] = __fmul_rn(dt[k], v[k]);
+            }
+            if (REV && a.z.p) {
+                const Pack<T, E> pz = slot_pack<E>(&sm.raw_z[i & 3][E * tid]);
+#pragma unroll
+                for (int k = 0; k < E; k++) {
+                    const float z = to_f(pz.v[k]);
+                    v[k] = __fmul_rn(v[k], __fmul_rn(z, sigmoid(z)));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < E; k++) dt[k] = v[k] = 0.0f;
+        }
+        stage_steps<E>(sm.sd[i & 1][lt], lc, lt, dt, v);
+#pragma unroll
+        for (int q = 0; q < PER; q++) {
+            const int e = tid + q * STAGERS, r = tq + q * (STAGERS / LN);
+            if (e >= F::QUADS) break;
+            *reinterpret_cast<float4*>(&sm.B[i & 1][r][nq]) = quad(slot_pack<4>(&sm.raw_bc[i & 1][0][4 * e]));
+            if (MODE == SCAN)
+                *reinterpret_cast<float4*>(&sm.C[i & 1][r][nq]) = quad(slot_pack<4>(&sm.raw_bc[i & 1][MODE == SCAN][4 * e]));
+        }
+    };
+    auto finish = [&](int i) {
+        const int t = tb + i * TT + lt;
+        if (t < te && have > 0) {
+            float o[E];
+            getk<E>(&sm.y[i & 1][lt][lc], o);
+            if (a.Dskip) {
+                const Pack<T, E> eu = slot_pack<E>(&sm.raw_u[i & 3][E * tid]);
+                float skip[E];
+                getk<E>(&sm.skip[lc], skip);
+#pragma unroll
+                for (int k = 0; k < E; k++) o[k] = __fmaf_rn(skip[k], to_f(eu.v[k]), o[k]);
+            }
+            if (a.z.p) {
+                const Pack<T, E> ez = slot_pack<E>(&sm.raw_z[i & 3][E * tid]);
+#pragma unroll
+                for (int k = 0; k < E; k++) {
+                    const float z = to_f(ez.v[k]);
+                    o[k] = __fmul_rn(o[k], __fmul_rn(z, sigmoid(z)));
+                }
+            }
+            if (t >= end) {
+#pragma unroll
+                for (int k = 0; k < E; k++) o[k] = 0.0f;
+            }
+            store_pack<E>(yp, o, have, a.ovec);
+        }
+        yp += (int64_t)TT * a.D;
+    };
+    load(0), load(1);
+    cp_async_wait<1>();
+    if (tiles > 0) stage(0);
+    cta_barrier();
+#pragma unroll 1
+    for (int i = 0; i < tiles; i++) {
+        load(i + 2);
+        if (MODE == SCAN && i > 0) finish(i - 1);
+        cp_async_wait<1>();
+        if (i + 1 < tiles) stage(i + 1);
+        cta_barrier();
+    }
+    if (MODE == SCAN) {
+        if (tiles > 0) finish(tiles - 1);
+        if (have > 0) {  // behind the length
+            float zero[E];
+#pragma unroll
+            for (int k = 0; k < E; k++) zero[k] = 0.0f;
+            for (int t = tb + tiles * TT + lt; t < te; t += TT, yp += (int64_t)TT * a.D)
+                store_pack<E>(yp, zero, have, a.ovec);
+        }
+    }
+}
+
+// A chunk's own end state, from a zero start (REV = false), or the gradient
+// that a chunk passes to the one before it, from a zero one behind it (REV =
+// true; dy, z and C in the place of u, delta and B), and the sum of its dt.
+// Only chunks > 1 need it: one more exponential for each state.
+template <typename T, int LN, int CPL, bool REV>
+__global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
+    using F = Cfg<T, LN, CPL>;
+    constexpr int CB = F::CB, TT = F::TT;
+    using Smem = typename F::template Smem<false>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    typename F::ChunkSmem& sm = *reinterpret_cast<typename F::ChunkSmem*>(smem_raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int d0 = blockIdx.x * CB, b = blockIdx.y, ck = blockIdx.z + (REV ? 1 : 0);
     const int len = length_of(a, b);
     const int tb = ck * a.span, te = tb + a.span < a.L ? tb + a.span : a.L;
     const int end = te < len ? te : len;  // past it nothing changes the state
     const int tiles = end > tb ? cdiv(end - tb, TT) : 0;
-    const int lt = tid / F::VPR, lv = tid % F::VPR, d = d0 + 8 * lv;
-    const int first = tb + (REV ? (tiles - 1) * TT : 0), rows = REV ? -TT : TT;
-    const Seq &su = REV ? a.dy : a.u, &sB = REV ? a.C : a.B;
-    const int have = a.D - d;
-    const int nq = 4 * (tid % LN), tq = tid / LN;
     stage_param(sm.bias, a.bias, d0, a.D);
     __syncthreads();
-    const T *wd = row_of<T>(a.delta, b, first + lt) + d, *wu = row_of<T>(su, b, first + lt) + d;
-    const T *wz = row_of<T>(a.z, b, first + lt) + d, *wB = row_of<T>(sB, b, first + tq) + nq;
-    auto load = [&](int i) {
-        const int t0 = first + i * rows, valid = t0 + lt < end ? have : 0;
-        fetch_pack<8>(&sm.raw[0][8 * tid], wd, a.delta.p, valid, a.delta.vec);
-        fetch_pack<8>(&sm.raw[1][8 * tid], wu, su.p, valid, su.vec);
-        if (REV && a.z.p) fetch_pack<8>(&sm.raw[2][8 * tid], wz, a.z.p, valid, a.z.vec);
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++) {
-            const int r = tq + q * (THREADS / LN);
-            if (r < TT)
-                fetch_pack<4>(&sm.raw_bc[q][4 * tid], wB + q * (THREADS / LN) * sB.sl, sB.p, t0 + r < end ? a.N - nq : 0,
-                              sB.vec);
-        }
-        cp_async_commit();
-        wd += rows * a.delta.sl, wu += rows * su.sl, wz += rows * a.z.sl, wB += rows * sB.sl;
-    };
-    auto stage = [&](int i) {
-        cp_async_wait();
-        if (first + i * rows + lt < end) {
-            const Pack<T, 8> pd = slot_pack<8>(&sm.raw[0][8 * tid]), pu = slot_pack<8>(&sm.raw[1][8 * tid]);
-            Pack<T, 8> pz;
-            if (REV && a.z.p) pz = slot_pack<8>(&sm.raw[2][8 * tid]);
-            float dt[8];
-            getk<8>(&sm.bias[8 * lv], dt);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                dt[k] = __fadd_rn(to_f(pd.v[k]), dt[k]);
-                if (a.softplus) dt[k] = softplus(dt[k]);
-            }
-            float v[8];
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                v[k] = to_f(pu.v[k]);
-                if (!REV)
-                    v[k] = __fmul_rn(dt[k], v[k]);
-                else if (a.z.p) {
-                    const float z = to_f(pz.v[k]);
-                    v[k] = __fmul_rn(v[k], __fmul_rn(z, sigmoid(z)));
-                }
-            }
-            stage_steps<8>(sm.sd[lt], 8 * lv, lt, dt, v);
-        } else {
-            const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-            stage_steps<8>(sm.sd[lt], 8 * lv, lt, zero, zero);
-        }
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++)
-            if (tq + q * (THREADS / LN) < TT)
-                *reinterpret_cast<float4*>(&sm.B[tq + q * (THREADS / LN)][nq]) = quad(slot_pack<4>(&sm.raw_bc[q][4 * tid]));
-    };
+    if (threadIdx.x >= WORKERS) {
+        give_registers();
+        stagers<T, LN, CPL, REV ? RCHUNK : CHUNK>(a, sm, d0, b, tb, te, end, tiles);
+        return;
+    }
+    take_registers();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
-    int ch[CPL];
+    const int c0 = warp * F::CL * CPL + cl * CPL;
     St A2[CPL], h[CPL];
-    float sum[CPL];
+    float sum[CPL], lim[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
-        ch[j] = warp * F::CL * CPL + cl * CPL + j;
-        const int c = d0 + ch[j];
+        const int c = d0 + c0 + j;
         A2[j] = mul(st(c < a.D ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
-        h[j] = keep_nan(st(make_float4(0, 0, 0, 0)), A2[j]);
+        h[j] = st(make_float4(0, 0, 0, 0));
+        lim[j] = limit(A2[j], h[j]);
         sum[j] = 0.0f;
     }
-    if (tiles > 0) load(0);
-    for (int i = 0; i < tiles; i++) {
-        stage(i);
-        __syncthreads();
-        if (i + 1 < tiles) load(i + 1);
+    auto run = [&](auto exact) {
+#pragma unroll 1
+        for (int i = 0; i < tiles; i++) {
+            const int buf = i & 1;
 #pragma unroll 2
-        for (int q4 = 0; q4 < TT; q4 += 4) {
-            const int r4 = REV ? TT - 4 - q4 : q4;
-            St m[4];
-            float dt[4][CPL], v[4][CPL];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                m[k] = st(*reinterpret_cast<const float4*>(&sm.B[r4 + k][n0]));
-                staged<CPL>(sm.sd[r4 + k], ch[0], k, dt[k], v[k]);
-            }
-#pragma unroll
-            for (int j = 0; j < CPL; j++) {
-                const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
-                St e[4];
-                decays<true>(A2[j], dj, e);
-                sum[j] = __fadd_rn(sum[j], __fadd_rn(__fadd_rn(dj[0], dj[1]), __fadd_rn(dj[2], dj[3])));
+            for (int q4 = 0; q4 < TT; q4 += 4) {
+                const int r4 = REV ? TT - 4 - q4 : q4;
+                St m[4];
+                float dt[4][CPL], v[4][CPL];
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    const int r = REV ? 3 - k : k;
-                    h[j] = REV ? mul(e[r], fma(m[r], dup(v[r][j]), h[j])) : fma(e[r], h[j], mul(m[r], dup(v[r][j])));
+                    m[k] = st(*reinterpret_cast<const float4*>(&sm.B[buf][r4 + k][n0]));
+                    staged<CPL>(sm.sd[buf][r4 + k], c0, k, dt[k], v[k]);
+                }
+#pragma unroll
+                for (int j = 0; j < CPL; j++) {
+                    const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                    St e[4];
+                    decays<decltype(exact)::value>(A2[j], lim[j], dj, e);
+                    sum[j] = __fadd_rn(sum[j], __fadd_rn(__fadd_rn(dj[0], dj[1]), __fadd_rn(dj[2], dj[3])));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int r = REV ? 3 - k : k;
+                        h[j] = REV ? mul(e[r], fma(m[r], dup(v[r][j]), h[j])) : fma(e[r], h[j], mul(m[r], dup(v[r][j])));
+                    }
                 }
             }
+            cta_barrier();
         }
-        __syncthreads();
-    }
+    };
+    cta_barrier();
+    if (a.softplus)
+        run(std::true_type());
+    else
+        run(std::false_type());
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
-        const int c = d0 + ch[j];
+        const int c = d0 + c0 + j;
         if (c >= a.D) continue;
         const int64_t row = ((int64_t)b * a.chunks + ck) * a.D + c;
         *reinterpret_cast<float4*>(a.cst + row * F::NP + n0) = f4(h[j]);
@@ -439,106 +537,36 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// The scan of one chunk (the whole sequence with chunks = 1).  A tile's loads
-// are issued before the tile in front of it is worked on, and wait in
-// registers; its outputs are gated and stored while the next one is staged.
-template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS, 3) scan_kernel(const Args a) {
-    using F = Cfg<T, LN>;
-    constexpr int NP = F::NP, CB = F::CB, TT = F::TT, CPL = F::CPL;
+// The scan of one chunk (the whole sequence with chunks = 1).
+template <typename T, int LN, int CPL>
+__global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
+    using F = Cfg<T, LN, CPL>;
+    constexpr int NP = F::NP, CB = F::CB, TT = F::TT;
+    using Smem = typename F::template Smem<true>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
-    typename F::Smem& sm = *reinterpret_cast<typename F::Smem*>(smem_raw);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
     const int d0 = blockIdx.x * CB, b = blockIdx.y, ck = blockIdx.z;
     const int len = length_of(a, b);
     const int tb = ck * a.span, te = tb + a.span < a.L ? tb + a.span : a.L;
     const int end = te < len ? te : len;
     const int tiles = end > tb ? cdiv(end - tb, TT) : 0;  // tiles behind the length only get their zeros
-    const int lt = tid / F::VPR, lv = tid % F::VPR, d = d0 + 8 * lv;
-    T* yp = static_cast<T*>(a.y) + ((int64_t)b * a.L + tb + lt) * a.D + d;
-    const int have = a.D - d;
-    const int nq = 4 * (tid % LN), tq = tid / LN;
-    const T *wu = row_of<T>(a.u, b, tb + lt) + d, *wd = row_of<T>(a.delta, b, tb + lt) + d;
-    const T *wz = row_of<T>(a.z, b, tb + lt) + d;
-    const T *wB = row_of<T>(a.B, b, tb + tq) + nq, *wC = row_of<T>(a.C, b, tb + tq) + nq;
     stage_param(sm.bias, a.bias, d0, a.D);
     stage_param(sm.skip, a.Dskip, d0, a.D);
     __syncthreads();
-    auto load = [&](int i) {
-        const int t0 = tb + i * TT, valid = t0 + lt < end ? have : 0;
-        fetch_pack<8>(&sm.raw[i & 1][0][8 * tid], wu, a.u.p, valid, a.u.vec);
-        fetch_pack<8>(&sm.raw[i & 1][1][8 * tid], wd, a.delta.p, valid, a.delta.vec);
-        if (a.z.p) fetch_pack<8>(&sm.raw[i & 1][2][8 * tid], wz, a.z.p, valid, a.z.vec);
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++) {
-            const int r = tq + q * (THREADS / LN), valid4 = t0 + r < end ? a.N - nq : 0;
-            if (r >= TT) break;
-            fetch_pack<4>(&sm.raw_bc[0][q][4 * tid], wB + q * (THREADS / LN) * a.B.sl, a.B.p, valid4, a.B.vec);
-            fetch_pack<4>(&sm.raw_bc[1][q][4 * tid], wC + q * (THREADS / LN) * a.C.sl, a.C.p, valid4, a.C.vec);
-        }
-        cp_async_commit();
-        wu += TT * a.u.sl, wd += TT * a.delta.sl, wz += TT * a.z.sl, wB += TT * a.B.sl, wC += TT * a.C.sl;
-    };
-    auto stage = [&](int i) {
-        cp_async_wait();
-        float dt[8], v[8];
-        if (tb + i * TT + lt < end) {
-            const Pack<T, 8> pu = slot_pack<8>(&sm.raw[i & 1][0][8 * tid]), pd = slot_pack<8>(&sm.raw[i & 1][1][8 * tid]);
-            getk<8>(&sm.bias[8 * lv], dt);
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                dt[k] = __fadd_rn(to_f(pd.v[k]), dt[k]);
-                if (a.softplus) dt[k] = softplus(dt[k]);
-                v[k] = __fmul_rn(dt[k], to_f(pu.v[k]));
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++) dt[k] = v[k] = 0.0f;
-        }
-        stage_steps<8>(sm.sd[lt], 8 * lv, lt, dt, v);
-#pragma unroll
-        for (int q = 0; q < F::QUADS; q++) {
-            const int r = tq + q * (THREADS / LN);
-            if (r >= TT) break;
-            *reinterpret_cast<float4*>(&sm.B[r][nq]) = quad(slot_pack<4>(&sm.raw_bc[0][q][4 * tid]));
-            *reinterpret_cast<float4*>(&sm.C[r][nq]) = quad(slot_pack<4>(&sm.raw_bc[1][q][4 * tid]));
-        }
-    };
-    auto finish = [&](int i) {
-        const int t = tb + i * TT + lt;
-        if (t < te && d < a.D) {
-            float o[8];
-            getk<8>(&sm.y[lt][8 * lv], o);
-            if (a.Dskip) {
-                const Pack<T, 8> eu = slot_pack<8>(&sm.raw[i & 1][0][8 * tid]);
-                float skip[8];
-                getk<8>(&sm.skip[8 * lv], skip);
-#pragma unroll
-                for (int k = 0; k < 8; k++) o[k] = __fmaf_rn(skip[k], to_f(eu.v[k]), o[k]);
-            }
-            if (a.z.p) {
-                const Pack<T, 8> ez = slot_pack<8>(&sm.raw[i & 1][2][8 * tid]);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float z = to_f(ez.v[k]);
-                    o[k] = __fmul_rn(o[k], __fmul_rn(z, sigmoid(z)));
-                }
-            }
-            if (t >= end) {
-#pragma unroll
-                for (int k = 0; k < 8; k++) o[k] = 0.0f;
-            }
-            store_pack<8>(yp, o, a.D - d, a.ovec);
-        }
-        yp += (int64_t)TT * a.D;
-    };
+    if (threadIdx.x >= WORKERS) {
+        give_registers();
+        stagers<T, LN, CPL, SCAN>(a, sm, d0, b, tb, te, end, tiles);
+        return;
+    }
+    take_registers();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
-    int ch[CPL];
+    const int c0 = warp * F::CL * CPL + cl * CPL;
     St A2[CPL], h[CPL];
+    float lim[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
-        ch[j] = warp * F::CL * CPL + cl * CPL + j;
-        const int c = d0 + ch[j];
+        const int c = d0 + c0 + j;
         const bool in = c < a.D;
         A2[j] = mul(st(in ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
         float4 v = make_float4(0, 0, 0, 0);
@@ -546,71 +574,70 @@ __global__ void __launch_bounds__(THREADS, 3) scan_kernel(const Args a) {
             v = *reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + c) * NP + n0);
         else if (in && a.h0)
             v = load4(a.h0 + ((int64_t)b * a.D + c) * a.N, n0, a.N);
-        h[j] = tiles > 0 ? keep_nan(st(v), A2[j]) : st(v);
+        h[j] = st(v);
+        St none = h[j];
+        lim[j] = limit(A2[j], tiles > 0 ? h[j] : none);
     }
-    float* keep = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK) * a.D + d0 + ch[0]) * NP + n0;
-    if (tiles > 0) load(0);
-    for (int i = 0; i < tiles; i++) {
-        const int t0 = tb + i * TT;
-        if (i > 0) finish(i - 1);
-        stage(i);
-        __syncthreads();
-        if (i + 1 < tiles) load(i + 1);
+    float* keep = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK) * a.D + d0 + c0) * NP + n0;
+    auto run = [&](auto exact) {
 #pragma unroll 1
-        for (int r16 = 0; r16 < TT; r16 += CK) {
-            if (a.ckpt && t0 + r16 < a.L) {
+        for (int i = 0; i < tiles; i++) {
+            const int buf = i & 1, t0 = tb + i * TT;
+#pragma unroll 1
+            for (int r16 = 0; r16 < TT; r16 += CK) {
+                if (a.ckpt && t0 + r16 < a.L) {
 #pragma unroll
-                for (int j = 0; j < CPL; j++)
-                    if (d0 + ch[j] < a.D) *reinterpret_cast<float4*>(keep + j * NP) = f4(h[j]);
-                keep += (int64_t)a.D * NP;
-            }
-            // 16 positions without a store in between, which would hold back the loads behind it
-            constexpr int KEEP = LN == 2 ? 2 : 1;
-            float out[CPL][4][KEEP];
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int r4 = r16 + 4 * g;
-                St Bv[4], Cv[4];
-                float dt[4][CPL], v[4][CPL];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[r4 + k][n0]));
-                    Cv[k] = st(*reinterpret_cast<const float4*>(&sm.C[r4 + k][n0]));
-                    staged<CPL>(sm.sd[r4 + k], ch[0], k, dt[k], v[k]);
+                    for (int j = 0; j < CPL; j++)
+                        if (d0 + c0 + j < a.D) *reinterpret_cast<float4*>(keep + j * NP) = f4(h[j]);
+                    keep += (int64_t)a.D * NP;
                 }
+                // 16 positions without a store in between, which would hold back the loads behind it
+                constexpr int KEEP = LN == 2 ? 2 : 1;
+                float out[CPL][4][KEEP];
 #pragma unroll
-                for (int j = 0; j < CPL; j++) {
-                    const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
-                    St e[4];
-                    float y[4];
-                    decays<true>(A2[j], dj, e);
+                for (int g = 0; g < 4; g++) {
+                    const int r4 = r16 + 4 * g;
+                    St Bv[4], Cv[4];
+                    float dt[4][CPL], v[4][CPL];
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
-                        y[k] = dot(h[j], Cv[k]);
+                        Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[buf][r4 + k][n0]));
+                        Cv[k] = st(*reinterpret_cast<const float4*>(&sm.C[buf][r4 + k][n0]));
+                        staged<CPL>(sm.sd[buf][r4 + k], c0, k, dt[k], v[k]);
                     }
-                    over_states<LN>(y);
 #pragma unroll
-                    for (int m = 0; m < KEEP; m++) out[j][g][m] = y[m];
+                    for (int j = 0; j < CPL; j++) {
+                        const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
+                        St e[4];
+                        float y[4];
+                        decays<decltype(exact)::value>(A2[j], lim[j], dj, e);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
+                            y[k] = dot(h[j], Cv[k]);
+                        }
+                        over_states<LN>(y);
+#pragma unroll
+                        for (int m = 0; m < KEEP; m++) out[j][g][m] = y[m];
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < CPL; j++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) store_positions<LN, F::YS>(&sm.y[buf][r16 + 4 * g][c0 + j], out[j][g], nl);
             }
-#pragma unroll
-            for (int j = 0; j < CPL; j++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) store_positions<LN, F::YS>(&sm.y[r16 + 4 * g][ch[j]], out[j][g], nl);
+            cta_barrier();
         }
-        __syncthreads();
-    }
-    if (tiles > 0) finish(tiles - 1);
-    if (d < a.D) {
-        const float zero[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        for (int t = tb + tiles * TT + lt; t < te; t += TT, yp += (int64_t)TT * a.D)
-            store_pack<8>(yp, zero, a.D - d, a.ovec);
-    }
+    };
+    cta_barrier();
+    if (a.softplus)
+        run(std::true_type());
+    else
+        run(std::false_type());
     if (a.hT && ck == a.chunks - 1) {
 #pragma unroll
         for (int j = 0; j < CPL; j++)
-            if (d0 + ch[j] < a.D) store4(a.hT + ((int64_t)b * a.D + d0 + ch[j]) * a.N, n0, a.N, f4(h[j]));
+            if (d0 + c0 + j < a.D) store4(a.hT + ((int64_t)b * a.D + d0 + c0 + j) * a.N, n0, a.N, f4(h[j]));
     }
 }
 
@@ -664,7 +691,7 @@ __device__ __forceinline__ float take(float keep, float send, int mask) {
 }
 
 template <typename T, int LN>
-__global__ void __launch_bounds__(THREADS, 3) bwd_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
     using F = BCfg<T, LN>;
     constexpr int NP = F::NP, CB = F::CB, CPL = F::CPL, TT = F::TT, CL = F::CL, PERMS = F::PERMS, E = F::E;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -822,7 +849,7 @@ __global__ void __launch_bounds__(THREADS, 3) bwd_kernel(const Args a) {
                 for (int j = 0; j < CPL; j++) {
                     const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                     St e[4];
-                    decays<false>(A2[j], dj, e);
+                    decays<false>(A2[j], 0.0f, dj, e);
 #pragma unroll
                     for (int k = 0; k < 4; k++) h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
                     mid[q][j] = h[j];
@@ -850,7 +877,7 @@ __global__ void __launch_bounds__(THREADS, 3) bwd_kernel(const Args a) {
                 const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                 const St h0 = q ? st(sm.mid[warp][j][q ? q - 1 : 0][lane]) : permute<PERMS>(st(sm.kept[j][tid]), perm);
                 St e[4], h[4];
-                decays<false>(A2[j], dj, e);
+                decays<false>(A2[j], 0.0f, dj, e);
 #pragma unroll
                 for (int k = 0; k < 4; k++) h[k] = fma(e[k], k ? h[k ? k - 1 : 0] : h0, mul(Bv[k], dup(v[k][j])));
 #pragma unroll
@@ -1093,27 +1120,56 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 static inline int lanes_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
-static inline int fwd_channels(int N) { return lanes_of(N) <= 4 ? Cfg<float, 4>::CB : Cfg<float, 8>::CB; }
 static inline int bwd_channels(int N) { return lanes_of(N) <= 4 ? BCfg<float, 4>::CB : BCfg<float, 8>::CB; }
-static_assert(Cfg<float, 2>::CB == Cfg<float, 4>::CB && Cfg<float, 8>::CB == Cfg<float, 16>::CB, "fwd_channels");
 static_assert(BCfg<float, 2>::CB == BCfg<float, 4>::CB && BCfg<float, 8>::CB == BCfg<float, 16>::CB, "bwd_channels");
 
-// Chunks of the sequence: one where the channels alone give every SM 2 CTAs;
-// else as many as bring it there, of 64 positions at least (a chunked scan
-// makes each exponential twice).
+// Channels a lane of the forward kernels.  Two share their loads of B and C,
+// but make CTAs of 64 channels: with fewer than 4 of those an SM, the SMs with
+// one more than the others cost more than the loads.
+static inline int fwd_cpl(int batch, int D, int N) {
+    const int LN = lanes_of(N);
+    if (LN == 4) return (int64_t)batch * cdiv(D, 64) >= 148 * 4 ? 2 : 1;
+    return LN == 2 ? 1 : LN == 8 ? 2 : 4;
+}
+static inline int fwd_channels(int batch, int D, int N) { return 4 * (32 / lanes_of(N)) * fwd_cpl(batch, D, N); }
+
+// Chunks of the sequence, of 64 positions at least.  The chunks' states cost a
+// pass of their own over all but one of them, which makes each exponential
+// once more.
 struct Plan {
     int chunks, span;
 };
-static inline Plan plan_of(int batch, int L, int D, int channels) {
-    const int64_t ctas = (int64_t)batch * cdiv(D, channels);
+static inline Plan plan_of(int L, int64_t n) {
     Plan p = {1, cdiv(L, 32) * 32};
-    const int64_t want = 148 * 2;
-    if (ctas >= want || L < 128) return p;
-    int64_t n = (want + ctas - 1) / ctas;
-    if (n > L / 64) n = L / 64;
+    if (n * 64 > L) n = L / 64;
+    if (n < 2) return p;
     p.span = cdiv(cdiv(L, (int)n), 32) * 32;
     p.chunks = cdiv(L, p.span);
     return p;
+}
+// Forward: only where the channels alone leave SMs idle, and then as many as
+// bring 2 CTAs to each.  With 384 CTAs (8 x 2048 x 1536) one chunk took 229 us,
+// three 194 and 104 for their states; with 48 (one sequence of it) one took
+// 157, six 28 and 20.
+static inline Plan forward_plan(int batch, int L, int D, int N) {
+    const int64_t ctas = (int64_t)batch * cdiv(D, fwd_channels(batch, D, N));
+    return plan_of(L, ctas >= 148 || ctas == 0 ? 1 : 2 * 148 / ctas);
+}
+// Backward: 2 CTAs an SM at once, in rounds of 296 that take as long for one
+// CTA on an SM as for two.  The number of least rounds / chunks +
+// (chunks - 1) / 4 chunks, a quarter being what the pass for all chunks'
+// states takes of the kernel's time: 8 x 2048 x 1536, 192 CTAs, 923 us in one
+// chunk and 617 in three, with 104 for their states.
+static inline Plan backward_plan(int batch, int L, int D, int N) {
+    const int64_t ctas = (int64_t)batch * cdiv(D, bwd_channels(N));
+    Plan best = {1, cdiv(L, 32) * 32};
+    double least = 1e30;
+    for (int n = 1; n <= 16 && (n == 1 || n * 64 <= L); n++) {
+        const Plan p = plan_of(L, n);
+        const double cost = (double)((ctas * p.chunks + 295) / 296) * p.span / L + 0.25 * (p.chunks - 1) / p.chunks;
+        if (cost < least) least = cost, best = p;
+    }
+    return best;
 }
 
 static inline int64_t align16(int64_t floats) { return (floats + 3) & ~(int64_t)3; }
@@ -1123,7 +1179,7 @@ struct Ws {  // floats from the workspace's start
 };
 static inline Ws ws_of(int batch, int L, int D, int N, bool backward) {
     const int LN = lanes_of(N), NP = 4 * LN;
-    const Plan p = plan_of(batch, L, D, backward ? bwd_channels(N) : fwd_channels(N));
+    const Plan p = backward ? backward_plan(batch, L, D, N) : forward_plan(batch, L, D, N);
     Ws w = {};
     int64_t at = 0;
     auto take = [&](int64_t n) {
@@ -1165,12 +1221,12 @@ static bool allow_smem(K* kernel, size_t bytes) {
 }
 
 // the chunks' starting states (REV: what they receive from behind), in a.cst
-template <typename T, int LN, bool REV>
+template <typename T, int LN, int CPL, bool REV>
 static int start_chunks(const Args& a, cudaStream_t s) {
-    using F = Cfg<T, LN>;
-    constexpr size_t smem = sizeof(typename F::ChunkSmem);
-    if (!allow_smem(chunk_kernel<T, LN, REV>, smem)) return MI_ERR_CUDA;
-    chunk_kernel<T, LN, REV><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), THREADS, smem, s>>>(a);
+    using F = Cfg<T, LN, CPL>;
+    constexpr size_t smem = sizeof(typename F::template Smem<false>);
+    if (!allow_smem(chunk_kernel<T, LN, CPL, REV>, smem)) return MI_ERR_CUDA;
+    chunk_kernel<T, LN, CPL, REV><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     const int64_t items = (int64_t)a.batch * a.D * LN;
     join_kernel<LN, REV><<<(unsigned)((items + THREADS - 1) / THREADS), THREADS, 0, s>>>(a);
@@ -1178,22 +1234,32 @@ static int start_chunks(const Args& a, cudaStream_t s) {
     return MI_OK;
 }
 
-template <typename T, int LN>
-static int forward(Args& a, float* ws, cudaStream_t s) {
-    using F = Cfg<T, LN>;
-    const Plan p = plan_of(a.batch, a.L, a.D, F::CB);
+template <typename T, int LN, int CPL>
+static int forward_cpl(Args& a, float* ws, cudaStream_t s) {
+    using F = Cfg<T, LN, CPL>;
+    const Plan p = forward_plan(a.batch, a.L, a.D, a.N);
     a.chunks = p.chunks, a.span = p.span;
     if (p.chunks > 1) {
         const Ws w = ws_of(a.batch, a.L, a.D, a.N, false);
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, false>(a, s);
+        const int rc = start_chunks<T, LN, CPL, false>(a, s);
         if (rc != MI_OK) return rc;
     }
-    constexpr size_t smem = sizeof(typename F::Smem);
-    if (!allow_smem(scan_kernel<T, LN>, smem)) return MI_ERR_CUDA;
-    scan_kernel<T, LN><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
+    constexpr size_t smem = sizeof(typename F::template Smem<true>);
+    if (!allow_smem(scan_kernel<T, LN, CPL>, smem)) return MI_ERR_CUDA;
+    scan_kernel<T, LN, CPL><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
+}
+
+template <typename T, int LN>
+static int forward(Args& a, float* ws, cudaStream_t s) {
+    if constexpr (LN == 4) {
+        if (fwd_cpl(a.batch, a.D, a.N) == 2) return forward_cpl<T, 4, 2>(a, ws, s);
+        return forward_cpl<T, 4, 1>(a, ws, s);
+    } else {
+        return forward_cpl<T, LN, LN == 2 ? 1 : LN == 8 ? 2 : 4>(a, ws, s);
+    }
 }
 
 template <typename T, int LN, int ROWS, bool VEC>
@@ -1214,13 +1280,13 @@ static int step(Args& a, float*, cudaStream_t s) {
 template <typename T, int LN>
 static int backward(Args& a, float* ws, cudaStream_t s) {
     using F = BCfg<T, LN>;
-    const Plan p = plan_of(a.batch, a.L, a.D, F::CB);
+    const Plan p = backward_plan(a.batch, a.L, a.D, a.N);
     a.chunks = p.chunks, a.span = p.span;
     const Ws w = ws_of(a.batch, a.L, a.D, a.N, true);
     a.part_bc = ws + w.part_bc, a.part_a = ws + w.part_a, a.part_d = ws + w.part_d;
     if (p.chunks > 1) {
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, true>(a, s);
+        const int rc = start_chunks<T, LN, LN == 2 ? 1 : LN == 16 ? 4 : LN == 8 ? 2 : 1, true>(a, s);
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::Smem);
