@@ -88,11 +88,14 @@ __device__ __forceinline__ void load_w(const Args& a, int c, float (&w)[W][K], f
 // beyond the last read the row's first ones; nothing comes of them.
 template <bool VEC, int K, typename T>
 __device__ __forceinline__ Pack<T, K> raw_row(const T* p, int have) {
-    if (VEC) return *reinterpret_cast<const Pack<T, K>*>(p);
-    Pack<T, K> r;
+    if constexpr (VEC) {
+        return *reinterpret_cast<const Pack<T, K>*>(p);
+    } else {
+        Pack<T, K> r;
 #pragma unroll
-    for (int i = 0; i < K; i++) r.v[i] = p[i < have ? i : 0];
-    return r;
+        for (int i = 0; i < K; i++) r.v[i] = p[i < have ? i : 0];
+        return r;
+    }
 }
 
 // The W - 1 inputs in front of position t0 (a run's first)

@@ -22,6 +22,7 @@
 // Tiles of TT positions by CB channels are staged in shared memory as
 // (dt, dt u); positions from the length on are staged with dt = 0, B = C = 0,
 // where the recurrence leaves the state as it is.
+#include <atomic>
 #include <type_traits>
 
 #include "mi_elem.cuh"
@@ -119,8 +120,8 @@ __device__ __forceinline__ St exp2s(St x) {
 
 // 2^(A dt) of two positions on the FMA pipe: with x = A dt and n = x rounded,
 // 2^x = 2^n 2^r, r = x - n in [-1/2, 1/2], and 2^r = 1 + r q(r), q of degree 5
-// with the least relative error (2^-27.9, by Remez's exchange).  dt is from 0
-// to 126 / |A|, where the decay is 2^-126 and no more than rounding.
+// with the least relative error (2^-27.9, by Remez's exchange).  |dt| is at
+// most 126 / |A|, where the decay is 2^-126 and no more than rounding.
 __device__ __forceinline__ float2 exp2_poly(float A, float2 dt) {
     const float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers and leaves them in the low bits
     const float2 t = __ffma2_rn(dup(A), dt, dup(magic));
@@ -135,31 +136,45 @@ __device__ __forceinline__ float2 exp2_poly(float A, float2 dt) {
                        __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
 }
 
-// The decays of 4 positions.  With EXACT (step sizes from softplus, which are
-// not negative) one state of a lane's four goes through the FMA pipe, the
-// others through the special-function unit.  The polynomial is the exacter of
-// the two near 1, where a decay's error adds up over the longest memory; A
-// usually begins with its slowest state, so it is the first of the four: dA's
-// error against 64 bits is 6e-7 with it and 1.6e-6 without (8 x 2048 x 1536),
-// and the special-function unit, the slower of the two, has a quarter less to
-// do.  `lim` is 126 / |A| of the first state.
-template <bool EXACT>
+// 2^x of two states, the same way; a NaN in x is not kept
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    x = make_float2(fminf(fmaxf(x.x, -126.0f), 126.0f), fminf(fmaxf(x.y, -126.0f), 126.0f));
+    return exp2_poly(1.0f, x);
+}
+
+// The decays of 4 positions: one state of a lane's four goes through the FMA
+// pipe, the others through the special-function unit.  The polynomial is the
+// exacter of the two near 1, where a decay's error adds up over the longest
+// memory; A usually begins with its slowest state, so it is the first of the
+// four: dA's error against 64 bits is 6e-7 with it and 1.6e-6 without (8 x 2048
+// x 1536), and the special-function unit, the slower of the two, has a quarter
+// less to do.  `lim` is 126 / |A| of the first state.  SIGNED: step sizes may
+// be negative (they are not from softplus).
+template <bool SIGNED>
 __device__ __forceinline__ void decays(const St& A2, float lim, const float (&dt)[4], St (&e)[4]) {
-    if constexpr (!EXACT) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) e[k] = exp2s(mul(A2, dup(dt[k])));
-    } else {
+    for (int k = 0; k < 4; k += 2) {
+        float2 d = make_float2(fminf(dt[k], lim), fminf(dt[k + 1], lim));
+        if (SIGNED) d = make_float2(fmaxf(d.x, -lim), fmaxf(d.y, -lim));
+        const float2 p = exp2_poly(A2.a.x, d);
+        e[k].a.x = p.x, e[k + 1].a.x = p.y;
+    }
 #pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-            const float2 p = exp2_poly(A2.a.x, make_float2(fminf(dt[k], lim), fminf(dt[k + 1], lim)));
-            e[k].a.x = p.x, e[k + 1].a.x = p.y;
-        }
+    for (int k = 0; k < 4; k++) {
+        const float2 x = __fmul2_rn(A2.b, dup(dt[k]));
+        e[k].a.y = exp2_fast(__fmul_rn(A2.a.y, dt[k]));
+        e[k].b = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+    }
+}
+// The backward pass's, whose lanes hold the states in different orders: all
+// by the special-function unit, which has time beside that pass's many
+// multiply-adds; with EXACT (fp32 gradients) all by the polynomial.
+template <bool EXACT>
+__device__ __forceinline__ void decays(const St& A2, const float (&dt)[4], St (&e)[4]) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float2 x = __fmul2_rn(A2.b, dup(dt[k]));
-            e[k].a.y = exp2_fast(__fmul_rn(A2.a.y, dt[k]));
-            e[k].b = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-        }
+    for (int k = 0; k < 4; k++) {
+        const St x = mul(A2, dup(dt[k]));
+        e[k] = EXACT ? St{exp2_poly(x.a), exp2_poly(x.b)} : exp2s(x);
     }
 }
 
@@ -226,6 +241,14 @@ __device__ __forceinline__ void stage_steps(float4* row, int c, int t, const flo
     for (int k = 0; k < K; k += 2) row[place((c + k) >> 1, t)] = make_float4(dt[k], v[k], dt[k + 1], v[k + 1]);
 }
 
+// NaNs in A, which the polynomial would lose, are put into the states.
+__device__ __forceinline__ St keep_nan(St h, St A) {
+    if (isnan(A.a.x)) h.a.x = A.a.x;
+    if (isnan(A.a.y)) h.a.y = A.a.y;
+    if (isnan(A.b.x)) h.b.x = A.b.x;
+    if (isnan(A.b.y)) h.b.y = A.b.y;
+    return h;
+}
 // A NaN in the A of a lane's first state, which the polynomial would lose, is
 // put into the state; an infinite one becomes a large one.
 __device__ __forceinline__ float limit(St& A2, St& h) {
@@ -266,6 +289,7 @@ struct Cfg {
 // launch gives each of the 256 threads 128 (two CTAs an SM), 32768 in all:
 // 128 x 176 + 128 x 80.  Three CTAs with 96 and 64 measured 210 us against 229
 // at 8 x 2048 x 1536, but 62 against 53 for ragged prompts of 6 x 777 x 2048.
+constexpr int CTA_REGS = 128;
 __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 176;\n"); }
 __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n"); }
 __device__ __forceinline__ void cta_barrier() { asm volatile("bar.sync 1, 256;\n" ::: "memory"); }
@@ -465,7 +489,7 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
         lim[j] = limit(A2[j], h[j]);
         sum[j] = 0.0f;
     }
-    auto run = [&](auto exact) {
+    auto run = [&](auto signed_steps) {
 #pragma unroll 1
         for (int i = 0; i < tiles; i++) {
             const int buf = i & 1;
@@ -483,7 +507,7 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
                 for (int j = 0; j < CPL; j++) {
                     const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                     St e[4];
-                    decays<decltype(exact)::value>(A2[j], lim[j], dj, e);
+                    decays<decltype(signed_steps)::value>(A2[j], lim[j], dj, e);
                     sum[j] = __fadd_rn(sum[j], __fadd_rn(__fadd_rn(dj[0], dj[1]), __fadd_rn(dj[2], dj[3])));
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
@@ -497,9 +521,9 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
     };
     cta_barrier();
     if (a.softplus)
-        run(std::true_type());
-    else
         run(std::false_type());
+    else
+        run(std::true_type());
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
         const int c = d0 + c0 + j;
@@ -579,7 +603,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
         lim[j] = limit(A2[j], tiles > 0 ? h[j] : none);
     }
     float* keep = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK) * a.D + d0 + c0) * NP + n0;
-    auto run = [&](auto exact) {
+    auto run = [&](auto signed_steps) {
 #pragma unroll 1
         for (int i = 0; i < tiles; i++) {
             const int buf = i & 1, t0 = tb + i * TT;
@@ -610,7 +634,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
                         const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                         St e[4];
                         float y[4];
-                        decays<decltype(exact)::value>(A2[j], lim[j], dj, e);
+                        decays<decltype(signed_steps)::value>(A2[j], lim[j], dj, e);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
                             h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
@@ -631,9 +655,9 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
     };
     cta_barrier();
     if (a.softplus)
-        run(std::true_type());
-    else
         run(std::false_type());
+    else
+        run(std::true_type());
     if (a.hT && ck == a.chunks - 1) {
 #pragma unroll
         for (int j = 0; j < CPL; j++)
@@ -719,6 +743,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
             else if (a.dhT)
                 gc[j] = st(load4(a.dhT + ((int64_t)b * a.D + c) * a.N, n0, a.N));
             gc[j] = permute<PERMS>(gc[j], perm);
+            if (sizeof(T) == 4 && active > 0) gc[j] = keep_nan(gc[j], A2[j]);
         }
     }
     constexpr int AK = E / 4;  // dD and dbias of a quarter of this thread's channels, over 4 positions of each tile
@@ -849,7 +874,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                 for (int j = 0; j < CPL; j++) {
                     const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                     St e[4];
-                    decays<false>(A2[j], 0.0f, dj, e);
+                    decays<sizeof(T) == 4>(A2[j], dj, e);
 #pragma unroll
                     for (int k = 0; k < 4; k++) h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
                     mid[q][j] = h[j];
@@ -877,7 +902,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                 const float dj[4] = {dt[0][j], dt[1][j], dt[2][j], dt[3][j]};
                 const St h0 = q ? st(sm.mid[warp][j][q ? q - 1 : 0][lane]) : permute<PERMS>(st(sm.kept[j][tid]), perm);
                 St e[4], h[4];
-                decays<false>(A2[j], 0.0f, dj, e);
+                decays<sizeof(T) == 4>(A2[j], dj, e);
 #pragma unroll
                 for (int k = 0; k < 4; k++) h[k] = fma(e[k], k ? h[k ? k - 1 : 0] : h0, mul(Bv[k], dup(v[k][j])));
 #pragma unroll
@@ -1006,44 +1031,43 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
     }
 }
 
-// dB and dC: the channel blocks' partial sums, added in order
-template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const float* __restrict__ part, T* __restrict__ dB,
-                                                     T* __restrict__ dC, int blocks, int64_t rows, int N, int NP) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= rows * 2 * NP) return;
-    const int k = (int)(e % (2 * NP));
-    const int64_t row = e / (2 * NP);
-    const int n = k % NP;
-    if (n >= N) return;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int p = 0;
-    for (; p + 3 < blocks; p += 4)
+// The partial sums, added in order.  The first `bc` blocks: dB and dC, over the
+// channel blocks; the others: dA, dD and dbias, over the sequences and chunks.
+struct Sums {
+    const float *part_bc, *part_a, *part_d;
+    void *dB, *dC;
+    float *dA, *dD, *db;
+    int64_t rows;
+    int blocks, bc, P, D, N, NP;
+};
+__device__ __forceinline__ float strands(const float* p, int64_t step, int n) {
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    int i = 0;
+    for (; i + 7 < n; i += 8)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[j] = __fadd_rn(s[j], part[(p + j) * rows * 2 * NP + e]);
-    for (; p < blocks; p++) s[0] = __fadd_rn(s[0], part[p * rows * 2 * NP + e]);
-    const float x = __fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3]));
-    T* o = k < NP ? dB : dC;
-    if (o) o[row * N + n] = from_f<T>(x);
+        for (int j = 0; j < 8; j++) s[j] = __fadd_rn(s[j], p[(i + j) * step]);
+    for (int j = 0; i < n; i++, j++) s[0] = __fadd_rn(s[0], p[i * step]);
+    return __fadd_rn(__fadd_rn(__fadd_rn(s[0], s[1]), __fadd_rn(s[2], s[3])),
+                     __fadd_rn(__fadd_rn(s[4], s[5]), __fadd_rn(s[6], s[7])));
 }
-
-// dA, dD and dbias: the partial sums of P sequences and chunks, added in order
-__global__ void __launch_bounds__(256) sum_params_kernel(const float* __restrict__ pa, const float* __restrict__ pd,
-                                                         float* __restrict__ dA, float* __restrict__ dD,
-                                                         float* __restrict__ db, int P, int D, int N, int NP) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e < (int64_t)D * NP) {
-        const int n = (int)(e % NP);
-        if (n >= N || !dA) return;
-        float s = 0.0f;
-        for (int p = 0; p < P; p++) s = __fadd_rn(s, pa[(int64_t)p * D * NP + e]);
-        dA[e / NP * N + n] = s;
-    } else if (e < (int64_t)D * (NP + 2)) {
-        const int64_t f = e - (int64_t)D * NP;
-        float s = 0.0f;
-        for (int p = 0; p < P; p++) s = __fadd_rn(s, pd[(int64_t)p * 2 * D + f]);
-        float* o = f < D ? dD : db;
-        if (o) o[f % D] = s;
+template <typename T>
+__global__ void __launch_bounds__(256) sum_kernel(const Sums a) {
+    if ((int)blockIdx.x < a.bc) {
+        const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        const int k = (int)(e % (2 * a.NP)), n = k % a.NP;
+        T* o = static_cast<T*>(k < a.NP ? a.dB : a.dC);
+        if (e >= a.rows * 2 * a.NP || n >= a.N || !o) return;
+        o[e / (2 * a.NP) * a.N + n] = from_f<T>(strands(a.part_bc + e, a.rows * 2 * a.NP, a.blocks));
+        return;
+    }
+    const int64_t e = (int64_t)(blockIdx.x - a.bc) * 256 + threadIdx.x, DN = (int64_t)a.D * a.NP;
+    if (e < DN) {
+        const int n = (int)(e % a.NP);
+        if (n < a.N && a.dA) a.dA[e / a.NP * a.N + n] = strands(a.part_a + e, DN, a.P);
+    } else if (e < DN + 2 * a.D) {
+        const int64_t f = e - DN;
+        float* o = f < a.D ? a.dD : a.db;
+        if (o) o[f % a.D] = strands(a.part_d + f, 2 * a.D, a.P);
     }
 }
 
@@ -1215,9 +1239,22 @@ static int check(int batch, int L, int D, int N, int dtype) {
     return MI_OK;
 }
 
+// Lets `kernel` have its shared memory, once for each device (by bit).  `regs`:
+// the registers a thread that its launch must bring along (what setmaxnreg
+// deals out has to be there, or the workers would wait for it without end).
 template <typename K>
-static bool allow_smem(K* kernel, size_t bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+static bool allow_smem(K* kernel, size_t bytes, std::atomic<uint64_t>& done, int regs = 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (regs) {
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, kernel) != cudaSuccess || f.numRegs < regs) return false;
+    }
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 // the chunks' starting states (REV: what they receive from behind), in a.cst
@@ -1225,7 +1262,8 @@ template <typename T, int LN, int CPL, bool REV>
 static int start_chunks(const Args& a, cudaStream_t s) {
     using F = Cfg<T, LN, CPL>;
     constexpr size_t smem = sizeof(typename F::template Smem<false>);
-    if (!allow_smem(chunk_kernel<T, LN, CPL, REV>, smem)) return MI_ERR_CUDA;
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow_smem(chunk_kernel<T, LN, CPL, REV>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
     chunk_kernel<T, LN, CPL, REV><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     const int64_t items = (int64_t)a.batch * a.D * LN;
@@ -1246,7 +1284,8 @@ static int forward_cpl(Args& a, float* ws, cudaStream_t s) {
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::template Smem<true>);
-    if (!allow_smem(scan_kernel<T, LN, CPL>, smem)) return MI_ERR_CUDA;
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow_smem(scan_kernel<T, LN, CPL>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
     scan_kernel<T, LN, CPL><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
@@ -1290,7 +1329,8 @@ static int backward(Args& a, float* ws, cudaStream_t s) {
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::Smem);
-    if (!allow_smem(bwd_kernel<T, LN>, smem)) return MI_ERR_CUDA;
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow_smem(bwd_kernel<T, LN>, smem, allowed)) return MI_ERR_CUDA;
     bwd_kernel<T, LN><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
@@ -1406,19 +1446,15 @@ extern "C" int mi_selective_scan_backward(
     int rc2 = MI_OK;
     MI_DISPATCH_DTYPE(dtype, T, rc2 = mi_sscan_backward_states<T>(a, ws, s));
     if (rc2 != MI_OK) return rc2;
-    const int NP = 4 * lanes_of(N), blocks = mi::cdiv(Dm, bwd_channels(N));
-    const int64_t rows = (int64_t)batch * L;
-    if (dB || dC) {
-        const int64_t n = rows * 2 * NP;
-        MI_DISPATCH_DTYPE(dtype, T,
-                          sum_bc_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(
-                              a.part_bc, static_cast<T*>(dB), static_cast<T*>(dC), blocks, rows, N, NP));
-        MI_CHECK_LAUNCH();
-    }
-    if (dA || dD || ddelta_bias) {
-        const int64_t n = (int64_t)Dm * (NP + 2);
-        sum_params_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a.part_a, a.part_d, dA, dD, ddelta_bias,
-                                                                      batch * a.chunks, Dm, N, NP);
+    Sums t = {};
+    t.part_bc = a.part_bc, t.part_a = a.part_a, t.part_d = a.part_d;
+    t.dB = dB, t.dC = dC, t.dA = dA, t.dD = dD, t.db = ddelta_bias;
+    t.rows = (int64_t)batch * L, t.blocks = mi::cdiv(Dm, bwd_channels(N));
+    t.P = batch * a.chunks, t.D = Dm, t.N = N, t.NP = 4 * lanes_of(N);
+    t.bc = dB || dC ? (int)((t.rows * 2 * t.NP + 255) / 256) : 0;
+    const int params = dA || dD || ddelta_bias ? (int)(((int64_t)Dm * (t.NP + 2) + 255) / 256) : 0;
+    if (t.bc + params) {
+        MI_DISPATCH_DTYPE(dtype, T, sum_kernel<T><<<t.bc + params, 256, 0, s>>>(t));
         MI_CHECK_LAUNCH();
     }
     return MI_OK;

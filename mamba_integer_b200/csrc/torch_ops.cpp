@@ -77,6 +77,16 @@ void like(const Tensor& t, const Tensor& first, at::IntArrayRef shape, const cha
     TORCH_CHECK_VALUE(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have a unit last stride");
 }
 
+// The kernels count positions, channels and rows in 32 bits (offsets in 64).
+void countable(const Tensor& t, const char* name) {
+    for (const int64_t n : t.sizes()) TORCH_CHECK_VALUE(n <= int64_t(1) << 30, name, " is too long: ", t.sizes());
+}
+
+// After a kernel has written to it: saved copies of the tensor are stale.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // Contiguous and on a 16-byte boundary (a copy where it is not).
 Tensor aligned(const Tensor& t) {
     Tensor c = t.contiguous();
@@ -235,6 +245,7 @@ struct ScanParams {
 ScanParams scan_arguments(at::IntArrayRef lead, const Tensor& u, const Tensor& delta, const Tensor& A, const Tensor& B,
                           const Tensor& C, const OptTensor& D, const OptTensor& z, const OptTensor& bias) {
     activation(u, "u");
+    countable(u, "u");
     const int64_t d = u.size(-1);
     TORCH_CHECK_VALUE(A.dim() == 2 && A.size(0) == d, "A must be [", d, ", states], got ", A.sizes());
     const int64_t N = A.size(1);
@@ -287,6 +298,7 @@ Tensor selective_scan_step(const Tensor& h, const Tensor& u, const Tensor& delta
                                     st(C, 0), fptr(p.D), ptr(p.z), st(p.z, 0), fptr(p.bias), fptr(h), ptr(y), batch, d,
                                     p.N, softplus, dtype_code(u), place.stream),
           "mi_selective_scan_step");
+    written(h);
     return y;
 }
 
@@ -348,6 +360,7 @@ struct CausalConv1d : torch::autograd::Function<CausalConv1d> {
 std::tuple<Tensor, Tensor> conv_arguments(at::IntArrayRef lead, const Tensor& x, const Tensor& weight,
                                           const OptTensor& bias) {
     activation(x, "x");
+    countable(x, "x");
     const int64_t d = x.size(-1);
     Tensor w = weight.dim() == 3 && weight.size(1) == 1 ? weight.squeeze(1) : weight;  // nn.Conv1d's [channels, 1, taps]
     TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) == d && d > 0 && w.size(1) >= 2 && w.size(1) <= 4, "weight must be [", d,
@@ -386,6 +399,7 @@ Tensor causal_conv1d_step(const Tensor& x, const Tensor& weight, const Tensor& w
     check(mi.mi_causal_conv1d_step(ptr(x), st(x, 0), fptr(w), fptr(bias), ptr(win), ptr(y), batch, d, w.size(1), silu,
                                    dtype_code(x), place.stream),
           "mi_causal_conv1d_step");
+    written(win);
     return y;
 }
 
@@ -459,6 +473,7 @@ Rows rms_arguments(const Tensor& x, const Tensor& weight, const OptTensor& resid
     }
     const Tensor w = plain(weight, x, {d}, at::kFloat, "weight");
     on_gpu(x, "x");
+    TORCH_CHECK_VALUE(x.numel() / d <= int64_t(1) << 30, "x has too many rows: ", x.sizes());
     auto rows = [&](const Tensor& t) { return unit(t.dim() == 2 ? t : t.reshape({-1, d})); };
     return {rows(x), w, residual.has_value() ? rows(*residual) : Tensor()};
 }

@@ -269,6 +269,18 @@ def test_scan_step(sel, cuda_dev, size, dtype):
     check_scan(torch.stack(ys, 1), h, a)
 
 
+def test_steps_in_place_are_seen_by_autograd(sel, cuda_dev):
+    """A state that a graph has saved and a step then overwrites is an error in that graph's backward pass."""
+    h = torch.randn(1, 8, 4, device=cuda_dev)
+    w = torch.ones(1, 8, 4, device=cuda_dev, requires_grad=True)
+    out = (h * w).sum()  # saves h
+    z = lambda *s: torch.randn(*s, device=cuda_dev)  # noqa: E731
+    with torch.no_grad():
+        sel.selective_scan_step(h, z(1, 8), z(1, 8), -z(8, 4).exp(), z(1, 4), z(1, 4))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
+
+
 def test_empty_calls(sel, cuda_dev):
     z = lambda *s, dtype=F32: torch.randn(*s, device=cuda_dev).to(dtype)  # noqa: E731
     for b, n in ((0, 5), (2, 0)):

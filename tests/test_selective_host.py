@@ -104,6 +104,17 @@ def test_norm_refuses(change, error):
             fn(**{**dict(x=_t(4, 8), weight=_t(8)), **change})
 
 
+def test_sizes_past_32_bits_are_refused():
+    """Expanded views: no such memory is there."""
+    n = (1 << 30) + 1
+    one = _t(1, 1, 1)
+    with pytest.raises(ValueError, match="too long"):
+        selective.selective_scan(one.expand(1, n, 1), one.expand(1, n, 1), _t(1, 1), one.expand(1, n, 1),
+                                 one.expand(1, n, 1))
+    with pytest.raises(ValueError, match="too long"):
+        selective.causal_conv1d(one.expand(1, n, 1), _t(1, 4))
+
+
 def test_entry_points_refuse_on_the_host():
     """Before any CUDA call; the pointers are not touched."""
     lib = _lib.load()
