@@ -469,7 +469,7 @@ extern "C" int mi_causal_conv1d(const void* x, int64_t x_batch, int64_t x_row, c
 extern "C" int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const float* bias, void* win,
                                      void* y, int batch, int D, int W, int silu, int dtype, void* stream) {
     using namespace mi::conv1d;
-    const int rc = check(batch, 1, D, W, dtype);
+    const int rc = check(batch < 0 ? -1 : 0, 1, D, W, dtype);
     if (rc != MI_OK) return rc;
     if (batch == 0) return MI_OK;
     if (!x || !w || !win || !y) return MI_ERR_INVALID;

@@ -63,7 +63,6 @@ struct Args {
     int softplus;
     int chunks, span;  // positions a chunk (a multiple of 32)
     int ovec;          // outputs' rows start on 8 elements' alignment
-    int pvec;          // D and delta_bias start on 16 bytes
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
@@ -113,6 +112,14 @@ __device__ __forceinline__ St fma(St x, float2 v, St z) { return {__ffma2_rn(x.a
 __device__ __forceinline__ float dot(St x, St y) {
     const float2 p = __ffma2_rn(x.b, y.b, __fmul2_rn(x.a, y.a));
     return __fadd_rn(p.x, p.y);
+}
+// A row of A for base 2.  An infinite A becomes a large one: it forgets the
+// state at once all the same, and a position of dt = 0 behind a length, which
+// must leave the state alone, stays clear of 0 times infinity.
+__device__ __forceinline__ float finite(float v) { return fabsf(v) > 1e20f ? copysignf(1e20f, v) : v; }
+__device__ __forceinline__ St scaled(float4 A) {
+    return {make_float2(finite(__fmul_rn(A.x, LOG2E)), finite(__fmul_rn(A.y, LOG2E))),
+            make_float2(finite(__fmul_rn(A.z, LOG2E)), finite(__fmul_rn(A.w, LOG2E)))};
 }
 __device__ __forceinline__ St exp2s(St x) {
     return {make_float2(exp2_fast(x.a.x), exp2_fast(x.a.y)), make_float2(exp2_fast(x.b.x), exp2_fast(x.b.y))};
@@ -250,10 +257,9 @@ __device__ __forceinline__ St keep_nan(St h, St A) {
     return h;
 }
 // A NaN in the A of a lane's first state, which the polynomial would lose, is
-// put into the state; an infinite one becomes a large one.
-__device__ __forceinline__ float limit(St& A2, St& h) {
+// put into the state.
+__device__ __forceinline__ float limit(const St& A2, St& h) {
     if (isnan(A2.a.x)) h.a.x = A2.a.x;
-    A2.a.x = fminf(fmaxf(A2.a.x, -1e30f), 1e30f);
     return __fdiv_rn(126.0f, fmaxf(fabsf(A2.a.x), 1e-30f));
 }
 
@@ -484,7 +490,7 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
         const int c = d0 + c0 + j;
-        A2[j] = mul(st(c < a.D ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
+        A2[j] = scaled(c < a.D ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0));
         h[j] = st(make_float4(0, 0, 0, 0));
         lim[j] = limit(A2[j], h[j]);
         sum[j] = 0.0f;
@@ -543,7 +549,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a) {
     const int64_t item = (int64_t)blockIdx.x * THREADS + threadIdx.x;
     if (item >= (int64_t)a.batch * a.D * LN) return;
     const int n0 = 4 * (int)(item % LN), d = (int)(item / LN % a.D), b = (int)(item / LN / a.D);
-    const St A2 = mul(st(load4(a.A + (int64_t)d * a.N, n0, a.N)), LOG2E);
+    const St A2 = scaled(load4(a.A + (int64_t)d * a.N, n0, a.N));
     const float* init = REV ? a.dhT : a.h0;
     St h = st(init ? load4(init + ((int64_t)b * a.D + d) * a.N, n0, a.N) : make_float4(0, 0, 0, 0));
     const int last = REV ? 0 : a.chunks - 1;  // its own part is not needed
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
     for (int j = 0; j < CPL; j++) {
         const int c = d0 + c0 + j;
         const bool in = c < a.D;
-        A2[j] = mul(st(in ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0)), LOG2E);
+        A2[j] = scaled(in ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0));
         float4 v = make_float4(0, 0, 0, 0);
         if (in && a.chunks > 1)
             v = *reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + c) * NP + n0);
@@ -737,7 +743,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
         const int c = d0 + c0 + j;
         A2[j] = gc[j] = dA[j] = st(make_float4(0, 0, 0, 0));
         if (c < a.D) {
-            A2[j] = permute<PERMS>(mul(st(load4(a.A + (int64_t)c * a.N, n0, a.N)), LOG2E), perm);
+            A2[j] = permute<PERMS>(scaled(load4(a.A + (int64_t)c * a.N, n0, a.N)), perm);
             if (a.chunks > 1)
                 gc[j] = st(*reinterpret_cast<const float4*>(a.cst + (((int64_t)b * a.chunks + ck) * a.D + c) * NP + n0));
             else if (a.dhT)
@@ -1117,7 +1123,7 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
             for (int i = 0; i < 4; i++) pB[r].v[i] = pC[r].v[i] = from_f<T>(0.0f);
         }
     }
-    const St A2 = mul(st(Av), LOG2E);
+    const St A2 = scaled(Av);
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
         const int b = b0 + r;
@@ -1387,7 +1393,6 @@ extern "C" int mi_selective_scan(const void* u, int64_t u_batch, int64_t u_row, 
     a.y = y, a.hT = h_out, a.ckpt = checkpoints;
     a.batch = batch, a.L = L, a.D = Dm, a.N = N, a.softplus = softplus;
     a.ovec = Dm % 8 == 0 && mi::aligned16(y);
-    a.pvec = mi::aligned16(D) && mi::aligned16(delta_bias);
     float* ws = static_cast<float*>(workspace);
     MI_DISPATCH_DTYPE(dtype, T, MI_SSCAN_STATES(N, forward, T, a, ws, (cudaStream_t)stream));
     return MI_ERR_INVALID;
@@ -1399,7 +1404,7 @@ extern "C" int mi_selective_scan_step(const void* u, int64_t u_batch, const void
                                       float* h, void* y, int batch, int Dm, int N, int softplus, int dtype,
                                       void* stream) {
     using namespace mi::sscan;
-    const int rc = check(batch, 1, Dm, N, dtype);
+    const int rc = check(batch < 0 ? -1 : 0, 1, Dm, N, dtype);
     if (rc != MI_OK) return rc;
     if (batch == 0) return MI_OK;
     if (!u || !delta || !A || !B || !C || !h || !y) return MI_ERR_INVALID;
@@ -1440,7 +1445,6 @@ extern "C" int mi_selective_scan_backward(
     a.du = du, a.ddelta = ddelta, a.dz = dz, a.dh0 = dh0;
     a.batch = batch, a.L = L, a.D = Dm, a.N = N, a.softplus = softplus;
     a.ovec = Dm % 8 == 0 && mi::aligned16(du) && mi::aligned16(ddelta) && mi::aligned16(dz);
-    a.pvec = mi::aligned16(D) && mi::aligned16(delta_bias);
     float* ws = static_cast<float*>(workspace);
     cudaStream_t s = (cudaStream_t)stream;
     int rc2 = MI_OK;

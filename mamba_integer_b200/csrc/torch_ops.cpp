@@ -8,12 +8,15 @@
 // same checks and nodes in Python took 15 to 25 us a call and 130 us a backward
 // pass, more than their kernels.
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
+
+#include <unordered_set>
 
 #include "../../include/mi_b200.h"
 
@@ -77,6 +80,9 @@ void like(const Tensor& t, const Tensor& first, at::IntArrayRef shape, const cha
     TORCH_CHECK_VALUE(t.size(-1) <= 1 || t.stride(-1) == 1, name, " must have a unit last stride");
 }
 
+// The kernels' grids: sequences, and a convolution's positions.
+constexpr int64_t MAX_BATCH = 65535, MAX_CONV_L = 65535 * 128;
+
 // The kernels count positions, channels and rows in 32 bits (offsets in 64).
 void countable(const Tensor& t, const char* name) {
     for (const int64_t n : t.sizes()) TORCH_CHECK_VALUE(n <= int64_t(1) << 30, name, " is too long: ", t.sizes());
@@ -130,6 +136,40 @@ template <typename... Ts>
 void no_grad_needed(const Ts&... ts) {
     TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad(ts...),
                 "the single-token and quantised forms have no backward pass: call them under torch.no_grad()");
+}
+
+// A training call that is being captured.  Where an earlier autograd graph is
+// alive over one of its leaves, the leaf's gradient is added on that graph's
+// stream; if that is the default stream, which no capture can join, the
+// captured backward pass would end the process.
+void capturable(c10::ArrayRef<const Tensor*> inputs, c10::Device device) {
+    using torch::autograd::Node;
+    c10::cuda::CUDAGuard guard(device);
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    std::vector<std::shared_ptr<Node>> todo;
+    std::unordered_set<Node*> seen;
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad()) continue;
+        todo.push_back(t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t));
+    }
+    while (!todo.empty()) {
+        const std::shared_ptr<Node> node = todo.back();
+        todo.pop_back();
+        if (!node || !seen.insert(node.get()).second) continue;
+        const auto on = node->stream();
+        TORCH_CHECK(!on || !on->device().is_cuda() || on->id() != c10::cuda::getDefaultCUDAStream(on->device_index()).id(),
+                    "a training step is being captured while an autograd graph made on the default stream is alive over "
+                    "one of its leaves: drop that graph's results first");
+        for (const auto& edge : node->next_edges()) todo.push_back(edge.function);
+    }
+}
+
+// `t`, empty, as a result that depends on the others, so that they get their zero gradients
+Tensor reached(Tensor t, c10::ArrayRef<const Tensor*> inputs) {
+    if (!at::GradMode::is_enabled()) return t;
+    for (const Tensor* o : inputs)
+        if (o->defined() && o->requires_grad()) t = t + o->sum().to(t.scalar_type());
+    return t;
 }
 
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -271,10 +311,13 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& delta, 
     const auto p = scan_arguments({batch, L}, u, delta, A_, B, C, D_, z_, bias_);
     const Tensor h0 = plain(h0_, u, {batch, d, p.N}, at::kFloat, "h0");
     const Tensor lengths = lengths_of(lengths_, u, batch);
+    TORCH_CHECK_VALUE(batch <= MAX_BATCH, "at most ", MAX_BATCH, " sequences, got u ", u.sizes());
     on_gpu(u, "u");
     if (batch == 0 || L == 0)  // nothing to scan
-        return {u * 1, h0.defined() ? h0 * 1 : at::zeros({batch, d, p.N}, u.options().dtype(at::kFloat))};
+        return {reached(u * 1, {&delta, &p.A, &B, &C, &p.D, &p.z, &p.bias, &h0}),
+                h0.defined() ? h0 * 1 : at::zeros({batch, d, p.N}, u.options().dtype(at::kFloat))};
     if (at::GradMode::is_enabled() && any_requires_grad(u, delta, p.A, B, C, p.D, p.z, p.bias, h0)) {
+        capturable({&u, &delta, &p.A, &B, &C, &p.D, &p.z, &p.bias, &h0}, u.device());
         const auto out = SelectiveScan::apply(u, delta, p.A, B, C, maybe(p.D), maybe(p.z), maybe(p.bias), maybe(h0),
                                               maybe(lengths), softplus);
         return {out[0], out[1]};
@@ -378,9 +421,14 @@ std::tuple<Tensor, Tensor> causal_conv1d(const Tensor& x, const Tensor& weight, 
     const auto [w, bias] = conv_arguments({batch, L}, x, weight, bias_);
     const Tensor win = plain(win_, x, {batch, w.size(1) - 1, d}, x.scalar_type(), "win");
     const Tensor lengths = lengths_of(lengths_, x, batch);
+    TORCH_CHECK_VALUE(batch <= MAX_BATCH && L <= MAX_CONV_L, "at most ", MAX_BATCH, " sequences of ", MAX_CONV_L,
+                      " positions, got x ", x.sizes());
     on_gpu(x, "x");
-    if (batch == 0 || L == 0) return {x * 1, win.defined() ? win * 1 : at::zeros({batch, w.size(1) - 1, d}, x.options())};
+    if (batch == 0 || L == 0)
+        return {reached(x * 1, {&w, &bias, &win}),
+                win.defined() ? win * 1 : at::zeros({batch, w.size(1) - 1, d}, x.options())};
     if (at::GradMode::is_enabled() && any_requires_grad(x, w, bias, win)) {
+        capturable({&x, &w, &bias, &win}, x.device());
         const auto out = CausalConv1d::apply(x, w, maybe(bias), maybe(win), maybe(lengths), silu);
         return {out[0], out[1]};
     }
@@ -481,8 +529,10 @@ Rows rms_arguments(const Tensor& x, const Tensor& weight, const OptTensor& resid
 std::tuple<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual) {
     const Rows a = rms_arguments(x, weight, residual);
     auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : t.view(x.sizes()); };
-    if (a.x.size(0) == 0) return {x * 1, residual.has_value() ? OptTensor(*residual * 1) : OptTensor()};
+    if (a.x.size(0) == 0)
+        return {reached(x * 1, {&a.w, &a.r}), residual.has_value() ? OptTensor(reached(*residual * 1, {&a.x})) : OptTensor()};
     if (at::GradMode::is_enabled() && any_requires_grad(a.x, a.w, a.r)) {
+        capturable({&a.x, &a.w, &a.r}, a.x.device());
         const auto out = RMSNorm::apply(a.x, a.w, maybe(a.r), eps);
         return {shaped(out[0]), out.size() > 1 ? OptTensor(shaped(out[1])) : OptTensor()};
     }

@@ -22,10 +22,11 @@ Every call launches on the current stream of its tensors' device, allocates its
 outputs and workspaces with torch, and gives the same bits for the same inputs.
 Wrong shapes and placements raise ValueError, wrong types TypeError.  The calls
 are native (csrc/torch_ops.cpp, over the C ABI of include/mi_b200.h).
-CUDA tensors only; gradients are of first order.  To capture a training step in
-a CUDA graph, drop any earlier result that still holds an autograd graph over
-the same leaves first (torch ties a leaf's gradient to the stream of the graph
-that is alive).
+CUDA tensors only; gradients are of first order; a prompt or training call has
+at most 65535 sequences.  To capture a training step in a CUDA graph, drop any
+earlier result that still holds an autograd graph over the same leaves first
+(torch ties a leaf's gradient to the stream of the graph that is alive; the
+calls refuse such a capture where that is the default stream).
 """
 from __future__ import annotations
 
@@ -79,7 +80,8 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
 
     u, delta, z [batch, L, channels]; B, C [batch, L, states]; A [channels,
     states]; D, delta_bias [channels]; h0 [batch, channels, states].  Returns
-    y, or (y, final state) with ``return_state``.  1 to 64 states."""
+    y, or (y, final state) with ``return_state``.  1 to 64 states.  An infinite
+    A counts as a very large one (0 times it is 0)."""
     y, h = (_ops or _load()).selective_scan(u, delta, A, B, C, D, z, delta_bias, delta_softplus, h0, lengths)
     return (y, h) if return_state else y
 
@@ -103,7 +105,8 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     weight [channels, taps] (or nn.Conv1d's [channels, 1, taps]), 2 to 4 taps;
     win [batch, taps - 1, channels] of x's type holds the inputs before
     position 0 (zeros without one).  Returns y, or (y, window) with
-    ``return_window``: the last taps - 1 inputs, as causal_conv1d_step takes it."""
+    ``return_window``: the last taps - 1 inputs, as causal_conv1d_step takes it.
+    Sequences of up to 8388480 positions."""
     y, out = (_ops or _load()).causal_conv1d(x, weight, bias, silu, win, lengths)
     return (y, out) if return_window else y
 

@@ -144,6 +144,30 @@ def test_scan_extreme_steps(sel, cuda_dev):
     assert not y[0, :5].isnan().any() and y[0, 5:].isnan().all() and h.isnan().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [21, 300])
+def test_scan_infinite_decays(sel, cuda_dev, n, dtype):
+    """States that are forgotten at once: the formula with a large A, also behind a length and in the backward pass."""
+    a = scan_inputs(cuda_dev, dtype, 3, n, 40, 16, h0=True, lengths=[n, n - 9, 2])
+    large = dict(a, A=a["A"].clone())
+    a["A"][:, 3::5], large["A"][:, 3::5] = float("-inf"), -1e12
+    a["A"][::7], large["A"][::7] = float("-inf"), -1e12
+    check_scan(*call_scan(sel, a), large)
+    dy, dh = torch.randn_like(a["u"]), torch.randn(3, 40, 16, device=cuda_dev)
+    _, _, got = scan_grads(sel, a, dy, dh)
+    # what only such a decay passes on: fp32 decays end at 2^-126 = 1.2e-38, so dh0 = a g and dA = sum a g h dt are at
+    # most that many times values of order 10 (and 300 positions of 3 sequences for dA), where the formula has 0
+    for name, gone in (("A", a["A"].isinf()), ("h0", a["A"].isinf().expand(3, -1, -1))):
+        assert (got[name][gone].abs() < 1e-30).all()
+        got[name] = got[name].masked_fill(gone, 0.0)
+    check_scan_grads(got, large, dy, dh)
+    h = a["h0"].clone()
+    y = sel.selective_scan_step(h, a["u"][:, 0], a["delta"][:, 0], a["A"], a["B"][:, 0], a["C"][:, 0], D=a["D"],
+                                z=a["z"][:, 0], delta_bias=a["bias"], delta_softplus=True)
+    first = {key: large[key][:, :1] for key in ("u", "delta", "B", "C", "z")}
+    check_scan(y[:, None], h, dict(large, **first, lengths=None))
+
+
 def scan_grads(sel, a, dy, dh):
     names = [k for k in ("u", "delta", "A", "B", "C", "D", "z", "bias", "h0") if a[k] is not None]
     leaves = {k: a[k].detach().clone().requires_grad_(True) for k in names}
@@ -292,6 +316,15 @@ def test_empty_calls(sel, cuda_dev):
         win = z(b, 3, 8)
         y, out = sel.causal_conv1d(z(b, n, 8), z(8, 4), win=win, return_window=True)
         assert y.shape == (b, n, 8) and torch.equal(out, win)
+        # all that could have changed the result gets a gradient of zeros
+        leaves = [t.requires_grad_(True) for t in (z(b, n, 8), z(b, n, 8), z(8, 4), z(b, n, 4), z(b, n, 4), z(8), z(8))]
+        y = sel.selective_scan(*leaves[:5], D=leaves[5], delta_bias=leaves[6])
+        assert not any(t.any() for t in torch.autograd.grad(y.sum(), leaves))
+        leaves = [t.requires_grad_(True) for t in (z(b, n, 8, dtype=BF16), z(8, 4), z(8))]
+        assert not any(t.any() for t in torch.autograd.grad(sel.causal_conv1d(*leaves).sum(), leaves))
+    leaves = [t.requires_grad_(True) for t in (z(0, 8, dtype=BF16), z(8), z(0, 8))]
+    y, s = sel.rms_norm(leaves[0], leaves[1], residual=leaves[2])
+    assert s.dtype == F32 and not any(t.any() for t in torch.autograd.grad(y.sum() + s.sum(), leaves))
     assert sel.selective_scan_step(z(0, 8, 4), z(0, 8), z(0, 8), z(8, 4), z(0, 4), z(0, 4)).shape == (0, 8)
     assert sel.causal_conv1d_step(z(0, 8), z(8, 4), z(0, 3, 8)).shape == (0, 8)
     y, s = sel.rms_norm(z(0, 8), z(8), residual=z(0, 8))
@@ -636,6 +669,43 @@ def test_graphs_of_prompts_and_training_steps(sel, cuda_dev):
         for a, dy, train, graph, out in made:
             y, grads = train()
             assert torch.equal(y, out[0]) and all(torch.equal(p, q) for p, q in zip(grads, out[1]))
+
+
+def test_capture_beside_an_eager_graph_is_refused(sel, cuda_dev):
+    """The leaves' gradients would be added on the default stream, which a capture cannot join."""
+    x, w = torch.randn(1, 9, 8, device=cuda_dev), torch.randn(8, device=cuda_dev, requires_grad=True)
+    taps = torch.randn(8, 4, device=cuda_dev, requires_grad=True)
+    A = torch.randn(8, 4, device=cuda_dev, requires_grad=True)
+    calls = {"norm": lambda: sel.rms_norm(x, w)[0], "conv": lambda: sel.causal_conv1d(x, taps * 2),
+             "scan": lambda: sel.selective_scan(x, x, A, x[..., :4], x[..., :4])}
+    for call in calls.values():
+        call()
+        alive = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            kept = x * 2  # a graph is not empty
+            with pytest.raises(RuntimeError, match="autograd graph made on the default stream is alive"):
+                call()
+            with torch.no_grad():
+                y = call()
+        graph.replay()
+        assert torch.equal(y, alive) and torch.equal(kept, x * 2)
+
+
+def test_many_streams(sel, cuda_dev):
+    """Steps have no limit of 65535 streams."""
+    b = 65537
+    a = scan_inputs(cuda_dev, F32, 1, 1, 3, 4, h0=True)
+    step = {k: a[k][:, 0].expand(b, -1).contiguous() for k in ("u", "delta", "B", "C")}
+    h = a["h0"].expand(b, -1, -1).contiguous()
+    y = sel.selective_scan_step(h, step["u"], step["delta"], a["A"], step["B"], step["C"])
+    assert torch.equal(y, y[:1].expand(b, -1)) and torch.equal(h, h[:1].expand(b, -1, -1))
+    assert not torch.equal(h[:1], a["h0"])
+    win = torch.zeros(b, 3, 3, device=cuda_dev)
+    taps = torch.ones(3, 4, device=cuda_dev)
+    assert torch.equal(sel.causal_conv1d_step(step["u"], taps, win), step["u"])
+    assert torch.equal(win[:, 2], step["u"]) and not win[:, :2].any()
 
 
 def test_graph_of_decode_steps(sel, cuda_dev):

@@ -115,6 +115,17 @@ def test_sizes_past_32_bits_are_refused():
         selective.causal_conv1d(one.expand(1, n, 1), _t(1, 4))
 
 
+def test_too_many_sequences_are_refused():
+    one = _t(1, 1, 1)
+    for b, n in ((65536, 1), (65536, 0)):
+        rows = one.expand(b, 1, 1)[:, :n]
+        with pytest.raises(ValueError, match="at most 65535 sequences"):
+            selective.selective_scan(rows, rows, _t(1, 1), rows, rows)
+    for b, n in ((65536, 1), (1, 65535 * 128 + 1)):
+        with pytest.raises(ValueError, match="at most 65535 sequences of 8388480"):
+            selective.causal_conv1d(one.expand(b, n, 1), _t(1, 4))
+
+
 def test_entry_points_refuse_on_the_host():
     """Before any CUDA call; the pointers are not touched."""
     lib = _lib.load()
