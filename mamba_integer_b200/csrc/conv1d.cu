@@ -185,126 +185,201 @@ __global__ void __launch_bounds__(128, 5) fwd_kernel(const Args a) {
     }
 }
 
-// Backward.  A CTA is 32 channel packs by 8 runs of one sequence.  A thread
-// walks its run forward, 4 positions at a time: dc[t] needs x up to t, dx[t]
-// needs dc up to t + W - 1, so it goes W - 1 positions past its run, and dx
-// comes out W - 1 positions late.  Its own positions' terms of dw and dbias stay in registers;
-// the CTA adds its 8 runs in shared memory, in order, and writes one partial
-// row, which sum_kernel adds.
-constexpr int BWD_RUNS = 8;  // of a.run positions: 16 or 32
+// Backward.  A CTA is 32 pairs of channels by 8 runs of one sequence, a run to
+// a warp.  A thread walks its run forward, 4 positions at a time: dc[t] needs x
+// up to t, dx[t] needs dc up to t + W - 1, so it goes W - 1 positions past its
+// run, and dx comes out W - 1 positions late.  Its own positions' terms of dw
+// and dbias stay in registers; the CTA adds its 8 runs in shared memory, in
+// order, and writes one partial row, which sum_kernel adds.
+//
+// A position of x and dy is 128 bytes of each for a warp (16-bit types), too
+// little to cover HBM's latency with the rows that registers can hold, and a
+// copy for each pair costs as many instructions as the arithmetic: asynchronous
+// copies of 16 bytes a lane bring the next DEPTH - 1 groups of 4 positions into
+// the warp's ring (zeros behind the sequence's length).  Rows off 16 bytes
+// (VEC = false) go through registers, one group ahead.  8 x 2048 x 1536 bf16:
+// 52 us (150 MB, 2.9 TB/s), bound by the instructions' issue; 74 with each
+// lane's rows in registers, 80 with a copy for each pair, 56 with 4 CTAs an SM,
+// whose 64 registers spill.
+constexpr int BWD_RUNS = 8, DEPTH = 4, PAIR = 2;
 
-template <typename T, int W, int K, bool VEC>
-__global__ void __launch_bounds__(256, 2) bwd_kernel(const Args a) {
+template <int W>
+constexpr int BWD_SUMS = BWD_RUNS * 32 * ((W + 1) * PAIR + 1) * (int)sizeof(float);
+template <typename T, int W, bool VEC>
+constexpr int bwd_smem() {
+    constexpr int ring = DEPTH * 8 * 256 * PAIR * (int)sizeof(T);
+    return VEC && ring > BWD_SUMS<W> ? ring : BWD_SUMS<W>;
+}
+template <typename T>
+__device__ __forceinline__ float2 pair(const Pack<T, PAIR>& p) { return make_float2(to_f(p.v[0]), to_f(p.v[1])); }
+
+template <typename T, int W, bool VEC>
+__global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
+    constexpr int K = PAIR;
     using P = Pack<T, K>;
     constexpr int S = (W + 1) * K;
-    __shared__ float sh[BWD_RUNS][32][S + 1];
+    extern __shared__ __align__(16) unsigned char smem[];
     const int cx = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int c = (blockIdx.x * 32 + cx) * K, have = a.D - c;
+    const int c0 = blockIdx.x * 32 * K, have = a.D - c0 - cx * K;
+    const int c = have > 0 ? c0 + cx * K : c0;  // lanes beyond the last channel copy along and store nothing
     const int b = blockIdx.z;
     const int t0 = (blockIdx.y * BWD_RUNS + g) * a.run, t1 = t0 + a.run < a.L ? t0 + a.run : a.L;
     const int len = length_of(a.lengths, b, a.L);
-    float dw[W][K], db[K];
+    const float2 zero = make_float2(0.0f, 0.0f);
+    float2 dw[W], db = zero;
 #pragma unroll
-    for (int i = 0; i < K; i++) {
-        db[i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; k++) dw[k][i] = 0.0f;
-    }
-    if (have > 0 && t0 < a.L) {
-        const T* xb = static_cast<const T*>(a.x) + b * a.xb + c;
-        const T* gb = static_cast<const T*>(a.dy) + b * a.gb + c;
+    for (int k = 0; k < W; k++) dw[k] = zero;
+    if (t0 < a.L && (VEC || have > 0)) {
+        const T* xb = static_cast<const T*>(a.x) + b * a.xb;
+        const T* gb = static_cast<const T*>(a.dy) + b * a.gb;
         const T* gwin = static_cast<const T*>(a.dwin_out);
+        T* dxb = static_cast<T*>(a.dx);
+        if (dxb) dxb += (int64_t)b * a.L * a.D + c;
         const int last = len > 0 ? len - 1 : 0;
+        // VEC: the ring [DEPTH][x, dy][4][64 channels]; a lane's part of a group is pack q of row r, or of rows r and r + 2
+        constexpr int PACK = 16 / (int)sizeof(T), ROW = 32 * K, PER = ROW / PACK, PARTS = 4 * PER / 32;
+        T* ring = reinterpret_cast<T*>(smem) + g * (DEPTH * 8 * ROW);
+        const int q = cx % PER, r0 = cx / PER;
+        const bool exists = c0 + q * PACK < a.D;
+        const T *xq = xb + (exists ? c0 + q * PACK : 0), *gq = gb + (exists ? c0 + q * PACK : 0);
         P nx[4], ng[4];
-        auto fetch = [&](int t) {
+        auto fetch = [&](int t, int slot) {
+            if constexpr (VEC) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int64_t r = t + j < last ? t + j : last;
-                nx[j] = raw_row<VEC, K>(xb + r * a.xl, have);
-                ng[j] = raw_row<VEC, K>(gb + r * a.gl, have);
+                for (int i = 0; i < PARTS; i++) {
+                    const int r = r0 + i * (32 / PER), bytes = exists && t + r < len ? 16 : 0;
+                    const int64_t row = t + r < last ? t + r : last;
+                    T* to = ring + (slot * 8 + r) * ROW + q * PACK;
+                    cp_async<16>(to, xq + row * a.xl, bytes);
+                    cp_async<16>(to + 4 * ROW, gq + row * a.gl, bytes);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int64_t row = t + j < last ? t + j : last;
+                    nx[j] = raw_row<VEC, K>(xb + row * a.xl + c, have);
+                    ng[j] = raw_row<VEC, K>(gb + row * a.gl + c, have);
+                }
             }
         };
-        fetch(t0);
-        float w[W][K], bias[K];
-        float x[W + 3][K], dc[W + 3][K];  // inputs and dc from W - 1 positions before a group to its end
-        rows_before<W, K, VEC, T>(a, b, t0, len, c, reinterpret_cast<float(&)[W - 1][K]>(x));
-        load_w<W, K>(a, c, w, bias);
+        const int te = t1 + W - 1;
+        if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < W - 1; j++)
+            for (int i = 0; i < DEPTH - 1; i++) {
+                if (t0 + 4 * i < te) fetch(t0 + 4 * i, i);
+                cp_async_commit();
+            }
+        } else {
+            fetch(t0, 0);
+        }
+        float2 x[W + 3], dc[W + 3], w[W], bias;  // inputs and dc from W - 1 positions before a group to its end
+        {
+            float xf[W - 1][K], wf[W][K], bf[K];
+            rows_before<W, K, VEC, T>(a, b, t0, len, c, xf);
+            load_w<W, K>(a, c, wf, bf);
 #pragma unroll
-            for (int i = 0; i < K; i++) dc[j][i] = 0.0f;
+            for (int k = 0; k < W - 1; k++) x[k] = make_float2(xf[k][0], xf[k][1]), dc[k] = zero;
+#pragma unroll
+            for (int k = 0; k < W; k++) w[k] = make_float2(wf[k][0], wf[k][1]);
+            bias = make_float2(bf[0], bf[1]);
+        }
         // the run that begins the sequence also makes the window's gradients, dx at t = -(W-1) .. -1
         const int first = t0 == 0 ? -(W - 1) : t0;
+        const int inner = gwin && len - (W - 1) < t1 ? len - (W - 1) : t1;  // dx up to here is the sum alone
+        int slot = 0;
 #pragma unroll 1
-        for (int t = t0; t < t1 + W - 1; t += 4) {
+        for (int t = t0; t < te; t += 4) {
+            if constexpr (VEC) {
+                cp_async_wait<DEPTH - 2>();
+                __syncwarp();  // every lane's part has come, and the slot behind this one has been read
+                if (t + 4 * (DEPTH - 1) < te) fetch(t + 4 * (DEPTH - 1), (slot + DEPTH - 1) % DEPTH);
+                cp_async_commit();
+                const P* at = reinterpret_cast<const P*>(ring + slot * 8 * ROW) + cx;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 4; j++) x[W - 1 + j] = pair(at[j * 32]), dc[W - 1 + j] = pair(at[(4 + j) * 32]);
+                slot = (slot + 1) % DEPTH;
+            } else {
 #pragma unroll
-                for (int i = 0; i < K; i++) {
-                    x[W - 1 + j][i] = t + j < len ? to_f(nx[j].v[i]) : 0.0f;
-                    dc[W - 1 + j][i] = t + j < len ? to_f(ng[j].v[i]) : 0.0f;
+                for (int j = 0; j < 4; j++) {
+                    x[W - 1 + j] = t + j < len ? pair(nx[j]) : zero;
+                    dc[W - 1 + j] = t + j < len ? pair(ng[j]) : zero;
                 }
-            fetch(t + 4);
+                fetch(t + 4, 0);
+            }
             if (a.silu) {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int j = 0; j < 4; j++) {
+                    float2 s = bias;
 #pragma unroll
-                    for (int i = 0; i < K; i++) {
-                        float s = bias[i];
-#pragma unroll
-                        for (int k = 0; k < W; k++) s = __fmaf_rn(w[k][i], x[j + k][i], s);
-                        const float sg = sigmoid(s);
-                        const float f = __fmul_rn(sg, __fmaf_rn(s, __fsub_rn(1.0f, sg), 1.0f));
-                        dc[W - 1 + j][i] = t + j < len ? __fmul_rn(dc[W - 1 + j][i], f) : 0.0f;
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (t + j < t1) {  // the run's own positions
-#pragma unroll
-                    for (int i = 0; i < K; i++) {
-                        db[i] = __fadd_rn(db[i], dc[W - 1 + j][i]);
-#pragma unroll
-                        for (int k = 0; k < W; k++) dw[k][i] = __fmaf_rn(dc[W - 1 + j][i], x[j + k][i], dw[k][i]);
-                    }
+                    for (int k = 0; k < W; k++) s = __ffma2_rn(w[k], x[j + k], s);
+                    const float2 sg = make_float2(sigmoid(s.x), sigmoid(s.y));
+                    const float2 rest = __fadd2_rn(make_float2(1.0f, 1.0f), make_float2(-sg.x, -sg.y));
+                    const float2 f = __fmul2_rn(sg, __ffma2_rn(s, rest, make_float2(1.0f, 1.0f)));
+                    dc[W - 1 + j] = __fmul2_rn(dc[W - 1 + j], f);
                 }
+                if (t + 4 > len) {  // 0 whatever f is
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (t + j >= len) dc[W - 1 + j] = zero;
+                }
+            }
+            if (t < t1) {  // the run's own positions (those behind t1, only behind the last run's, have dc = 0)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    db = __fadd2_rn(db, dc[W - 1 + j]);
+#pragma unroll
+                    for (int k = 0; k < W; k++) dw[k] = __ffma2_rn(dc[W - 1 + j], x[j + k], dw[k]);
+                }
+            }
             // dx of the positions W - 1 earlier
+            float2 o[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int td = t + j - (W - 1);
-                T* to = td >= 0 ? static_cast<T*>(a.dx) : static_cast<T*>(a.dwin);
-                if (td < first || td >= t1 || !to) continue;
-                float o[K];
+                o[j] = __fmul2_rn(w[0], dc[j + W - 1]);
 #pragma unroll
-                for (int i = 0; i < K; i++) {
-                    float s = __fmul_rn(w[0][i], dc[j + W - 1][i]);
+                for (int k = 1; k < W; k++) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
+            }
+            const int td0 = t - (W - 1);
+            if (td0 >= t0 && td0 + 4 <= inner) {
+                if (dxb && have > 0) {
+                    T* to = dxb + (int64_t)td0 * a.D;
 #pragma unroll
-                    for (int k = 1; k < W; k++) s = __fmaf_rn(w[k][i], dc[j + W - 1 - k][i], s);
-                    o[i] = s;
+                    for (int j = 0; j < 4; j++) {
+                        const float v[K] = {o[j].x, o[j].y};
+                        store_pack<K>(to + (int64_t)j * a.D, v, have, VEC);
+                    }
                 }
-                // this input's place in the window that leaves, if it has one
-                const int kw = td - (len - (W - 1));
-                if (gwin && kw >= 0 && kw < W - 1) {
-                    const P p = raw_row<VEC, K>(gwin + ((int64_t)b * (W - 1) + kw) * a.D + c, have);
+            } else if (have > 0) {
 #pragma unroll
-                    for (int i = 0; i < K; i++) o[i] = __fadd_rn(o[i], to_f(p.v[i]));
+                for (int j = 0; j < 4; j++) {
+                    const int td = td0 + j;
+                    if (td < first || td >= t1) continue;
+                    // this input's place in the window that leaves, if it has one
+                    const int kw = td - (len - (W - 1));
+                    if (gwin && kw >= 0 && kw < W - 1)
+                        o[j] = __fadd2_rn(o[j],
+                                          pair(raw_row<VEC, K>(gwin + ((int64_t)b * (W - 1) + kw) * a.D + c, have)));
+                    const float v[K] = {o[j].x, o[j].y};
+                    T* dwin = static_cast<T*>(a.dwin);
+                    if (td >= 0 ? dxb != nullptr : dwin != nullptr)
+                        store_pack<K>(td >= 0 ? dxb + (int64_t)td * a.D
+                                              : dwin + ((int64_t)b * (W - 1) + td + W - 1) * a.D + c,
+                                      v, have, VEC);
                 }
-                store_pack<K>(to + (td >= 0 ? (int64_t)b * a.L + td : (int64_t)b * (W - 1) + td + W - 1) * a.D + c, o, have,
-                              VEC);
             }
 #pragma unroll
-            for (int j = 0; j < W - 1; j++)
-#pragma unroll
-                for (int i = 0; i < K; i++) x[j][i] = x[j + 4][i], dc[j][i] = dc[j + 4][i];
+            for (int j = 0; j < W - 1; j++) x[j] = x[j + 4], dc[j] = dc[j + 4];
         }
     }
     if (!a.part) return;
-#pragma unroll
-    for (int i = 0; i < K; i++) {
-#pragma unroll
-        for (int k = 0; k < W; k++) sh[g][cx][i * (W + 1) + k] = dw[k][i];
-        sh[g][cx][i * (W + 1) + W] = db[i];
+    if constexpr (VEC) {
+        cp_async_wait();
+        __syncthreads();  // the slots are done with
     }
+    float(*sh)[32][S + 1] = reinterpret_cast<float(*)[32][S + 1]>(smem);
+#pragma unroll
+    for (int k = 0; k < W; k++) sh[g][cx][k] = dw[k].x, sh[g][cx][W + 1 + k] = dw[k].y;
+    sh[g][cx][W] = db.x, sh[g][cx][2 * W + 1] = db.y;
     __syncthreads();
     float* part = a.part + ((int64_t)b * gridDim.y + blockIdx.y) * a.D * (W + 1);
     for (int e = threadIdx.x; e < 32 * S; e += 256) {
@@ -383,11 +458,12 @@ __global__ void __launch_bounds__(128) step_kernel(const Args a) {
     for (int k = 0; k < W - 1; k++) store_pack<K>(win + (int64_t)k * a.D, row[k + 1], valid, vec);
 }
 
-// Channels a thread.  Wider packs need fewer loads, but what a thread holds for
-// each channel (4 taps, 7 inputs; backward 4 sums and 7 dc more) costs
-// registers, and occupancy is worth more than the loads: 8 x 2048 x 1536 bf16
-// took 41 us forward with 8 channels (209 registers) and 37 with 4.
-constexpr int KF = 4, KB = 2;
+// Channels a thread of the forward kernels.  Wider packs need fewer loads, but
+// what a thread holds for each channel (4 taps, 7 inputs) costs registers, and
+// occupancy is worth more than the loads: 8 x 2048 x 1536 bf16 took 41 us with
+// 8 channels (209 registers) and 37 with 4; with the loads off their branches
+// 27 us (100 MB, 3.7 TB/s).
+constexpr int KF = 4;
 
 template <typename T, int W>
 static int forward(Args& a, cudaStream_t s) {
@@ -412,24 +488,36 @@ static int step(const Args& a, cudaStream_t s) {
     return MI_OK;
 }
 
-// positions a thread: 32 where that still gives every SM 4 CTAs
+// Positions a thread: of 16, 32 and 64 the one with the least rounds of 3 CTAs
+// an SM times what a run walks, 4 positions beyond its own.  8 x 2048 x 1536:
+// 52 us with 64 (2 rounds), 61 with 32 (4 rounds).
 static inline int bwd_run(int batch, int L, int D) {
-    return (int64_t)cdiv(D, 32 * KB) * cdiv(L, 32 * BWD_RUNS) * batch >= 148 * 4 ? 32 : 16;
+    int64_t best = 16, least = INT64_MAX;
+    for (int run = 64; run >= 16; run /= 2) {
+        const int64_t ctas = (int64_t)cdiv(D, 32 * PAIR) * cdiv(L, run * BWD_RUNS) * batch;
+        const int64_t cost = (ctas + 148 * 3 - 1) / (148 * 3) * (run + 4);
+        if (cost < least) least = cost, best = run;
+    }
+    return (int)best;
 }
 static inline int64_t parts(int batch, int L, int D) {
     return (int64_t)batch * cdiv(L, bwd_run(batch, L, D) * BWD_RUNS);
 }
 
+template <typename T, int W, bool VEC>
+static int backward_vec(const Args& a, cudaStream_t s) {
+    constexpr int smem = bwd_smem<T, W, VEC>();
+    static std::atomic<uint64_t> allowed{0};
+    if (!allow_smem(bwd_kernel<T, W, VEC>, smem, allowed)) return MI_ERR_CUDA;
+    const dim3 grid(cdiv(a.D, 32 * PAIR), cdiv(a.L, a.run * BWD_RUNS), a.batch);
+    bwd_kernel<T, W, VEC><<<grid, 256, smem, s>>>(a);
+    MI_CHECK_LAUNCH();
+    return MI_OK;
+}
 template <typename T, int W>
 static int backward(Args& a, cudaStream_t s) {
     a.run = bwd_run(a.batch, a.L, a.D);
-    const dim3 grid(cdiv(a.D, 32 * KB), cdiv(a.L, a.run * BWD_RUNS), a.batch);
-    if (a.vec)
-        bwd_kernel<T, W, KB, true><<<grid, 256, 0, s>>>(a);
-    else
-        bwd_kernel<T, W, KB, false><<<grid, 256, 0, s>>>(a);
-    MI_CHECK_LAUNCH();
-    return MI_OK;
+    return a.vec ? backward_vec<T, W, true>(a, s) : backward_vec<T, W, false>(a, s);
 }
 
 static int check(int batch, int L, int D, int W, int dtype) {
@@ -504,7 +592,8 @@ extern "C" int mi_causal_conv1d_backward(const void* dy, int64_t dy_batch, int64
     a.dy = dy, a.gb = dy_batch, a.gl = dy_row, a.dwin_out = dwin_out, a.dx = dx, a.dwin = dwin;
     a.part = dw || dbias ? static_cast<float*>(workspace) : nullptr;
     a.batch = batch, a.L = L, a.D = D, a.silu = silu;
-    a.vec = D % KF == 0 && x_batch % KF == 0 && x_row % KF == 0 && dy_batch % KF == 0 && dy_row % KF == 0 &&
+    const int pack = dtype == MI_DT_F32 ? 4 : 8;
+    a.vec = D % pack == 0 && x_batch % pack == 0 && x_row % pack == 0 && dy_batch % pack == 0 && dy_row % pack == 0 &&
             mi::aligned16(x) && mi::aligned16(dy) && mi::aligned16(win) && mi::aligned16(dwin_out) &&
             mi::aligned16(dx) && mi::aligned16(dwin) && mi::aligned16(w) && mi::aligned16(bias);
     int (*fn)(Args&, cudaStream_t) = nullptr;

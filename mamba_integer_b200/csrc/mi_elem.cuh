@@ -8,6 +8,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "mi_common.cuh"
 
 namespace mi {
@@ -92,6 +94,24 @@ __device__ __forceinline__ void fetch_pack(T* slot, const T* p, const void* any,
 #pragma unroll
         for (int i = 0; i < K; i++) slot[i] = i < valid ? p[i] : from_f<T>(0.0f);
     }
+}
+
+// Lets `kernel` have its shared memory, once for each device (by bit).  `regs`:
+// the registers a thread that its launch must bring along (what setmaxnreg
+// deals out has to be there, or the workers would wait for it without end).
+template <typename K>
+static bool allow_smem(K* kernel, size_t bytes, std::atomic<uint64_t>& done, int regs = 0) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return true;
+    if (regs) {
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, kernel) != cudaSuccess || f.numRegs < regs) return false;
+    }
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 // 2^x to 2 ulp; results below the normal range are zero.

@@ -22,7 +22,6 @@
 // Tiles of TT positions by CB channels are staged in shared memory as
 // (dt, dt u); positions from the length on are staged with dt = 0, B = C = 0,
 // where the recurrence leaves the state as it is.
-#include <atomic>
 #include <type_traits>
 
 #include "mi_elem.cuh"
@@ -1243,24 +1242,6 @@ static int check(int batch, int L, int D, int N, int dtype) {
     if (dtype != MI_DT_F32 && dtype != MI_DT_BF16 && dtype != MI_DT_F16) return MI_ERR_INVALID;
     if (N > MAX_N || batch > 65535) return MI_ERR_UNSUPPORTED;
     return MI_OK;
-}
-
-// Lets `kernel` have its shared memory, once for each device (by bit).  `regs`:
-// the registers a thread that its launch must bring along (what setmaxnreg
-// deals out has to be there, or the workers would wait for it without end).
-template <typename K>
-static bool allow_smem(K* kernel, size_t bytes, std::atomic<uint64_t>& done, int regs = 0) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return false;
-    const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return true;
-    if (regs) {
-        cudaFuncAttributes f;
-        if (cudaFuncGetAttributes(&f, kernel) != cudaSuccess || f.numRegs < regs) return false;
-    }
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) return false;
-    done.fetch_or(bit, std::memory_order_relaxed);
-    return true;
 }
 
 // the chunks' starting states (REV: what they receive from behind), in a.cst
