@@ -13,12 +13,14 @@
 // output, so the bound is HBM: x and r in, s and y out.  A row belongs to TPR
 // threads (a warp up to 1024 columns of 16 bits); rows that need more than a
 // warp reduce through shared memory.
+#include <type_traits>
+
 #include "mi_elem.cuh"
 
 namespace mi {
 namespace rms {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256, CTAS = 148 * 2;  // two CTAs an SM at most
 
 struct Args {
     const void* x;
@@ -78,102 +80,140 @@ __device__ __forceinline__ Pack<T, K> row_pack(const T* p, int valid) {
     return r;
 }
 
+template <typename T, typename R, int K, int NV, int TPR>
+struct InSlots {  // by thread
+    static constexpr int BLOCK = TPR > THREADS ? TPR : THREADS;
+    Pack<T, K> x[NV][BLOCK];
+    Pack<R, K> r[NV][BLOCK];
+};
+
+// Rows are dealt to at most CTAS CTAs; the next row's packs come into the
+// thread's own slots while a row is worked on.  32768 x 768 bf16 to int8 with a
+// residual 31 us (177 MB, 5.7 TB/s) against 40 with a warp for each row, whose
+// loads and arithmetic take turns, and 39 with 3 CTAs an SM (80 registers
+// instead of 102); 16384 x 768 to bf16 17 us (100 MB, 6.0 TB/s) against 21.
 // T: element type of x and y; R: of the residual and s.  A thread holds NV
 // packs of K elements, TPR * K apart.
 template <typename T, typename R, int K, int NV, int TPR, bool VEC, bool QUANT>
-__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ? 1 : 2) fwd_kernel(const Args a) {
     __shared__ float red[32];
+    extern __shared__ __align__(16) unsigned char smem[];
+    InSlots<T, R, K, NV, TPR>& slots = *reinterpret_cast<InSlots<T, R, K, NV, TPR>*>(smem);
     constexpr int ROWS = (TPR > THREADS ? TPR : THREADS) / TPR;
-    const int lane = threadIdx.x % TPR;
+    const int tid = threadIdx.x, lane = tid % TPR;
     grid_dependency_sync();
-    const int64_t t = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-    // the threads of a row that does not exist still take part in the barriers
-    const bool live = t < a.T;
-    const T* x = static_cast<const T*>(a.x) + t * a.ldx;
-    const R* r = static_cast<const R*>(a.r) + t * a.ldr;
-    float s[NV][K];
-    float acc = 0.0f;
-    Pack<T, K> px[NV];
-    Pack<R, K> pr[NV];
+    auto fetch = [&](int64_t t) {
+        const T* x = static_cast<const T*>(a.x) + t * a.ldx + lane * K;
+        const R* r = static_cast<const R*>(a.r) + t * a.ldr + lane * K;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int c = (j * TPR + lane) * K;
-        const int valid = live ? a.D - c : 0;
-        px[j] = row_pack<VEC, K>(x + c, valid);
-        if (a.r) pr[j] = row_pack<VEC, K>(r + c, valid);
-    }
+        for (int j = 0; j < NV; j++) {
+            const int c = j * TPR * K, valid = t < a.T ? a.D - c - lane * K : 0;
+            fetch_pack<K>(slots.x[j][tid].v, x + c, a.x, valid, true);
+            if (a.r) fetch_pack<K>(slots.r[j][tid].v, r + c, a.r, valid, true);
+        }
+        cp_async_commit();
+    };
+    if (VEC) fetch((int64_t)blockIdx.x * ROWS + tid / TPR);
+#pragma unroll 1
+    for (int64_t t0 = (int64_t)blockIdx.x * ROWS; t0 < a.T; t0 += (int64_t)gridDim.x * ROWS) {
+        const int64_t t = t0 + tid / TPR;
+        // the threads of a row that does not exist still take part in the barriers
+        const bool live = t < a.T;
+        float s[NV][K];
+        float acc = 0.0f;
+        Pack<T, K> px[NV];
+        Pack<R, K> pr[NV];
+        if constexpr (VEC) {
+            cp_async_wait();
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int c = (j * TPR + lane) * K;
-        const int valid = live ? a.D - c : 0;
-#pragma unroll
-        for (int i = 0; i < K; i++) s[j][i] = to_f(px[j].v[i]);
-        if (a.r) {  // the norm is of the sum as it is kept, so that a backward pass finds the same one
-#pragma unroll
-            for (int i = 0; i < K; i++) {
-                pr[j].v[i] = from_f<R>(__fadd_rn(s[j][i], to_f(pr[j].v[i])));
-                s[j][i] = to_f(pr[j].v[i]);
+            for (int j = 0; j < NV; j++) {
+                px[j] = slots.x[j][tid];
+                if (a.r) pr[j] = slots.r[j][tid];
             }
-            R* o = static_cast<R*>(a.sum) + t * a.D + c;
-            if (VEC) {
-                if (valid > 0) *reinterpret_cast<Pack<R, K>*>(o) = pr[j];
-            } else {
+            fetch(t + (int64_t)gridDim.x * ROWS);
+        } else {
 #pragma unroll
-                for (int i = 0; i < K; i++)
-                    if (i < valid) o[i] = pr[j].v[i];
+            for (int j = 0; j < NV; j++) {
+                const int c = (j * TPR + lane) * K;
+                const int valid = live ? a.D - c : 0;
+                px[j] = row_pack<VEC, K>(static_cast<const T*>(a.x) + t * a.ldx + c, valid);
+                if (a.r) pr[j] = row_pack<VEC, K>(static_cast<const R*>(a.r) + t * a.ldr + c, valid);
             }
         }
-#pragma unroll
-        for (int i = 0; i < K; i++) acc = __fmaf_rn(s[j][i], s[j][i], acc);
-    }
-    acc = row_reduce<TPR, false>(acc, red);
-    const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(acc, (float)a.D), a.eps)));
-    if (live && lane == 0 && a.rstd) a.rstd[t] = rstd;
-    float amax = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NV; j++) {
-        const int c = (j * TPR + lane) * K;
-        const Pack<float, K> w = row_pack<VEC, K>(a.w + c, a.D - c);
-#pragma unroll
-        for (int i = 0; i < K; i++) {
-            s[j][i] = __fmul_rn(__fmul_rn(s[j][i], rstd), w.v[i]);
-            if (QUANT) amax = max_nan(amax, fabsf(s[j][i]));
-        }
-        if (!QUANT && live && c < a.D) store_pack<K>(static_cast<T*>(a.y) + t * a.D + c, s[j], a.D - c, VEC);
-    }
-    if (QUANT) {
-        amax = row_reduce<TPR, true>(amax, red);
-        float scale;
-        const float inv = quant_inv_scale(amax, scale);
-        const uint32_t some = amax < __int_as_float(0x7f800000) ? 0xffffffffu : 0u;
-        if (live && lane == 0) a.xscale[t] = scale;
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int c = (j * TPR + lane) * K;
-            if (!live || c >= a.D) continue;
-            int8_t* o = a.xq + t * a.D + c;
-            static_assert(K == 8, "two words of 4");
-            alignas(8) uint32_t word[2];
-            // 1.5 2^23 + v holds v rounded to even in its low bits: |v| is at most 127 as it is rounded, or the
-            // row has an infinity or a NaN, and then all of its q are 0 (infinity times 0, NaN) like quantise_rows'
+            const int valid = live ? a.D - c : 0;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                uint32_t b[4];
+            for (int i = 0; i < K; i++) s[j][i] = to_f(px[j].v[i]);
+            if (a.r) {  // the norm is of the sum as it is kept, so that a backward pass finds the same one
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    b[i] = __float_as_uint(__fadd_rn(__fmul_rn(s[j][4 * h + i], inv), 12582912.0f));
-                word[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & some;
+                for (int i = 0; i < K; i++) {
+                    pr[j].v[i] = from_f<R>(__fadd_rn(s[j][i], to_f(pr[j].v[i])));
+                    s[j][i] = to_f(pr[j].v[i]);
+                }
+                R* o = static_cast<R*>(a.sum) + t * a.D + c;
+                if (VEC) {
+                    if (valid > 0) *reinterpret_cast<Pack<R, K>*>(o) = pr[j];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K; i++)
+                        if (i < valid) o[i] = pr[j].v[i];
+                }
             }
-            const Pack<int8_t, K>& q = reinterpret_cast<const Pack<int8_t, K>&>(word);
-            if (VEC) {
-                *reinterpret_cast<Pack<int8_t, K>*>(o) = q;
-            } else {
 #pragma unroll
-                for (int i = 0; i < K; i++)
-                    if (i < a.D - c) o[i] = q.v[i];
+            for (int i = 0; i < K; i++) acc = __fmaf_rn(s[j][i], s[j][i], acc);
+        }
+        acc = row_reduce<TPR, false>(acc, red);
+        const float rstd = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(acc, (float)a.D), a.eps)));
+        if (live && lane == 0 && a.rstd) a.rstd[t] = rstd;
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int c = (j * TPR + lane) * K;
+            const Pack<float, K> w = row_pack<VEC, K>(a.w + c, a.D - c);
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                s[j][i] = __fmul_rn(__fmul_rn(s[j][i], rstd), w.v[i]);
+                if (QUANT) amax = max_nan(amax, fabsf(s[j][i]));
+            }
+            if (!QUANT && live && c < a.D) store_pack<K>(static_cast<T*>(a.y) + t * a.D + c, s[j], a.D - c, VEC);
+        }
+        if (QUANT) {
+            amax = row_reduce<TPR, true>(amax, red);
+            float scale;
+            const float inv = quant_inv_scale(amax, scale);
+            const uint32_t some = amax < __int_as_float(0x7f800000) ? 0xffffffffu : 0u;
+            if (live && lane == 0) a.xscale[t] = scale;
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int c = (j * TPR + lane) * K;
+                if (!live || c >= a.D) continue;
+                int8_t* o = a.xq + t * a.D + c;
+                static_assert(K == 8, "two words of 4");
+                alignas(8) uint32_t word[2];
+                // 1.5 2^23 + v holds v rounded to even in its low bits: |v| is at most 127 as it is rounded, or the
+                // row has an infinity or a NaN, and then all of its q are 0 (infinity times 0, NaN) like quantise_rows'
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t b[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        b[i] = __float_as_uint(__fadd_rn(__fmul_rn(s[j][4 * h + i], inv), 12582912.0f));
+                    word[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410) & some;
+                }
+                const Pack<int8_t, K>& q = reinterpret_cast<const Pack<int8_t, K>&>(word);
+                if (VEC) {
+                    *reinterpret_cast<Pack<int8_t, K>*>(o) = q;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K; i++)
+                        if (i < a.D - c) o[i] = q.v[i];
+                }
             }
         }
     }
+    if (VEC) cp_async_wait();
 }
 
 // Rows are dealt to the CTAs in a fixed order; each thread keeps the sums of
@@ -181,8 +221,7 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS) fwd_kernel(cons
 // through shared memory and writes one row of partial sums, and
 // column_sum_kernel adds those.  Those sums leave registers for two CTAs an SM
 // and none for the next row, which asynchronous copies bring into the thread's
-// own slots while a row is worked on: 16384 x 768 bf16 27 us (100 MB, 3.7 TB/s)
-// against 40 with the rows loaded as they are needed.
+// own slots while a row is worked on.
 // registers that a thread of the backward pass holds for its packs, and the CTAs an SM that they leave room for
 template <typename T, typename R, int K, int NV>
 constexpr int held = (2 * K + (sizeof(T) + 2 * sizeof(R)) * K / 4) * NV;
@@ -346,11 +385,11 @@ static inline int threads_per_row(int T, int D, int K) {
     return packs > 4 * 32 || (packs > 32 && T <= 148 * 4) ? 128 : 32;
 }
 
-// two CTAs an SM, as many as the backward pass's registers allow: each keeps its sums of dw to the end
+// the backward pass's CTAs: each keeps its sums of dw to the end
 static inline int grid_of(int T, int D) {
     const int tpr = threads_per_row(T, D, 8);
     const int grid = cdiv(T, (tpr > THREADS ? tpr : THREADS) / tpr);
-    return grid < 148 * 2 ? grid : 148 * 2;
+    return grid < CTAS ? grid : CTAS;
 }
 
 template <typename T, typename R, int K, int TPR, bool BWD, bool QUANT>
@@ -358,13 +397,16 @@ static int launch_nv(const Args& a, int grid, int block, cudaStream_t s) {
     const int nv = cdiv(cdiv(a.D, K), TPR);
 #define MI_RMS_CASE(NV, VEC)                                                                     \
     do {                                                                                         \
+        using S = std::conditional_t<BWD, Slots<T, R, K, NV, TPR>, InSlots<T, R, K, NV, TPR>>;   \
+        constexpr int smem = sizeof(S);                                                          \
+        static std::atomic<uint64_t> allowed{0};                                                 \
         if constexpr (BWD) {                                                                     \
-            constexpr int smem = sizeof(Slots<T, R, K, NV, TPR>);                                \
-            static std::atomic<uint64_t> allowed{0};                                             \
             if (!allow_smem(bwd_kernel<T, R, K, NV, TPR, VEC>, smem, allowed)) return MI_ERR_CUDA; \
             bwd_kernel<T, R, K, NV, TPR, VEC><<<grid, block, smem, s>>>(a);                      \
-        } else                                                                                   \
-            MI_LAUNCH_DEPENDENT(fwd_kernel<T, R, K, NV, TPR, VEC, QUANT>, grid, block, 0, s, a); \
+        } else {                                                                                 \
+            if (!allow_smem(fwd_kernel<T, R, K, NV, TPR, VEC, QUANT>, smem, allowed)) return MI_ERR_CUDA; \
+            MI_LAUNCH_DEPENDENT(fwd_kernel<T, R, K, NV, TPR, VEC, QUANT>, grid, block, smem, s, a); \
+        }                                                                                        \
     } while (0)
     if (!a.vec)
         MI_RMS_CASE(4, false);
@@ -387,7 +429,7 @@ static int launch(const Args& a, int grid_cap, cudaStream_t s) {
     const int tpr = threads_per_row(a.T, a.D, K);
     const int block = tpr > THREADS ? tpr : THREADS;
     int grid = cdiv(a.T, block / tpr);
-    if (grid_cap && grid > grid_cap) grid = grid_cap;
+    if (grid > grid_cap) grid = grid_cap;
     switch (tpr) {
         case 32: return launch_nv<T, R, K, 32, BWD, QUANT>(a, grid, block, s);
         case 128: return launch_nv<T, R, K, 128, BWD, QUANT>(a, grid, block, s);
@@ -429,8 +471,8 @@ static int mi_rms_forward(const void* x, int64_t ldx, const void* r, int64_t ldr
     if (r) vec = vec && ldr % 8 == 0 && mi::aligned16(r) && mi::aligned16(sum);
     vec = vec && (xq ? (reinterpret_cast<uintptr_t>(xq) & 7) == 0 : mi::aligned16(y));
     a.vec = vec;
-    if (xq) return mi::rms::dispatch<false, true>(a, dtype, r ? rdtype : dtype, 0, (cudaStream_t)stream);
-    return mi::rms::dispatch<false, false>(a, dtype, r ? rdtype : dtype, 0, (cudaStream_t)stream);
+    if (xq) return mi::rms::dispatch<false, true>(a, dtype, r ? rdtype : dtype, mi::rms::CTAS, (cudaStream_t)stream);
+    return mi::rms::dispatch<false, false>(a, dtype, r ? rdtype : dtype, mi::rms::CTAS, (cudaStream_t)stream);
 }
 
 extern "C" int mi_rms_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight, void* y,
