@@ -378,6 +378,29 @@ def test_conv(sel, cuda_dev, size, dtype, bias, silu, win):
         ref.check(t, want["d" + m], mag["d" + m], 64 + (b * n if m in ("w", "bias") else 0), "d" + m)
 
 
+@pytest.mark.parametrize("size", [(222, 509, 8, 4), (444, 510, 8, 3), (2, 300, 72, 4)])
+def test_conv_gradients_of_long_runs(sel, cuda_dev, size):
+    """Runs of 32 and of 64 positions, lengths that end in them, lanes beyond the last channel."""
+    b, n, d, k = size
+    lens = [(37 * i) % (n + 1) for i in range(b)]
+    a = conv_inputs(cuda_dev, BF16, *size, win=True, lengths=lens)
+    clean = {key: t.clone() if isinstance(t, torch.Tensor) else t for key, t in a.items()}
+    dy = torch.randn(b, n, d, device=cuda_dev).to(BF16)
+    dwin = torch.randn(b, k - 1, d, device=cuda_dev).to(BF16)
+    for i, v in enumerate(lens):
+        a["x"][i, v:] = dy[i, v:] = float("nan")
+        clean["x"][i, v:] = 0
+    args = dict(clean, dy=dy.nan_to_num(0.0), dwin=dwin)
+    want, mag = ref.conv(args), ref.conv(args, mag=True)
+    leaves = {m: a[m].clone().requires_grad_(True) for m in ("x", "w", "bias", "win")}
+    y, out = call_conv(sel, a, **leaves)
+    ref.check(y, want["y"], mag["y"], 32, "y")
+    got = torch.autograd.grad([y, out], list(leaves.values()), [dy, dwin])
+    for m, t in zip(leaves, got):
+        ref.check(t, want["d" + m], mag["d" + m], 64 + (b * n if m in ("w", "bias") else 0), "d" + m)
+    assert not any(got[0][i, v:].any() for i, v in enumerate(lens))
+
+
 @pytest.mark.parametrize("n", [5, 40, 150])
 def test_conv_lengths(sel, cuda_dev, n):
     lens = [0, 1, 2, n - 1, n, n + 7, -1]
@@ -438,7 +461,7 @@ def test_conv_step(sel, cuda_dev, dtype, d, k, silu):
 # norm
 # ---------------------------------------------------------------------------
 NORM_SIZES = [(1, 1), (3, 7), (2, 32), (5, 100), (9, 256), (4, 768), (3, 1000), (2, 1025), (1, 2048), (2, 4096), (3, 8191),
-              (1, 16384), (700, 264)]
+              (1, 16384), (700, 264), (2500, 40), (1250, 1032), (900, 4104)]  # the last: several rows a warp, or block
 
 
 @pytest.mark.parametrize("size", NORM_SIZES)
@@ -497,6 +520,29 @@ def test_norm_strides_zeros_and_infinities(sel, cuda_dev):
     _, s = sel.rms_norm(x2, w, residual=x2)
     (g,) = torch.autograd.grad(s.sum(), x2)
     assert torch.equal(g, torch.full_like(x2, 2))
+
+
+def test_norm_quant_gives_the_rows_of_quantize_rows(sel, cuda_dev):
+    """Bit for bit from the fp32 norm, rows with infinities and NaN (no value of theirs is kept) too."""
+    from mamba_integer_b200 import kernels
+    x, w = 3 * torch.randn(3000, 200, device=cuda_dev), torch.randn(200, device=cuda_dev)
+    x[5, 7], x[6, 199] = float("nan"), float("inf")
+    x[7] = 0
+    y, _ = sel.rms_norm(x, w)
+    one = torch.ones(200, device=cuda_dev)
+    q, scale, _ = sel.rms_norm_quant(x, w)
+    want, wscale = kernels.quantize_rows(y[:8])
+    assert torch.equal(q[:8], want[:, :200]) and torch.equal(scale[:8].isnan(), wscale.isnan())
+    fine = ~wscale.isnan()
+    assert torch.equal(scale[:8][fine], wscale[fine])
+    want, wscale = kernels.quantize_rows(y[10:])
+    assert torch.equal(q[10:], want[:, :200]) and torch.equal(scale[10:], wscale)
+    # infinite values of the norm itself: an infinite weight
+    one[4] = float("inf")
+    y, _ = sel.rms_norm(x[10:], one)
+    q, scale, _ = sel.rms_norm_quant(x[10:], one)
+    want, wscale = kernels.quantize_rows(y)
+    assert torch.equal(q, want[:, :200]) and torch.equal(scale, wscale)
 
 
 def test_norm_quant_feeds_the_ternary_product(sel, cuda_dev):
