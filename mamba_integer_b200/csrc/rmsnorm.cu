@@ -378,7 +378,8 @@ constexpr int MAX_D = 16384;  // 512 threads of 4 packs
 
 // Threads of a row: a warp where 4 packs of 8 a thread hold it, 128 or 512
 // where they do not, and 128 too for the few rows of a decode batch, which
-// would leave most of the GPU without a warp.
+// would leave most of the GPU without a warp: 256 x 1024 2.7 us with 128 and
+// 4.3 with 32; 32768 x 768 59 and 31.
 static inline int threads_per_row(int T, int D, int K) {
     const int packs = cdiv(D, K);
     if (packs > 4 * 128) return 512;
