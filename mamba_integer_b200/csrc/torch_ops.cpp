@@ -14,6 +14,7 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <unordered_set>
@@ -201,16 +202,21 @@ Tensor empty_as(const Tensor& t, bool want = true) {
     return want && t.defined() ? at::empty(t.sizes(), t.options()) : Tensor();
 }
 
-// Gradients of first order: a second backward pass through them is refused when it is taken.
-variable_list once(variable_list grads, const variable_list& incoming) {
-    if (!at::GradMode::is_enabled()) return grads;
-    bool any = false;
-    for (const auto& t : incoming) any = any || (t.defined() && t.requires_grad());
-    if (!any) return grads;
-    for (auto& t : grads)
-        if (t.defined()) t = t.detach().requires_grad_(true);
-    return torch::autograd::DelayedError("the float Mamba operators have gradients of first order only",
-                                         (int64_t)grads.size())(std::move(grads));
+// The gradients as backward() returns them: of first order.  Under create_graph
+// (`create`: the backward pass was entered with gradients on) they depend on
+// what the forward pass saved, whatever came in, so they get a node over all of
+// that: a second backward pass that reaches it, by whichever way, is refused.
+variable_list once(variable_list grads, bool create, const variable_list& saved, const variable_list& incoming) {
+    using namespace torch::autograd;
+    if (!create || !(any_variable_requires_grad(saved) || any_variable_requires_grad(incoming))) return grads;
+    const auto refusal = std::make_shared<Error>("the float Mamba operators have gradients of first order only",
+                                                 collect_next_edges(saved, incoming));
+    for (auto& t : grads) {
+        if (!t.defined()) continue;
+        t = t.detach();
+        set_history(t, refusal);
+    }
+    return grads;
 }
 
 // ---------------------------------------------------------------------------
@@ -255,6 +261,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
         const bool softplus = ctx->saved_data["softplus"].toBool();
         const int64_t need = ctx->saved_data["need"].toInt();
         const int64_t batch = u.size(0), L = u.size(1), d = u.size(2), N = A.size(1);
+        const bool create = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         Place place(u);
         const Tensor dy = g[0].defined() ? unit(g[0]) : at::zeros({batch, L, d}, u.options());
@@ -271,8 +278,7 @@ struct SelectiveScan : torch::autograd::Function<SelectiveScan> {
                   fptr(dA), ptr(dB), ptr(dC), fptr(dD), ptr(dz), fptr(dbias), fptr(dh0), ptr(ws), batch, L, d, N,
                   softplus, dtype_code(u), place.stream),
               "mi_selective_scan_backward");
-        at::AutoGradMode back(true);
-        return once({du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, Tensor(), Tensor()}, g);
+        return once({du, ddelta, dA, dB, dC, dD, dz, dbias, dh0, Tensor(), Tensor()}, create, s, g);
     }
 };
 
@@ -381,6 +387,7 @@ struct CausalConv1d : torch::autograd::Function<CausalConv1d> {
         const bool silu = ctx->saved_data["silu"].toBool();
         const int64_t need = ctx->saved_data["need"].toInt();
         const int64_t batch = x.size(0), L = x.size(1), d = x.size(2), W = w.size(1);
+        const bool create = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         Place place(x);
         const Tensor dy = g[0].defined() ? unit(g[0]) : at::zeros({batch, L, d}, x.options());
@@ -394,8 +401,7 @@ struct CausalConv1d : torch::autograd::Function<CausalConv1d> {
                                            fptr(dbias), ptr(dwin), ptr(ws), batch, L, d, W, silu, dtype_code(x),
                                            place.stream),
               "mi_causal_conv1d_backward");
-        at::AutoGradMode back(true);
-        return once({dx, dw, dbias, dwin, Tensor(), Tensor()}, g);
+        return once({dx, dw, dbias, dwin, Tensor(), Tensor()}, create, s, g);
     }
 };
 
@@ -488,6 +494,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
             return {need & 1 ? dtotal.to(type) : Tensor(), Tensor(), need & 4 ? dtotal : Tensor(), Tensor()};
         }
         const int64_t T = sum.size(0), d = sum.size(1);
+        const bool create = at::GradMode::is_enabled();
         at::NoGradGuard no_grad;
         Place place(sum);
         const Tensor dy = aligned(g[0]);
@@ -500,8 +507,7 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
         check(mi.mi_rms_norm_backward(ptr(dy), ptr(dtotal), ptr(sum), st(sum, 0), fptr(w), fptr(rstd), ptr(dx), ptr(dr),
                                       fptr(dw), ptr(ws), T, d, dtype_code(dy), dtype_code(sum), place.stream),
               "mi_rms_norm_backward");
-        at::AutoGradMode back(true);
-        return once({need & 1 ? dx : Tensor(), dw, want_r ? (same ? dx : dr) : Tensor(), Tensor()}, g);
+        return once({need & 1 ? dx : Tensor(), dw, want_r ? (same ? dx : dr) : Tensor(), Tensor()}, create, s, g);
     }
 };
 

@@ -778,3 +778,36 @@ def test_graph_of_decode_steps(sel, cuda_dev):
         x.copy_(a["u"][:, t])
         assert all(torch.equal(p, q) for p, q in zip(token(), got[t]))
     assert torch.equal(h, h2) and torch.equal(win, win2)
+
+
+# ---------------------------------------------------------------------------
+# second order, values that are not finite, the variants that only large calls take
+# ---------------------------------------------------------------------------
+def test_gradients_of_gradients_are_refused(sel, cuda_dev):
+    """Under create_graph every gradient refuses a second pass, whatever the incoming one; without it none has a graph."""
+    z = lambda *s: torch.randn(*s, device=cuda_dev).requires_grad_(True)  # noqa: E731
+    x, w, A, B = z(2, 9, 8), z(8), z(8, 4), z(2, 9, 4)
+    calls = {"norm": (lambda: sel.rms_norm(x, w)[0], [x, w]),
+             "residual": (lambda: sel.rms_norm(x, w, residual=x * 2)[0], [x, w]),
+             "conv": (lambda: sel.causal_conv1d(x, A, bias=w, silu=True), [x, A, w]),
+             "scan": (lambda: sel.selective_scan(x, x, A, B, B, D=w, z=x, delta_softplus=True), [x, A, B, w])}
+    for name, (call, leaves) in calls.items():
+        got = torch.autograd.grad(call().sum(), leaves, create_graph=True)
+        for g in got:
+            assert g.requires_grad, name
+            with pytest.raises(RuntimeError, match="first order"):
+                g.sum().backward(retain_graph=True)
+        y = call()
+        plain = torch.autograd.grad(y, leaves, torch.ones_like(y).requires_grad_(True))
+        assert not any(g.requires_grad for g in plain), name
+        assert all(torch.equal(g, p) for g, p in zip(got, plain)), name
+    # beside another way to the leaf too: the term is not left out
+    y, _ = sel.rms_norm(x, w)
+    (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(y.sum() + (g * g).sum(), x)
+    # the sum alone is linear: its gradient may be differentiated
+    _, s = sel.rms_norm(x, w, residual=x * 2)
+    (g,) = torch.autograd.grad((s * s).sum(), x, create_graph=True)
+    (gg,) = torch.autograd.grad(g.sum(), x)
+    assert torch.equal(gg, torch.full_like(x, 18))
