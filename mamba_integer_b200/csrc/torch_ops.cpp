@@ -8,6 +8,7 @@
 // same checks and nodes in Python took 15 to 25 us a call and 130 us a backward
 // pass, more than their kernels.
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -137,6 +138,15 @@ template <typename... Ts>
 void no_grad_needed(const Ts&... ts) {
     TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad(ts...),
                 "the single-token and quantised forms have no backward pass: call them under torch.no_grad()");
+}
+
+// No formulas for tangents: forward-mode differentiation would lose them.
+template <typename... Ts>
+void no_tangents(const Ts&... ts) {
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        !((ts.defined() && ts._fw_grad(/*level=*/0).defined()) || ...) ||
+            !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+        "the float Mamba operators have no forward-mode derivative: an argument is a dual tensor");
 }
 
 // A training call that is being captured.  Where an earlier autograd graph is
@@ -312,6 +322,7 @@ std::tuple<Tensor, Tensor> selective_scan(const Tensor& u, const Tensor& delta, 
                                           const Tensor& C, const OptTensor& D_, const OptTensor& z_,
                                           const OptTensor& bias_, bool softplus, const OptTensor& h0_,
                                           const OptTensor& lengths_) {
+    no_tangents(u, delta, A_, B, C, given(D_), given(z_), given(bias_), given(h0_));
     TORCH_CHECK_VALUE(u.dim() == 3, "u must be [batch, L, channels], got ", u.sizes());
     const int64_t batch = u.size(0), L = u.size(1), d = u.size(2);
     const auto p = scan_arguments({batch, L}, u, delta, A_, B, C, D_, z_, bias_);
@@ -337,6 +348,7 @@ Tensor selective_scan_step(const Tensor& h, const Tensor& u, const Tensor& delta
                            bool softplus) {
     TORCH_CHECK_VALUE(u.dim() == 2, "u must be [batch, channels], got ", u.sizes());
     const int64_t batch = u.size(0), d = u.size(1);
+    no_tangents(h, u, delta, A_, B, C, given(D_), given(z_), given(bias_));
     no_grad_needed(h, u, delta, A_, B, C, given(D_), given(z_), given(bias_));
     const auto p = scan_arguments({batch}, u, delta, A_, B, C, D_, z_, bias_);
     in_place(h, u, {batch, d, p.N}, at::kFloat, "h");
@@ -422,6 +434,7 @@ std::tuple<Tensor, Tensor> conv_arguments(at::IntArrayRef lead, const Tensor& x,
 
 std::tuple<Tensor, Tensor> causal_conv1d(const Tensor& x, const Tensor& weight, const OptTensor& bias_, bool silu,
                                          const OptTensor& win_, const OptTensor& lengths_) {
+    no_tangents(x, weight, given(bias_), given(win_));
     TORCH_CHECK_VALUE(x.dim() == 3, "x must be [batch, L, channels], got ", x.sizes());
     const int64_t batch = x.size(0), L = x.size(1), d = x.size(2);
     const auto [w, bias] = conv_arguments({batch, L}, x, weight, bias_);
@@ -444,6 +457,7 @@ std::tuple<Tensor, Tensor> causal_conv1d(const Tensor& x, const Tensor& weight, 
 Tensor causal_conv1d_step(const Tensor& x, const Tensor& weight, const Tensor& win, const OptTensor& bias_, bool silu) {
     TORCH_CHECK_VALUE(x.dim() == 2, "x must be [batch, channels], got ", x.sizes());
     const int64_t batch = x.size(0), d = x.size(1);
+    no_tangents(x, weight, win, given(bias_));
     no_grad_needed(x, weight, win, given(bias_));
     const auto [w, bias] = conv_arguments({batch}, x, weight, bias_);
     in_place(win, x, {batch, w.size(1) - 1, d}, x.scalar_type(), "win");
@@ -516,6 +530,7 @@ struct Rows {
 };
 
 Rows rms_arguments(const Tensor& x, const Tensor& weight, const OptTensor& residual) {
+    no_tangents(x, weight, given(residual));
     activation(x, "x");
     const int64_t d = x.dim() ? x.size(-1) : 0;
     TORCH_CHECK_VALUE(d >= 1 && d <= 16384, "rows of 1 to 16384 columns, got x ", x.sizes());

@@ -22,8 +22,9 @@ Every call launches on the current stream of its tensors' device, allocates its
 outputs and workspaces with torch, and gives the same bits for the same inputs.
 Wrong shapes and placements raise ValueError, wrong types TypeError.  The calls
 are native (csrc/torch_ops.cpp, over the C ABI of include/mi_b200.h).
-CUDA tensors only; gradients are of first order; a prompt or training call has
-at most 65535 sequences.  To capture a training step in a CUDA graph, drop any
+CUDA tensors only; gradients are of first order and by backward passes (dual
+tensors of forward-mode differentiation raise NotImplementedError); a prompt or
+training call has at most 65535 sequences.  To capture a training step in a CUDA graph, drop any
 earlier result that still holds an autograd graph over the same leaves first
 (torch ties a leaf's gradient to the stream of the graph that is alive; the
 calls refuse such a capture where that is the default stream).

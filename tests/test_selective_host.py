@@ -215,3 +215,28 @@ def test_norm_formula_against_autograd():
     ds, dw = torch.autograd.grad(y, [s, w], dy)
     got = ref.norm(s, w, 1e-6, dy)
     assert torch.allclose(got["ds"], ds, rtol=1e-12, atol=1e-12) and torch.allclose(got["dw"], dw, rtol=1e-12)
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost; any argument may carry it, a view of a dual tensor too."""
+    from torch.autograd import forward_ad
+
+    step = dict(h=_t(2, 8, 4), u=_t(2, 8), delta=_t(2, 8), A=_t(8, 4), B=_t(2, 4), C=_t(2, 4), D=_t(8), z=_t(2, 8),
+                delta_bias=_t(8))
+    calls = [
+        (selective.selective_scan, dict(scan_args(), D=_t(8), z=_t(2, 5, 8), delta_bias=_t(8), h0=_t(2, 8, 4))),
+        (selective.selective_scan_step, step),
+        (selective.causal_conv1d, dict(x=_t(2, 5, 8), weight=_t(8, 4), bias=_t(8), win=_t(2, 3, 8))),
+        (selective.causal_conv1d_step, dict(x=_t(2, 8), weight=_t(8, 4), win=_t(2, 3, 8), bias=_t(8))),
+        (selective.rms_norm, dict(x=_t(4, 8), weight=_t(8), residual=_t(4, 8))),
+        (selective.rms_norm_quant, dict(x=_t(4, 8), weight=_t(8), residual=_t(4, 8))),
+    ]
+    for fn, args in calls:
+        for name, t in args.items():
+            with forward_ad.dual_level():
+                wide = forward_ad.make_dual(torch.zeros(2, *t.shape), torch.ones(2, *t.shape))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(**{**args, name: wide[0]})
+        with pytest.raises(ValueError, match="must be a CUDA tensor"):  # and without one the call goes on
+            fn(**args)
