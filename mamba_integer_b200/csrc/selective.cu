@@ -17,8 +17,10 @@
 // states, 8 x 2048 x 1536 positions and channels, are 86 us of exponentials
 // against 31 us of 16-bit loads and stores.
 //
-// Layout: LN lanes share a channel and hold 4 states each (N <= 4 LN; states
-// beyond N have A = B = C = 0 and stay 0), so a warp spans 32 / LN channels.
+// Layout: LN lanes share a channel and hold 4 states each (N <= 4 LN), so a warp
+// spans 32 / LN channels.  States beyond N have A = B = C = 0, and where there
+// are any (PAD) they are put back to 0 after each step: the channel's step size
+// and input reach them too, and 0 times an infinite one is not 0.
 // Tiles of TT positions by CB channels are staged in shared memory as
 // (dt, dt u); positions from the length on are staged with dt = 0, B = C = 0,
 // where the recurrence leaves the state as it is.
@@ -102,7 +104,6 @@ struct St {  // 4 states in two f32x2 pairs
 __device__ __forceinline__ St st(float4 v) { return {make_float2(v.x, v.y), make_float2(v.z, v.w)}; }
 __device__ __forceinline__ float4 f4(St s) { return make_float4(s.a.x, s.a.y, s.b.x, s.b.y); }
 __device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 neg(float2 v) { return make_float2(-v.x, -v.y); }
 __device__ __forceinline__ St mul(St x, float v) { return {__fmul2_rn(x.a, dup(v)), __fmul2_rn(x.b, dup(v))}; }
 __device__ __forceinline__ St mul(St x, St y) { return {__fmul2_rn(x.a, y.a), __fmul2_rn(x.b, y.b)}; }
 __device__ __forceinline__ St fma(St x, St y, St z) { return {__ffma2_rn(x.a, y.a, z.a), __ffma2_rn(x.b, y.b, z.b)}; }
@@ -111,6 +112,20 @@ __device__ __forceinline__ St fma(St x, float2 v, St z) { return {__ffma2_rn(x.a
 __device__ __forceinline__ float dot(St x, St y) {
     const float2 p = __ffma2_rn(x.b, y.b, __fmul2_rn(x.a, y.a));
     return __fadd_rn(p.x, p.y);
+}
+// Which of a lane's 4 states n0 .. n0 + 3 (lane order `perm`: n0 + (i ^ perm)) there are.
+template <bool PAD>
+__device__ __forceinline__ uint4 within(int n0, int N, int perm = 0) {
+    if (!PAD) return make_uint4(~0u, ~0u, ~0u, ~0u);
+    return make_uint4(n0 + perm < N ? ~0u : 0u, n0 + (1 ^ perm) < N ? ~0u : 0u, n0 + (2 ^ perm) < N ? ~0u : 0u,
+                      n0 + (3 ^ perm) < N ? ~0u : 0u);
+}
+__device__ __forceinline__ float2 masked(float2 v, uint32_t x, uint32_t y) {
+    return make_float2(__uint_as_float(__float_as_uint(v.x) & x), __uint_as_float(__float_as_uint(v.y) & y));
+}
+template <bool PAD>
+__device__ __forceinline__ St only(St s, uint4 m) {
+    return PAD ? St{masked(s.a, m.x, m.y), masked(s.b, m.z, m.w)} : s;
 }
 // A row of A for base 2.  An infinite A becomes a large one: it forgets the
 // state at once all the same, and a position of dt = 0 behind a length, which
@@ -461,7 +476,7 @@ __device__ __forceinline__ void stagers(const Args& a, typename Cfg<T, LN, CPL>:
 // that a chunk passes to the one before it, from a zero one behind it (REV =
 // true; dy, z and C in the place of u, delta and B), and the sum of its dt.
 // Only chunks > 1 need it: one more exponential for each state.
-template <typename T, int LN, int CPL, bool REV>
+template <typename T, int LN, int CPL, bool REV, bool PAD>
 __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
     using F = Cfg<T, LN, CPL>;
     constexpr int CB = F::CB, TT = F::TT;
@@ -484,6 +499,7 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
     const int c0 = warp * F::CL * CPL + cl * CPL;
+    const uint4 there = within<PAD>(n0, a.N);
     St A2[CPL], h[CPL];
     float sum[CPL], lim[CPL];
 #pragma unroll
@@ -518,6 +534,7 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
                     for (int k = 0; k < 4; k++) {
                         const int r = REV ? 3 - k : k;
                         h[j] = REV ? mul(e[r], fma(m[r], dup(v[r][j]), h[j])) : fma(e[r], h[j], mul(m[r], dup(v[r][j])));
+                        h[j] = only<PAD>(h[j], there);
                     }
                 }
             }
@@ -525,8 +542,8 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
         }
     };
     cta_barrier();
-    if (a.softplus)
-        run(std::false_type());
+    if (!PAD && a.softplus)  // with PAD one loop takes steps of either sign
+        run(std::bool_constant<PAD>());
     else
         run(std::true_type());
 #pragma unroll
@@ -568,7 +585,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a) {
 // ---------------------------------------------------------------------------
 // The scan of one chunk (the whole sequence with chunks = 1).  16 states, bf16,
 // 8 x 2048 x 1536: 233 us, 1.7e12 decays a second, the issue slots 71% busy.
-template <typename T, int LN, int CPL>
+template <typename T, int LN, int CPL, bool PAD>
 __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
     using F = Cfg<T, LN, CPL>;
     constexpr int NP = F::NP, CB = F::CB, TT = F::TT;
@@ -592,6 +609,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int nl = lane % LN, cl = lane / LN, n0 = 4 * nl;
     const int c0 = warp * F::CL * CPL + cl * CPL;
+    const uint4 there = within<PAD>(n0, a.N);
     St A2[CPL], h[CPL];
     float lim[CPL];
 #pragma unroll
@@ -643,7 +661,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
                         decays<decltype(signed_steps)::value>(A2[j], lim[j], dj, e);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
+                            h[j] = only<PAD>(fma(e[k], h[j], mul(Bv[k], dup(v[k][j]))), there);
                             y[k] = dot(h[j], Cv[k]);
                         }
                         over_states<LN>(y);
@@ -660,8 +678,8 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
         }
     };
     cta_barrier();
-    if (a.softplus)
-        run(std::false_type());
+    if (!PAD && a.softplus)  // with PAD one loop takes steps of either sign
+        run(std::bool_constant<PAD>());
     else
         run(std::true_type());
     if (a.hT && ck == a.chunks - 1) {
@@ -724,7 +742,7 @@ __device__ __forceinline__ float take(float keep, float send, int mask) {
     return __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, send, mask));
 }
 
-template <typename T, int LN>
+template <typename T, int LN, bool PAD>
 __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
     using F = BCfg<T, LN>;
     constexpr int NP = F::NP, CB = F::CB, CPL = F::CPL, TT = F::TT, CL = F::CL, PERMS = F::PERMS, E = F::E;
@@ -740,6 +758,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
     const int active = end > tb ? cdiv(end - tb, TT) : 0;  // tiles behind the length change nothing
     const int lt = tid / F::VPR, lc = E * (tid % F::VPR), d = d0 + lc, have = a.D - d;
     const int c0 = warp * CL * CPL + cl * CPL;  // this lane's first channel in the CTA
+    const uint4 there = within<PAD>(n0, a.N, perm);
 
     St A2[CPL], gc[CPL], dA[CPL];
 #pragma unroll
@@ -886,7 +905,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                     St e[4];
                     decays<sizeof(T) == 4>(A2[j], dj, e);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) h[j] = fma(e[k], h[j], mul(Bv[k], dup(v[k][j])));
+                    for (int k = 0; k < 4; k++) h[j] = only<PAD>(fma(e[k], h[j], mul(Bv[k], dup(v[k][j]))), there);
                     mid[q][j] = h[j];
                 }
             }
@@ -914,15 +933,16 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                 St e[4], h[4];
                 decays<sizeof(T) == 4>(A2[j], dj, e);
 #pragma unroll
-                for (int k = 0; k < 4; k++) h[k] = fma(e[k], k ? h[k ? k - 1 : 0] : h0, mul(Bv[k], dup(v[k][j])));
+                for (int k = 0; k < 4; k++)
+                    h[k] = only<PAD>(fma(e[k], k ? h[k ? k - 1 : 0] : h0, mul(Bv[k], dup(v[k][j]))), there);
 #pragma unroll
                 for (int k = 3; k >= 0; k--) {
                     const float2 dsk = dup(ds[k][j]);
-                    const St g = fma(Cv[k], dsk, gc[j]);
+                    const St g = only<PAD>(fma(Cv[k], dsk, gc[j]), there);
                     vB[k] = j ? fma(g, dup(v[k][j]), vB[k]) : mul(g, dup(v[k][j]));
                     vC[k] = j ? fma(h[k], dsk, vC[k]) : mul(h[k], dsk);
                     out[0][j][k] = dot(g, Bv[k]);
-                    gc[j] = mul(e[k], g);
+                    gc[j] = only<PAD>(mul(e[k], g), there);
                     const St w = mul(gc[j], k ? h[k ? k - 1 : 0] : h0);
                     out[1][j][k] = dot(w, A2[j]);
                     out[2][j][k] = dot(h[k], Cv[k]);
@@ -1129,6 +1149,7 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
         }
     }
     const St A2 = scaled(Av);
+    const uint4 there = within<true>(n0, a.N);
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
         const int b = b0 + r;
@@ -1136,7 +1157,7 @@ __global__ void __launch_bounds__(THREADS) step_kernel(const Args a) {
         const float u = to_f(tu[r]);
         float t = __fadd_rn(to_f(td[r]), bias);
         if (a.softplus) t = softplus(t);
-        const St h = fma(exp2s(mul(A2, dup(t))), st(hv[r]), mul(st(quad(pB[r])), dup(__fmul_rn(t, u))));
+        const St h = only<true>(fma(exp2s(mul(A2, dup(t))), st(hv[r]), mul(st(quad(pB[r])), dup(__fmul_rn(t, u)))), there);
         if (live) store4(a.hT + ((int64_t)b * a.D + d) * a.N, n0, a.N, f4(h));
         float y = dot(h, st(quad(pC[r])));
 #pragma unroll
@@ -1253,13 +1274,13 @@ static int check(int batch, int L, int D, int N, int dtype) {
 }
 
 // the chunks' starting states (REV: what they receive from behind), in a.cst
-template <typename T, int LN, int CPL, bool REV>
+template <typename T, int LN, int CPL, bool REV, bool PAD>
 static int start_chunks(const Args& a, cudaStream_t s) {
     using F = Cfg<T, LN, CPL>;
     constexpr size_t smem = sizeof(typename F::template Smem<false>);
     static std::atomic<uint64_t> allowed{0};
-    if (!allow_smem(chunk_kernel<T, LN, CPL, REV>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
-    chunk_kernel<T, LN, CPL, REV><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), CTA, smem, s>>>(a);
+    if (!allow_smem(chunk_kernel<T, LN, CPL, REV, PAD>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
+    chunk_kernel<T, LN, CPL, REV, PAD><<<dim3(cdiv(a.D, F::CB), a.batch, a.chunks - 1), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     const int64_t items = (int64_t)a.batch * a.D * LN;
     join_kernel<LN, REV><<<(unsigned)((items + THREADS - 1) / THREADS), THREADS, 0, s>>>(a);
@@ -1267,7 +1288,7 @@ static int start_chunks(const Args& a, cudaStream_t s) {
     return MI_OK;
 }
 
-template <typename T, int LN, int CPL>
+template <typename T, int LN, int CPL, bool PAD>
 static int forward_cpl(Args& a, float* ws, cudaStream_t s) {
     using F = Cfg<T, LN, CPL>;
     const Plan p = forward_plan(a.batch, a.L, a.D, a.N);
@@ -1275,25 +1296,29 @@ static int forward_cpl(Args& a, float* ws, cudaStream_t s) {
     if (p.chunks > 1) {
         const Ws w = ws_of(a.batch, a.L, a.D, a.N, false);
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, CPL, false>(a, s);
+        const int rc = start_chunks<T, LN, CPL, false, PAD>(a, s);
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::template Smem<true>);
     static std::atomic<uint64_t> allowed{0};
-    if (!allow_smem(scan_kernel<T, LN, CPL>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
-    scan_kernel<T, LN, CPL><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), CTA, smem, s>>>(a);
+    if (!allow_smem(scan_kernel<T, LN, CPL, PAD>, smem, allowed, CTA_REGS)) return MI_ERR_CUDA;
+    scan_kernel<T, LN, CPL, PAD><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), CTA, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }
 
+template <typename T, int LN, bool PAD>
+static int forward_pad(Args& a, float* ws, cudaStream_t s) {
+    if constexpr (LN == 4) {
+        if (fwd_cpl(a.batch, a.D, a.N) == 2) return forward_cpl<T, 4, 2, PAD>(a, ws, s);
+        return forward_cpl<T, 4, 1, PAD>(a, ws, s);
+    } else {
+        return forward_cpl<T, LN, LN == 2 ? 1 : LN == 8 ? 2 : 4, PAD>(a, ws, s);
+    }
+}
 template <typename T, int LN>
 static int forward(Args& a, float* ws, cudaStream_t s) {
-    if constexpr (LN == 4) {
-        if (fwd_cpl(a.batch, a.D, a.N) == 2) return forward_cpl<T, 4, 2>(a, ws, s);
-        return forward_cpl<T, 4, 1>(a, ws, s);
-    } else {
-        return forward_cpl<T, LN, LN == 2 ? 1 : LN == 8 ? 2 : 4>(a, ws, s);
-    }
+    return a.N < 4 * LN ? forward_pad<T, LN, true>(a, ws, s) : forward_pad<T, LN, false>(a, ws, s);
 }
 
 template <typename T, int LN, int ROWS, bool VEC>
@@ -1313,8 +1338,8 @@ static int step(Args& a, float*, cudaStream_t s) {
     return step_rows<T, LN, 1, true>(a, s);
 }
 
-template <typename T, int LN>
-static int backward(Args& a, float* ws, cudaStream_t s) {
+template <typename T, int LN, bool PAD>
+static int backward_pad(Args& a, float* ws, cudaStream_t s) {
     using F = BCfg<T, LN>;
     const Plan p = backward_plan(a.batch, a.L, a.D, a.N);
     a.chunks = p.chunks, a.span = p.span;
@@ -1322,15 +1347,19 @@ static int backward(Args& a, float* ws, cudaStream_t s) {
     a.part_bc = ws + w.part_bc, a.part_a = ws + w.part_a, a.part_d = ws + w.part_d;
     if (p.chunks > 1) {
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, LN == 2 ? 1 : LN == 16 ? 4 : LN == 8 ? 2 : 1, true>(a, s);
+        const int rc = start_chunks<T, LN, LN == 2 ? 1 : LN == 16 ? 4 : LN == 8 ? 2 : 1, true, PAD>(a, s);
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::Smem);
     static std::atomic<uint64_t> allowed{0};
-    if (!allow_smem(bwd_kernel<T, LN>, smem, allowed)) return MI_ERR_CUDA;
-    bwd_kernel<T, LN><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
+    if (!allow_smem(bwd_kernel<T, LN, PAD>, smem, allowed)) return MI_ERR_CUDA;
+    bwd_kernel<T, LN, PAD><<<dim3(cdiv(a.D, F::CB), a.batch, p.chunks), THREADS, smem, s>>>(a);
     MI_CHECK_LAUNCH();
     return MI_OK;
+}
+template <typename T, int LN>
+static int backward(Args& a, float* ws, cudaStream_t s) {
+    return a.N < 4 * LN ? backward_pad<T, LN, true>(a, ws, s) : backward_pad<T, LN, false>(a, ws, s);
 }
 
 }  // namespace sscan

@@ -811,3 +811,53 @@ def test_gradients_of_gradients_are_refused(sel, cuda_dev):
     (g,) = torch.autograd.grad((s * s).sum(), x, create_graph=True)
     (gg,) = torch.autograd.grad(g.sum(), x)
     assert torch.equal(gg, torch.full_like(x, 18))
+
+
+def same_infinities(got, want, name):
+    """Where the formula has no finite value the result is the same; elsewhere it is finite."""
+    got, odd = got.detach().cpu().double(), want.isinf()
+    assert torch.equal(got.isnan(), want.isnan()), (name, int(got.isnan().sum()), int(want.isnan().sum()))
+    assert torch.equal(got[odd], want[odd]) and got[want.isfinite()].isfinite().all(), name
+
+
+def infinite_inputs(dev, dtype, n, k):
+    """Inputs whose formula has infinities and, in y, no NaN; no single decay leaves the range of fp32."""
+    a = scan_inputs(dev, dtype, 3, n, 40, k, h0=True)
+    for name in ("B", "C", "D"):
+        a[name] = a[name].abs() + 0.125
+    a["A"] *= 2 / k
+    a["u"][0, 7, 3] = float("inf")
+    a["delta"][1, 9, 5], a["u"][1, 9, 5] = float("inf"), 1.0
+    return a
+
+
+INFINITE = [(k, n, dtype) for k in (1, 5, 16, 20, 24, 33) for n in (20,) for dtype in (F32, BF16)]
+
+
+@pytest.mark.parametrize("k,n,dtype", INFINITE)
+def test_scan_infinite_inputs(sel, cuda_dev, k, n, dtype):
+    """States that only fill a lane up are reached by an infinite input or step size, and stay 0."""
+    a = infinite_inputs(cuda_dev, dtype, n, k)
+    want = ref.scan(a)
+    assert not want["y"].isnan().any() and want["y"][0, 7:, 3].isinf().all() and want["y"][1, 9:, 5].isinf().all()
+    y, h = call_scan(sel, a)
+    same_infinities(y, want["y"], "y")
+    same_infinities(h, want["h"], "h")
+    h, ys = a["h0"].clone(), []
+    for t in range(11):  # one token at a time
+        ys.append(sel.selective_scan_step(h, a["u"][:, t], a["delta"][:, t], a["A"], a["B"][:, t], a["C"][:, t], D=a["D"],
+                                          z=a["z"][:, t], delta_bias=a["bias"], delta_softplus=True))
+    same_infinities(torch.stack(ys, 1), want["y"][:, :11], "steps")
+
+
+@pytest.mark.parametrize("k,n,dtype", INFINITE)
+def test_scan_infinite_gradients(sel, cuda_dev, k, n, dtype):
+    a = infinite_inputs(cuda_dev, dtype, n, k)
+    a["u"][0, 7, 3], a["delta"][1, 9, 5] = 1.0, 0.5
+    g = torch.Generator().manual_seed(1)
+    dy, dh = torch.randn(3, n, 40, generator=g).to(cuda_dev, dtype), torch.randn(3, 40, k, generator=g).to(cuda_dev)
+    dy[0, 12, 4] = float("inf")
+    _, _, got = scan_grads(sel, a, dy, dh)
+    want = ref.scan(dict(a, dy=dy, dh=dh))
+    for name, t in got.items():
+        same_infinities(t, want["d" + name], "d" + name)
