@@ -157,10 +157,22 @@ __device__ __forceinline__ float2 exp2_poly(float A, float2 dt) {
                        __int_as_float((__float_as_int(t.y) << 23) + __float_as_int(p.y)));
 }
 
-// 2^x of two states, the same way; a NaN in x is not kept
+// 2^x of two states by the same polynomial, twice 2^r times 2^(n - 1): the
+// product keeps a NaN, is infinite from 2^128 on, and 0 below 2^-125.5, where
+// 2^(n - 1) has left the normal range.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-    x = make_float2(fminf(fmaxf(x.x, -126.0f), 126.0f), fminf(fmaxf(x.y, -126.0f), 126.0f));
-    return exp2_poly(1.0f, x);
+    x = make_float2(min_nan(max_nan(x.x, -126.0f), 128.0f), min_nan(max_nan(x.y, -126.0f), 128.0f));
+    const float magic = 12582912.0f;
+    const float2 t = __fadd2_rn(x, dup(magic));
+    const float2 r = __fadd2_rn(x, __ffma2_rn(t, dup(-1.0f), dup(magic)));
+    float2 p = __ffma2_rn(dup(2 * 1.5469732170458883e-4f), r, dup(2 * 1.3410000829026103e-3f));
+    p = __ffma2_rn(p, r, dup(2 * 9.618030861020088e-3f));
+    p = __ffma2_rn(p, r, dup(2 * 5.550297349691391e-2f));
+    p = __ffma2_rn(p, r, dup(2 * 2.4022650718688965e-1f));
+    p = __ffma2_rn(p, r, dup(2 * 6.931472420692444e-1f));
+    p = __ffma2_rn(p, r, dup(2.0f));
+    return __fmul2_rn(p, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f000000),
+                                     __int_as_float((__float_as_int(t.y) << 23) + 0x3f000000)));
 }
 
 // The decays of 4 positions: one state of a lane's four goes through the FMA
@@ -262,14 +274,6 @@ __device__ __forceinline__ void stage_steps(float4* row, int c, int t, const flo
     for (int k = 0; k < K; k += 2) row[place((c + k) >> 1, t)] = make_float4(dt[k], v[k], dt[k + 1], v[k + 1]);
 }
 
-// NaNs in A, which the polynomial would lose, are put into the states.
-__device__ __forceinline__ St keep_nan(St h, St A) {
-    if (isnan(A.a.x)) h.a.x = A.a.x;
-    if (isnan(A.a.y)) h.a.y = A.a.y;
-    if (isnan(A.b.x)) h.b.x = A.b.x;
-    if (isnan(A.b.y)) h.b.y = A.b.y;
-    return h;
-}
 // A NaN in the A of a lane's first state, which the polynomial would lose, is
 // put into the state.
 __device__ __forceinline__ float limit(const St& A2, St& h) {
@@ -772,7 +776,6 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
             else if (a.dhT)
                 gc[j] = st(load4(a.dhT + ((int64_t)b * a.D + c) * a.N, n0, a.N));
             gc[j] = permute<PERMS>(gc[j], perm);
-            if (sizeof(T) == 4 && active > 0) gc[j] = keep_nan(gc[j], A2[j]);
         }
     }
     constexpr int AK = E / 4;  // dD and dbias of a quarter of this thread's channels, over 4 positions of each tile

@@ -861,3 +861,18 @@ def test_scan_infinite_gradients(sel, cuda_dev, k, n, dtype):
     want = ref.scan(dict(a, dy=dy, dh=dh))
     for name, t in got.items():
         same_infinities(t, want["d" + name], "d" + name)
+
+
+@pytest.mark.parametrize("k", [1, 5, 16])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [20, 300])
+def test_scan_nan_steps_reach_the_gradients(sel, cuda_dev, n, dtype, k):
+    """A step size that is NaN makes the same gradients NaN as in the formula, those of earlier positions among them."""
+    a = scan_inputs(cuda_dev, dtype, 2, n, 40, k, h0=True)
+    a["delta"][0, 9, 5] = float("nan")
+    dy, dh = torch.randn(2, n, 40, device=cuda_dev).to(dtype), torch.randn(2, 40, k, device=cuda_dev)
+    y, h, got = scan_grads(sel, a, dy, dh)
+    want = ref.scan(dict(a, dy=dy, dh=dh))
+    assert want["dh0"][0, 5].isnan().all() and not want["dD"].isnan().any()
+    for name, t in dict(got, y=y, h=h).items():
+        same_infinities(t, want[name if name in ("y", "h") else "d" + name], name)
