@@ -921,6 +921,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
         for (int q = 3; q >= 0; q--) {
             St Bv[4], Cv[4], vB[4], vC[4];
             float dt[4][CPL], v[4][CPL], ds[4][CPL];
+            const int inside = end - (t0 + 4 * q);  // behind the end dt is 0, which an infinite state times it is not
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 Bv[k] = st(*reinterpret_cast<const float4*>(&sm.B[perm][4 * q + k][n0]));
@@ -949,7 +950,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                     const St w = mul(gc[j], k ? h[k ? k - 1 : 0] : h0);
                     out[1][j][k] = dot(w, A2[j]);
                     out[2][j][k] = dot(h[k], Cv[k]);
-                    dA[j] = fma(w, dup(dj[k]), dA[j]);
+                    if (k < inside) dA[j] = fma(w, dup(dj[k]), dA[j]);
                 }
 #pragma unroll
                 for (int m = 0; m < 3; m++) over_states<LN>(out[m][j]);

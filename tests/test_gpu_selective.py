@@ -876,3 +876,21 @@ def test_scan_nan_steps_reach_the_gradients(sel, cuda_dev, n, dtype, k):
     assert want["dh0"][0, 5].isnan().all() and not want["dD"].isnan().any()
     for name, t in dict(got, y=y, h=h).items():
         same_infinities(t, want[name if name in ("y", "h") else "d" + name], name)
+
+
+
+@pytest.mark.parametrize("lengths", [None, [20, 13, 17]])
+@pytest.mark.parametrize("k,n,dtype", INFINITE)
+def test_scan_gradients_of_infinite_states(sel, cuda_dev, k, n, dtype, lengths):
+    """Positions behind the end, whose step size is 0, add nothing to dA, also where the state is infinite."""
+    a = infinite_inputs(cuda_dev, dtype, n, k)
+    a["lengths"] = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_dev)
+    g = torch.Generator().manual_seed(1)
+    # gradients of one sign: the formula's dA is an infinity for the infinite input, and NaN for the infinite step
+    dy, dh = torch.rand(3, n, 40, generator=g).to(cuda_dev, dtype), torch.rand(3, 40, k, generator=g).to(cuda_dev)
+    a["z"] = a["z"].abs()
+    _, _, got = scan_grads(sel, a, dy, dh)
+    want = ref.scan(dict(a, dy=dy, dh=dh))
+    assert want["dA"][3].isinf().all()
+    for name, t in got.items():
+        same_infinities(t, want["d" + name], "d" + name)
