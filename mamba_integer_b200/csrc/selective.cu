@@ -560,6 +560,18 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
     }
 }
 
+// 2^x h + own, x of a whole chunk: not 0 below 2^-126, so that an infinite state
+// stays one, and not infinite where the state is 0, as the product of a growing
+// state's factors is not.
+__device__ __forceinline__ float over_chunk(float x, float h, float own) {
+    const float e = exp2_fast(max_nan(x, -126.0f));
+    return h == 0.0f && isinf(e) ? own : __fmaf_rn(e, h, own);
+}
+__device__ __forceinline__ St over_chunk(St x, St h, St own) {
+    return {make_float2(over_chunk(x.a.x, h.a.x, own.a.x), over_chunk(x.a.y, h.a.y, own.a.y)),
+            make_float2(over_chunk(x.b.x, h.b.x, own.b.x), over_chunk(x.b.y, h.b.y, own.b.y))};
+}
+
 // Turns each chunk's own end state into the state it starts from: a walk along
 // the chunks, h <- exp(A sum dt) h + own.  REV: from the last chunk to the
 // first, turning what each chunk passes on into what it receives from behind.
@@ -582,7 +594,7 @@ __global__ void __launch_bounds__(THREADS) join_kernel(const Args a) {
         float sum = 0.0f;
         if (ck != last) own = st(*p), sum = a.cdt[row];
         *p = f4(h);
-        h = fma(exp2s(mul(A2, sum)), h, own);
+        h = over_chunk(mul(A2, sum), h, own);
     }
 }
 

@@ -894,3 +894,43 @@ def test_scan_gradients_of_infinite_states(sel, cuda_dev, k, n, dtype, lengths):
     assert want["dA"][3].isinf().all()
     for name, t in got.items():
         same_infinities(t, want["d" + name], "d" + name)
+
+
+@pytest.mark.parametrize("k,dtype", [(k, dtype) for k in (1, 16, 20) for dtype in (F32, BF16)])
+def test_scan_infinities_over_chunks(sel, cuda_dev, k, dtype):
+    """An infinite state, and an infinite gradient, stay infinite over chunks whose decay as a whole is 0 in fp32."""
+    n = 300
+    a = infinite_inputs(cuda_dev, dtype, n, k)
+    a["A"] *= 4
+    a["delta"] += 2
+    want = ref.scan(a)
+    y, h = call_scan(sel, a)
+    same_infinities(y, want["y"], "y")
+    same_infinities(h, want["h"], "h")
+    a["u"][0, 7, 3], a["delta"][1, 9, 5] = 1.0, 0.5
+    g = torch.Generator().manual_seed(1)
+    dy, dh = torch.randn(3, n, 40, generator=g).to(cuda_dev, dtype), torch.randn(3, 40, k, generator=g).to(cuda_dev)
+    dy[0, 290, 4] = float("inf")
+    _, _, got = scan_grads(sel, a, dy, dh)
+    want = ref.scan(dict(a, dy=dy, dh=dh))
+    same_infinities(got["u"], want["du"], "du")
+    same_infinities(got["h0"], want["dh0"], "dh0")
+
+
+def test_scan_growth_over_chunks(sel, cuda_dev):
+    """Growing states: a chunk's growth leaves the range of fp32, the states do not, being 0 there."""
+    n = 2048
+    a = scan_inputs(cuda_dev, F32, 1, n, 8, 16, softplus=False, bias=False, z=False)
+    a["A"] = a["A"].abs().clamp(0.5, 1.0)
+    a["delta"].fill_(2.0)
+    a["u"][:, :n - 20] = 0
+    dy = torch.randn(1, n, 8, device=cuda_dev)
+    dy[:, 20:] = 0
+    y, h, got = scan_grads(sel, a, dy, None)
+    args = dict(a, dy=dy)
+    want, mag = ref.scan(args), ref.scan(args, mag=True)
+    # a factor e^2 = 2^2.9 has 4 + 8 * 2.9 roundings, the step one more; 20 positions and what lies around them; twice for gradients
+    ref.check(y, want["y"], mag["y"], 28 * 20 + 64, "y")
+    ref.check(h, want["h"], mag["h"], 28 * 20 + 64, "h")
+    for name, t in got.items():
+        ref.check(t, want["d" + name], mag["d" + name], 2 * (28 * 20 + 64) + n, "d" + name)
