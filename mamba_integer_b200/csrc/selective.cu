@@ -141,8 +141,10 @@ __device__ __forceinline__ St exp2s(St x) {
 
 // 2^(A dt) of two positions on the FMA pipe: with x = A dt and n = x rounded,
 // 2^x = 2^n 2^r, r = x - n in [-1/2, 1/2], and 2^r = 1 + r q(r), q of degree 5
-// with the least relative error (2^-27.9, by Remez's exchange).  |dt| is at
-// most 126 / |A|, where the decay is 2^-126 and no more than rounding.
+// with the least relative error (2^-27.9, by Remez's exchange).  A dt is at
+// most -126, where the decay is 2^-126 and no more than rounding, and at most
+// 128, where the largest fp32 number or infinity comes out (behind 128 the sum
+// of the exponents would be a NaN): `limits` keeps dt there.
 __device__ __forceinline__ float2 exp2_poly(float A, float2 dt) {
     const float magic = 12582912.0f;  // 1.5 2^23: adding it rounds to whole numbers and leaves them in the low bits
     const float2 t = __ffma2_rn(dup(A), dt, dup(magic));
@@ -181,14 +183,14 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
 // memory; A usually begins with its slowest state, so it is the first of the
 // four: dA's error against 64 bits is 6e-7 with it and 1.6e-6 without (8 x 2048
 // x 1536), and the special-function unit, the slower of the two, has a quarter
-// less to do.  `lim` is 126 / |A| of the first state.  SIGNED: step sizes may
-// be negative (they are not from softplus).
+// less to do.  `lim`: the limits of the first state's step sizes.  SIGNED: they
+// may be negative (they are not from softplus).
 template <bool SIGNED>
-__device__ __forceinline__ void decays(const St& A2, float lim, const float (&dt)[4], St (&e)[4]) {
+__device__ __forceinline__ void decays(const St& A2, float2 lim, const float (&dt)[4], St (&e)[4]) {
 #pragma unroll
     for (int k = 0; k < 4; k += 2) {
-        float2 d = make_float2(fminf(dt[k], lim), fminf(dt[k + 1], lim));
-        if (SIGNED) d = make_float2(fmaxf(d.x, -lim), fmaxf(d.y, -lim));
+        float2 d = make_float2(fminf(dt[k], lim.y), fminf(dt[k + 1], lim.y));
+        if (SIGNED) d = make_float2(fmaxf(d.x, lim.x), fmaxf(d.y, lim.x));
         const float2 p = exp2_poly(A2.a.x, d);
         e[k].a.x = p.x, e[k + 1].a.x = p.y;
     }
@@ -274,11 +276,12 @@ __device__ __forceinline__ void stage_steps(float4* row, int c, int t, const flo
     for (int k = 0; k < K; k += 2) row[place((c + k) >> 1, t)] = make_float4(dt[k], v[k], dt[k + 1], v[k + 1]);
 }
 
-// A NaN in the A of a lane's first state, which the polynomial would lose, is
-// put into the state.
-__device__ __forceinline__ float limit(const St& A2, St& h) {
+// The least and the largest step size with -126 <= A dt <= 128, A of a lane's
+// first state; a NaN in it, which the polynomial would lose, is put into the state.
+__device__ __forceinline__ float2 limits(const St& A2, St& h) {
     if (isnan(A2.a.x)) h.a.x = A2.a.x;
-    return __fdiv_rn(126.0f, fmaxf(fabsf(A2.a.x), 1e-30f));
+    const float A = fmaxf(fabsf(A2.a.x), 1e-30f), decay = __fdiv_rn(126.0f, A), growth = __fdiv_rd(128.0f, A);
+    return A2.a.x > 0.0f ? make_float2(-decay, growth) : make_float2(-growth, decay);
 }
 
 // The forward kernels' CTA: 4 warps that carry the recurrence, 4 that stage
@@ -505,13 +508,14 @@ __global__ void __launch_bounds__(CTA, 2) chunk_kernel(const Args a) {
     const int c0 = warp * F::CL * CPL + cl * CPL;
     const uint4 there = within<PAD>(n0, a.N);
     St A2[CPL], h[CPL];
-    float sum[CPL], lim[CPL];
+    float sum[CPL];
+    float2 lim[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
         const int c = d0 + c0 + j;
         A2[j] = scaled(c < a.D ? load4(a.A + (int64_t)c * a.N, n0, a.N) : make_float4(0, 0, 0, 0));
         h[j] = st(make_float4(0, 0, 0, 0));
-        lim[j] = limit(A2[j], h[j]);
+        lim[j] = limits(A2[j], h[j]);
         sum[j] = 0.0f;
     }
     auto run = [&](auto signed_steps) {
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
     const int c0 = warp * F::CL * CPL + cl * CPL;
     const uint4 there = within<PAD>(n0, a.N);
     St A2[CPL], h[CPL];
-    float lim[CPL];
+    float2 lim[CPL];
 #pragma unroll
     for (int j = 0; j < CPL; j++) {
         const int c = d0 + c0 + j;
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
             v = load4(a.h0 + ((int64_t)b * a.D + c) * a.N, n0, a.N);
         h[j] = st(v);
         St none = h[j];
-        lim[j] = limit(A2[j], tiles > 0 ? h[j] : none);
+        lim[j] = limits(A2[j], tiles > 0 ? h[j] : none);
     }
     float* keep = a.ckpt + (((int64_t)b * cdiv(a.L, CK) + tb / CK) * a.D + d0 + c0) * NP + n0;
     auto run = [&](auto signed_steps) {

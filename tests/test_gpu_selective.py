@@ -934,3 +934,30 @@ def test_scan_growth_over_chunks(sel, cuda_dev):
     ref.check(h, want["h"], mag["h"], 28 * 20 + 64, "h")
     for name, t in got.items():
         ref.check(t, want["d" + name], mag["d" + name], 2 * (28 * 20 + 64) + n, "d" + name)
+
+
+@pytest.mark.parametrize("softplus,sign", [(False, 1), (False, -1), (True, 1)])
+def test_scan_growth_to_the_end_of_fp32(sel, cuda_dev, softplus, sign):
+    """Factors between 2^126 and 2^128, and one beyond, which ends in an infinity or next to it."""
+    a = scan_inputs(cuda_dev, F32, 1, 1, 8, 16, softplus=softplus, bias=False, z=False, h0=True)
+    a["A"] = sign * torch.ones(8, 16, device=cuda_dev)
+    a["delta"].fill_(sign * 88.0)
+    a["C"] *= 2.0 ** -10
+    a["h0"] = a["h0"].clamp(-1, 1)
+    dh = torch.randn(1, 8, 16, device=cuda_dev).clamp(-1, 1)
+    y, h, got = scan_grads(sel, a, None, dh)
+    args = dict(a, dh=dh)
+    want, mag = ref.scan(args), ref.scan(args, mag=True)
+    # the factor: x = 127, 4 + 8 * 127 roundings; 64 around it
+    ref.check(h, want["h"], mag["h"], 1100, "h")
+    ref.check(y, want["y"], mag["y"], 1100, "y")
+    ref.check(got["h0"], want["dh0"], mag["dh0"], 1100, "dh0")
+    a["delta"][:] = sign * 200.0
+    a["h0"] = a["h0"].sign() * 2
+    h = call_scan(sel, a)[1]
+    assert torch.equal(h, a["h0"] * float("inf"))
+    if not softplus:  # the other way, what is left is the input's part
+        a["delta"][:] = sign * -200.0
+        h = call_scan(sel, a)[1]
+        want, mag = ref.scan(a), ref.scan(a, mag=True)
+        ref.check(h, want["h"], mag["h"], 64, "h")
