@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
         }
         // the run that begins the sequence also makes the window's gradients, dx at t = -(W-1) .. -1
         const int first = t0 == 0 ? -(W - 1) : t0;
-        const int inner = gwin && len - (W - 1) < t1 ? len - (W - 1) : t1;  // dx up to here is the sum alone
+        const int inner = gwin ? len - (W - 1) : len;  // dx up to here is the sum alone
         int slot = 0;
 #pragma unroll 1
         for (int t = t0; t < te; t += 4) {
@@ -340,7 +340,8 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
                 for (int k = 1; k < W; k++) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
             }
             const int td0 = t - (W - 1);
-            if (td0 >= t0 && td0 + 4 <= inner) {
+            if (td0 >= t0 && td0 + 4 <= t1 && (td0 + 4 <= inner || td0 >= len)) {
+                if (td0 >= len) o[0] = o[1] = o[2] = o[3] = zero;  // whatever the weights are
                 if (dxb && have > 0) {
                     T* to = dxb + (int64_t)td0 * a.D;
 #pragma unroll
@@ -354,6 +355,11 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
                 for (int j = 0; j < 4; j++) {
                     const int td = td0 + j;
                     if (td < first || td >= t1) continue;
+                    // of the positions that there are: 0 times an infinite weight is not 0
+                    o[j] = zero;
+#pragma unroll
+                    for (int k = 0; k < W; k++)
+                        if (td + W - 1 - k >= 0 && td + W - 1 - k < len) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
                     // this input's place in the window that leaves, if it has one
                     const int kw = td - (len - (W - 1));
                     if (gwin && kw >= 0 && kw < W - 1)

@@ -961,3 +961,22 @@ def test_scan_growth_to_the_end_of_fp32(sel, cuda_dev, softplus, sign):
         h = call_scan(sel, a)[1]
         want, mag = ref.scan(a), ref.scan(a, mag=True)
         ref.check(h, want["h"], mag["h"], 64, "h")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("d", [24, 21])
+@pytest.mark.parametrize("n", [33, 160])
+def test_conv_infinite_weights_behind_lengths(sel, cuda_dev, n, d, silu, dtype):
+    """What lies behind a length has gradients of 0 and adds nothing to others, also where a weight is infinite or NaN."""
+    lens = [0, 1, 7, 30, n]
+    a = conv_inputs(cuda_dev, dtype, 5, n, d, 4, silu=silu, win=True, lengths=lens)
+    a["w"][3, 1], a["w"][5, 0], a["w"][5, 3] = float("inf"), float("nan"), float("-inf")
+    leaves = {m: a[m].clone().requires_grad_(True) for m in ("x", "w", "bias", "win")}
+    y, out = call_conv(sel, a, **leaves)
+    for given in ((y,), (out,), (y, out)):
+        grads = [torch.randn_like(t) for t in given]
+        dx, dwin = torch.autograd.grad(given, [leaves["x"], leaves["win"]], grads, retain_graph=True)
+        for i, v in enumerate(lens):
+            assert not y[i, v:].any() and not dx[i, v:].any()
+        assert torch.equal(dwin[0], torch.zeros_like(dwin[0]) if given[-1] is y else grads[-1][0])  # the empty sequence's
