@@ -980,3 +980,49 @@ def test_conv_infinite_weights_behind_lengths(sel, cuda_dev, n, d, silu, dtype):
         for i, v in enumerate(lens):
             assert not y[i, v:].any() and not dx[i, v:].any()
         assert torch.equal(dwin[0], torch.zeros_like(dwin[0]) if given[-1] is y else grads[-1][0])  # the empty sequence's
+
+
+@pytest.mark.parametrize("size", [(600, 33, 40, 16), (300, 20, 72, 13), (592, 49, 64, 9)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_two_channels_a_lane(sel, cuda_dev, size, dtype):
+    """From 592 CTAs of 64 channels on, a lane of a scan of 9 to 16 states carries two channels."""
+    b, n, d, k = size
+    assert b * -(-d // 64) >= 592
+    lens = [(7 * i) % (n + 1) for i in range(b)]
+    a = scan_inputs(cuda_dev, dtype, *size, h0=True, lengths=lens)
+    g = torch.Generator().manual_seed(5)
+    dy, dh = torch.randn(b, n, d, generator=g).to(cuda_dev, dtype), torch.randn(b, d, k, generator=g).to(cuda_dev)
+    y, h, got = scan_grads(sel, a, dy, dh)
+    check_scan(y, h, a)
+    check_scan_grads(got, a, dy, dh)
+    y2, h2 = call_scan(sel, a)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+@pytest.mark.parametrize("b,k,lanes", [(8193, 8, 2), (4099, 16, 4), (2051, 24, 8), (2050, 32, 8), (1027, 64, 16),
+                                       (1029, 44, 16)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_scan_step_of_many_streams(sel, cuda_dev, b, k, lanes, dtype):
+    """From 606208 lanes on a thread takes 4 streams, the last ones fewer."""
+    assert b * 37 * lanes >= 606208 and b % 4
+    a = scan_inputs(cuda_dev, dtype, b, 1, 37, k, h0=True)
+    h = a["h0"].clone()
+    y = sel.selective_scan_step(h, a["u"][:, 0], a["delta"][:, 0], a["A"], a["B"][:, 0], a["C"][:, 0], D=a["D"],
+                                z=a["z"][:, 0], delta_bias=a["bias"], delta_softplus=True)
+    check_scan(y[:, None], h, a)
+
+
+@pytest.mark.parametrize("b,d,run", [(57000, 4, 64), (28500, 5, 64), (40000, 4, 32), (20000, 5, 32), (24000, 4, 16),
+                                     (12000, 5, 16)])
+@pytest.mark.parametrize("dtype,k", [(F32, 4), (BF16, 4), (F16, 3), (BF16, 2)])
+def test_conv_forward_runs(sel, cuda_dev, b, d, run, dtype, k):
+    """The longest runs that leave 113664 threads, each with a run of one position behind the full ones."""
+    n = 65
+    threads = lambda r: b * -(-d // 4) * -(-n // r)  # noqa: E731
+    assert threads(run) >= 113664 and (run == 64 or threads(2 * run) < 113664)
+    lens = [(11 * i) % (n + 1) for i in range(b)]
+    a = conv_inputs(cuda_dev, dtype, b, n, d, k, win=True, lengths=lens)
+    y, out = call_conv(sel, a)
+    want, mag = ref.conv(a), ref.conv(a, mag=True)
+    ref.check(y, want["y"], mag["y"], 32, "y")
+    assert torch.equal(out.cpu().double(), want["win"])
