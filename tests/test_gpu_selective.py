@@ -1026,3 +1026,32 @@ def test_conv_forward_runs(sel, cuda_dev, b, d, run, dtype, k):
     want, mag = ref.conv(a), ref.conv(a, mag=True)
     ref.check(y, want["y"], mag["y"], 32, "y")
     assert torch.equal(out.cpu().double(), want["win"])
+
+
+def test_integration_example(sel, cuda_dev):
+    """The calls of INTEGRATION.md as they are written there."""
+    import os
+    from mamba_integer_b200.rational_bitnet import BitLinear
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
+        code = f.read().split("## 1b.")[1].split("```python\n")[1].split("```")[0]
+    b, n, d, k, width = 3, 10, 64, 16, 32
+    r = lambda *s: torch.randn(*s, device=cuda_dev)  # noqa: E731
+    linear = BitLinear(width, 48).to(cuda_dev)
+    v = dict(torch=torch, d=d, x=r(b, n, width), residual=r(b, n, width), norm_w=torch.ones(width, device=cuda_dev),
+             xz=r(b, n, 2 * d), conv_w=r(d, 4), conv_b=r(d), delta=r(b, n, d), A=-r(d, k).exp(), B=r(b, n, k), C=r(b, n, k),
+             D=r(d), dt_bias=r(d) - 4, lengths=torch.tensor([10, 4, 0], dtype=torch.int32, device=cuda_dev), xz1=r(b, 2 * d),
+             delta1=r(b, d), B1=r(b, k), C1=r(b, k), linear=linear)
+    exec(code, v)
+    # the tokens go on from each sequence's own length
+    for i, e in enumerate((10, 4, 0)):
+        one = lambda t, t1: torch.cat([t[i:i + 1, :e], t1[i:i + 1, None]], 1)  # noqa: E731
+        xz = one(v["xz"], v["xz1"])
+        c = sel.causal_conv1d(xz[..., :d], v["conv_w"], bias=v["conv_b"], silu=True)
+        assert torch.equal(c[0, -1], v["c1"][i])
+        whole = dict(u=c, delta=one(v["delta"], v["delta1"]), A=v["A"], B=one(v["B"], v["B1"]), C=one(v["C"], v["C1"]),
+                     D=v["D"], z=xz[..., d:], bias=v["dt_bias"], softplus=True)
+        want, mag = ref.scan(whole), ref.scan(whole, mag=True)
+        ref.check(v["s1"][i], want["y"][0, -1], mag["y"][0, -1], 8 * (e + 1) + 64, "s1")
+    with torch.no_grad():
+        y, total = sel.rms_norm(v["x"], v["norm_w"], residual=v["residual"])
+        assert torch.equal(v["out"], linear(y).flatten(0, -2)) and torch.equal(v["total"], total)
