@@ -56,18 +56,37 @@ def build_bpe(force: bool = False) -> str:
 
 TORCH_SO = os.path.join(HERE, "_mi_torch.so")
 TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_STAMP = TORCH_SO + ".stamp"
+
+
+def torch_stamp() -> str:
+    """What _mi_torch.so is tied to beside its sources: another torch or Python than it was built for needs a new one."""
+    import torch
+
+    return "\n".join([torch.__version__, os.path.dirname(torch.__file__), str(int(torch._C._GLIBCXX_USE_CXX11_ABI)),
+                      sys.version, sys.implementation.cache_tag]) + "\n"
+
+
+def torch_needs_build() -> bool:
+    deps = [TORCH_SRC, os.path.join(ROOT, "include", "mi_b200.h")]
+    if not os.path.exists(TORCH_SO) or any(os.path.getmtime(d) > os.path.getmtime(TORCH_SO) for d in deps):
+        return True
+    try:
+        with open(TORCH_STAMP) as f:
+            return f.read() != torch_stamp()
+    except OSError:
+        return True
 
 
 def build_torch(force: bool = False) -> str:
     """The float operators' calls from torch, _mi_torch.so (g++, C++17; no CUDA compiler)."""
+    if not force and not torch_needs_build():
+        return TORCH_SO
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    deps = [TORCH_SRC, os.path.join(ROOT, "include", "mi_b200.h")]
-    if not force and os.path.exists(TORCH_SO) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_SO) for d in deps):
-        return TORCH_SO
     cxx = shutil.which("g++") or "g++"
     cuda = os.path.dirname(os.path.dirname(shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"))
     includes = [*cpp_extension.include_paths(), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
@@ -77,7 +96,11 @@ def build_torch(force: bool = False) -> str:
                     *[arg for path in includes for arg in ("-isystem", path)], "-o", TORCH_SO + ".tmp", TORCH_SRC,
                     "-L" + libs, "-Wl,-rpath," + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"],
                    check=True)
+    if os.path.exists(TORCH_STAMP):
+        os.remove(TORCH_STAMP)  # never an old stamp beside a new library
     os.replace(TORCH_SO + ".tmp", TORCH_SO)
+    with open(TORCH_STAMP, "w") as f:
+        f.write(torch_stamp())
     return TORCH_SO
 
 

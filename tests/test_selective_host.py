@@ -240,3 +240,25 @@ def test_forward_mode_is_refused():
                         fn(**{**args, name: wide[0]})
         with pytest.raises(ValueError, match="must be a CUDA tensor"):  # and without one the call goes on
             fn(**args)
+
+
+def test_the_native_calls_are_built_again_for_another_torch(tmp_path, monkeypatch):
+    from mamba_integer_b200 import build
+
+    monkeypatch.setattr(build, "TORCH_SO", str(tmp_path / "x.so"))
+    monkeypatch.setattr(build, "TORCH_STAMP", str(tmp_path / "x.so.stamp"))
+    assert build.torch_needs_build()
+    (tmp_path / "x.so").write_bytes(b"")
+    assert build.torch_needs_build()  # of unknown origin
+    (tmp_path / "x.so.stamp").write_text(build.torch_stamp())
+    assert not build.torch_needs_build()
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert build.torch_needs_build()
+
+
+def test_the_most_states():
+    most = selective.MAX_STATES
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        selective.selective_scan(**scan_args(k=most))
+    with pytest.raises(ValueError, match=f"1 to {most} states"):
+        selective.selective_scan(**scan_args(k=most + 1))
