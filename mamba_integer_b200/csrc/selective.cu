@@ -1313,11 +1313,13 @@ static int forward_cpl(Args& a, float* ws, cudaStream_t s) {
     using F = Cfg<T, LN, CPL>;
     const Plan p = forward_plan(a.batch, a.L, a.D, a.N);
     a.chunks = p.chunks, a.span = p.span;
-    if (p.chunks > 1) {
-        const Ws w = ws_of(a.batch, a.L, a.D, a.N, false);
-        a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, CPL, false, PAD>(a, s);
-        if (rc != MI_OK) return rc;
+    if constexpr (LN != 4 || CPL != 2) {  // two channels a lane come with 592 CTAs, and those with one chunk
+        if (p.chunks > 1) {
+            const Ws w = ws_of(a.batch, a.L, a.D, a.N, false);
+            a.cst = ws + w.cst, a.cdt = ws + w.cdt;
+            const int rc = start_chunks<T, LN, CPL, false, PAD>(a, s);
+            if (rc != MI_OK) return rc;
+        }
     }
     constexpr size_t smem = sizeof(typename F::template Smem<true>);
     static std::atomic<uint64_t> allowed{0};
