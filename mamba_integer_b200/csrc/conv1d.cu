@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(128, 5) fwd_kernel(const Args a) {
 // copies of 16 bytes a lane bring the next DEPTH - 1 groups of 4 positions into
 // the warp's ring (zeros behind the sequence's length).  Rows off 16 bytes
 // (VEC = false) go through registers, one group ahead.  8 x 2048 x 1536 bf16:
-// 52 us (150 MB, 2.9 TB/s), bound by the instructions' issue; 74 with each
+// 53 us (150 MB, 2.8 TB/s), the issue slots 68 % busy; 74 with each
 // lane's rows in registers, 80 with a copy for each pair, 56 with 4 CTAs an SM,
 // whose 64 registers spill.
 constexpr int BWD_RUNS = 8, DEPTH = 4, PAIR = 2;
@@ -283,9 +283,6 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
             for (int k = 0; k < W; k++) w[k] = make_float2(wf[k][0], wf[k][1]);
             bias = make_float2(bf[0], bf[1]);
         }
-        // the run that begins the sequence also makes the window's gradients, dx at t = -(W-1) .. -1
-        const int first = t0 == 0 ? -(W - 1) : t0;
-        const int inner = gwin ? len - (W - 1) : len;  // dx up to here is the sum alone
         int slot = 0;
 #pragma unroll 1
         for (int t = t0; t < te; t += 4) {
@@ -323,9 +320,10 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
                         if (t + j >= len) dc[W - 1 + j] = zero;
                 }
             }
-            if (t < t1) {  // the run's own positions (those behind t1, only behind the last run's, have dc = 0)
+            if (t < t1) {  // the run's own positions that there are (an infinite input times the others' 0 is not 0)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
+                    if (t + j >= len) continue;
                     db = __fadd2_rn(db, dc[W - 1 + j]);
 #pragma unroll
                     for (int k = 0; k < W; k++) dw[k] = __ffma2_rn(dc[W - 1 + j], x[j + k], dw[k]);
@@ -340,8 +338,7 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
                 for (int k = 1; k < W; k++) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
             }
             const int td0 = t - (W - 1);
-            if (td0 >= t0 && td0 + 4 <= t1 && (td0 + 4 <= inner || td0 >= len)) {
-                if (td0 >= len) o[0] = o[1] = o[2] = o[3] = zero;  // whatever the weights are
+            if (t > t0 && t + 4 <= len && td0 + 4 <= t1) {  // inside, and in front of the window that leaves
                 if (dxb && have > 0) {
                     T* to = dxb + (int64_t)td0 * a.D;
 #pragma unroll
@@ -350,16 +347,30 @@ __global__ void __launch_bounds__(256, VEC ? 3 : 2) bwd_kernel(const Args a) {
                         store_pack<K>(to + (int64_t)j * a.D, v, have, VEC);
                     }
                 }
+            } else if (t > t0 && td0 >= len && td0 + 4 <= t1) {  // behind the length
+                if (dxb && have > 0) {
+                    const float none[K] = {};
+                    T* to = dxb + (int64_t)td0 * a.D;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) store_pack<K>(to + (int64_t)j * a.D, none, have, VEC);
+                }
             } else if (have > 0) {
+                if (t == 0 || t + 4 > len) {  // of the positions that there are: 0 times an infinite weight is not 0
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        o[j] = zero;
+#pragma unroll
+                        for (int k = 0; k < W; k++) {
+                            const int of = td0 + j + W - 1 - k;
+                            if (of >= 0 && of < len) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int td = td0 + j;
-                    if (td < first || td >= t1) continue;
-                    // of the positions that there are: 0 times an infinite weight is not 0
-                    o[j] = zero;
-#pragma unroll
-                    for (int k = 0; k < W; k++)
-                        if (td + W - 1 - k >= 0 && td + W - 1 - k < len) o[j] = __ffma2_rn(w[k], dc[j + W - 1 - k], o[j]);
+                    // the run that begins the sequence also makes the window's gradients, dx at t = -(W-1) .. -1
+                    if ((t0 > 0 && td < t0) || td >= t1) continue;
                     // this input's place in the window that leaves, if it has one
                     const int kw = td - (len - (W - 1));
                     if (gwin && kw >= 0 && kw < W - 1)
@@ -468,7 +479,8 @@ __global__ void __launch_bounds__(128) step_kernel(const Args a) {
 // what a thread holds for each channel (4 taps, 7 inputs) costs registers, and
 // occupancy is worth more than the loads: 8 x 2048 x 1536 bf16 took 41 us with
 // 8 channels (209 registers) and 37 with 4; with the loads off their branches
-// 27 us (100 MB, 3.7 TB/s).
+// 27 us (100 MB, 3.7 TB/s).  fp32 with 4 taps spills 32 bytes at the 96
+// registers that 5 CTAs an SM leave: 46 us (201 MB, 4.4 TB/s).
 constexpr int KF = 4;
 
 template <typename T, int W>

@@ -1055,3 +1055,37 @@ def test_integration_example(sel, cuda_dev):
     with torch.no_grad():
         y, total = sel.rms_norm(v["x"], v["norm_w"], residual=v["residual"])
         assert torch.equal(v["out"], linear(y).flatten(0, -2)) and torch.equal(v["total"], total)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("d", [24, 21])
+@pytest.mark.parametrize("n,lens", [(33, [33, 32, 9]), (162, [162, 160, 131]), (30, None)])
+def test_conv_gradients_of_infinities_at_the_end(sel, cuda_dev, n, lens, d, silu, dtype):
+    """Infinite inputs in a sequence's last positions, and infinite weights: the formula's gradients, in which there are
+    no positions behind them."""
+    a = conv_inputs(cuda_dev, dtype, 3, n, d, 4, silu=silu, win=True, lengths=lens)
+    ends = [n] * 3 if lens is None else lens
+    for i, e in enumerate(ends):
+        for back in (1, 2, 3):
+            a["x"][i, e - back, back] = float("inf")
+    a["w"][7, 0], a["w"][8, 1], a["w"][9, 2] = (float("inf"),) * 3
+    a["w"][10, 0] = float("nan")
+    dy = torch.randn(3, n, d, generator=torch.Generator().manual_seed(9)).to(cuda_dev, dtype)
+    dwin = torch.randn(3, 3, d, generator=torch.Generator().manual_seed(8)).to(cuda_dev, dtype)
+    leaves = {m: a[m].clone().requires_grad_(True) for m in ("x", "w", "bias", "win")}
+    y, out = call_conv(sel, a, **leaves)
+    for given in (dy, None), (dy, dwin):
+        outs = [y] if given[1] is None else [y, out]
+        got = torch.autograd.grad(outs, list(leaves.values()), [g for g in given if g is not None], retain_graph=True)
+        got = dict(zip(leaves, got), y=y)
+        parts = []  # each sequence by itself, as long as it is
+        for i, e in enumerate(ends):
+            one = {m: None if t is None else t[i:i + 1] for m, t in (("win", a["win"]), ("dwin", given[1]))}
+            parts.append(ref.conv(dict(a, x=a["x"][i:i + 1, :e], dy=given[0][i:i + 1, :e], lengths=None, **one)))
+            for m in ("x", "y"):
+                same_infinities(got[m][i:i + 1, :e], parts[-1]["dx" if m == "x" else "y"], m)
+                assert not got[m][i, e:].any()
+            same_infinities(got["win"][i:i + 1], parts[-1]["dwin"], "dwin")
+        for m in ("w", "bias"):
+            same_infinities(got[m], sum(p["d" + m] for p in parts), "d" + m)
