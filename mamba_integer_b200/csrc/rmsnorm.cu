@@ -222,7 +222,13 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR > THREADS ?
 // column_sum_kernel adds those.  Those sums leave registers for two CTAs an SM
 // and none for the next row, which asynchronous copies bring into the thread's
 // own slots while a row is worked on.
-// registers that a thread of the backward pass holds for its packs, and the CTAs an SM that they leave room for
+// Registers that a thread of the backward pass holds for its packs; up to 92 of
+// them it runs in two CTAs an SM, which leave it 128 in all.  Two packs of 8 fit
+// those; three do not quite (without the bound they take about 195) and spill,
+// bf16 180 bytes, fp16 96.  us with the sums' kernel (2.8), in two CTAs an SM
+// and in one: 16384 x 512 bf16 20.5 and 23.0; x 768 bf16 32.7 and 28.8, fp16
+// 26.7 and 28.8, with fp32 residuals 43.6 and 39.0, fp32 46.3 and 39.2; x 1024
+// bf16 49.3 and 33.0.  So the bound is right but for three packs of bf16.
 template <typename T, typename R, int K, int NV>
 constexpr int held = (2 * K + (sizeof(T) + 2 * sizeof(R)) * K / 4) * NV;
 template <typename T, typename R, int K, int NV, int TPR>

@@ -262,3 +262,26 @@ def test_the_most_states():
         selective.selective_scan(**scan_args(k=most))
     with pytest.raises(ValueError, match=f"1 to {most} states"):
         selective.selective_scan(**scan_args(k=most + 1))
+
+
+def test_the_error_of_the_decays_polynomial():
+    """2^r on [-1/2, 1/2] by the kernels' coefficients: 2^-26.1, as the source says; the fp32 backward pass has them doubled."""
+    import os
+    import re
+
+    import numpy as np
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    with open(os.path.join(root, "mamba_integer_b200", "csrc", "selective.cu")) as f:
+        source = f.read()
+    found = []
+    for head in ("exp2_poly(float A, float2 dt) {", "exp2_poly(float2 x) {"):
+        body = source.split(head)[1].split("return")[0]
+        body = body[body.index("float2 p ="):]
+        found.append([float(np.float32(v)) for v in re.findall(r"dup\((?:2 \* )?([0-9.e-]+)f\)", body)])
+    assert len(found[0]) == 7 and found[0][:6] == found[1][:6] and found[0][6] == 1 and found[1][6] == 2
+    r = np.linspace(-0.5, 0.5, 200001)
+    p = np.zeros_like(r)
+    for c in found[0]:
+        p = p * r + c
+    worst = np.abs(p / np.exp2(r) - 1).max()
+    assert 2 ** -26.2 < worst < 2 ** -26.1
