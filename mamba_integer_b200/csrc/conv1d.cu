@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(128, 5) fwd_kernel(const Args a) {
 // copies of 16 bytes a lane bring the next DEPTH - 1 groups of 4 positions into
 // the warp's ring (zeros behind the sequence's length).  Rows off 16 bytes
 // (VEC = false) go through registers, one group ahead.  8 x 2048 x 1536 bf16:
-// 53 us (150 MB, 2.8 TB/s), the issue slots 68 % busy; 74 with each
+// 53 us (150 MB, 2.8 TB/s), the issue slots 69 % busy; 74 with each
 // lane's rows in registers, 80 with a copy for each pair, 56 with 4 CTAs an SM,
 // whose 64 registers spill.
 constexpr int BWD_RUNS = 8, DEPTH = 4, PAIR = 2;
