@@ -721,7 +721,9 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
 // from the last, is run again with its decays and states held in registers,
 // and walked backwards.  dB and dC are added over a lane's channels (where it
 // has more than one), across the warp's channel lanes, and once a tile across
-// the warps; sum_bc_kernel adds the channel blocks.
+// the warps; sum_kernel adds the channel blocks.  PAD: also where lanes have
+// channels beyond the last, which take no part in those sums (their zeros times
+// an infinite B or C are none).
 //
 // Across the channel lanes, a lane sends the half of its states that it does
 // not keep.  Lanes hold their 4 states in an order of their own (state
@@ -967,8 +969,13 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                 for (int k = 3; k >= 0; k--) {
                     const float2 dsk = dup(ds[k][j]);
                     const St g = only<PAD>(fma(Cv[k], dsk, gc[j]), there);
-                    vB[k] = j ? fma(g, dup(v[k][j]), vB[k]) : mul(g, dup(v[k][j]));
-                    vC[k] = j ? fma(h[k], dsk, vC[k]) : mul(h[k], dsk);
+                    if constexpr (PAD) {
+                        if (!j) vB[k] = vC[k] = st(make_float4(0, 0, 0, 0));
+                        if (d0 + c0 + j < a.D) vB[k] = fma(g, dup(v[k][j]), vB[k]), vC[k] = fma(h[k], dsk, vC[k]);
+                    } else {
+                        vB[k] = j ? fma(g, dup(v[k][j]), vB[k]) : mul(g, dup(v[k][j]));
+                        vC[k] = j ? fma(h[k], dsk, vC[k]) : mul(h[k], dsk);
+                    }
                     out[0][j][k] = dot(g, Bv[k]);
                     gc[j] = only<PAD>(mul(e[k], g), there);
                     const St w = mul(gc[j], k ? h[k ? k - 1 : 0] : h0);
@@ -1377,7 +1384,8 @@ static int backward_pad(Args& a, float* ws, cudaStream_t s) {
     a.part_bc = ws + w.part_bc, a.part_a = ws + w.part_a, a.part_d = ws + w.part_d;
     if (p.chunks > 1) {
         a.cst = ws + w.cst, a.cdt = ws + w.cdt;
-        const int rc = start_chunks<T, LN, LN == 2 ? 1 : LN == 16 ? 4 : LN == 8 ? 2 : 1, true, PAD>(a, s);
+        constexpr int CPL = LN == 2 ? 1 : LN == 16 ? 4 : LN == 8 ? 2 : 1;
+        const int rc = a.N < 4 * LN ? start_chunks<T, LN, CPL, true, true>(a, s) : start_chunks<T, LN, CPL, true, false>(a, s);
         if (rc != MI_OK) return rc;
     }
     constexpr size_t smem = sizeof(typename F::Smem);
@@ -1389,7 +1397,7 @@ static int backward_pad(Args& a, float* ws, cudaStream_t s) {
 }
 template <typename T, int LN>
 static int backward(Args& a, float* ws, cudaStream_t s) {
-    return a.N < 4 * LN ? backward_pad<T, LN, true>(a, ws, s) : backward_pad<T, LN, false>(a, ws, s);
+    return a.N < 4 * LN || a.D % BCfg<T, LN>::CB ? backward_pad<T, LN, true>(a, ws, s) : backward_pad<T, LN, false>(a, ws, s);
 }
 
 }  // namespace sscan

@@ -1089,3 +1089,24 @@ def test_conv_gradients_of_infinities_at_the_end(sel, cuda_dev, n, lens, d, silu
             same_infinities(got["win"][i:i + 1], parts[-1]["dwin"], "dwin")
         for m in ("w", "bias"):
             same_infinities(got[m], sum(p["d" + m] for p in parts), "d" + m)
+
+
+@pytest.mark.parametrize("k,d", [(1, 40), (5, 33), (8, 70), (16, 40), (16, 65), (16, 64), (20, 33), (32, 31), (64, 33), (50, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [20, 300])
+def test_scan_infinite_B_and_C(sel, cuda_dev, n, dtype, k, d):
+    """dB and dC are sums over the channels that there are, and no others of a block of channels."""
+    a = scan_inputs(cuda_dev, dtype, 2, n, d, k, h0=True)
+    for name in ("u", "B", "C", "D", "h0", "z"):
+        a[name] = a[name].abs() + 0.125
+    a["A"] *= 2 / k
+    a["B"][0, 7, k - 1] = a["C"][1, 12, 0] = float("inf")
+    g = torch.Generator().manual_seed(1)
+    dy, dh = torch.rand(2, n, d, generator=g).to(cuda_dev, dtype), torch.rand(2, d, k, generator=g).to(cuda_dev)
+    dy += 0.125
+    y, h, got = scan_grads(sel, a, dy, dh)
+    want = ref.scan(dict(a, dy=dy, dh=dh))
+    assert want["dC"][0, 7:, k - 1].isinf().all() and want["dB"][1, :13, 0].isinf().all()
+    assert want["dB"][0].isfinite().all() and want["dC"][1].isfinite().all()
+    for name, t in dict(got, y=y, h=h).items():
+        same_infinities(t, want[name if name in ("y", "h") else "d" + name], name)
