@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(CTA, 2) scan_kernel(const Args a) {
 // has more than one), across the warp's channel lanes, and once a tile across
 // the warps; sum_kernel adds the channel blocks.  PAD: also where lanes have
 // channels beyond the last, which take no part in those sums (their zeros times
-// an infinite B or C are none).
+// an infinite B or C are none): 8 x 2048 x 1528 1010 us in training, 994 without.
 //
 // Across the channel lanes, a lane sends the half of its states that it does
 // not keep.  Lanes hold their 4 states in an order of their own (state
