@@ -441,6 +441,40 @@ int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const 
                           int batch, int D, int W, int silu, int dtype, void* stream);
 
 /*
+ * Gated linear recurrence: a = sigmoid(f + bias[d]), c = 1 - a with `convex`,
+ * 1 without;
+ *   h[t] = a[t] h[t-1] + c[t] x[t],  h[-1] = h0 (0 if NULL)
+ *   y[t] = h[t] * z sigmoid(z) (h[t] with z NULL)
+ * x, f, z, y [batch, L, D]; bias [D]; h0, h_out [batch, D]; z, bias, h0,
+ * lengths, h_out may be NULL.  checkpoints (NULL without a backward pass):
+ * mi_gated_recurrence_checkpoints() floats.  L >= 1.  Gates never reach 0 (e^-|f|
+ * is 2^-126 at least): infinite states stay infinite.
+ */
+int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,
+                        const void* z, int64_t z_batch, int64_t z_row, const float* bias, const float* h0,
+                        const int32_t* lengths, void* y, float* h_out, float* checkpoints, int batch, int L, int D,
+                        int convex, int dtype, void* stream);
+int64_t mi_gated_recurrence_checkpoints(int batch, int L, int D);
+
+/* Its gradients, from dy [batch, L, D] and dh_out (NULL: 0): dx, df, dz [batch,
+ * L, D] (dz with z); dbias [D] and dh0 [batch, D], which may be NULL.
+ * workspace (for dbias): mi_gated_recurrence_backward_workspace() bytes.  The
+ * same inputs give the same bits. */
+int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const float* dh_out, const void* x,
+                                 int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,
+                                 const void* z, int64_t z_batch, int64_t z_row, const float* bias,
+                                 const int32_t* lengths, const float* checkpoints, void* dx, void* df, void* dz,
+                                 float* dbias, float* dh0, void* workspace, int batch, int L, int D, int convex,
+                                 int dtype, void* stream);
+int64_t mi_gated_recurrence_backward_workspace(int batch, int L, int D);
+
+/* One new token a stream: x, f, z, y [batch, D]; h [batch, D] is advanced in
+ * place. */
+int mi_gated_recurrence_step(const void* x, int64_t x_batch, const void* f, int64_t f_batch, const void* z,
+                             int64_t z_batch, const float* bias, float* h, void* y, int batch, int D, int convex,
+                             int dtype, void* stream);
+
+/*
  * RMS norm with the residual's addition: s = x + residual (s = x with residual
  * NULL), kept in the residual's type (`rdtype`: dtype, or MI_DT_F32) as `sum`;
  * rstd = 1 / sqrt(mean(s^2) + eps); y = s * rstd * weight.  The norm is of s

@@ -157,6 +157,26 @@ __device__ __forceinline__ float softplus(float x) {
     return __fadd_rn(fmaxf(x, 0.0f), l);
 }
 
+// out[c] = sum over p of part[p, c]: 32 strands of rows, then the strands in order
+static __global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, float* __restrict__ out,
+                                                                 int P, int D) {
+    __shared__ float sh[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+    float s = 0.0f;
+    if (c < D) {
+#pragma unroll 8
+        for (int p = g; p < P; p += 32) s = __fadd_rn(s, part[(int64_t)p * D + c]);
+    }
+    sh[g][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (g == 0 && c < D) {
+        float v = sh[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < 32; i++) v = __fadd_rn(v, sh[i][threadIdx.x]);
+        out[c] = v;
+    }
+}
+
 __host__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace mi

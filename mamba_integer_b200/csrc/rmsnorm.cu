@@ -360,26 +360,6 @@ __global__ void __launch_bounds__(TPR > THREADS ? TPR : THREADS, TPR <= THREADS 
     }
 }
 
-// out[c] = sum over p of part[p, c]: 32 strands of rows, then the strands in order
-__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, float* __restrict__ out, int P,
-                                                          int D) {
-    __shared__ float sh[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-    float s = 0.0f;
-    if (c < D) {
-#pragma unroll 8
-        for (int p = g; p < P; p += 32) s = __fadd_rn(s, part[(int64_t)p * D + c]);
-    }
-    sh[g][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (g == 0 && c < D) {
-        float v = sh[0][threadIdx.x];
-#pragma unroll
-        for (int i = 1; i < 32; i++) v = __fadd_rn(v, sh[i][threadIdx.x]);
-        out[c] = v;
-    }
-}
-
 constexpr int MAX_D = 16384;  // 512 threads of 4 packs
 
 // Threads of a row: a warp where 4 packs of 8 a thread hold it, 128 or 512
@@ -525,7 +505,7 @@ extern "C" int mi_rms_norm_backward(const void* dy, const void* dsum, const void
     const int grid = mi::rms::grid_of(T, D);
     const int rc2 = mi::rms::dispatch<true, false>(a, dtype, rdtype, grid, st);
     if (rc2 != MI_OK || !dweight) return rc2;
-    mi::rms::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, st>>>(a.dw_part, dweight, grid, D);
+    mi::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, st>>>(a.dw_part, dweight, grid, D);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }

@@ -33,7 +33,9 @@ using OptTensor = std::optional<Tensor>;
     X(mi_status_string) X(mi_selective_scan) X(mi_selective_scan_checkpoints) X(mi_selective_scan_workspace) \
     X(mi_selective_scan_backward) X(mi_selective_scan_step) X(mi_causal_conv1d) X(mi_causal_conv1d_backward) \
     X(mi_causal_conv1d_backward_workspace) X(mi_causal_conv1d_step) X(mi_rms_norm) X(mi_rms_norm_quant)      \
-    X(mi_rms_norm_backward) X(mi_rms_norm_backward_workspace)
+    X(mi_rms_norm_backward) X(mi_rms_norm_backward_workspace) X(mi_gated_recurrence)                         \
+    X(mi_gated_recurrence_checkpoints) X(mi_gated_recurrence_backward)                                       \
+    X(mi_gated_recurrence_backward_workspace) X(mi_gated_recurrence_step)
 
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -472,6 +474,116 @@ Tensor causal_conv1d_step(const Tensor& x, const Tensor& weight, const Tensor& w
 }
 
 // ---------------------------------------------------------------------------
+// gated linear recurrence
+// ---------------------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor> rec_forward(const Tensor& x, const Tensor& f, const Tensor& z, const Tensor& bias,
+                                               const Tensor& h0, const Tensor& lengths, bool convex, bool keep) {
+    const int64_t batch = x.size(0), L = x.size(1), d = x.size(2);
+    Place place(x);
+    Tensor y = at::empty({batch, L, d}, x.options()), h = floats({batch, d}, x), ckpt;
+    if (keep) ckpt = floats({mi.mi_gated_recurrence_checkpoints(batch, L, d)}, x);
+    check(mi.mi_gated_recurrence(ptr(x), st(x, 0), st(x, 1), ptr(f), st(f, 0), st(f, 1), ptr(z), st(z, 0), st(z, 1),
+                                 fptr(bias), fptr(h0), static_cast<int32_t*>(ptr(lengths)), ptr(y), fptr(h), fptr(ckpt),
+                                 batch, L, d, convex, dtype_code(x), place.stream),
+          "mi_gated_recurrence");
+    return {y, h, ckpt};
+}
+
+struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& f, const OptTensor& z_,
+                                 const OptTensor& bias_, const OptTensor& h0_, const OptTensor& lengths_, bool convex) {
+        const Tensor z = given(z_), bias = given(bias_), h0 = given(h0_), lengths = given(lengths_);
+        auto [y, h, ckpt] = rec_forward(x, f, z, bias, h0, lengths, convex, true);
+        ctx->save_for_backward({x, f, z, bias, lengths, ckpt});
+        ctx->saved_data["convex"] = convex;
+        ctx->saved_data["need"] = (int64_t)(bias.defined() && bias.requires_grad()) |
+                                  (int64_t)(h0.defined() && h0.requires_grad()) << 1;
+        ctx->set_materialize_grads(false);
+        return {y, h};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        if (!g[0].defined() && !g[1].defined()) return variable_list(7);
+        const auto s = ctx->get_saved_variables();
+        const Tensor &x = s[0], &f = s[1], &z = s[2], &bias = s[3], &lengths = s[4], &ckpt = s[5];
+        const bool convex = ctx->saved_data["convex"].toBool();
+        const int64_t need = ctx->saved_data["need"].toInt();
+        const int64_t batch = x.size(0), L = x.size(1), d = x.size(2);
+        const bool create = at::GradMode::is_enabled();
+        at::NoGradGuard no_grad;
+        Place place(x);
+        const Tensor dy = g[0].defined() ? unit(g[0]) : at::zeros({batch, L, d}, x.options());
+        const Tensor dh = g[1].defined() ? aligned(g[1]) : Tensor();
+        Tensor dx = empty_as(x), df = empty_as(f), dz = empty_as(z), dbias = empty_as(bias, need & 1);
+        Tensor dh0 = need & 2 ? floats({batch, d}, x) : Tensor(), ws;
+        if (need & 1) ws = workspace(mi.mi_gated_recurrence_backward_workspace(batch, L, d), x);
+        check(mi.mi_gated_recurrence_backward(
+                  ptr(dy), st(dy, 0), st(dy, 1), fptr(dh), ptr(x), st(x, 0), st(x, 1), ptr(f), st(f, 0), st(f, 1), ptr(z),
+                  st(z, 0), st(z, 1), fptr(bias), static_cast<int32_t*>(ptr(lengths)), fptr(ckpt), ptr(dx), ptr(df),
+                  ptr(dz), fptr(dbias), fptr(dh0), ptr(ws), batch, L, d, convex, dtype_code(x), place.stream),
+              "mi_gated_recurrence_backward");
+        return once({dx, df, dz, dbias, dh0, Tensor(), Tensor()}, create, s, g);
+    }
+};
+
+// lead: {batch, L} or {batch}; returns the bias
+Tensor rec_arguments(at::IntArrayRef lead, const Tensor& x, const Tensor& gate, const OptTensor& z, const OptTensor& bias) {
+    activation(x, "x");
+    countable(x, "x");
+    const int64_t d = x.size(-1);
+    TORCH_CHECK_VALUE(d > 0 && d <= 1 << 24, "x must have 1 to ", 1 << 24, " channels, got ", x.sizes());
+    c10::SmallVector<int64_t, 3> full(lead.begin(), lead.end());
+    full.push_back(d);
+    like(x, x, full, "x");
+    like(gate, x, full, "gate");
+    if (z.has_value()) like(*z, x, full, "z");
+    return plain(bias, x, {d}, at::kFloat, "gate_bias");
+}
+
+std::tuple<Tensor, Tensor> gated_recurrence(const Tensor& x, const Tensor& gate, const OptTensor& z_,
+                                            const OptTensor& bias_, bool convex, const OptTensor& h0_,
+                                            const OptTensor& lengths_) {
+    const Tensor z = given(z_);
+    no_tangents(x, gate, z, given(bias_), given(h0_));
+    TORCH_CHECK_VALUE(x.dim() == 3, "x must be [batch, L, channels], got ", x.sizes());
+    const int64_t batch = x.size(0), L = x.size(1), d = x.size(2);
+    const Tensor bias = rec_arguments({batch, L}, x, gate, z_, bias_);
+    const Tensor h0 = plain(h0_, x, {batch, d}, at::kFloat, "h0");
+    const Tensor lengths = lengths_of(lengths_, x, batch);
+    TORCH_CHECK_VALUE(batch <= MAX_BATCH, "at most ", MAX_BATCH, " sequences, got x ", x.sizes());
+    on_gpu(x, "x");
+    if (batch == 0 || L == 0)
+        return {reached(x * 1, {&gate, &z, &bias, &h0}),
+                h0.defined() ? h0 * 1 : at::zeros({batch, d}, x.options().dtype(at::kFloat))};
+    if (at::GradMode::is_enabled() && any_requires_grad(x, gate, z, bias, h0)) {
+        capturable({&x, &gate, &z, &bias, &h0}, x.device());
+        const auto out = GatedRecurrence::apply(x, gate, maybe(z), maybe(bias), maybe(h0), maybe(lengths), convex);
+        return {out[0], out[1]};
+    }
+    auto [y, h, ckpt] = rec_forward(x, gate, z, bias, h0, lengths, convex, false);
+    return {y, h};
+}
+
+Tensor gated_recurrence_step(const Tensor& h, const Tensor& x, const Tensor& gate, const OptTensor& z_,
+                             const OptTensor& bias_, bool convex) {
+    const Tensor z = given(z_);
+    TORCH_CHECK_VALUE(x.dim() == 2, "x must be [batch, channels], got ", x.sizes());
+    const int64_t batch = x.size(0), d = x.size(1);
+    no_tangents(h, x, gate, z, given(bias_));
+    no_grad_needed(h, x, gate, z, given(bias_));
+    const Tensor bias = rec_arguments({batch}, x, gate, z_, bias_);
+    in_place(h, x, {batch, d}, at::kFloat, "h");
+    TORCH_CHECK_VALUE(batch <= MAX_BATCH, "at most ", MAX_BATCH, " streams, got x ", x.sizes());
+    on_gpu(x, "x");
+    Place place(x);
+    Tensor y = at::empty({batch, d}, x.options());
+    check(mi.mi_gated_recurrence_step(ptr(x), st(x, 0), ptr(gate), st(gate, 0), ptr(z), st(z, 0), fptr(bias), fptr(h),
+                                      ptr(y), batch, d, convex, dtype_code(x), place.stream),
+          "mi_gated_recurrence_step");
+    written(h);
+    return y;
+}
+
+// ---------------------------------------------------------------------------
 // RMS norm
 // ---------------------------------------------------------------------------
 std::tuple<Tensor, Tensor, Tensor> rms_forward(const Tensor& x, const Tensor& w, double eps, const Tensor& r, bool keep) {
@@ -588,6 +700,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("selective_scan_step", &selective_scan_step, free);
     m.def("causal_conv1d", &causal_conv1d, free);
     m.def("causal_conv1d_step", &causal_conv1d_step, free);
+    m.def("gated_recurrence", &gated_recurrence, free);
+    m.def("gated_recurrence_step", &gated_recurrence_step, free);
     m.def("rms_norm", &rms_norm, free);
     m.def("rms_norm_quant", &rms_norm_quant, free);
 }

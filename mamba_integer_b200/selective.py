@@ -6,6 +6,8 @@ pass), for prompts, and for single tokens.
     y    = selective_scan_step(h, u, delta, A, B, C, D=.., z=..)      # h in place
     y, w = causal_conv1d(x, weight, bias=.., silu=True, return_window=True)
     y    = causal_conv1d_step(x, weight, w, bias=.., silu=True)       # w in place
+    y, h = gated_recurrence(x, gate, z=.., gate_bias=.., return_state=True)
+    y    = gated_recurrence_step(h, x, gate, z=.., gate_bias=..)      # h in place
     y, s = rms_norm(x, weight, residual=r)                            # s = x + r
     q, scale, s = rms_norm_quant(x, weight, residual=r)               # int8 rows for the ternary GEMMs
 
@@ -118,6 +120,33 @@ def causal_conv1d_step(x: torch.Tensor, weight: torch.Tensor, win: torch.Tensor,
     win [batch, taps - 1, channels] is advanced in place.  Returns y [batch,
     channels].  No backward pass."""
     return (_ops or _load()).causal_conv1d_step(x, weight, win, bias, silu)
+
+
+def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, z: Optional[torch.Tensor] = None,
+                     gate_bias: Optional[torch.Tensor] = None, convex: bool = True,
+                     h0: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                     return_state: bool = False):
+    """Gated linear recurrence over [batch, L, channels], the float form of the
+    convex dyadic one with an input-dependent gate:
+
+        a = sigmoid(gate + gate_bias)
+        h[t] = a[t] h[t-1] + (1 - a[t]) x[t],  h[-1] = h0 (zeros without one)
+        y[t] = h[t] * z sigmoid(z)  (h[t] without z)
+
+    Without ``convex`` the input is not weighed: h[t] = a[t] h[t-1] + x[t].
+    x, gate, z [batch, L, channels]; gate_bias [channels]; h0 [batch,
+    channels].  Returns y, or (y, final state) with ``return_state``.  A gate is
+    at least 2^-127, so that an infinite state stays one."""
+    y, h = (_ops or _load()).gated_recurrence(x, gate, z, gate_bias, convex, h0, lengths)
+    return (y, h) if return_state else y
+
+
+def gated_recurrence_step(h: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, z: Optional[torch.Tensor] = None,
+                          gate_bias: Optional[torch.Tensor] = None, convex: bool = True) -> torch.Tensor:
+    """One position of gated_recurrence for every stream: x, gate, z [batch,
+    channels]; h [batch, channels] is advanced in place.  Returns y [batch,
+    channels].  No backward pass."""
+    return (_ops or _load()).gated_recurrence_step(h, x, gate, z, gate_bias, convex)
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None

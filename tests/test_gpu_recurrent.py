@@ -1,0 +1,244 @@
+"""The float recurrent layer's operators against their 64-bit formulas (tests/recurrent_ref.py, where the tolerances are
+derived)."""
+import pytest
+import torch
+
+import recurrent_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def sel(cuda_dev):
+    from mamba_integer_b200 import selective
+    return selective
+
+
+def rec_inputs(dev, dtype, b, n, d, seed=0, z=True, bias=True, h0=False, convex=True, lengths=None):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(x=r(b, n, d).to(dtype), f=(r(b, n, d) + (0 if bias else 2)).to(dtype), z=r(b, n, d).to(dtype) if z else None,
+             bias=2 + 2 * r(d) if bias else None, h0=r(b, d) if h0 else None, convex=convex)
+    a["lengths"] = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    return {k: t.to(dev) if isinstance(t, torch.Tensor) else t for k, t in a.items()}
+
+
+def call_rec(sel, a, **over):
+    a = {**a, **over}
+    return sel.gated_recurrence(a["x"], a["f"], z=a["z"], gate_bias=a["bias"], convex=a["convex"], h0=a["h0"],
+                                lengths=a["lengths"], return_state=True)
+
+
+def check_rec(y, h, a):
+    want = ref.recurrence(a)
+    ref.check(y, want["y"], "y")
+    ref.check(h, want["h"], "h")
+
+
+REC_SIZES = [
+    # batch, L, channels: blocks of 64 channels, stretches of 8 and 16 positions, tiles of 64 and 128, clusters of 1 to 8
+    (1, 1, 1), (2, 1, 64), (1, 2, 33), (3, 7, 31), (2, 8, 64), (2, 9, 65), (1, 15, 100), (2, 16, 128), (1, 17, 8),
+    (2, 63, 72), (1, 64, 2), (1, 65, 130), (3, 128, 40), (2, 129, 64), (1, 255, 16), (1, 257, 66), (1, 513, 24),
+    (1, 1100, 72), (40, 70, 520), (2, 2050, 12),
+]
+
+
+@pytest.mark.parametrize("size", REC_SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_prompt(sel, cuda_dev, size, dtype):
+    a = rec_inputs(cuda_dev, dtype, *size, h0=size[1] % 2 == 1)
+    check_rec(*call_rec(sel, a), a)
+
+
+def rec_grads(sel, a, dy, dh, need=None):
+    names = [k for k in ("x", "f", "z", "bias", "h0") if a[k] is not None and (need is None or k in need)]
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in names}
+    y, h = call_rec(sel, a, **leaves)
+    outs = [(o, g) for o, g in ((y, dy), (h, dh)) if g is not None]
+    got = torch.autograd.grad([o for o, _ in outs], list(leaves.values()), [g for _, g in outs], allow_unused=True)
+    return y, h, dict(zip(names, got))
+
+
+def check_rec_grads(got, a, dy, dh):
+    want = ref.recurrence(dict(a, dy=dy, dh=dh))
+    for name, t in got.items():
+        assert t.dtype == a[name].dtype
+        ref.check(t, want["d" + name], "d" + name)
+
+
+@pytest.mark.parametrize("size", REC_SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_gradients(sel, cuda_dev, size, dtype):
+    b, n, d = size
+    a = rec_inputs(cuda_dev, dtype, *size, h0=True)
+    g = torch.Generator().manual_seed(5)
+    dy, dh = torch.randn(b, n, d, generator=g).to(cuda_dev, dtype), torch.randn(b, d, generator=g).to(cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+
+
+@pytest.mark.parametrize("convex", [True, False])
+@pytest.mark.parametrize("z,bias,h0", [(False, False, False), (True, False, True), (False, True, True)])
+@pytest.mark.parametrize("n", [40, 300])
+def test_recurrence_options(sel, cuda_dev, n, convex, z, bias, h0):
+    a = rec_inputs(cuda_dev, F32, 2, n, 48, z=z, bias=bias, h0=h0, convex=convex)
+    dy = torch.randn(2, n, 48, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, None)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, None)
+    dh = torch.randn(2, 48, device=cuda_dev)
+    _, _, got = rec_grads(sel, a, None, dh, need=("x", "f"))
+    check_rec_grads(got, a, None, dh)
+
+
+@pytest.mark.parametrize("n", [37, 260])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_recurrence_lengths(sel, cuda_dev, n, dtype):
+    # 0, 1, inside and at a stretch's border, past the end (clamped), negative (clamped)
+    lens = [0, 1, 8, 16, 20, n, n + 5, -3]
+    a = rec_inputs(cuda_dev, dtype, len(lens), n, 40, h0=True, lengths=lens)
+    clamped = dict(a, lengths=torch.tensor([min(max(v, 0), n) for v in lens], dtype=torch.int32))
+    dy, dh = torch.randn(len(lens), n, 40, device=cuda_dev).to(dtype), torch.randn(len(lens), 40, device=cuda_dev)
+    for i, v in enumerate(clamped["lengths"].tolist()):  # what lies behind a length is not used
+        for name in ("x", "f", "z"):
+            a[name][i, v:] = float("nan") if i % 2 else float("inf")
+        dy[i, v:] = float("nan")
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, clamped)
+    check_rec_grads(got, clamped, dy, dh)
+    for i, v in enumerate(clamped["lengths"].tolist()):
+        assert not y[i, v:].any() and not got["x"][i, v:].any() and not got["f"][i, v:].any() and not got["z"][i, v:].any()
+    assert torch.equal(h[0], a["h0"][0]) and torch.equal(got["h0"][0], dh[0])
+
+
+def test_recurrence_strides_slices_and_broadcasts(sel, cuda_dev):
+    b, n, d = 3, 70, 48
+    a = rec_inputs(cuda_dev, BF16, b, n, d)
+    want = call_rec(sel, a)
+    for pad in (8, 3):  # columns of wider rows, aligned and not; every other row
+        wide = torch.randn(b, 2 * n, 3 * d + pad, device=cuda_dev).to(BF16)
+        cut = {}
+        for i, key in enumerate(("x", "f", "z")):
+            cut[key] = wide[:, ::2, pad + i * d:pad + (i + 1) * d]
+            cut[key].copy_(a[key])
+        got = call_rec(sel, a, **cut)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    one = {key: a[key][:1] for key in ("x", "f", "z")}
+    spread = call_rec(sel, a, **{key: t.expand(b, -1, -1) for key, t in one.items()})
+    copied = call_rec(sel, a, **{key: t.repeat(b, 1, 1) for key, t in one.items()})
+    assert torch.equal(spread[0], copied[0]) and torch.equal(spread[1], copied[1])
+    flat = torch.empty(d + 1, device=cuda_dev)
+    flat[1:].copy_(a["bias"])
+    assert torch.equal(call_rec(sel, a, bias=flat[1:])[0], want[0])
+    # gradients of a sequence that several share
+    dy = torch.randn(b, n, d, device=cuda_dev).to(BF16)
+    x = one["x"].detach().clone().requires_grad_(True)
+    y, _ = call_rec(sel, a, x=x.expand(b, -1, -1))
+    got, = torch.autograd.grad(y, x, dy)
+    xs = one["x"].repeat(b, 1, 1).requires_grad_(True)
+    y, _ = call_rec(sel, a, x=xs)
+    each, = torch.autograd.grad(y, xs, dy.transpose(1, 2).contiguous().transpose(1, 2))  # a gradient with another layout
+    assert torch.equal(got, each.sum(0, keepdim=True))
+
+
+def test_recurrence_offsets_past_32_bits(sel, cuda_dev):
+    n, d = 20, 32
+    a = rec_inputs(cuda_dev, BF16, 2, n, d)
+    want = call_rec(sel, a)
+    big = torch.empty(2 ** 31 + 64 * n, dtype=BF16, device=cuda_dev)
+    for i, key in enumerate(("x", "f", "z")):
+        far = big[i * 8 * d:].as_strided((2, n, d), (2 ** 31 + 3 * d - 2 ** 10, d, 1))
+        far.copy_(a[key])
+        got = call_rec(sel, a, **{key: far})
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_recurrence_extreme_gates(sel, cuda_dev, dtype):
+    """Gates that keep the state, that drop it at once, and NaN and infinities of inputs and states."""
+    n = 300
+    a = rec_inputs(cuda_dev, dtype, 1, n, 64, h0=True, bias=False, z=False)
+    a["f"][0, ::3], a["f"][0, 1::7] = 60.0, -60.0
+    dy, dh = torch.randn_like(a["x"]), torch.randn(1, 64, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+    a["f"][0, ::3], a["f"][0, 1::7] = float("inf"), float("-inf")  # a convention: 2^-126 is as good as 0
+    y2, h2 = call_rec(sel, a)
+    assert torch.isfinite(y2).all() and torch.isfinite(h2).all()
+    a = rec_inputs(cuda_dev, dtype, 1, n, 64, h0=True)
+    a["x"][0, 150, :32] = float("inf")
+    a["h0"][0, 40] = float("-inf")
+    a["x"][0, 200, 50] = float("nan")
+    y, h = call_rec(sel, a, z=None)
+    assert (y[0, 150:, :32] == float("inf")).all() and torch.isfinite(y[0, :150, :32]).all()
+    assert (y[0, :, 40] == float("-inf")).all() and h[0, 40] == float("-inf")
+    assert torch.isfinite(y[0, :200, 50]).all() and y[0, 200:, 50].isnan().all() and h[0, 50].isnan()
+    rest = [i for i in range(32, 64) if i not in (40, 50)]
+    assert torch.isfinite(y[..., rest]).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("size", [(1, 1), (3, 33), (4, 512), (2, 130), (256, 64), (5, 1021)])
+@pytest.mark.parametrize("convex,z,bias", [(True, True, True), (False, False, False), (True, False, True), (False, True, False)])
+def test_recurrence_step(sel, cuda_dev, dtype, size, convex, z, bias):
+    b, d = size
+    a = rec_inputs(cuda_dev, dtype, b, 3, d, z=z, bias=bias, h0=True, convex=convex)
+    h = a["h0"].clone()
+    ys = []
+    for t in range(3):
+        with torch.no_grad():
+            ys.append(sel.gated_recurrence_step(h, a["x"][:, t], a["f"][:, t], z=None if a["z"] is None else a["z"][:, t],
+                                                gate_bias=a["bias"], convex=convex))
+    check_rec(torch.stack(ys, 1), h, a)
+
+
+def test_recurrence_same_bits_and_streams(sel, cuda_dev):
+    """The same inputs give the same bits, on another stream and captured in a graph that is replayed."""
+    a = rec_inputs(cuda_dev, BF16, 2, 700, 192, h0=True)
+    dy, dh = torch.randn(2, 700, 192, device=cuda_dev).to(BF16), torch.randn(2, 192, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    y, h, got = y.detach(), h.detach(), {k: t.clone() for k, t in got.items()}
+    for _ in range(3):
+        y2, h2, got2 = rec_grads(sel, a, dy, dh)
+        assert torch.equal(y, y2) and torch.equal(h, h2) and all(torch.equal(got[k], got2[k]) for k in got)
+    del y2, h2, got2
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in got}
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        call_rec(sel, a, **leaves)
+        s.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            y3, h3 = call_rec(sel, a, **leaves)
+            got3 = torch.autograd.grad([y3, h3], list(leaves.values()), [dy, dh])
+    for _ in range(2):
+        y3.detach().zero_(), h3.detach().zero_(), [t.zero_() for t in got3]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, y3) and torch.equal(h, h3)
+        assert all(torch.equal(got[k], t) for k, t in zip(leaves, got3))
+
+
+def test_recurrence_empty_calls(sel, cuda_dev):
+    for b, n in ((0, 5), (2, 0)):
+        a = rec_inputs(cuda_dev, F32, b, n, 8, h0=True)
+        leaves = {k: a[k].detach().clone().requires_grad_(True) for k in ("x", "f", "z", "bias", "h0")}
+        y, h = call_rec(sel, a, **leaves)
+        assert y.shape == (b, n, 8) and torch.equal(h, a["h0"])
+        got = torch.autograd.grad([y.sum() + h.sum()], list(leaves.values()))
+        assert not got[3].any() and (got[4] == 1).all()
+
+
+def test_recurrence_second_order_is_refused(sel, cuda_dev):
+    a = rec_inputs(cuda_dev, F32, 1, 9, 8)
+    x = a["x"].requires_grad_(True)
+    y, _ = call_rec(sel, a)
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(g.sum(), x)

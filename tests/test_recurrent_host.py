@@ -1,0 +1,141 @@
+"""The float recurrent layer's operators without a GPU: the refusals of the Python functions and of the C entry points, and
+the 64-bit formulas that the GPU tests compare with against differences."""
+import pytest
+import torch
+
+import recurrent_ref as ref
+from mamba_integer_b200 import _lib, selective
+
+
+def _t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def _rand(g, *shape):
+    return torch.randn(*shape, generator=g, dtype=torch.float64)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(x=_t(2, 5, 8, dtype=torch.float64)), TypeError),
+    (dict(x=_t(2, 8)), ValueError),
+    (dict(x=_t(2, 5, 0), gate=_t(2, 5, 0)), ValueError),
+    (dict(gate=_t(2, 5, 7)), ValueError),
+    (dict(gate=_t(2, 5, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(x=_t(2, 8, 5).transpose(1, 2)), ValueError),
+    (dict(gate=_t(2, 8, 5).transpose(1, 2)), ValueError),
+    (dict(z=_t(2, 4, 8)), ValueError),
+    (dict(z=_t(2, 5, 8, dtype=torch.float16)), TypeError),
+    (dict(gate_bias=_t(7)), ValueError),
+    (dict(gate_bias=_t(8, dtype=torch.bfloat16)), TypeError),
+    (dict(h0=_t(2, 7)), ValueError),
+    (dict(h0=_t(2, 8, dtype=torch.float64)), TypeError),
+    (dict(lengths=torch.zeros(2, dtype=torch.int64)), ValueError),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), ValueError),
+    (dict(), ValueError),  # CPU tensors
+])
+def test_recurrence_refuses(change, error):
+    with pytest.raises(error):
+        selective.gated_recurrence(**{**dict(x=_t(2, 5, 8), gate=_t(2, 5, 8)), **change})
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(h=_t(2, 7)), ValueError),
+    (dict(h=_t(2, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(h=_t(8, 2).t()), ValueError),
+    (dict(h=_t(17)[1:].view(2, 8)), ValueError),  # off the 16-byte boundary
+    (dict(x=_t(2, 1, 8)), ValueError),
+    (dict(gate=_t(3, 8)), ValueError),
+    (dict(z=_t(2, 8, dtype=torch.float16)), TypeError),
+    (dict(gate_bias=_t(8).requires_grad_(True)), RuntimeError),
+    (dict(), ValueError),
+])
+def test_recurrence_step_refuses(change, error):
+    with pytest.raises(error):
+        selective.gated_recurrence_step(**{**dict(h=_t(2, 8), x=_t(2, 8), gate=_t(2, 8)), **change})
+
+
+def test_sizes_past_the_counters_are_refused():
+    """Expanded views: no such memory is there."""
+    for shape, what in (((1, (1 << 30) + 1, 1), "too long"), ((65536, 1, 1), "at most 65535"),
+                        ((65536, 0, 1), "at most 65535"), ((1, 1, (1 << 24) + 1), "channels")):
+        x = _t(1).as_strided(shape, (0, 0, 0))
+        with pytest.raises(ValueError, match=what):
+            selective.gated_recurrence(x, x)
+    with pytest.raises(ValueError, match="at most 65535 streams"):
+        selective.gated_recurrence_step(_t(65536, 1), _t(65536, 1), _t(65536, 1))
+
+
+def test_entry_points_refuse_on_the_host():
+    """Before any CUDA call; the pointers are not touched."""
+    lib = _lib.load()
+    p, s, none = 256, (256, 512, 64), (None, 0, 0)
+
+    def fwd(x=s, f=s, z=none, y=p, batch=2, L=8, D=64, dtype=0):
+        return lib.mi_gated_recurrence(*x, *f, *z, None, None, None, y, p, None, batch, L, D, 1, dtype, None)
+    assert fwd(x=none) == -1 and fwd(f=none) == -1 and fwd(y=None) == -1
+    assert fwd(L=0) == -1 and fwd(L=-1) == -1 and fwd(D=0) == -1 and fwd(batch=-1) == -1
+    assert fwd(dtype=3) == -1 and fwd(dtype=-1) == -1 and fwd(z=(256, -1, 64)) == -1
+    assert fwd(batch=65536) == -2
+    assert fwd(batch=0) == 0
+    bwd = lambda dy=s, ck=p, dx=p, df=p, dz=p, dbias=p, ws=p, z=s: lib.mi_gated_recurrence_backward(  # noqa: E731
+        *dy, None, *s, *s, *z, None, None, ck, dx, df, dz, dbias, None, ws, 2, 8, 64, 1, 0, None)
+    assert bwd(dy=none) == -1 and bwd(ck=None) == -1 and bwd(dx=None) == -1 and bwd(df=None) == -1 and bwd(dz=None) == -1
+    assert bwd(ws=None) == -1
+    step = lambda h=p, y=p, dtype=0, D=64: lib.mi_gated_recurrence_step(p, 64, p, 64, None, 0, None, h, y, 2, D, 1, dtype,  # noqa: E731
+                                                                       None)
+    assert step(h=None) == -1 and step(y=None) == -1 and step(dtype=7) == -1 and step(D=0) == -1
+    assert lib.mi_gated_recurrence_checkpoints(2, 17, 5) == 2 * 3 * 5
+    assert lib.mi_gated_recurrence_backward_workspace(1, 64, 64) == 4 * 64
+
+
+def slopes(value, leaves, got, prefix="d"):
+    """Central differences of 1e-6 in 64 bits: 1e-12 of curvature and 1e-10 of rounding next to values of order 10."""
+    g = torch.Generator().manual_seed(77)
+    for name, t in leaves.items():
+        v = _rand(g, *t.shape)
+        up, down = (value({**leaves, name: t + s * 1e-6 * v}) for s in (1, -1))
+        slope = float(up - down) / 2e-6
+        have = float((got[prefix + name][0] * v).sum())
+        assert abs(have - slope) < 1e-7 * max(1, abs(slope)) + 1e-7, (name, have, slope)
+
+
+@pytest.mark.parametrize("convex", [True, False])
+def test_recurrence_formula_against_differences(convex):
+    g = torch.Generator().manual_seed(0)
+    b, n, d = 3, 7, 4
+    leaves = dict(x=_rand(g, b, n, d), f=_rand(g, b, n, d), z=_rand(g, b, n, d), bias=_rand(g, d), h0=_rand(g, b, d))
+    rest = dict(convex=convex, lengths=torch.tensor([7, 4, 0], dtype=torch.int32))
+    dy, dh = _rand(g, b, n, d), _rand(g, b, d)
+
+    def value(vals):
+        out = ref.recurrence({**vals, **rest})
+        return (out["y"][0] * dy).sum() + (out["h"][0] * dh).sum()
+    slopes(value, leaves, ref.recurrence({**leaves, **rest, "dy": dy, "dh": dh}))
+    # the formula itself, written out for one channel
+    one = {k: (t[:1, :, :1] if t.dim() == 3 else t[..., :1] if t.dim() == 1 else t[:1, :1]) for k, t in leaves.items()}
+    out, h = ref.recurrence({**one, "convex": convex}), float(one["h0"])
+    for t in range(n):
+        a = float(torch.sigmoid(one["f"][0, t, 0] + one["bias"][0]))
+        h = a * h + (1 - a if convex else 1) * float(one["x"][0, t, 0])
+        z = float(one["z"][0, t, 0])
+        assert abs(float(out["y"][0][0, t, 0]) - h * z / (1 + 2.718281828459045 ** -z)) < 1e-12
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost; any argument may carry it, a view of a dual tensor too."""
+    from torch.autograd import forward_ad
+
+    x = lambda: _t(2, 5, 8)  # noqa: E731
+    calls = [
+        (selective.gated_recurrence, dict(x=x(), gate=x(), z=x(), gate_bias=_t(8), h0=_t(2, 8))),
+        (selective.gated_recurrence_step, dict(h=_t(2, 8), x=_t(2, 8), gate=_t(2, 8), z=_t(2, 8), gate_bias=_t(8))),
+    ]
+    for fn, args in calls:
+        for name, t in args.items():
+            with forward_ad.dual_level():
+                wide = forward_ad.make_dual(torch.zeros(2, *t.shape), torch.ones(2, *t.shape))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="forward-mode"):
+                        fn(**{**args, name: wide[0]})
+        with pytest.raises(ValueError, match="must be a CUDA tensor"):  # and without one the call goes on
+            fn(**args)
