@@ -498,6 +498,23 @@ int mi_rms_norm_backward(const void* dy, const void* dsum, const void* s, int64_
                          int dtype, int rdtype, void* stream);
 int64_t mi_rms_norm_backward_workspace(int T, int D);
 
+/*
+ * Layer norm with the residual's addition: s = x + residual as in mi_rms_norm;
+ * mean and variance of s as it is kept, rstd = 1 / sqrt(var + eps),
+ * y = (s - mean) * rstd * weight + bias (bias may be NULL).  stats [T, 2] (may be
+ * NULL): mean and rstd of each row for the backward pass, 8-byte aligned.
+ * D <= 16384.
+ */
+int mi_layer_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, const float* weight, const float* bias,
+                  void* y, void* sum, float* stats, int T, int D, float eps, int dtype, int rdtype, void* stream);
+
+/* Gradients of mi_layer_norm, as mi_rms_norm_backward's, and dbias [D].
+ * workspace (for dweight or dbias): mi_layer_norm_backward_workspace() bytes. */
+int mi_layer_norm_backward(const void* dy, const void* dsum, const void* s, int64_t lds, const float* weight,
+                           const float* stats, void* dx, void* dresidual, float* dweight, float* dbias,
+                           void* workspace, int T, int D, int dtype, int rdtype, void* stream);
+int64_t mi_layer_norm_backward_workspace(int T, int D);
+
 #ifdef __cplusplus
 }
 #endif

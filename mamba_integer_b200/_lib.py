@@ -76,10 +76,14 @@ SIGNATURES = {
     "mi_rms_norm_quant": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
     "mi_rms_norm_backward": [_p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     "mi_rms_norm_backward_workspace": [_i, _i],
+    "mi_layer_norm": [_p, _i64, _p, _i64] + [_p] * 5 + [_i, _i, _f, _i, _i, _p],
+    "mi_layer_norm_backward": [_p, _p, _p, _i64] + [_p] * 7 + [_i] * 4 + [_p],
+    "mi_layer_norm_backward_workspace": [_i, _i],
 }
 _RESTYPE = {"mi_status_string": ctypes.c_char_p, "mi_selective_scan_checkpoints": _i64,
             "mi_selective_scan_workspace": _i64, "mi_causal_conv1d_backward_workspace": _i64,
             "mi_rms_norm_backward_workspace": _i64, "mi_gated_recurrence_checkpoints": _i64,
+            "mi_layer_norm_backward_workspace": _i64,
             "mi_gated_recurrence_backward_workspace": _i64}
 
 _lib = None

@@ -35,7 +35,8 @@ using OptTensor = std::optional<Tensor>;
     X(mi_causal_conv1d_backward_workspace) X(mi_causal_conv1d_step) X(mi_rms_norm) X(mi_rms_norm_quant)      \
     X(mi_rms_norm_backward) X(mi_rms_norm_backward_workspace) X(mi_gated_recurrence)                         \
     X(mi_gated_recurrence_checkpoints) X(mi_gated_recurrence_backward)                                       \
-    X(mi_gated_recurrence_backward_workspace) X(mi_gated_recurrence_step)
+    X(mi_gated_recurrence_backward_workspace) X(mi_gated_recurrence_step) X(mi_layer_norm)                   \
+    X(mi_layer_norm_backward) X(mi_layer_norm_backward_workspace)
 
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -638,11 +639,11 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
 };
 
 struct Rows {
-    Tensor x, w, r;
+    Tensor x, w, r, b;
 };
 
-Rows rms_arguments(const Tensor& x, const Tensor& weight, const OptTensor& residual) {
-    no_tangents(x, weight, given(residual));
+Rows norm_arguments(const Tensor& x, const Tensor& weight, const OptTensor& residual, const OptTensor& bias = {}) {
+    no_tangents(x, weight, given(residual), given(bias));
     activation(x, "x");
     const int64_t d = x.dim() ? x.size(-1) : 0;
     TORCH_CHECK_VALUE(d >= 1 && d <= 16384, "rows of 1 to 16384 columns, got x ", x.sizes());
@@ -652,15 +653,15 @@ Rows rms_arguments(const Tensor& x, const Tensor& weight, const OptTensor& resid
                          "residual must be ", x.scalar_type(), " or float32, got ", residual->scalar_type());
         same_device(*residual, x, "residual");
     }
-    const Tensor w = plain(weight, x, {d}, at::kFloat, "weight");
+    const Tensor w = plain(weight, x, {d}, at::kFloat, "weight"), b = plain(bias, x, {d}, at::kFloat, "bias");
     on_gpu(x, "x");
     TORCH_CHECK_VALUE(x.numel() / d <= int64_t(1) << 30, "x has too many rows: ", x.sizes());
     auto rows = [&](const Tensor& t) { return unit(t.dim() == 2 ? t : t.reshape({-1, d})); };
-    return {rows(x), w, residual.has_value() ? rows(*residual) : Tensor()};
+    return {rows(x), w, residual.has_value() ? rows(*residual) : Tensor(), b};
 }
 
 std::tuple<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual) {
-    const Rows a = rms_arguments(x, weight, residual);
+    const Rows a = norm_arguments(x, weight, residual);
     auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : t.view(x.sizes()); };
     if (a.x.size(0) == 0)
         return {reached(x * 1, {&a.w, &a.r}), residual.has_value() ? OptTensor(reached(*residual * 1, {&a.x})) : OptTensor()};
@@ -676,7 +677,7 @@ std::tuple<Tensor, OptTensor> rms_norm(const Tensor& x, const Tensor& weight, do
 std::tuple<Tensor, Tensor, OptTensor> rms_norm_quant(const Tensor& x, const Tensor& weight, double eps,
                                                      const OptTensor& residual) {
     no_grad_needed(x, weight, given(residual));
-    const Rows a = rms_arguments(x, weight, residual);
+    const Rows a = norm_arguments(x, weight, residual);
     const int64_t T = a.x.size(0), d = a.x.size(1);
     Place place(a.x);
     Tensor q = at::empty({T, d}, x.options().dtype(at::kChar)), scale = floats({T}, x);
@@ -691,6 +692,81 @@ std::tuple<Tensor, Tensor, OptTensor> rms_norm_quant(const Tensor& x, const Tens
             total.defined() ? OptTensor(total.view(x.sizes())) : OptTensor()};
 }
 
+// ---------------------------------------------------------------------------
+// layer norm
+// ---------------------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor> ln_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps,
+                                              const Tensor& r, bool keep) {
+    const int64_t T = x.size(0), d = x.size(1);
+    Place place(x);
+    Tensor y = at::empty({T, d}, x.options()), total = r.defined() ? at::empty({T, d}, r.options()) : Tensor();
+    Tensor stats = keep ? floats({T, 2}, x) : Tensor();
+    check(mi.mi_layer_norm(ptr(x), st(x, 0), ptr(r), st(r, 0), fptr(w), fptr(b), ptr(y), ptr(total), fptr(stats), T, d,
+                           eps, dtype_code(x), dtype_code(r.defined() ? r : x), place.stream),
+          "mi_layer_norm");
+    return {y, total, stats};
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b_,
+                                 const OptTensor& r_, double eps) {
+        const Tensor b = given(b_), r = given(r_);
+        auto [y, total, stats] = ln_forward(x, w, b, eps, r, true);
+        ctx->save_for_backward({total.defined() ? total : x, w, stats});
+        ctx->saved_data["type"] = (int64_t)x.scalar_type();
+        ctx->saved_data["need"] = (int64_t)x.requires_grad() | (int64_t)w.requires_grad() << 1 |
+                                  (int64_t)(r.defined() && r.requires_grad()) << 2 |
+                                  (int64_t)(b.defined() && b.requires_grad()) << 3;
+        ctx->set_materialize_grads(false);
+        if (total.defined()) return {y, total};
+        return {y};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const auto s = ctx->get_saved_variables();
+        const Tensor &sum = s[0], &w = s[1], &stats = s[2];
+        const auto type = static_cast<at::ScalarType>(ctx->saved_data["type"].toInt());
+        const int64_t need = ctx->saved_data["need"].toInt();
+        Tensor dtotal = g.size() > 1 ? g[1] : Tensor();
+        if (!g[0].defined()) {
+            if (!dtotal.defined()) return variable_list(5);
+            return {need & 1 ? dtotal.to(type) : Tensor(), Tensor(), Tensor(), need & 4 ? dtotal : Tensor(), Tensor()};
+        }
+        const int64_t T = sum.size(0), d = sum.size(1);
+        const bool create = at::GradMode::is_enabled();
+        at::NoGradGuard no_grad;
+        Place place(sum);
+        const Tensor dy = aligned(g[0]);
+        if (dtotal.defined()) dtotal = aligned(dtotal);
+        const bool same = sum.scalar_type() == type, want_r = need & 4;
+        Tensor dx = need & 1 || (same && want_r) ? at::empty({T, d}, sum.options().dtype(type)) : Tensor();
+        Tensor dr = want_r && !same ? at::empty({T, d}, sum.options()) : Tensor();
+        Tensor dw = need & 2 ? floats({d}, sum) : Tensor(), db = need & 8 ? floats({d}, sum) : Tensor();
+        Tensor ws = need & 10 ? workspace(mi.mi_layer_norm_backward_workspace(T, d), sum) : Tensor();
+        check(mi.mi_layer_norm_backward(ptr(dy), ptr(dtotal), ptr(sum), st(sum, 0), fptr(w), fptr(stats), ptr(dx),
+                                        ptr(dr), fptr(dw), fptr(db), ptr(ws), T, d, dtype_code(dy), dtype_code(sum),
+                                        place.stream),
+              "mi_layer_norm_backward");
+        return once({need & 1 ? dx : Tensor(), dw, db, want_r ? (same ? dx : dr) : Tensor(), Tensor()}, create, s, g);
+    }
+};
+
+std::tuple<Tensor, OptTensor> layer_norm(const Tensor& x, const Tensor& weight, const OptTensor& bias, double eps,
+                                         const OptTensor& residual) {
+    const Rows a = norm_arguments(x, weight, residual, bias);
+    const Tensor& b = a.b;
+    auto shaped = [&](const Tensor& t) { return x.dim() == 2 ? t : t.view(x.sizes()); };
+    if (a.x.size(0) == 0)
+        return {reached(x * 1, {&a.w, &b, &a.r}),
+                residual.has_value() ? OptTensor(reached(*residual * 1, {&a.x})) : OptTensor()};
+    if (at::GradMode::is_enabled() && any_requires_grad(a.x, a.w, b, a.r)) {
+        capturable({&a.x, &a.w, &b, &a.r}, a.x.device());
+        const auto out = LayerNorm::apply(a.x, a.w, maybe(b), maybe(a.r), eps);
+        return {shaped(out[0]), out.size() > 1 ? OptTensor(shaped(out[1])) : OptTensor()};
+    }
+    auto [y, total, stats] = ln_forward(a.x, a.w, b, eps, a.r, false);
+    return {shaped(y), total.defined() ? OptTensor(shaped(total)) : OptTensor()};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -700,6 +776,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("selective_scan_step", &selective_scan_step, free);
     m.def("causal_conv1d", &causal_conv1d, free);
     m.def("causal_conv1d_step", &causal_conv1d_step, free);
+    m.def("layer_norm", &layer_norm, free);
     m.def("gated_recurrence", &gated_recurrence, free);
     m.def("gated_recurrence_step", &gated_recurrence_step, free);
     m.def("rms_norm", &rms_norm, free);

@@ -10,6 +10,7 @@ pass), for prompts, and for single tokens.
     y    = gated_recurrence_step(h, x, gate, z=.., gate_bias=..)      # h in place
     y, s = rms_norm(x, weight, residual=r)                            # s = x + r
     q, scale, s = rms_norm_quant(x, weight, residual=r)               # int8 rows for the ternary GEMMs
+    y, s = layer_norm(x, weight, bias, residual=r)
 
 Activations are fp32, bf16 or fp16, one type for all of a call's; parameters
 (A, D, delta_bias, the convolution's weight and bias, the norm's weight), scan
@@ -159,6 +160,19 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     x and residual [..., width]; residual is of x's type or fp32; the norm is of
     s as it is kept.  Returns (y, s), s None without a residual."""
     return (_ops or _load()).rms_norm(x, weight, eps, residual)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Layer norm over the last dimension, with the residual's addition:
+
+        s = x + residual (s = x without one), in the residual's type
+        y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias
+
+    x and residual [..., width]; residual is of x's type or fp32; weight, bias
+    [width]; the norm is of s as it is kept.  Returns (y, s), s None without a
+    residual."""
+    return (_ops or _load()).layer_norm(x, weight, bias, eps, residual)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: Optional[torch.Tensor] = None

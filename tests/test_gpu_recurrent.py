@@ -242,3 +242,139 @@ def test_recurrence_second_order_is_refused(sel, cuda_dev):
     g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="first order"):
         torch.autograd.grad(g.sum(), x)
+
+
+# ---------------------------------------------------------------------------
+# layer norm
+# ---------------------------------------------------------------------------
+EPS = 1e-5
+NORM_SIZES = [
+    # rows, width: rows within a warp (4 to 32 threads), of several warps, of 1, 2 and 4 packs a thread, odd widths
+    (1, 1), (5, 8), (3, 31), (70, 32), (9, 72), (33, 129), (2, 256), (700, 264), (17, 509), (4, 512), (37, 768), (300, 1024),
+    (6, 1032), (3, 2000), (5, 4096), (3, 4100), (2, 5000), (2, 8192), (3, 8200), (1, 9001), (2, 16384), (1, 16380),
+]
+
+
+def norm_inputs(dev, dtype, t, d, rdtype=None, bias=True, seed=0, offset=0.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    a = dict(x=(r(t, d) + offset).to(dtype), w=1 + 0.5 * r(d), b=r(d) if bias else None,
+             r=None if rdtype is None else (2 * r(t, d)).to(rdtype), dy=r(t, d).to(dtype))
+    a["dsum"] = None if rdtype is None else r(t, d).to(rdtype)
+    return {k: None if v is None else v.to(dev) for k, v in a.items()}
+
+
+def check_norm(sel, a):
+    names = [k for k in ("x", "w", "b", "r") if a[k] is not None]
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in names}
+    y, s = sel.layer_norm(leaves["x"], leaves["w"], leaves.get("b"), eps=EPS, residual=leaves.get("r"))
+    outs = [(y, a["dy"])] + ([] if s is None else [(s, a["dsum"])])
+    got = dict(zip(names, torch.autograd.grad([o for o, _ in outs], list(leaves.values()), [g for _, g in outs])))
+    kept = a["x"] if s is None else (a["x"].float() + a["r"].float()).to(a["r"].dtype)
+    if s is not None:
+        assert torch.equal(s, kept)
+    want = ref.norm(kept, a["w"], a["b"], EPS, a["dy"], a["dsum"])
+    ref.check(y, want["y"], "y")
+    ref.check(got["x"], want["ds"], "dx")
+    ref.check(got["w"], want["dw"], "dw")
+    if a["b"] is not None:
+        ref.check(got["b"], want["dbias"], "db")
+    if a["r"] is not None:
+        ref.check(got["r"], want["ds"], "dr")
+    with torch.no_grad():
+        again, s2 = sel.layer_norm(a["x"], a["w"], a["b"], eps=EPS, residual=a["r"])
+    assert torch.equal(again, y) and (s is None or torch.equal(s, s2))
+
+
+@pytest.mark.parametrize("size", NORM_SIZES)
+@pytest.mark.parametrize("dtype,rdtype", [(F32, None), (F32, F32), (BF16, None), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+def test_layer_norm(sel, cuda_dev, size, dtype, rdtype):
+    check_norm(sel, norm_inputs(cuda_dev, dtype, *size, rdtype=rdtype, bias=size[0] % 3 != 0))
+
+
+@pytest.mark.parametrize("t,d", [(5000, 64), (2500, 768), (1301, 509), (700, 4096)])
+def test_layer_norm_many_rows(sel, cuda_dev, t, d):
+    check_norm(sel, norm_inputs(cuda_dev, BF16, t, d, rdtype=BF16))
+
+
+def test_layer_norm_rows_far_from_zero(sel, cuda_dev):
+    """A mean a thousand times the spread, rows that are constant, and rows of zeros."""
+    a = norm_inputs(cuda_dev, F32, 40, 700, offset=1000.0)
+    a["x"][3], a["x"][4] = 7.25, 0.0
+    check_norm(sel, a)
+    y, _ = sel.layer_norm(a["x"], a["w"], a["b"], eps=EPS)
+    assert torch.allclose(y[4], a["b"])
+    a["x"][5, 9], a["x"][6, 2] = float("nan"), float("inf")
+    y, _ = sel.layer_norm(a["x"], a["w"], a["b"], eps=EPS)
+    assert y[5].isnan().all() and y[6].isnan().all() and torch.isfinite(y[[0, 1, 2, 3, 4, 7]]).all()
+
+
+def test_layer_norm_shapes_strides_and_parts(sel, cuda_dev):
+    a = norm_inputs(cuda_dev, BF16, 24, 96, rdtype=F32)
+    want = sel.layer_norm(a["x"], a["w"], a["b"], residual=a["r"])
+    got = sel.layer_norm(a["x"].view(2, 3, 4, 96), a["w"], a["b"], residual=a["r"].view(2, 3, 4, 96))
+    assert got[0].shape == (2, 3, 4, 96) and torch.equal(got[0].view(24, 96), want[0]) and torch.equal(got[1].view(24, 96), want[1])
+    for pad in (8, 3):
+        wide = torch.empty(24, 96 + 2 * pad, dtype=BF16, device=cuda_dev)
+        x = wide[:, pad:pad + 96]
+        x.copy_(a["x"])
+        got = sel.layer_norm(x, a["w"], a["b"], residual=a["r"])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    flat = torch.empty(97, device=cuda_dev)
+    flat[1:].copy_(a["w"])
+    assert torch.equal(sel.layer_norm(a["x"], flat[1:], a["b"], residual=a["r"])[0], want[0])
+    row = a["x"][:1].detach().clone().requires_grad_(True)  # a row that many share
+    y, _ = sel.layer_norm(row.expand(24, -1), a["w"], a["b"])
+    g, = torch.autograd.grad(y, row, a["dy"])
+    each = a["x"][:1].repeat(24, 1).requires_grad_(True)
+    y, _ = sel.layer_norm(each, a["w"], a["b"])
+    assert torch.equal(g, torch.autograd.grad(y, each, a["dy"])[0].sum(0, keepdim=True))
+    # gradients of some of the arguments, and of the sum alone
+    full = {}
+    for names in (("x", "w", "b", "r"), ("x",), ("w",), ("b",), ("r",)):
+        leaves = {k: a[k].detach().clone().requires_grad_(k in names) for k in ("x", "w", "b", "r")}
+        y, s = sel.layer_norm(leaves["x"], leaves["w"], leaves["b"], residual=leaves["r"])
+        outs, givens = ([y, s], [a["dy"], a["dsum"]]) if set(names) & {"x", "r"} else ([y], [a["dy"]])
+        got = dict(zip(names, torch.autograd.grad(outs, [leaves[k] for k in names], givens)))
+        full = full or got
+        assert all(torch.equal(full[k], got[k]) for k in names)
+    x, r = a["x"].detach().requires_grad_(True), a["r"].detach().requires_grad_(True)
+    _, s = sel.layer_norm(x, a["w"], a["b"], residual=r)
+    gx, gr = torch.autograd.grad(s, [x, r], a["dsum"])
+    assert torch.equal(gx, a["dsum"].to(BF16)) and torch.equal(gr, a["dsum"])
+
+
+def test_layer_norm_empty_and_refused(sel, cuda_dev):
+    w = torch.ones(8, device=cuda_dev, requires_grad=True)
+    b = torch.ones(8, device=cuda_dev, requires_grad=True)
+    y, s = sel.layer_norm(torch.zeros(0, 8, device=cuda_dev), w, b)
+    assert y.shape == (0, 8) and s is None
+    gw, gb = torch.autograd.grad(y.sum(), [w, b])
+    assert not gw.any() and not gb.any()
+    x = torch.randn(3, 8, device=cuda_dev, requires_grad=True)
+    y, _ = sel.layer_norm(x, w, b)
+    g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="first order"):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_layer_norm_captured(sel, cuda_dev):
+    a = norm_inputs(cuda_dev, BF16, 333, 768, rdtype=BF16)
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in ("x", "w", "b", "r")}
+
+    def step():
+        y, s = sel.layer_norm(leaves["x"], leaves["w"], leaves["b"], residual=leaves["r"])
+        return [y.detach(), s.detach(), *torch.autograd.grad([y, s], list(leaves.values()), [a["dy"], a["dsum"]])]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        want = [t.clone() for t in step()]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            got = step()
+    for _ in range(2):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))

@@ -54,6 +54,23 @@ def test_recurrence_step_refuses(change, error):
         selective.gated_recurrence_step(**{**dict(h=_t(2, 8), x=_t(2, 8), gate=_t(2, 8)), **change})
 
 
+@pytest.mark.parametrize("change,error", [
+    (dict(x=_t(4, 8, dtype=torch.float64)), TypeError),
+    (dict(weight=_t(7)), ValueError),
+    (dict(weight=_t(8, dtype=torch.bfloat16)), TypeError),
+    (dict(bias=_t(9)), ValueError),
+    (dict(bias=_t(8, dtype=torch.float16)), TypeError),
+    (dict(residual=_t(4, 7)), ValueError),
+    (dict(residual=_t(4, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(x=_t(1, selective.MAX_NORM_WIDTH + 1), weight=_t(selective.MAX_NORM_WIDTH + 1)), ValueError),
+    (dict(x=torch.zeros(())), ValueError),
+    (dict(), ValueError),
+])
+def test_layer_norm_refuses(change, error):
+    with pytest.raises(error):
+        selective.layer_norm(**{**dict(x=_t(4, 8), weight=_t(8)), **change})
+
+
 def test_sizes_past_the_counters_are_refused():
     """Expanded views: no such memory is there."""
     for shape, what in (((1, (1 << 30) + 1, 1), "too long"), ((65536, 1, 1), "at most 65535"),
@@ -84,6 +101,13 @@ def test_entry_points_refuse_on_the_host():
     step = lambda h=p, y=p, dtype=0, D=64: lib.mi_gated_recurrence_step(p, 64, p, 64, None, 0, None, h, y, 2, D, 1, dtype,  # noqa: E731
                                                                        None)
     assert step(h=None) == -1 and step(y=None) == -1 and step(dtype=7) == -1 and step(D=0) == -1
+    norm = lambda x=p, y=p, r=None, s_=None, D=64, rdtype=0, dtype=0, w=p: lib.mi_layer_norm(  # noqa: E731
+        x, 64, r, 64, w, None, y, s_, None, 4, D, 1e-5, dtype, rdtype, None)
+    assert norm(x=None) == -1 and norm(y=None) == -1 and norm(w=None) == -1 and norm(r=p) == -1
+    assert norm(D=16385) == -2 and norm(D=0) == -1 and norm(dtype=3) == -1 and norm(r=p, s_=p, rdtype=1) == -1
+    back = lambda dx=p, dw=None, db=None, ws=None, stats=p: lib.mi_layer_norm_backward(  # noqa: E731
+        p, None, p, 64, p, stats, dx, None, dw, db, ws, 4, 64, 0, 0, None)
+    assert back(dx=None) == -1 and back(dw=p) == -1 and back(db=p) == -1 and back(stats=None) == -1
     assert lib.mi_gated_recurrence_checkpoints(2, 17, 5) == 2 * 3 * 5
     assert lib.mi_gated_recurrence_backward_workspace(1, 64, 64) == 4 * 64
 
@@ -121,6 +145,18 @@ def test_recurrence_formula_against_differences(convex):
         assert abs(float(out["y"][0][0, t, 0]) - h * z / (1 + 2.718281828459045 ** -z)) < 1e-12
 
 
+def test_norm_formula_against_differences():
+    g = torch.Generator().manual_seed(2)
+    leaves = dict(s=_rand(g, 5, 9), w=_rand(g, 9), bias=_rand(g, 9))
+    dy, dsum = _rand(g, 5, 9), _rand(g, 5, 9)
+
+    def value(v):
+        return (ref.norm(v["s"], v["w"], v["bias"], 1e-5)["y"][0] * dy).sum() + (v["s"] * dsum).sum()
+    slopes(value, leaves, ref.norm(leaves["s"], leaves["w"], leaves["bias"], 1e-5, dy, dsum))
+    y = ref.norm(leaves["s"], leaves["w"], leaves["bias"], 1e-5)["y"][0]
+    assert torch.allclose(y, torch.nn.functional.layer_norm(leaves["s"], (9,), leaves["w"], leaves["bias"], 1e-5), rtol=1e-12)
+
+
 def test_forward_mode_is_refused():
     """A tangent would be lost; any argument may carry it, a view of a dual tensor too."""
     from torch.autograd import forward_ad
@@ -129,6 +165,7 @@ def test_forward_mode_is_refused():
     calls = [
         (selective.gated_recurrence, dict(x=x(), gate=x(), z=x(), gate_bias=_t(8), h0=_t(2, 8))),
         (selective.gated_recurrence_step, dict(h=_t(2, 8), x=_t(2, 8), gate=_t(2, 8), z=_t(2, 8), gate_bias=_t(8))),
+        (selective.layer_norm, dict(x=_t(4, 8), weight=_t(8), bias=_t(8), residual=_t(4, 8))),
     ]
     for fn, args in calls:
         for name, t in args.items():
