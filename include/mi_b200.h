@@ -515,6 +515,26 @@ int mi_layer_norm_backward(const void* dy, const void* dsum, const void* s, int6
                            void* workspace, int T, int D, int dtype, int rdtype, void* stream);
 int64_t mi_layer_norm_backward_workspace(int T, int D);
 
+/*
+ * The choice of a token from each row of logits [rows, V] (row stride ld) by a
+ * uniform number u [rows] in [0, 1).  With w = exp((l - max l) / temperature)
+ * and the tokens in the order (l downwards, index upwards): the first top_k are
+ * kept (all with top_k <= 0); of those, each whose mass before it is below top_p
+ * times their total, the first always (all with top_p >= 1 or NaN); of those,
+ * w >= min_p (min_p > 1 counts as 1; all with min_p <= 0 or NaN).  token [rows]:
+ * the first index whose running sum of the kept w, in index order, exceeds u
+ * times their total (u outside [0, 1) counts as its nearest end, NaN as 0);
+ * prob [rows] (may be NULL): its w over that total.
+ * temperature <= 0 or NaN, or a row whose maximum is infinite, NaN or -infinity:
+ * mi_argmax_rows' choice and prob 1.  -infinity is never chosen beside finite
+ * logits, nor is a w below 2^-45.  The parameters are arrays [rows], or scalars
+ * where the array is NULL.  dtype: MI_DT_*.  V <= 262144.  The same inputs give
+ * the same bits.
+ */
+int mi_sample_rows(const void* logits, int64_t ld, const float* u, const float* temperature, const int32_t* top_k,
+                   const float* top_p, const float* min_p, float temperature1, int top_k1, float top_p1, float min_p1,
+                   int64_t* token, float* prob, int rows, int V, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

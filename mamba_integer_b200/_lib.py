@@ -76,6 +76,7 @@ SIGNATURES = {
     "mi_rms_norm_quant": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
     "mi_rms_norm_backward": [_p, _p, _p, _i64, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p],
     "mi_rms_norm_backward_workspace": [_i, _i],
+    "mi_sample_rows": [_p, _i64] + [_p] * 5 + [_f, _i, _f, _f, _p, _p, _i, _i, _i, _p],
     "mi_layer_norm": [_p, _i64, _p, _i64] + [_p] * 5 + [_i, _i, _f, _i, _i, _p],
     "mi_layer_norm_backward": [_p, _p, _p, _i64] + [_p] * 7 + [_i] * 4 + [_p],
     "mi_layer_norm_backward_workspace": [_i, _i],

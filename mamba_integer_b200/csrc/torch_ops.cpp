@@ -19,6 +19,7 @@
 #include <torch/extension.h>
 
 #include <unordered_set>
+#include <variant>
 
 #include "../../include/mi_b200.h"
 
@@ -36,7 +37,7 @@ using OptTensor = std::optional<Tensor>;
     X(mi_rms_norm_backward) X(mi_rms_norm_backward_workspace) X(mi_gated_recurrence)                         \
     X(mi_gated_recurrence_checkpoints) X(mi_gated_recurrence_backward)                                       \
     X(mi_gated_recurrence_backward_workspace) X(mi_gated_recurrence_step) X(mi_layer_norm)                   \
-    X(mi_layer_norm_backward) X(mi_layer_norm_backward_workspace)
+    X(mi_layer_norm_backward) X(mi_layer_norm_backward_workspace) X(mi_sample_rows)
 
 struct Entries {
 #define X(name) decltype(&::name) name = nullptr;
@@ -577,6 +578,7 @@ Tensor gated_recurrence_step(const Tensor& h, const Tensor& x, const Tensor& gat
     on_gpu(x, "x");
     Place place(x);
     Tensor y = at::empty({batch, d}, x.options());
+    if (batch == 0) return y;
     check(mi.mi_gated_recurrence_step(ptr(x), st(x, 0), ptr(gate), st(gate, 0), ptr(z), st(z, 0), fptr(bias), fptr(h),
                                       ptr(y), batch, d, convex, dtype_code(x), place.stream),
           "mi_gated_recurrence_step");
@@ -767,6 +769,59 @@ std::tuple<Tensor, OptTensor> layer_norm(const Tensor& x, const Tensor& weight, 
     return {shaped(y), total.defined() ? OptTensor(shaped(total)) : OptTensor()};
 }
 
+// ---------------------------------------------------------------------------
+// the choice of a token
+// ---------------------------------------------------------------------------
+// A setting of all rows, or of each.
+template <typename V>
+struct Setting {
+    Tensor rows;
+    V value{};
+    Setting(const std::variant<Tensor, V>& s, const Tensor& logits, at::ScalarType type, const char* name) {
+        if (std::holds_alternative<Tensor>(s))
+            rows = plain(std::get<Tensor>(s), logits, {logits.size(0)}, type, name);
+        else
+            value = std::get<V>(s);
+    }
+};
+
+std::tuple<Tensor, OptTensor> sample_rows(const Tensor& logits, const Tensor& u_, const std::variant<Tensor, double>& t_,
+                                          const std::variant<Tensor, int64_t>& k_, const std::variant<Tensor, double>& p_,
+                                          const std::variant<Tensor, double>& m_, const OptTensor& out, bool return_prob) {
+    no_grad_needed(logits);
+    activation(logits, "logits");
+    TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) <= 262144,
+                      "logits must be [rows, 1 to 262144 tokens], got ", logits.sizes());
+    const int64_t rows = logits.size(0), V = logits.size(1);
+    like(logits, logits, {rows, V}, "logits");
+    TORCH_CHECK_VALUE(rows <= 1 << 27, "logits has too many rows: ", logits.sizes());
+    const Tensor u = plain(u_, logits, {rows}, at::kFloat, "u");
+    const Setting<double> t(t_, logits, at::kFloat, "temperature"), p(p_, logits, at::kFloat, "top_p"),
+        m(m_, logits, at::kFloat, "min_p");
+    const Setting<int64_t> k(k_, logits, at::kInt, "top_k");
+    TORCH_CHECK_VALUE(t.rows.defined() || t.value >= 0, "temperature must be 0 (greedy) or more, got ", t.value);
+    TORCH_CHECK_VALUE(k.rows.defined() || k.value >= 0, "top_k must be 0 (off) or more, got ", k.value);
+    TORCH_CHECK_VALUE(p.rows.defined() || (p.value >= 0 && p.value <= 1), "top_p must be from 0 to 1, got ", p.value);
+    TORCH_CHECK_VALUE(m.rows.defined() || (m.value >= 0 && m.value <= 1), "min_p must be from 0 to 1, got ", m.value);
+    if (out.has_value()) {
+        TORCH_CHECK_VALUE(out->sizes() == at::IntArrayRef({rows}) && out->is_contiguous(), "out must be contiguous [", rows,
+                          "], got ", out->sizes());
+        TORCH_CHECK_TYPE(out->scalar_type() == at::kLong, "out must be int64, got ", out->scalar_type());
+        same_device(*out, logits, "out");
+    }
+    on_gpu(logits, "logits");
+    Place place(logits);
+    Tensor token = out.has_value() ? *out : at::empty({rows}, logits.options().dtype(at::kLong));
+    Tensor prob = return_prob ? floats({rows}, logits) : Tensor();
+    if (rows == 0) return {token, maybe(prob)};
+    check(mi.mi_sample_rows(ptr(logits), st(logits, 0), fptr(u), fptr(t.rows), static_cast<int32_t*>(ptr(k.rows)),
+                            fptr(p.rows), fptr(m.rows), t.value, std::min(k.value, V), p.value, m.value,
+                            static_cast<int64_t*>(ptr(token)), fptr(prob), rows, V, dtype_code(logits), place.stream),
+          "mi_sample_rows");
+    if (out.has_value()) written(token);
+    return {token, maybe(prob)};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -776,6 +831,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("selective_scan_step", &selective_scan_step, free);
     m.def("causal_conv1d", &causal_conv1d, free);
     m.def("causal_conv1d_step", &causal_conv1d_step, free);
+    m.def("sample_rows", &sample_rows, free);
     m.def("layer_norm", &layer_norm, free);
     m.def("gated_recurrence", &gated_recurrence, free);
     m.def("gated_recurrence_step", &gated_recurrence_step, free);

@@ -362,6 +362,26 @@ def argmax_rows(x: torch.Tensor, V: Optional[int] = None, out: Optional[torch.Te
     return out
 
 
+def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                out: Optional[torch.Tensor] = None, return_prob: bool = False):
+    """One token from each row of logits [rows, vocab] (fp32, bf16 or fp16) by a given uniform number u (fp32 [rows], in
+    [0, 1)).  With w = exp((l - max l) / temperature) and the tokens in the order (l downwards, index upwards):
+
+        top_k   the first k are kept (0: all)
+        top_p   of those, each whose mass before it is below p times their total; the first always (1: all)
+        min_p   of those, w >= min_p (0: all)
+
+    The token (int64 [rows]) is the first index whose running sum of the kept w, in index order, exceeds u times their
+    total; with ``return_prob`` also its share w / total (fp32 [rows]).  Temperature 0 is argmax_rows, with share 1; so
+    is a row whose maximum is infinite or NaN, or that is all -inf.  Every setting is a number or a tensor of one value a
+    row (fp32, top_k int32), whose values are not checked: a temperature below 0 counts as 0, and the filters of values
+    beyond their range as off or as their nearest end.  Up to 262144 tokens.  The same inputs give the same bits."""
+    from . import selective
+    token, prob = (selective._ops or selective._load()).sample_rows(logits, u, temperature, top_k, top_p, min_p, out,
+                                                                    return_prob)
+    return (token, prob) if return_prob else token
+
+
 def scan_convex(u: torch.Tensor, nums: torch.Tensor) -> torch.Tensor:
     _need(u, torch.float32, "u")
     _need(nums, torch.float32, "nums")

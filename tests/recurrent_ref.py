@@ -158,6 +158,7 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
         left = left[:top_k]
     mass = np.exp((row[left] - row[best]) / temperature)
     near = 1.0
+    whole = (mass == 1).all()  # equal tokens: their sums, and a number of 24 bits times those, are exact on both sides
     if top_p < 1:  # a NaN keeps all
         total = mass.sum()
         before = np.cumsum(mass) - mass
@@ -167,7 +168,7 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
         left, mass = left[ok], mass[ok]
     floor = min(max(min_p, 0.0), 1.0) if min_p == min_p else 0.0
     if floor > 0:
-        near = min(near, np.abs(mass / floor - 1).min())
+        near = min(near, np.abs(mass[mass < 1] / floor - 1).min(initial=1.0))  # that of the maximum is exact
         ok = mass >= floor
         left, mass = left[ok], mass[ok]
     order = np.argsort(left)
@@ -176,4 +177,4 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
     target = (min(max(u, 0.0), 1.0) if u == u else 0.0) * upto[-1]
     at = min(int(np.searchsorted(upto, target, side="right")), left.size - 1)
     near = min(near, np.abs(upto[:-1] / upto[-1] - target / upto[-1]).min(initial=1.0))
-    return int(left[at]), float(mass[at] / upto[-1]), float(near)
+    return int(left[at]), float(mass[at] / upto[-1]), 1.0 if whole else float(near)

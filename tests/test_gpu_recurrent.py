@@ -233,6 +233,8 @@ def test_recurrence_empty_calls(sel, cuda_dev):
         assert y.shape == (b, n, 8) and torch.equal(h, a["h0"])
         got = torch.autograd.grad([y.sum() + h.sum()], list(leaves.values()))
         assert not got[3].any() and (got[4] == 1).all()
+    none = torch.zeros(0, 8, device=cuda_dev)
+    assert sel.gated_recurrence_step(none, none, none).shape == (0, 8)
 
 
 def test_recurrence_second_order_is_refused(sel, cuda_dev):
@@ -378,3 +380,176 @@ def test_layer_norm_captured(sel, cuda_dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+# ---------------------------------------------------------------------------
+# the choice of a token
+# ---------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def kernels(cuda_dev):
+    from mamba_integer_b200 import kernels
+    return kernels
+
+
+# masses are whole numbers of 2^-44 from powers right to 2^-42: sums of up to 2^17 of them are off by less than 2^-30 of
+# the total, and a border that lies nearer than that to the number asked for may be taken from either side
+NEAR = 2.0 ** -30
+
+
+def check_sample(kernels, dev, logits, u, t, k, p, m):
+    """Settings: numbers, or lists of one a row."""
+    rows = logits.shape[0]
+    each = lambda v: v if isinstance(v, list) else [v] * rows  # noqa: E731
+    send = lambda v, d: torch.tensor(v, dtype=d, device=dev) if isinstance(v, list) else v  # noqa: E731
+    token, prob = kernels.sample_rows(logits.to(dev), torch.tensor(u, device=dev), send(t, F32), send(k, torch.int32),
+                                      send(p, F32), send(m, F32), return_prob=True)
+    f32 = lambda v: torch.tensor(v, dtype=F32).double().tolist()  # noqa: E731
+    token, prob = token.tolist(), prob.tolist()
+    unsure = 0
+    for i, row in enumerate(zip(f32(u), f32(each(t)), each(k), f32(each(p)), f32(each(m)))):
+        want, share, near = ref.sample(logits[i], *row)
+        if near < NEAR:
+            unsure += 1
+            continue
+        assert token[i] == want, (i, row, token[i], want, near)
+        # its own rounding, and the total's 2^-30
+        assert abs(prob[i] - share) <= share * (2.0 ** -24 + NEAR), (i, row, prob[i], share)
+    assert unsure <= max(1, rows // 50)
+
+
+def sample_logits(rows, v, seed=0, spread=2.5, dtype=F32):
+    g = torch.Generator().manual_seed(seed)
+    x = spread * torch.randn(rows, v, generator=g)
+    return torch.where(torch.rand(rows, v, generator=g) < 30 / v, 4 + 8 * torch.rand(rows, v, generator=g), x).to(dtype)
+
+
+def uniform(rows, seed=1):
+    return torch.rand(rows, generator=torch.Generator().manual_seed(seed)).tolist()
+
+
+SETTINGS = [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0, 1.0, 0.1), (0.9, 40, 0.8, 0.05),
+            (0.0, 5, 0.5, 0.5), (1.5, 1, 1.0, 0.0), (1.0, 700, 0.97, 0.0), (0.2, 0, 0.5, 0.01), (50.0, 0, 0.7, 0.0)]
+
+
+@pytest.mark.parametrize("setting", SETTINGS)
+@pytest.mark.parametrize("rows,v", [(1, 1), (3, 2), (5, 64), (7, 1000), (4, 4096), (9, 32768), (2, 50021), (1, 131072)])
+def test_sample(kernels, cuda_dev, rows, v, setting):
+    check_sample(kernels, cuda_dev, sample_logits(rows, v, seed=v), uniform(rows, v), *setting)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v", [300, 4100, 32768, 40000])
+def test_sample_rows_with_settings_of_their_own(kernels, cuda_dev, v, dtype):
+    rows = 160
+    g = torch.Generator().manual_seed(v)
+    r = lambda: torch.rand(rows, generator=g)  # noqa: E731
+    t = torch.where(r() < 0.2, 0.0, 0.3 + 1.5 * r()).tolist()
+    k = torch.where(r() < 0.4, 0, (r() * 2000).int() + 1).int().tolist()
+    p = torch.where(r() < 0.4, 1.0, r()).tolist()
+    m = torch.where(r() < 0.5, 0.0, 0.3 * r()).tolist()
+    check_sample(kernels, cuda_dev, sample_logits(rows, v, seed=v, dtype=dtype), uniform(rows, v), t, k, p, m)
+
+
+@pytest.mark.parametrize("v", [999, 32768, 70000])
+def test_sample_equal_logits(kernels, cuda_dev, v):
+    """Ties go to the lower index: rows of one value, of few values, and of values that differ in their last bits."""
+    flat = torch.zeros(1, v)
+    steps = torch.randint(0, 3, (1, v), generator=torch.Generator().manual_seed(3)).float()
+    close = 1000 + 2 ** -13 * torch.randint(0, 40, (1, v), generator=torch.Generator().manual_seed(4)).float()
+    zeros = torch.where(torch.arange(v)[None] % 2 == 0, -0.0, 0.0)
+    logits = torch.cat([flat, steps, close, zeros, torch.full((1, v), -3e38)])
+    for setting in ((1.0, 0, 1.0, 0.0), (1.0, 500, 1.0, 0.0), (1.0, 0, 0.37, 0.0), (0.5, 600, 0.9, 0.3), (0.0, 0, 1.0, 0.0),
+                    (1e-3, 0, 0.5, 0.0), (1e30, 300, 0.5, 0.0)):
+        check_sample(kernels, cuda_dev, logits, uniform(5, v), *setting)
+
+
+@pytest.mark.parametrize("v", [77, 32768])
+def test_sample_masks(kernels, cuda_dev, v):
+    """Banned tokens of -inf and of the type's lowest value, rows with one token left, rows with none, NaN and +inf."""
+    inf = float("inf")
+    base = sample_logits(8, v, seed=5)
+    base[0, v // 2:] = -inf
+    base[1, : v - 3] = torch.finfo(F32).min
+    base[2] = -inf
+    base[2, 40] = -7.0
+    base[3] = -inf
+    base[4, 50], base[4, 60] = inf, inf
+    base[5, 70], base[5, 30], base[5, 20] = float("nan"), float("nan"), inf
+    base[6] = torch.finfo(F32).min
+    base[7] = torch.where(torch.arange(v) % 2 == 0, 3.4e38, -3.4e38)
+    for setting in SETTINGS + [(1.0, v - 1, 0.999, 0.0), (1.0, 60, 1.0, 1.0), (1.0, 3, 0.0, 0.0)]:
+        check_sample(kernels, cuda_dev, base, uniform(8, v), *setting)
+
+
+def test_sample_numbers_at_the_ends(kernels, cuda_dev):
+    """u of 0, just below 1, 1, beyond and NaN; settings beyond their range, by row."""
+    nan = float("nan")
+    v = 5000
+    logits = sample_logits(1, v).repeat(9, 1)
+    u = [0.0, 1 - 2.0 ** -24, 1.0, 7.0, -1.0, nan, 0.5, 0.5, 0.5]
+    check_sample(kernels, cuda_dev, logits, u, 1.0, 0, 1.0, 0.0)
+    check_sample(kernels, cuda_dev, logits, u, 1.0, 20, 0.9, 0.0)
+    check_sample(kernels, cuda_dev, logits, [0.7] * 9, [1.0, -1.0, nan, float("inf"), 1e-38, 1e-45, 3e38, 1.0, 1.0],
+                 [-5, 3, 3, 0, 0, 0, 0, 2 ** 31 - 1, v + 1], [1.0, 0.5, 0.5, 1.0, 1.0, 0.5, 0.5, nan, 2.0],
+                 [nan, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, -1.0, 5.0])
+
+
+def test_sample_frequencies(kernels, cuda_dev):
+    """Many numbers over one row give every token its share: within 6 standard deviations."""
+    v, n = 200, 40000
+    row = sample_logits(1, v, seed=9)
+    u = (torch.arange(n, device=cuda_dev) + 0.5) / n
+    token = kernels.sample_rows(row.to(cuda_dev).expand(n, -1), u, temperature=0.8, top_p=0.9)
+    got = torch.bincount(token, minlength=v).cpu().double() / n
+    w = torch.softmax(row[0].double() / 0.8, 0)
+    s, order = torch.sort(w, descending=True, stable=True)
+    s = torch.where(torch.cumsum(s, 0) - s < torch.tensor(0.9).double(), s, 0)
+    want = torch.zeros(v, dtype=torch.float64).scatter_(0, order, s / s.sum())
+    assert (got - want).abs().max() <= 2.0 / n  # evenly spread numbers: two borders, half a number each
+
+
+def test_sample_strides_out_and_argmax(kernels, cuda_dev):
+    x = sample_logits(40, 3001).to(cuda_dev)
+    u = torch.rand(40, device=cuda_dev)
+    want = kernels.sample_rows(x, u, top_k=30)
+    wide = torch.zeros(40, 4000, device=cuda_dev)
+    for pad in (4, 3):
+        cut = wide[:, pad:pad + 3001]
+        cut.copy_(x)
+        assert torch.equal(kernels.sample_rows(cut, u, top_k=30), want)
+    out = torch.full((40,), -1, dtype=torch.int64, device=cuda_dev)
+    assert kernels.sample_rows(x, u, top_k=30, out=out) is not None and torch.equal(out, want)
+    assert torch.equal(kernels.sample_rows(x, u, temperature=0.0), kernels.argmax_rows(x))
+    assert torch.equal(kernels.sample_rows(x, u, top_k=1), kernels.argmax_rows(x))
+    assert kernels.sample_rows(x[:0], u[:0]).shape == (0,)
+    back = torch.flip(u, (0,)).flip(0)[::1]
+    assert torch.equal(kernels.sample_rows(x, torch.stack([u, back], 1)[:, 0], top_k=30), want)
+
+
+def test_sample_captured_and_on_streams(kernels, cuda_dev):
+    x = sample_logits(6, 32768).to(cuda_dev)
+    u, k = torch.rand(6, device=cuda_dev), torch.tensor([0, 5, 50, 500, 5000, 1], dtype=torch.int32, device=cuda_dev)
+    want = [t.clone() for t in kernels.sample_rows(x, u, 0.9, k, 0.95, 0.01, return_prob=True)]
+    for _ in range(20):
+        assert all(torch.equal(p, q) for p, q in zip(want, kernels.sample_rows(x, u, 0.9, k, 0.95, 0.01, return_prob=True)))
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            got = kernels.sample_rows(x, u, 0.9, k, 0.95, 0.01, return_prob=True)
+    for _ in range(2):
+        got[0].zero_(), got[1].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+def test_sample_offsets_past_32_bits(kernels, cuda_dev):
+    v, rows = 70000, 3
+    x = sample_logits(rows, v, dtype=BF16).to(cuda_dev)
+    u = torch.rand(rows, device=cuda_dev)
+    big = torch.empty(2 * 2 ** 31 + 2 ** 20, dtype=BF16, device=cuda_dev)
+    far = big.as_strided((rows, v), (2 ** 31 - 8, 1))
+    far.copy_(x)
+    assert torch.equal(kernels.sample_rows(far, u, 0.9, 40, 0.9), kernels.sample_rows(x, u, 0.9, 40, 0.9))

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import recurrent_ref as ref
-from mamba_integer_b200 import _lib, selective
+from mamba_integer_b200 import _lib, kernels, selective
 
 
 def _t(*shape, dtype=torch.float32):
@@ -71,6 +71,40 @@ def test_layer_norm_refuses(change, error):
         selective.layer_norm(**{**dict(x=_t(4, 8), weight=_t(8)), **change})
 
 
+@pytest.mark.parametrize("change,error", [
+    (dict(logits=_t(4, 9, dtype=torch.float64)), TypeError),
+    (dict(logits=_t(4)), ValueError),
+    (dict(logits=_t(4, 0)), ValueError),
+    (dict(logits=_t(9, 4).t()), ValueError),
+    (dict(logits=_t(4, 1).expand(4, 262145)), ValueError),
+    (dict(logits=_t(4, 9).requires_grad_(True)), RuntimeError),
+    (dict(u=_t(5)), ValueError),
+    (dict(u=_t(4, 1)), ValueError),
+    (dict(u=_t(4, dtype=torch.float64)), TypeError),
+    (dict(temperature=-0.1), ValueError),
+    (dict(temperature=float("nan")), ValueError),
+    (dict(temperature=_t(5)), ValueError),
+    (dict(temperature=_t(4, dtype=torch.bfloat16)), TypeError),
+    (dict(temperature="hot"), TypeError),
+    (dict(top_k=-1), ValueError),
+    (dict(top_k=2.5), TypeError),
+    (dict(top_k=torch.zeros(4, dtype=torch.int64)), TypeError),
+    (dict(top_p=1.1), ValueError),
+    (dict(top_p=-0.1), ValueError),
+    (dict(top_p=float("nan")), ValueError),
+    (dict(top_p=_t(1)), ValueError),
+    (dict(min_p=1.5), ValueError),
+    (dict(min_p=torch.zeros(4, dtype=torch.int32)), TypeError),
+    (dict(out=torch.zeros(4, dtype=torch.int32)), TypeError),
+    (dict(out=torch.zeros(5, dtype=torch.int64)), ValueError),
+    (dict(out=torch.zeros(8, dtype=torch.int64)[::2]), ValueError),
+    (dict(), ValueError),  # CPU tensors
+])
+def test_sample_refuses(change, error):
+    with pytest.raises(error):
+        kernels.sample_rows(**{**dict(logits=_t(4, 9), u=_t(4)), **change})
+
+
 def test_sizes_past_the_counters_are_refused():
     """Expanded views: no such memory is there."""
     for shape, what in (((1, (1 << 30) + 1, 1), "too long"), ((65536, 1, 1), "at most 65535"),
@@ -108,6 +142,10 @@ def test_entry_points_refuse_on_the_host():
     back = lambda dx=p, dw=None, db=None, ws=None, stats=p: lib.mi_layer_norm_backward(  # noqa: E731
         p, None, p, 64, p, stats, dx, None, dw, db, ws, 4, 64, 0, 0, None)
     assert back(dx=None) == -1 and back(dw=p) == -1 and back(db=p) == -1 and back(stats=None) == -1
+    pick = lambda x=p, u=p, token=p, rows=4, V=64, ld=64, dtype=0: lib.mi_sample_rows(  # noqa: E731
+        x, ld, u, None, None, None, None, 1.0, 0, 1.0, 0.0, token, None, rows, V, dtype, None)
+    assert pick(x=None) == -1 and pick(u=None) == -1 and pick(token=None) == -1 and pick(rows=-1) == -1 and pick(V=0) == -1
+    assert pick(ld=-1) == -1 and pick(dtype=3) == -1 and pick(V=262145) == -2 and pick(rows=0) == 0
     assert lib.mi_gated_recurrence_checkpoints(2, 17, 5) == 2 * 3 * 5
     assert lib.mi_gated_recurrence_backward_workspace(1, 64, 64) == 4 * 64
 
@@ -176,3 +214,17 @@ def test_forward_mode_is_refused():
                         fn(**{**args, name: wide[0]})
         with pytest.raises(ValueError, match="must be a CUDA tensor"):  # and without one the call goes on
             fn(**args)
+
+
+def test_the_choice_by_hand():
+    x = torch.log(torch.tensor([1.0, 4.0, 2.0, 4.0, 1.0, 8.0], dtype=torch.float64))  # shares of 20; order 5 1 3 2 0 4
+    pick = lambda u, t=1.0, k=0, p=1.0, m=0.0: ref.sample(x, u, t, k, p, m)[:2]  # noqa: E731
+    assert pick(0.0) == (0, pytest.approx(1 / 20)) and pick(0.049)[0] == 0 and pick(0.051)[0] == 1 and pick(0.99)[0] == 5
+    assert pick(0.6, t=0.0) == (5, 1.0)
+    assert pick(0.3, k=2) == (1, pytest.approx(1 / 3)) and pick(0.34, k=2)[0] == 5  # the lower index of the equal ones
+    assert pick(0.1, p=0.39) == (5, 1.0) and pick(0.1, p=0.41)[0] == 1  # 8 of 20 before the second
+    assert pick(0.0, m=0.4)[0] == 1 and pick(0.0, m=0.2)[0] == 1 and pick(0.0, m=0.12)[0] == 0
+    assert pick(0.3, t=2.0, k=2)[1] == pytest.approx(2 ** 0.5 / (1 + 2 ** 0.5) / 2 ** 0.5)
+    inf = float("inf")
+    assert ref.sample(torch.tensor([-inf, -inf]), 0.5, 1.0, 0, 1.0, 0.0)[:2] == (0, 1.0)
+    assert ref.sample(torch.tensor([1.0, float("nan"), inf]), 0.5, 1.0, 0, 1.0, 0.0)[:2] == (1, 1.0)
