@@ -105,20 +105,21 @@ Tensor aligned(const Tensor& t) {
     return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
+void fixed(const Tensor& t, const Tensor& first, at::IntArrayRef shape, at::ScalarType type, const char* name) {
+    TORCH_CHECK_VALUE(t.sizes() == shape, name, " must be ", shape, ", got ", t.sizes());
+    TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+    same_device(t, first, name);
+}
+
 // A contiguous operand of a fixed type (parameters, states), undefined if missing.
 Tensor plain(const OptTensor& o, const Tensor& first, at::IntArrayRef shape, at::ScalarType type, const char* name) {
     if (!o.has_value()) return Tensor();
-    const Tensor& t = *o;
-    TORCH_CHECK_VALUE(t.sizes() == shape, name, " must be ", shape, ", got ", t.sizes());
-    TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-    same_device(t, first, name);
-    return aligned(t);
+    fixed(*o, first, shape, type, name);
+    return aligned(*o);
 }
 
 void in_place(const Tensor& t, const Tensor& first, at::IntArrayRef shape, at::ScalarType type, const char* name) {
-    TORCH_CHECK_VALUE(t.sizes() == shape, name, " must be ", shape, ", got ", t.sizes());
-    TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
-    same_device(t, first, name);
+    fixed(t, first, shape, type, name);
     TORCH_CHECK_VALUE(t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, name,
                       " is advanced in place: it must be contiguous and start on a 16-byte boundary");
 }
@@ -778,10 +779,12 @@ struct Setting {
     Tensor rows;
     V value{};
     Setting(const std::variant<Tensor, V>& s, const Tensor& logits, at::ScalarType type, const char* name) {
-        if (std::holds_alternative<Tensor>(s))
-            rows = plain(std::get<Tensor>(s), logits, {logits.size(0)}, type, name);
-        else
+        if (std::holds_alternative<Tensor>(s)) {
+            fixed(std::get<Tensor>(s), logits, {logits.size(0)}, type, name);
+            rows = std::get<Tensor>(s).contiguous();
+        } else {
             value = std::get<V>(s);
+        }
     }
 };
 
@@ -795,7 +798,8 @@ std::tuple<Tensor, OptTensor> sample_rows(const Tensor& logits, const Tensor& u_
     const int64_t rows = logits.size(0), V = logits.size(1);
     like(logits, logits, {rows, V}, "logits");
     TORCH_CHECK_VALUE(rows <= 1 << 27, "logits has too many rows: ", logits.sizes());
-    const Tensor u = plain(u_, logits, {rows}, at::kFloat, "u");
+    fixed(u_, logits, {rows}, at::kFloat, "u");
+    const Tensor u = u_.contiguous();
     const Setting<double> t(t_, logits, at::kFloat, "temperature"), p(p_, logits, at::kFloat, "top_p"),
         m(m_, logits, at::kFloat, "min_p");
     const Setting<int64_t> k(k_, logits, at::kInt, "top_k");

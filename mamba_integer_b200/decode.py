@@ -20,7 +20,8 @@ The reference has no step API: its generation loop recomputes
 MambaIntegerModel.forward over the whole sequence for every token
 (scripts/inference.py:148-160, temperature sampling).  Each step here gives
 the logits that forward gives the last position, bit for bit; generation is
-greedy (argmax, first index of the maximum).
+greedy (argmax, first index of the maximum), or samples with a temperature,
+top-k, top-p and min-p (``Sampling``; kernels.sample_rows on the step's logits).
 
 Streams are independent, so multi-GPU decoding shards them across ranks
 (``mamba_integer_b200.distributed.shard_range``) with no collective until the
@@ -28,11 +29,41 @@ generated ids are gathered.
 """
 from __future__ import annotations
 
+from dataclasses import dataclass
+from typing import Optional
+
 import torch
 
 from . import kernels
 from .engine import PrefillEngine
 from .rational_bitnet import ternary_matmul
+
+
+@dataclass(frozen=True)
+class Sampling:
+    """How a stream's tokens are chosen from its logits (kernels.sample_rows): temperature 0 is greedy.  ``seed`` fixes
+    the random numbers; without one they are drawn from torch's default generator."""
+
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: Optional[int] = None
+
+    def __post_init__(self):
+        if not 0 <= self.temperature <= 3.4e38:
+            raise ValueError(f"temperature must be 0 (greedy) or more and finite, got {self.temperature}")
+        if not 0 <= int(self.top_k) < 2 ** 31 or int(self.top_k) != self.top_k:
+            raise ValueError(f"top_k must be a whole number from 0 (off) on, got {self.top_k}")
+        if not 0 <= self.top_p <= 1:
+            raise ValueError(f"top_p must be from 0 to 1, got {self.top_p}")
+        if not 0 <= self.min_p <= 1:
+            raise ValueError(f"min_p must be from 0 to 1, got {self.min_p}")
+
+    def numbers(self, *shape: int) -> torch.Tensor:
+        """Uniform numbers in [0, 1) on the CPU."""
+        g = None if self.seed is None else torch.Generator().manual_seed(self.seed)
+        return torch.rand(*shape, generator=g)
 
 
 class StreamStates:
@@ -203,20 +234,31 @@ class DecodeEngine:
         """Greedy choice over logits [k, V] (int64 [k])."""
         return kernels.argmax_rows(logits)
 
+    @staticmethod
+    def sample(logits: torch.Tensor, u: torch.Tensor, temperature, top_k, top_p, min_p,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The choice over logits [k, V] by uniform numbers [k] (int64 [k]); settings of all rows or of each."""
+        return kernels.sample_rows(logits, u, temperature, top_k, top_p, min_p, out=out)
+
     def next_ids(self) -> torch.Tensor:
         """argmax of the logits of the last step (int64 [batch])."""
         return self.ws.next_ids
 
-    def generate(self, prompt_ids: torch.Tensor, n_new: int) -> torch.Tensor:
-        """Greedy continuation: int64 [batch, n_new]."""
+    def generate(self, prompt_ids: torch.Tensor, n_new: int, sampling: Optional[Sampling] = None) -> torch.Tensor:
+        """Continuation int64 [batch, n_new]: greedy, or sampled where ``sampling`` is given (each stream and position has
+        a number of its own; the same seed, batch and length give the same tokens)."""
         logits = self.start(prompt_ids)
         batch = prompt_ids.shape[0]
         out = torch.empty(batch, n_new, dtype=torch.int64, device=self.pre.dev)
         if n_new == 0:
             return out
+        s = sampling if sampling is not None and sampling.temperature > 0 else None
+        u = None if s is None else s.numbers(n_new, batch).to(self.pre.dev)
         kernels.argmax_rows(logits, out=self.ws.next_ids)
         for t in range(n_new):
+            if s is not None:  # in the place of the argmax
+                self.sample(logits, u[t], s.temperature, s.top_k, s.top_p, s.min_p, out=self.ws.next_ids)
             out[:, t].copy_(self.ws.next_ids)
             if t + 1 < n_new:
-                self.step(self.ws.next_ids)
+                logits = self.step(self.ws.next_ids)
         return out

@@ -1,4 +1,4 @@
-"""Continuous-batching greedy generation over the decode kernels.
+"""Continuous-batching generation over the decode kernels, greedy or sampled.
 
 The reference generates for one prompt at a time by recomputing the whole
 forward per token (scripts/inference.py:148-160).  `DecodeServer` keeps a
@@ -22,9 +22,12 @@ step t runs.  A request that finished at step t-1 has had step t computed for
 its slot too; that token is dropped (each slot's step is credited only to the
 request that held the slot when the step was launched and still holds it).
 
-Every request gets exactly the tokens greedy full-recompute generation gives
-its prompt alone: streams never interact (every operation is per stream), so
-neither the other slots nor the admission time change a stream's bits.
+Every request gets exactly the tokens full-recompute generation gives its
+prompt alone: streams never interact (every operation is per stream), so
+neither the other slots nor the admission time change a stream's bits.  A
+request that samples (``Sampling``) has its own random numbers, one for each
+of its tokens; all slots' settings and numbers go to the GPU in one copy a
+step, and one kernel chooses every slot's token (a greedy one's by argmax).
 """
 from __future__ import annotations
 
@@ -34,7 +37,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
-from .decode import DecodeEngine
+from .decode import DecodeEngine, Sampling
 
 
 @dataclass
@@ -43,6 +46,9 @@ class Request:
     prompt: List[int]
     max_new_tokens: int
     tokens: List[int] = field(default_factory=list)
+    sampling: Optional[Sampling] = None
+    numbers: Optional[List[float]] = None  # one for each token, with sampling
+    issued: int = 0                        # tokens that were launched, credited or not
 
 
 class DecodeServer:
@@ -65,13 +71,22 @@ class DecodeServer:
         self._host_ids = [torch.empty(slots, dtype=torch.int64, pin_memory=on_gpu) for _ in range(2)]
         self._ready = [torch.cuda.Event() if on_gpu else None for _ in range(2)]
         self._inflight = None
+        # settings of the slots for the last two launched steps (rows: u, temperature, top_p, min_p, top_k's bits); a
+        # buffer is written again after the ids of its step were read
+        self._host_set = [torch.zeros(5, slots, pin_memory=on_gpu) for _ in range(2)]
+        self._set = torch.zeros(5, slots, device=self.eng.ws.ids.device)
 
-    def submit(self, prompt: Sequence[int], max_new_tokens: int) -> int:
+    def submit(self, prompt: Sequence[int], max_new_tokens: int, sampling: Optional[Sampling] = None) -> int:
+        """Queue a request; greedy, or sampled by ``sampling`` (its numbers are its own: whatever shares the slots, the
+        same seed gives the same tokens)."""
         if len(prompt) == 0 or max_new_tokens <= 0:
             raise ValueError("a request needs a non-empty prompt and max_new_tokens >= 1")
         rid = self._next_rid
         self._next_rid += 1
-        self.queue.append(Request(rid, [int(t) for t in prompt], int(max_new_tokens)))
+        r = Request(rid, [int(t) for t in prompt], int(max_new_tokens))
+        if sampling is not None and sampling.temperature > 0:
+            r.sampling, r.numbers = sampling, sampling.numbers(r.max_new_tokens).tolist()
+        self.queue.append(r)
         return rid
 
     def pending(self) -> int:
@@ -84,6 +99,27 @@ class DecodeServer:
         if len(r.tokens) >= r.max_new_tokens or (self.eos_id is not None and tok == self.eos_id):
             self.finished[r.rid] = r.tokens
             self.active[slot] = None
+
+    @staticmethod
+    def _settings(requests: List[Optional[Request]], into: torch.Tensor) -> bool:
+        """Each one's next number and settings into the columns of [5, n]; False, and nothing written, if all are greedy."""
+        if not any(r is not None and r.sampling is not None for r in requests):
+            return False
+        rows = [[], [], [], []]
+        top_k = []
+        for r in requests:
+            s = None if r is None else r.sampling
+            u = r.numbers[r.issued] if s is not None and r.issued < r.max_new_tokens else 0.0
+            for row, v in zip(rows, (u, s.temperature, s.top_p, s.min_p) if s is not None else (0.0, 0.0, 1.0, 0.0)):
+                row.append(v)
+            top_k.append(s.top_k if s is not None else 0)
+        into[:4].copy_(torch.tensor(rows))
+        into[4].view(torch.int32).copy_(torch.tensor(top_k, dtype=torch.int32))
+        return True
+
+    def _choose(self, logits: torch.Tensor, settings: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        u, temperature, top_p, min_p, top_k = settings.unbind(0)
+        return self.eng.sample(logits, u, temperature, top_k.view(torch.int32), top_p, min_p, out=out)
 
     def _admit(self) -> None:
         free = [i for i, r in enumerate(self.active) if r is None]
@@ -101,7 +137,13 @@ class DecodeServer:
             slots = [free.pop(0) for _ in group]
             ids = torch.tensor([r.prompt for r in group], dtype=torch.int64)
             logits = self.eng.prefill_slots(slots, ids)
-            first = self.eng.argmax(logits)
+            settings = torch.empty(5, len(group))
+            if self._settings(group, settings):
+                first = self._choose(logits, settings.to(logits.device))
+            else:
+                first = self.eng.argmax(logits)
+            for r in group:
+                r.issued += 1
             self.eng.ws.ids.index_copy_(0, torch.as_tensor(slots, device=first.device), first)
             for s, r, tok in zip(slots, group, first.tolist()):
                 self.active[s] = r
@@ -127,8 +169,14 @@ class DecodeServer:
             ws = self.eng.ws
             self.eng.step(ws.ids)
             nxt = self.eng.next_ids()
-            ws.ids.copy_(nxt)  # every slot's next input is its own last token
             k = self.steps & 1
+            if self._settings(self.active, self._host_set[k]):
+                self._set.copy_(self._host_set[k], non_blocking=self._ready[k] is not None)
+                self._choose(ws.logits, self._set, out=nxt)
+            for r in self.active:
+                if r is not None:
+                    r.issued += 1
+            ws.ids.copy_(nxt)  # every slot's next input is its own last token
             self._host_ids[k].copy_(nxt, non_blocking=self._ready[k] is not None)
             if self._ready[k] is not None:
                 self._ready[k].record()

@@ -553,3 +553,107 @@ def test_sample_offsets_past_32_bits(kernels, cuda_dev):
     far = big.as_strided((rows, v), (2 ** 31 - 8, 1))
     far.copy_(x)
     assert torch.equal(kernels.sample_rows(far, u, 0.9, 40, 0.9), kernels.sample_rows(x, u, 0.9, 40, 0.9))
+
+
+# ---------------------------------------------------------------------------
+# the three together: a small recurrent language model, trained, prompted and stepped
+# ---------------------------------------------------------------------------
+class Net:
+    """Two layers of norm, gates and recurrence, a norm and a head; `ops`: the framework's calls, or the formulas."""
+
+    def __init__(self, dev, dtype, d=64, v=500, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        r = lambda *s: torch.randn(*s, generator=g).to(dev, dtype)  # noqa: E731
+        self.p = {"emb": r(v, d), "head": r(v, d) / d ** 0.5, "fw": 1 + 0.1 * r(d), "fb": 0.1 * r(d)}
+        for i in range(2):
+            self.p.update({f"w{i}": 1 + 0.1 * r(d), f"b{i}": 0.1 * r(d), f"in{i}": r(3 * d, d) / d ** 0.5,
+                           f"out{i}": r(d, d) / d ** 0.5, f"bias{i}": 2 + r(d)})
+        self.d = d
+
+    def forward(self, ops, ids, states=None, lengths=None):
+        """ids [batch, L] (or [batch] with states, one token each): logits, and the states behind the prompt."""
+        p, d = self.p, self.d
+        x, kept = p["emb"][ids], []
+        delta = torch.zeros_like(x)
+        for i in range(2):
+            n, x = ops.norm(delta, p[f"w{i}"], p[f"b{i}"], x)
+            rows = n @ p[f"in{i}"].t()
+            y, h = ops.rec(rows[..., :d], rows[..., d:2 * d], rows[..., 2 * d:], p[f"bias{i}"],
+                           None if states is None else states[i], lengths)
+            kept.append(h)
+            delta = y @ p[f"out{i}"].t()
+        n, _ = ops.norm(delta, p["fw"], p["fb"], x)
+        return n @ p["head"].t(), kept
+
+
+class Ours:
+    def __init__(self, sel, step=False):
+        self.sel, self.step = sel, step
+
+    def norm(self, x, w, b, r):
+        return self.sel.layer_norm(x, w, b, residual=r)
+
+    def rec(self, x, f, z, bias, h, lengths):
+        if self.step:
+            return self.sel.gated_recurrence_step(h, x, f, z=z, gate_bias=bias), h
+        return self.sel.gated_recurrence(x, f, z=z, gate_bias=bias, h0=h, lengths=lengths, return_state=True)
+
+
+class Formula:
+    @staticmethod
+    def norm(x, w, b, r):
+        s = x + r
+        c = s - s.mean(-1, keepdim=True)
+        return c / torch.sqrt((c * c).mean(-1, keepdim=True) + 1e-5) * w + b, s
+
+    @staticmethod
+    def rec(x, f, z, bias, h, lengths):
+        a, out = torch.sigmoid(f + bias), []
+        h = torch.zeros_like(x[:, 0]) if h is None else h
+        for t in range(x.shape[1]):
+            new = a[:, t] * h + (1 - a[:, t]) * x[:, t]
+            h = new if lengths is None else torch.where((t < lengths)[:, None], new, h)
+            out.append(new if lengths is None else torch.where((t < lengths)[:, None], new, 0.0))
+        return torch.stack(out, 1) * z * torch.sigmoid(z), h
+
+
+def test_a_training_step_of_all(sel, cuda_dev):
+    net, ref64 = Net(cuda_dev, F32), Net(cuda_dev, torch.float64)
+    ids = torch.randint(0, 500, (3, 33), generator=torch.Generator().manual_seed(1)).to(cuda_dev)
+    lengths = torch.tensor([33, 20, 7], dtype=torch.int32, device=cuda_dev)
+    grads = []
+    for n, ops in ((net, Ours(sel)), (ref64, Formula())):
+        for k in n.p:
+            n.p[k] = n.p[k].double().to(n.p[k].dtype).requires_grad_(True)
+        logits, _ = n.forward(ops, ids[:, :-1], lengths=lengths - 1)
+        lp = torch.log_softmax(logits, -1).gather(2, ids[:, 1:, None])[..., 0]
+        live = torch.arange(32, device=cuda_dev)[None] < (lengths - 1)[:, None]
+        loss = -(lp * live).sum() / live.sum()
+        grads.append(torch.autograd.grad(loss, list(n.p.values())))
+    for name, a, b in zip(net.p, *grads):
+        # fp32 through two layers and products of 64 terms: each value's error is some hundred roundings of its terms,
+        # which the norm of the whole gradient bounds (2^-24 * 1000 = 6e-5); a wrong term would be of order 1
+        assert (a.double() - b).norm() <= 1e-3 * b.norm(), name
+
+
+def test_prompt_steps_and_choices_of_all(sel, kernels, cuda_dev):
+    """Tokens chosen step by step from the carried states are those chosen from the whole sequence in 64 bits."""
+    net, ref64 = Net(cuda_dev, F32), Net(cuda_dev, torch.float64)
+    for k in net.p:
+        ref64.p[k] = net.p[k].double()
+    prompt = torch.randint(0, 500, (4, 21), generator=torch.Generator().manual_seed(2)).to(cuda_dev)
+    u = torch.rand(12, 4, generator=torch.Generator().manual_seed(3)).to(cuda_dev)
+    t, k, p = 0.8, 40, 0.95
+    with torch.no_grad():
+        logits, states = net.forward(Ours(sel), prompt)
+        logits, seq = logits[:, -1].contiguous(), prompt
+        for i in range(12):
+            want64 = ref64.forward(Formula(), seq)[0][:, -1]
+            # a hundred roundings per layer on logits of order 1 to 10
+            assert (logits.double() - want64).abs().max() < 1e-3
+            tok = kernels.sample_rows(logits, u[i], t, k, p)
+            for b in range(4):
+                want, _, near = ref.sample(logits[b], float(u[i, b]), 0.8, k, 0.95, 0.0)
+                assert near < 1e-6 or int(tok[b]) == want  # 0.8 and 0.95 as fp32 numbers move a border by 1e-7
+            seq = torch.cat([seq, tok[:, None]], 1)
+            logits, states = net.forward(Ours(sel, step=True), tok, states)

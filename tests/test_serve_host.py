@@ -68,3 +68,69 @@ def test_eos_and_late_arrivals():
     out = srv.run()
     assert out[a] == [10, 11, 12]
     assert out[b] == expected([3, 3], 3, eos=12)
+
+
+class SamplingEngine(FakeEngine):
+    """Logits of a toy rule, and the choice by the 64-bit formula."""
+
+    @staticmethod
+    def logits_of(prev):
+        base = torch.arange(V).float()[None]
+        return 3 * torch.cos(base * (1 + prev[:, None].float() % 7)) + (base == (prev[:, None] + 1) % V)
+
+    def prefill_slots(self, slots, prompt_ids):
+        self.prefill_calls.append((list(slots), prompt_ids.shape[1]))
+        return self.logits_of(prompt_ids.sum(1) % V)
+
+    def step(self, ids):
+        self.ws.ids.copy_(ids)
+        self.ws.logits = self.logits_of(self.ws.ids)
+        self._next = torch.argmax(self.ws.logits, dim=-1)
+
+    @staticmethod
+    def sample(logits, u, temperature, top_k, top_p, min_p, out=None):
+        import recurrent_ref as ref
+        got = torch.tensor([ref.sample(*row)[0] for row in zip(logits, *(t.tolist() for t in (u, temperature, top_k, top_p, min_p)))])
+        return got if out is None else out.copy_(got)
+
+
+def sampled_alone(prompt, n, s, eos=None):
+    import recurrent_ref as ref
+    f32 = lambda v: float(torch.tensor(v))  # noqa: E731
+    prev, out = torch.tensor([sum(prompt) % V]), []
+    u = [0.0] * n if s is None else s.numbers(n).tolist()
+    for i in range(n):
+        row = SamplingEngine.logits_of(prev)[0]
+        tok = (int(torch.argmax(row)) if s is None else
+               ref.sample(row, u[i], f32(s.temperature), s.top_k, f32(s.top_p), f32(s.min_p))[0])
+        out.append(tok)
+        if tok == eos:
+            break
+        prev = torch.tensor([tok])
+    return out
+
+
+def test_sampled_requests_have_their_own_numbers():
+    from mamba_integer_b200.decode import Sampling
+    reqs = [([1, 2, 3], 6, Sampling(0.9, seed=1)), ([4, 5, 6], 3, None), ([7, 8], 5, Sampling(1.2, 8, 0.9, 0.01, seed=2)),
+            ([9, 9, 9], 1, Sampling(0.7, top_p=0.5, seed=3)), ([1], 4, Sampling(0.0, seed=9)), ([2], 7, Sampling(0.9, seed=1)),
+            ([3, 3], 6, None)]
+    for slots in (1, 2, 4):
+        srv = DecodeServer(None, slots=slots, engine=SamplingEngine())
+        rids = [srv.submit(p, n, s) for p, n, s in reqs[:4]]
+        srv.step(), srv.step()
+        rids += [srv.submit(p, n, s) for p, n, s in reqs[4:]]
+        out = srv.run()
+        for rid, (p, n, s) in zip(rids, reqs):
+            assert out[rid] == sampled_alone(p, n, None if s is not None and s.temperature == 0 else s), (slots, rid)
+
+
+def test_sampling_settings_are_checked():
+    import pytest
+    from mamba_integer_b200.decode import Sampling
+    for bad in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_k=-1),
+                dict(top_k=1.5), dict(top_k=2 ** 31), dict(top_p=1.1), dict(top_p=float("nan")), dict(min_p=-0.5)):
+        with pytest.raises(ValueError):
+            Sampling(**bad)
+    a, b = Sampling(seed=4).numbers(5), Sampling(seed=4).numbers(5)
+    assert torch.equal(a, b) and not torch.equal(a, Sampling(seed=5).numbers(5))
