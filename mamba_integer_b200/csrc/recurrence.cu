@@ -12,23 +12,26 @@
 //
 // A position and channel move 3 elements forward (4 with z) and meet 2 (4)
 // special-function results, so HBM bounds it as long as enough loads are in
-// flight: the recurrence must not wait for them, nor a long sequence for its
-// few channels.
+// flight and the instructions are few: at 45 of them a channel and position
+// (8 x 2048 x 1536 bf16 71 us, 3.2 TB/s) issue slots did.
 //
-// Layout: a CTA has 64 channels, two a lane, and walks the sequence in tiles;
-// a warp has SUB neighbouring positions of a tile, which asynchronous copies
-// bring into slots of its own one tile ahead.  A stretch of positions acts on
-// the state as h -> P h + H; the warps fold theirs through shared memory, once
-// a tile, and then run their own positions again from the state they start
-// from, with a and c x still in registers.  Where the channels leave SMs idle,
-// a cluster of up to 8 CTAs shares the tiles of a round and folds over
-// distributed shared memory; nothing is read twice.
+// Layout: a CTA has 64 channels, two a lane in f32x2 arithmetic, and walks the
+// sequence in tiles; a warp has SUB neighbouring positions of a tile, whose rows
+// asynchronous copies bring into slots of its own one tile ahead.  A stretch of
+// positions acts on the state as h -> P h + H; the warps fold theirs through
+// shared memory, once a tile, and then run their own positions again from the
+// state they start from, with a and c x still in registers.  Where the channels
+// leave SMs idle, a cluster of up to 8 CTAs shares the tiles of a round: each
+// sends its fold to the others' shared memory, counted by their mbarriers;
+// nothing is read twice.
 //
-// Gates never reach 0: e^-|f| is at least 2^-126, so that an infinite state
-// stays infinite and an infinite input reaches it, whether or not a stretch is
-// folded; and a fold adds to an infinite state, as a P that underflowed to 0
-// would make a NaN of it.
+// Gates and folds never reach 0: gate logits count as at most 87 from 0, and a
+// stretch's P is at least 2^-126, so that an infinite state stays infinite and an
+// infinite input reaches it, whether or not a stretch is folded.  (A state of
+// 1e38 leaves up to 1 of itself behind a stretch that forgets it.)
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "mi_elem.cuh"
 
@@ -38,15 +41,16 @@ namespace rec {
 constexpr int WARPS = 8, THREADS = WARPS * 32, CB = 64;  // channels a CTA
 constexpr int CK = 8;          // positions between the states kept for the backward pass
 constexpr int MAX_CLUSTER = 8;
-constexpr int STAGES = 2;
 
 struct Seq {  // a [batch, L, D] operand with unit last stride
     const void* p;
     int64_t sb, sl;
 };
 
+enum { X, F, Z, DY };  // operands that are read by rows
+
 struct Args {
-    Seq x, f, z, dy;
+    Seq in[4];
     const float* bias;   // [D] or NULL
     const float* h0;     // [batch, D] or NULL
     const float* dhT;    // gradient of the final state or NULL
@@ -58,7 +62,6 @@ struct Args {
     float* dh0;          // [batch, D] or NULL
     float* part;         // [batch * cluster, D]: the CTAs' sums of df, or NULL
     int batch, L, D;
-    int vec;             // inputs' rows start on 16 bytes
     int ovec;            // outputs' rows start on a lane's two elements' alignment
     int cs;              // CTAs of a cluster
 };
@@ -69,54 +72,43 @@ __device__ __forceinline__ int length_of(const Args& a, int b) {
     return n < 0 ? 0 : (n < a.L ? n : a.L);
 }
 
-// sigmoid(v) and sigmoid(-v), neither taken from 1 minus the other.  e^-|v| to
-// 2 ulp and the argument's rounding, |v| 2^-24 of it, are far below half a step
-// of 16 bits; fp32 values take expf and a Newton step for the reciprocal.
-template <typename T>
-__device__ __forceinline__ void sigmoids(float v, float& up, float& down) {
-    float e, r;
-    if constexpr (sizeof(T) == 4) {
-        e = max_nan(expf(-fabsf(v)), 1.17549435e-38f);
-        const float d = __fadd_rn(1.0f, e);
-        r = rcp_fast(d);
-        r = __fmaf_rn(r, __fmaf_rn(-d, r, 1.0f), r);
-    } else {
-        e = max_nan(exp2_fast(__fmul_rn(fabsf(v), -LOG2E)), 1.17549435e-38f);
-        r = rcp_fast(__fadd_rn(1.0f, e));
-    }
-    const float s = __fmul_rn(e, r);
-    up = v < 0.0f ? s : r;
-    down = v < 0.0f ? r : s;
+__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
+
+// sigmoid(v) and sigmoid(-v), neither taken from 1 minus the other, for |v| up
+// to 87 (beyond it counts as 87; a NaN stays one).  The product with log2(e) is
+// carried on in two parts, which keeps the power to 2 ulp where |v| is large.
+__device__ __forceinline__ void sigmoids(float2 v, float2& up, float2& down) {
+    v.x = max_nan(min_nan(v.x, 87.0f), -87.0f);
+    v.y = max_nan(min_nan(v.y, 87.0f), -87.0f);
+    const float2 t = __fmul2_rn(v, dup(-LOG2E));
+    const float2 r = __ffma2_rn(v, dup(1.92596299e-8f), __ffma2_rn(v, dup(LOG2E), t));  // t is too large by this
+    float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
+    e = __ffma2_rn(__fmul2_rn(e, dup(-LN2)), r, e);
+    const float2 d = __fadd2_rn(e, dup(1.0f));
+    up = make_float2(rcp_fast(d.x), rcp_fast(d.y));
+    down = __fmul2_rn(e, up);
 }
 
-// z sigmoid(z) and, from the same sigmoid, its derivative
-template <typename T>
-__device__ __forceinline__ float silu(float z, float& slope) {
-    float s, n;
-    sigmoids<T>(z, s, n);
-    slope = __fmaf_rn(__fmul_rn(z, s), n, s);
-    return __fmul_rn(z, s);
+// z sigmoid(z) and its derivative
+__device__ __forceinline__ float2 silu(float2 z, float2& slope) {
+    float2 s, n;
+    sigmoids(z, s, n);
+    const float2 zs = __fmul2_rn(z, s);
+    slope = __ffma2_rn(zs, n, s);
+    return zs;
 }
 template <typename T>
-__device__ __forceinline__ float silu(float z) {
+__device__ __forceinline__ float2 silu(float2 z) {
     if constexpr (sizeof(T) == 4) {
-        float s;
-        return silu<T>(z, s);
-    } else {
-        return __fmul_rn(z, sigmoid(z));
+        float2 slope;
+        return silu(z, slope);
+    } else {  // |z| 2^-24 of the power is far below half a step of 16 bits
+        const float2 t = __fmul2_rn(z, dup(-LOG2E));
+        const float2 d = __fadd2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), dup(1.0f));
+        return __fmul2_rn(z, make_float2(rcp_fast(d.x), rcp_fast(d.y)));
     }
 }
 
-template <typename T>
-__device__ __forceinline__ float2 pair(const T* p) {
-    const Pack<T, 2> v = *reinterpret_cast<const Pack<T, 2>*>(p);
-    return make_float2(to_f(v.v[0]), to_f(v.v[1]));
-}
-template <typename T>
-__device__ __forceinline__ void put(T* p, float2 v, int valid, bool vec) {
-    const float o[2] = {v.x, v.y};
-    store_pack<2>(p, o, valid, vec);
-}
 __device__ __forceinline__ float2 load2(const float* p, int valid) {
     return make_float2(valid > 0 ? p[0] : 0.0f, valid > 1 ? p[1] : 0.0f);
 }
@@ -124,257 +116,384 @@ __device__ __forceinline__ void store2(float* p, float2 v, int valid) {
     if (valid > 0) p[0] = v.x;
     if (valid > 1) p[1] = v.y;
 }
+// FAST: both exist, aligned
+template <bool FAST, typename T>
+__device__ __forceinline__ void put(T* p, float2 v, int valid, bool vec) {
+    if (FAST) {
+        Pack<T, 2> o;
+        o.v[0] = from_f<T>(v.x), o.v[1] = from_f<T>(v.y);
+        *reinterpret_cast<Pack<T, 2>*>(p) = o;
+    } else {
+        const float o[2] = {v.x, v.y};
+        store_pack<2>(p, o, valid, vec);
+    }
+}
 
 // what a stretch of positions does to the state of two channels: s -> p s + q
 struct Fold {
     float2 p, q;
 };
-__device__ __forceinline__ float fold1(float s, float p, float q) {
-    return fabsf(s) == __int_as_float(0x7f800000) ? __fadd_rn(s, q) : __fmaf_rn(p, s, q);
-}
-__device__ __forceinline__ float2 fold(float2 s, const Fold& f) {
-    return make_float2(fold1(s.x, f.p.x, f.q.x), fold1(s.y, f.p.y, f.q.y));
+__device__ __forceinline__ float2 fold(float2 s, const Fold& f) { return __ffma2_rn(f.p, s, f.q); }
+__device__ __forceinline__ float2 some(float2 p) {
+    return make_float2(max_nan(p.x, 1.17549435e-38f), max_nan(p.y, 1.17549435e-38f));
 }
 __device__ __forceinline__ Fold join(const Fold& a, const Fold& b) {  // a, then b
-    return {__fmul2_rn(a.p, b.p), make_float2(fold1(a.q.x, b.p.x, b.q.x), fold1(a.q.y, b.p.y, b.q.y))};
+    return {some(__fmul2_rn(a.p, b.p)), __ffma2_rn(b.p, a.q, b.q)};
 }
 
-// A warp's rows of one operand in shared memory, SUB rows of CB channels.
-template <typename T, int SUB>
-struct Rows {
-    alignas(16) T v[SUB][CB];
-};
-
-// Starts the copies of the operand's rows t0 .. t0 + SUB - 1 of sequence b,
-// channels c0 on, into this warp's slot; rows from `end` on and channels from D
-// on become zeros.
-template <typename T, int SUB>
-__device__ __forceinline__ void fetch_rows(Rows<T, SUB>& to, const Seq& s, int b, int t0, int end, int c0, int D, int vec) {
-    constexpr int K = 16 / sizeof(T), PER = CB / K;
-    const int lane = threadIdx.x & 31;
-    const T* base = static_cast<const T*>(s.p) + (int64_t)b * s.sb + c0;
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < SUB * PER / 32; i++) {
-            const int at = i * 32 + lane, row = at / PER, col = at % PER * K;
-            const int valid = t0 + row < end ? D - c0 - col : 0;
-            fetch_pack<K>(&to.v[row][col], base + (int64_t)(t0 + row) * s.sl + col, s.p, valid, true);
-        }
-    } else {
-#pragma unroll 4
-        for (int row = 0; row < SUB; row++) {
-            const T* p = base + (int64_t)(t0 + row) * s.sl;
-#pragma unroll
-            for (int col = 0; col < CB; col += 32)
-                to.v[row][col + lane] = t0 + row < end && c0 + col + lane < D ? p[col + lane] : from_f<T>(0.0f);
+// ---------------------------------------------------------------------------
+// barriers in shared memory
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t* bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_at(bar)) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok)
+                 : "r"(smem_at(bar)), "r"(parity)
+                 : "memory");
+    return ok != 0;
+}
+// Bounded: after about 2 s the device's error word is set and the wait given up.
+__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity) {
+    if (bar_try(bar, parity)) return;
+    const long long t0 = clock64();
+    while (!bar_try(bar, parity)) {
+        if (clock64() - t0 > 4000000000LL) {
+            raise_dev_error(MI_DEV_TIMEOUT);
+            return;
         }
     }
 }
 
+// ---------------------------------------------------------------------------
+// rows of the operands in shared memory
+// ---------------------------------------------------------------------------
+// A warp's rows of N operands: SUB rows of CB channels each.  Where rows start
+// off 16 bytes (not VEC), the 16-byte blocks that hold a row's channels are
+// copied whole, and the row starts inside the first one.
+template <typename T, int N, int SUB, bool VEC>
+struct Rows {
+    static constexpr int K = 16 / sizeof(T), PITCH = VEC ? CB : CB + K;
+    alignas(16) T v[N][SUB][PITCH];
+};
+
+// The copies of a warp's rows, 16 bytes each, dealt to its lanes.
+template <typename T, int N, int SUB, bool VEC>
+struct Fetch {
+    static constexpr int K = 16 / sizeof(T), PER = CB / K, STEP = 32 / PER;  // blocks a row, rows a turn of the warp
+    const char* base[N];  // VEC: this lane's block of the first row it copies; else row 0 of the sequence
+    int size;             // VEC: bytes of the lane's block that exist, 0 or 16; else bytes of a row's channels
+
+    template <typename... W>
+    __device__ __forceinline__ void init(const Args& a, int b, int c0, W... which) {
+        const int lane = threadIdx.x & 31, col = lane % PER * K;
+        const int w[N] = {which...};
+        size = VEC ? (c0 + col < a.D ? 16 : 0) : (a.D - c0 < CB ? a.D - c0 : CB) * (int)sizeof(T);
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const Seq& s = a.in[w[k]];
+            int64_t at = (int64_t)b * s.sb;
+            if (!VEC) at += c0;
+            if (VEC && size) at += c0 + col + lane / PER * s.sl;
+            base[k] = static_cast<const char*>(s.p) + at * (int64_t)sizeof(T);
+        }
+    }
+    // rows t0 .. t0 + n - 1, n > 0
+    template <typename... W>
+    __device__ __forceinline__ void start(const Args& a, Rows<T, N, SUB, VEC>& to, int t0, int n, W... which) const {
+        const int lane = threadIdx.x & 31;
+        const int w[N] = {which...};
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int64_t row = a.in[w[k]].sl * (int64_t)sizeof(T);
+            const char* from = base[k] + t0 * row;
+            if (VEC) {
+                char* slot = reinterpret_cast<char*>(&to.v[k][0][0]) + lane * 16;
+                if (n >= SUB) {
+#pragma unroll
+                    for (int i = 0; i < SUB / STEP; i++) {
+                        cp_async<16>(slot + i * 512, from, size);
+                        from += STEP * row;
+                    }
+                } else {
+                    for (int i = 0; i * STEP + lane / PER < n; i++) {
+                        cp_async<16>(slot + i * 512, from, size);
+                        from += STEP * row;
+                    }
+                }
+            } else {
+                // whole blocks of 16 bytes: what lies before a row in its first block is read and not used
+                for (int at = lane; at < SUB * (PER + 1); at += 32) {
+                    const int r = at / (PER + 1), col = at % (PER + 1);
+                    const char* p = from + r * row;
+                    const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15), left = off + size - col * 16;
+                    if (r < n && left > 0) cp_async<16>(&to.v[k][r][col * K], p - off + col * 16, left < 16 ? left : 16);
+                }
+            }
+        }
+    }
+};
+
+// A lane's two channels of a row; `off`: where a row off 16 bytes starts.
+template <bool VEC, typename T>
+__device__ __forceinline__ float2 pair(const T* row, uint32_t off) {
+    const int lane = threadIdx.x & 31;
+    if (VEC) {
+        const Pack<T, 2> v = *reinterpret_cast<const Pack<T, 2>*>(row + 2 * lane);
+        return make_float2(to_f(v.v[0]), to_f(v.v[1]));
+    }
+    return make_float2(to_f(row[off + 2 * lane]), to_f(row[off + 2 * lane + 1]));
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ uint32_t off16(const Seq& s, int b, int t, int c0) {
+    if (VEC) return 0;
+    return (uint32_t)((reinterpret_cast<uintptr_t>(s.p) / sizeof(T) + (int64_t)b * s.sb + (int64_t)t * s.sl + c0) %
+                      (16 / sizeof(T)));
+}
+
 // The folds of a round, in order: `mine` is this warp's, `s` the state that the
 // round starts from.  Returns the state that this warp starts from; s becomes
-// the state after the round.  Rounds alternate between two sets of slots, so one
-// barrier a round is enough.
+// the state after the round.  Rounds alternate between two sets of slots: whoever
+// writes to one has seen the other's round end, which all read the first before.
 struct Exchange {
     Fold warp[2][WARPS][32];
     Fold cta[2][MAX_CLUSTER][32];
+    uint64_t arrived[2];
 };
-template <bool CLUSTER>
-__device__ __forceinline__ float2 exchange(Exchange& ex, int round, int cs, const Fold& mine, float2& s) {
+
+// Slots a warp: as many as leave room for two CTAs an SM.
+template <typename R>
+constexpr int STAGES = sizeof(R) * WARPS * 2 + sizeof(Exchange) <= 113 * 1024 ? 2 : 1;
+
+__device__ __forceinline__ float2 exchange(Exchange& ex, int round, int cs, int rank, Fold mine, float2& s) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = round & 1;
+    mine.p = some(mine.p);
     ex.warp[k][warp][lane] = mine;
+    if (cs > 1 && threadIdx.x == 0) bar_expect(&ex.arrived[k], cs * 32 * sizeof(Fold));
     __syncthreads();
     float2 from = s;
-    if constexpr (!CLUSTER) {
+    if (cs == 1) {
 #pragma unroll
         for (int i = 0; i < WARPS; i++) {
             if (i == warp) from = s;
             s = fold(s, ex.warp[k][i][lane]);
         }
-    } else {
-        namespace cg = cooperative_groups;
-        cg::cluster_group cluster = cg::this_cluster();
-        const int rank = cluster.block_rank();
-        if (warp < cs) {  // warp i tells CTA i
-            Fold all = ex.warp[k][0][lane];
-#pragma unroll
-            for (int i = 1; i < WARPS; i++) all = join(all, ex.warp[k][i][lane]);
-            *cluster.map_shared_rank(&ex.cta[k][rank][lane], warp) = all;
-        }
-        cluster.sync();
-        for (int i = 0; i < cs; i++) {
-            if (i == rank) from = s;
-            s = fold(s, ex.cta[k][i][lane]);
-        }
-        for (int i = 0; i < warp; i++) from = fold(from, ex.warp[k][i][lane]);
+        return from;
     }
+    if (warp < cs) {  // warp i tells CTA i
+        Fold all = ex.warp[k][0][lane];
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) all = join(all, ex.warp[k][i][lane]);
+        uint32_t to, bar;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&ex.cta[k][rank][lane])), "r"(warp));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&ex.arrived[k])), "r"(warp));
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+                     "f"(all.p.x), "f"(all.p.y), "f"(all.q.x), "f"(all.q.y), "r"(bar)
+                     : "memory");
+    }
+    bar_wait(&ex.arrived[k], (round >> 1) & 1);
+    for (int i = 0; i < cs; i++) {
+        if (i == rank) from = s;
+        s = fold(s, ex.cta[k][i][lane]);
+    }
+    for (int i = 0; i < warp; i++) from = fold(from, ex.warp[k][i][lane]);
     return from;
 }
 
+__device__ __forceinline__ void begin(Exchange& ex, int cs) {
+    if (threadIdx.x < 2) bar_init(&ex.arrived[threadIdx.x]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (cs > 1)
+        cooperative_groups::this_cluster().sync();
+    else
+        __syncthreads();
+}
+
 template <typename T>
-constexpr int SUB_FWD = 32 / sizeof(T);  // 16 positions of 16 bits, 8 of fp32: slots of 2 KB
+constexpr int SUB_FWD = sizeof(T) == 2 ? 16 : 8;
 
-template <typename T, bool GATE>
-struct FwdSlots {
-    Rows<T, SUB_FWD<T>> x[STAGES][WARPS], f[STAGES][WARPS], z[GATE ? STAGES : 1][GATE ? WARPS : 1];
-};
-
-template <typename T, bool CONVEX, bool GATE, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const Args a) {
-    constexpr int SUB = SUB_FWD<T>, TT = SUB * WARPS;
+template <typename T, bool CONVEX, bool GATE, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__ Args a) {
+    constexpr int SUB = SUB_FWD<T>, TT = SUB * WARPS, N = GATE ? 3 : 2;
+    using R = Rows<T, N, SUB, VEC>;
+    constexpr int ST = STAGES<R>;
     extern __shared__ __align__(16) unsigned char smem[];
-    FwdSlots<T, GATE>& slots = *reinterpret_cast<FwdSlots<T, GATE>*>(smem);
-    Exchange& ex = *reinterpret_cast<Exchange*>(smem + sizeof(FwdSlots<T, GATE>));
+    Exchange& ex = *reinterpret_cast<Exchange*>(smem);
+    R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cs = CLUSTER ? a.cs : 1;
-    const int b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
+    const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
     const int c = c0 + 2 * lane, valid = a.D - c;
+    begin(ex, cs);
     grid_dependency_sync();
     const int len = length_of(a, b);
     const int rounds = cdiv(len, TT * cs);
-    const float2 bias = a.bias ? load2(a.bias + c, valid) : make_float2(0.0f, 0.0f);
-    float2 s = a.h0 ? load2(a.h0 + (int64_t)b * a.D + c, valid) : make_float2(0.0f, 0.0f);
+    const float2 bias = a.bias ? load2(a.bias + c, valid) : dup(0.0f);
+    float2 s = a.h0 ? load2(a.h0 + (int64_t)b * a.D + c, valid) : dup(0.0f);
+    Fetch<T, N, SUB, VEC> fetch;
+    if constexpr (GATE)
+        fetch.init(a, b, c0, X, F, Z);
+    else
+        fetch.init(a, b, c0, X, F);
     auto start = [&](int round) { return (round * cs + rank) * TT + warp * SUB; };
-    auto fetch = [&](int round) {
-        if (round < rounds) {
-            const int t0 = start(round), k = round % STAGES;
-            fetch_rows<T, SUB>(slots.x[k][warp], a.x, b, t0, len, c0, a.D, a.vec);
-            fetch_rows<T, SUB>(slots.f[k][warp], a.f, b, t0, len, c0, a.D, a.vec);
-            if (GATE) fetch_rows<T, SUB>(slots.z[k][warp], a.z, b, t0, len, c0, a.D, a.vec);
+    auto load = [&](int round) {
+        const int t0 = start(round);
+        if (round < rounds && t0 < len) {
+            if constexpr (GATE)
+                fetch.start(a, slots[round % ST][warp], t0, len - t0, X, F, Z);
+            else
+                fetch.start(a, slots[round % ST][warp], t0, len - t0, X, F);
         }
         cp_async_commit();
     };
 #pragma unroll
-    for (int i = 0; i < STAGES; i++) fetch(i);
-    if (CLUSTER) cooperative_groups::this_cluster().sync();  // the other CTAs' shared memory is there from here on
+    for (int i = 0; i < ST; i++) load(i);
     for (int round = 0; round < rounds; round++) {
-        const int t0 = start(round), k = round % STAGES;
+        const int t0 = start(round), k = round % ST;
         const int n = len - t0;  // positions of this stretch that exist
-        cp_async_wait<STAGES - 1>();
+        R& rows = slots[k][warp];
+        cp_async_wait<ST - 1>();
         __syncwarp();
         float2 av[SUB], uv[SUB];
-#pragma unroll
-        for (int i = 0; i < SUB; i++) {
-            const float2 f = __fadd2_rn(pair(&slots.f[k][warp].v[i][2 * lane]), bias);
-            const float2 x = pair(&slots.x[k][warp].v[i][2 * lane]);
-            float2 w;
-            sigmoids<T>(f.x, av[i].x, w.x);
-            sigmoids<T>(f.y, av[i].y, w.y);
-            uv[i] = CONVEX ? __fmul2_rn(w, x) : x;
-        }
-        if (n < SUB) {
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-                if (i >= n) av[i] = make_float2(1.0f, 1.0f), uv[i] = make_float2(0.0f, 0.0f);
-        }
-        Fold mine = {av[0], uv[0]};
-#pragma unroll
-        for (int i = 1; i < SUB; i++) {
-            mine.p = __fmul2_rn(mine.p, av[i]);
-            mine.q = __ffma2_rn(av[i], mine.q, uv[i]);
-        }
-        float2 h = exchange<CLUSTER>(ex, round, cs, mine, s);
+        Fold mine = {dup(1.0f), dup(0.0f)};
         if (n > 0) {
-            T* y = static_cast<T*>(a.y) + ((int64_t)b * a.L + t0) * a.D + c;
-            float* ck = a.ckpt ? a.ckpt + ((int64_t)b * cdiv(a.L, CK) + t0 / CK) * a.D + c : nullptr;
 #pragma unroll
             for (int i = 0; i < SUB; i++) {
-                if (i % CK == 0 && ck && i < n) put(ck + (int64_t)(i / CK) * a.D, h, valid, a.D % 2 == 0);
-                h = __ffma2_rn(av[i], h, uv[i]);
-                float2 o = h;
-                if (GATE) {
-                    const float2 z = pair(&slots.z[k][warp].v[i][2 * lane]);
-                    o = __fmul2_rn(o, make_float2(silu<T>(z.x), silu<T>(z.y)));
-                }
-                if (i < n) put(y + (int64_t)i * a.D, o, valid, a.ovec);
-            }
-        }
-        __syncwarp();
-        fetch(round + STAGES);
-    }
-    cp_async_wait();
-    if (a.hT && rank == 0 && warp == 0) store2(a.hT + (int64_t)b * a.D + c, s, valid);
-    for (int t = len + rank * WARPS + warp; t < a.L; t += cs * WARPS)
-        put(static_cast<T*>(a.y) + ((int64_t)b * a.L + t) * a.D + c, make_float2(0.0f, 0.0f), valid, a.ovec);
-}
-
-template <typename T, bool GATE>
-struct BwdSlots {
-    Rows<T, CK> x[STAGES][WARPS], f[STAGES][WARPS], dy[STAGES][WARPS], z[GATE ? STAGES : 1][GATE ? WARPS : 1];
-};
-
-// The tiles in reverse: warp 0 of CTA 0 has a round's last positions.  A stretch
-// is as long as the distance between the kept states, so each warp has its own.
-template <typename T, bool CONVEX, bool GATE, bool CLUSTER>
-__global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
-    constexpr int SUB = CK, TT = SUB * WARPS;
-    extern __shared__ __align__(16) unsigned char smem[];
-    BwdSlots<T, GATE>& slots = *reinterpret_cast<BwdSlots<T, GATE>*>(smem);
-    Exchange& ex = *reinterpret_cast<Exchange*>(smem + sizeof(BwdSlots<T, GATE>));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cs = CLUSTER ? a.cs : 1;
-    const int b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
-    const int c = c0 + 2 * lane, valid = a.D - c;
-    const int len = length_of(a, b);
-    const int stretches = cdiv(len, SUB), rounds = cdiv(stretches, WARPS * cs);
-    const float2 bias = a.bias ? load2(a.bias + c, valid) : make_float2(0.0f, 0.0f);
-    float2 s = a.dhT ? load2(a.dhT + (int64_t)b * a.D + c, valid) : make_float2(0.0f, 0.0f);
-    float2 dbias = make_float2(0.0f, 0.0f), next_h = make_float2(0.0f, 0.0f);
-    auto stretch = [&](int round) { return stretches - 1 - ((round * cs + rank) * WARPS + warp); };  // < 0: none
-    auto fetch = [&](int round) {
-        const int j = round < rounds ? stretch(round) : -1;
-        if (j >= 0) {
-            const int t0 = j * SUB, k = round % STAGES;
-            fetch_rows<T, SUB>(slots.x[k][warp], a.x, b, t0, len, c0, a.D, a.vec);
-            fetch_rows<T, SUB>(slots.f[k][warp], a.f, b, t0, len, c0, a.D, a.vec);
-            fetch_rows<T, SUB>(slots.dy[k][warp], a.dy, b, t0, len, c0, a.D, a.vec);
-            if (GATE) fetch_rows<T, SUB>(slots.z[k][warp], a.z, b, t0, len, c0, a.D, a.vec);
-        }
-        cp_async_commit();
-    };
-    auto fetch_h = [&](int round) {
-        const int j = round < rounds ? stretch(round) : -1;
-        if (j >= 0) next_h = load2(a.ckpt + ((int64_t)b * cdiv(a.L, CK) + j) * a.D + c, valid);
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES; i++) fetch(i);
-    fetch_h(0);
-    if (CLUSTER) cooperative_groups::this_cluster().sync();
-    for (int round = 0; round < rounds; round++) {
-        const int j = stretch(round), t0 = j * SUB, k = round % STAGES;
-        const int n = j >= 0 ? len - t0 : 0;
-        const int64_t at = ((int64_t)b * a.L + t0) * a.D + c;
-        cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        float2 av[SUB], wv[SUB], hv[SUB], dv[SUB];  // a, 1 - a, h[t-1], ds
-        Fold mine = {make_float2(1.0f, 1.0f), make_float2(0.0f, 0.0f)};
-        if (j >= 0) {
-            float2 h = next_h;
-            fetch_h(round + 1);
-#pragma unroll
-            for (int i = 0; i < SUB; i++) {
-                const float2 f = __fadd2_rn(pair(&slots.f[k][warp].v[i][2 * lane]), bias);
-                const float2 x = pair(&slots.x[k][warp].v[i][2 * lane]);
-                dv[i] = pair(&slots.dy[k][warp].v[i][2 * lane]);
-                sigmoids<T>(f.x, av[i].x, wv[i].x);
-                sigmoids<T>(f.y, av[i].y, wv[i].y);
-                hv[i] = h;
-                h = __ffma2_rn(av[i], h, CONVEX ? __fmul2_rn(wv[i], x) : x);
-                if (GATE) {
-                    const float2 z = pair(&slots.z[k][warp].v[i][2 * lane]);
-                    float2 gate, slope;
-                    gate.x = silu<T>(z.x, slope.x);
-                    gate.y = silu<T>(z.y, slope.y);
-                    if (i < n)
-                        put(static_cast<T*>(a.dz) + at + (int64_t)i * a.D, __fmul2_rn(__fmul2_rn(dv[i], h), slope), valid,
-                            a.ovec);
-                    dv[i] = __fmul2_rn(dv[i], gate);
-                }
+                const float2 f = __fadd2_rn(pair<VEC>(rows.v[1][i], off16<VEC, T>(a.in[F], b, t0 + i, c0)), bias);
+                const float2 x = pair<VEC>(rows.v[0][i], off16<VEC, T>(a.in[X], b, t0 + i, c0));
+                float2 w;
+                sigmoids(f, av[i], w);
+                uv[i] = CONVEX ? __fmul2_rn(w, x) : x;
             }
             if (n < SUB) {
 #pragma unroll
                 for (int i = 0; i < SUB; i++)
-                    if (i >= n) av[i] = make_float2(1.0f, 1.0f), dv[i] = make_float2(0.0f, 0.0f);
+                    if (i >= n) av[i] = dup(1.0f), uv[i] = dup(0.0f);
+            }
+            mine = {av[0], uv[0]};
+#pragma unroll
+            for (int i = 1; i < SUB; i++) {
+                mine.p = __fmul2_rn(mine.p, av[i]);
+                mine.q = __ffma2_rn(av[i], mine.q, uv[i]);
+            }
+        }
+        float2 h = exchange(ex, round, cs, rank, mine, s);
+        if (n > 0) {
+            T* y = static_cast<T*>(a.y) + ((int64_t)b * a.L + t0) * a.D + c;
+            float* ck = a.ckpt ? a.ckpt + ((int64_t)b * cdiv(a.L, CK) + t0 / CK) * a.D + c : nullptr;
+            auto finish = [&](auto fast) {
+                constexpr bool FAST = decltype(fast)::value;
+#pragma unroll
+                for (int i = 0; i < SUB; i++) {
+                    if (i % CK == 0 && ck && (FAST || i < n)) put<FAST>(ck + (int64_t)(i / CK) * a.D, h, valid, a.D % 2 == 0);
+                    h = __ffma2_rn(av[i], h, uv[i]);
+                    float2 o = h;
+                    if (GATE) o = __fmul2_rn(o, silu<T>(pair<VEC>(rows.v[N - 1][i], off16<VEC, T>(a.in[Z], b, t0 + i, c0))));
+                    if (FAST || i < n) put<FAST>(y + (int64_t)i * a.D, o, valid, a.ovec);
+                }
+            };
+            if (a.ovec && n >= SUB && c0 + CB <= a.D)
+                finish(std::true_type());
+            else
+                finish(std::false_type());
+        }
+        __syncwarp();
+        load(round + ST);
+    }
+    cp_async_wait();
+    if (a.hT && rank == 0 && warp == 0) store2(a.hT + (int64_t)b * a.D + c, s, valid);
+    for (int t = len + rank * WARPS + warp; t < a.L; t += cs * WARPS)
+        put<false>(static_cast<T*>(a.y) + ((int64_t)b * a.L + t) * a.D + c, dup(0.0f), valid, a.ovec);
+    if (cs > 1) cooperative_groups::this_cluster().sync();  // none leaves before the others are done with its memory
+}
+
+// The tiles in reverse: warp 0 of CTA 0 has a round's last positions.  A stretch
+// is as long as the distance between the kept states, so each warp has its own.
+template <typename T, bool CONVEX, bool GATE, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__ Args a) {
+    constexpr int SUB = CK, N = GATE ? 4 : 3;
+    using R = Rows<T, N, SUB, VEC>;
+    constexpr int ST = STAGES<R>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Exchange& ex = *reinterpret_cast<Exchange*>(smem);
+    R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
+    const int c = c0 + 2 * lane, valid = a.D - c;
+    begin(ex, cs);
+    const int len = length_of(a, b);
+    const int stretches = cdiv(len, SUB), rounds = cdiv(stretches, WARPS * cs);
+    const float2 bias = a.bias ? load2(a.bias + c, valid) : dup(0.0f);
+    float2 s = a.dhT ? load2(a.dhT + (int64_t)b * a.D + c, valid) : dup(0.0f);
+    float2 dbias = dup(0.0f), next_h = dup(0.0f);
+    Fetch<T, N, SUB, VEC> fetch;
+    if constexpr (GATE)
+        fetch.init(a, b, c0, X, F, DY, Z);
+    else
+        fetch.init(a, b, c0, X, F, DY);
+    auto stretch = [&](int round) { return stretches - 1 - ((round * cs + rank) * WARPS + warp); };  // < 0: none
+    auto load = [&](int round) {
+        const int j = stretch(round);
+        if (j >= 0) {
+            if constexpr (GATE)
+                fetch.start(a, slots[round % ST][warp], j * SUB, len - j * SUB, X, F, DY, Z);
+            else
+                fetch.start(a, slots[round % ST][warp], j * SUB, len - j * SUB, X, F, DY);
+        }
+        cp_async_commit();
+    };
+    auto load_h = [&](int round) {
+        const int j = stretch(round);
+        if (j >= 0) next_h = load2(a.ckpt + ((int64_t)b * cdiv(a.L, CK) + j) * a.D + c, valid);
+    };
+#pragma unroll
+    for (int i = 0; i < ST; i++) load(i);
+    load_h(0);
+    for (int round = 0; round < rounds; round++) {
+        const int j = stretch(round), t0 = j * SUB, k = round % ST;
+        const int n = j >= 0 ? len - t0 : 0;
+        const int64_t at = ((int64_t)b * a.L + t0) * a.D + c;
+        const bool fast = a.ovec && n >= SUB && c0 + CB <= a.D;
+        R& rows = slots[k][warp];
+        cp_async_wait<ST - 1>();
+        __syncwarp();
+        float2 av[SUB], wv[SUB], mv[SUB], dv[SUB];  // a, 1 - a, dh[t]/df, ds
+        Fold mine = {dup(1.0f), dup(0.0f)};
+        if (n > 0) {
+            float2 h = next_h;
+            load_h(round + 1);
+            auto enter = [&](auto quick) {
+                constexpr bool FAST = decltype(quick)::value;
+#pragma unroll
+                for (int i = 0; i < SUB; i++) {
+                    const float2 f = __fadd2_rn(pair<VEC>(rows.v[1][i], off16<VEC, T>(a.in[F], b, t0 + i, c0)), bias);
+                    const float2 x = pair<VEC>(rows.v[0][i], off16<VEC, T>(a.in[X], b, t0 + i, c0));
+                    dv[i] = pair<VEC>(rows.v[2][i], off16<VEC, T>(a.in[DY], b, t0 + i, c0));
+                    sigmoids(f, av[i], wv[i]);
+                    mv[i] = __fmul2_rn(__fmul2_rn(av[i], wv[i]), CONVEX ? __ffma2_rn(x, dup(-1.0f), h) : h);
+                    h = __ffma2_rn(av[i], h, CONVEX ? __fmul2_rn(wv[i], x) : x);
+                    if (GATE) {
+                        float2 slope;
+                        const float2 gate = silu(pair<VEC>(rows.v[N - 1][i], off16<VEC, T>(a.in[Z], b, t0 + i, c0)), slope);
+                        if (FAST || i < n)
+                            put<FAST>(static_cast<T*>(a.dz) + at + (int64_t)i * a.D, __fmul2_rn(__fmul2_rn(dv[i], h), slope),
+                                      valid, a.ovec);
+                        dv[i] = __fmul2_rn(dv[i], gate);
+                    }
+                }
+            };
+            if (fast) {
+                enter(std::true_type());
+            } else {
+                enter(std::false_type());
+#pragma unroll
+                for (int i = 0; i < SUB; i++)
+                    if (i >= n) av[i] = dup(1.0f), dv[i] = dup(0.0f);
             }
             mine = {av[SUB - 1], __fmul2_rn(av[SUB - 1], dv[SUB - 1])};
 #pragma unroll
@@ -383,47 +502,50 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const Args a) {
                 mine.q = __fmul2_rn(av[i], __fadd2_rn(dv[i], mine.q));
             }
         }
-        float2 G = exchange<CLUSTER>(ex, round, cs, mine, s);
-        if (j >= 0) {
+        float2 G = exchange(ex, round, cs, rank, mine, s);
+        if (n > 0) {
+            auto leave = [&](auto quick) {
+                constexpr bool FAST = decltype(quick)::value;
 #pragma unroll
-            for (int i = SUB - 1; i >= 0; i--) {
-                const float2 g = __fadd2_rn(dv[i], G);
-                G = __fmul2_rn(av[i], g);
-                if (i < n) {
-                    float2 d = hv[i];
-                    if (CONVEX) {
-                        const float2 x = pair(&slots.x[k][warp].v[i][2 * lane]);
-                        d = make_float2(__fsub_rn(d.x, x.x), __fsub_rn(d.y, x.y));
+                for (int i = SUB - 1; i >= 0; i--) {
+                    const float2 g = __fadd2_rn(dv[i], G);
+                    G = __fmul2_rn(av[i], g);
+                    if (FAST || i < n) {
+                        const float2 df = __fmul2_rn(g, mv[i]);
+                        dbias = __fadd2_rn(dbias, df);
+                        put<FAST>(static_cast<T*>(a.df) + at + (int64_t)i * a.D, df, valid, a.ovec);
+                        put<FAST>(static_cast<T*>(a.dx) + at + (int64_t)i * a.D, CONVEX ? __fmul2_rn(wv[i], g) : g, valid, a.ovec);
                     }
-                    const float2 df = __fmul2_rn(__fmul2_rn(G, wv[i]), d);
-                    dbias = make_float2(__fadd_rn(dbias.x, df.x), __fadd_rn(dbias.y, df.y));
-                    put(static_cast<T*>(a.df) + at + (int64_t)i * a.D, df, valid, a.ovec);
-                    put(static_cast<T*>(a.dx) + at + (int64_t)i * a.D, CONVEX ? __fmul2_rn(wv[i], g) : g, valid, a.ovec);
                 }
-            }
+            };
+            if (fast)
+                leave(std::true_type());
+            else
+                leave(std::false_type());
         }
         __syncwarp();
-        fetch(round + STAGES);
+        load(round + ST);
     }
     cp_async_wait();
     if (a.dh0 && rank == 0 && warp == 0) store2(a.dh0 + (int64_t)b * a.D + c, s, valid);
     for (int t = len + rank * WARPS + warp; t < a.L; t += cs * WARPS) {
         const int64_t at = ((int64_t)b * a.L + t) * a.D + c;
-        const float2 zero = make_float2(0.0f, 0.0f);
-        put(static_cast<T*>(a.dx) + at, zero, valid, a.ovec);
-        put(static_cast<T*>(a.df) + at, zero, valid, a.ovec);
-        if (GATE) put(static_cast<T*>(a.dz) + at, zero, valid, a.ovec);
+        put<false>(static_cast<T*>(a.dx) + at, dup(0.0f), valid, a.ovec);
+        put<false>(static_cast<T*>(a.df) + at, dup(0.0f), valid, a.ovec);
+        if (GATE) put<false>(static_cast<T*>(a.dz) + at, dup(0.0f), valid, a.ovec);
     }
-    if (!a.part) return;
-    float2* sums = reinterpret_cast<float2*>(smem);  // [WARPS][32], in the place of the slots
-    __syncthreads();
-    sums[threadIdx.x] = dbias;
-    __syncthreads();
-    if (warp == 0) {
+    if (a.part) {
+        float2(*sums)[32] = reinterpret_cast<float2(*)[32]>(slots);  // every copy into them has arrived
+        __syncthreads();
+        sums[warp][lane] = dbias;
+        __syncthreads();
+        if (warp == 0) {
 #pragma unroll
-        for (int i = 1; i < WARPS; i++) dbias = __fadd2_rn(dbias, sums[i * 32 + lane]);
-        store2(a.part + ((int64_t)b * cs + rank) * a.D + c, dbias, valid);
+            for (int i = 1; i < WARPS; i++) dbias = __fadd2_rn(dbias, sums[i][lane]);
+            store2(a.part + ((int64_t)b * cs + rank) * a.D + c, dbias, valid);
+        }
     }
+    if (cs > 1) cooperative_groups::this_cluster().sync();
 }
 
 // One position: 4 channels a thread.
@@ -445,33 +567,42 @@ __global__ void __launch_bounds__(128) step_kernel(const T* __restrict__ x, int6
     if (bias) pb = load_pack<4>(bias + c, valid, vec);
     float hn[4], o[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float up, down;
-        sigmoids<T>(__fadd_rn(to_f(pf.v[i]), pb.v[i]), up, down);
-        hn[i] = __fmaf_rn(up, hp.v[i], CONVEX ? __fmul_rn(down, to_f(px.v[i])) : to_f(px.v[i]));
-        o[i] = GATE ? __fmul_rn(hn[i], silu<T>(to_f(pz.v[i]))) : hn[i];
+    for (int i = 0; i < 4; i += 2) {
+        const float2 x = make_float2(to_f(px.v[i]), to_f(px.v[i + 1]));
+        float2 up, down;
+        sigmoids(make_float2(__fadd_rn(to_f(pf.v[i]), pb.v[i]), __fadd_rn(to_f(pf.v[i + 1]), pb.v[i + 1])), up, down);
+        const float2 hh = __ffma2_rn(up, make_float2(hp.v[i], hp.v[i + 1]), CONVEX ? __fmul2_rn(down, x) : x);
+        const float2 oo = GATE ? __fmul2_rn(hh, silu<T>(make_float2(to_f(pz.v[i]), to_f(pz.v[i + 1])))) : hh;
+        hn[i] = hh.x, hn[i + 1] = hh.y, o[i] = oo.x, o[i + 1] = oo.y;
     }
     store_pack<4>(ph, hn, valid, vec);
     store_pack<4>(y + b * D + c, o, valid, vec);
 }
 
-// CTAs of a cluster: as many as it takes to give every SM two CTAs, and no more
-// than the sequence has tiles.
+// CTAs of a cluster: doubled as long as SMs are left without a CTA, and further,
+// up to 800 CTAs, where each still has 4 tiles.
+// us forward and backward in bf16 (fp16) by CTAs of a cluster, 1, 2, 4, 8:
+// 1 x 2048 x 1536 37 22 12.5 12.2, 62 40 25 22; 6 x 777 x 2048 ragged
+// 23 24 28 43, 38 37 44 60; 8 x 2048 x 1536 64 54 57 68, 105 110 99 117;
+// 32 x 512 x 1536 48 55 72 145, 85 99 117 162.
 static inline int cluster_of(int batch, int L, int D, int tile) {
+    const int64_t base = (int64_t)batch * cdiv(D, CB);
     int cs = 1;
-    while (cs < MAX_CLUSTER && (int64_t)batch * cdiv(D, CB) * cs < 148 * 2 && cs * tile < L) cs *= 2;
+    while (cs < MAX_CLUSTER && cs * tile < L && base * cs * 2 <= 800 && (base * cs < 148 || L >= (int64_t)cs * 8 * tile)) cs *= 2;
     return cs;
 }
 
-template <typename T, bool CONVEX, bool GATE, bool CLUSTER, bool BWD>
+template <typename T, bool CONVEX, bool GATE, bool VEC, bool BWD>
 static int launch(const Args& a, cudaStream_t s) {
-    constexpr size_t smem = (BWD ? sizeof(BwdSlots<T, GATE>) : sizeof(FwdSlots<T, GATE>)) + sizeof(Exchange);
+    constexpr int N = (GATE ? 3 : 2) + BWD, SUB = BWD ? CK : SUB_FWD<T>;
+    using R = Rows<T, N, SUB, VEC>;
+    constexpr size_t smem = sizeof(R) * STAGES<R> * WARPS + sizeof(Exchange);
     static std::atomic<uint64_t> allowed{0};
     void (*kernel)(const Args);
     if constexpr (BWD)
-        kernel = bwd_kernel<T, CONVEX, GATE, CLUSTER>;
+        kernel = bwd_kernel<T, CONVEX, GATE, VEC>;
     else
-        kernel = fwd_kernel<T, CONVEX, GATE, CLUSTER>;
+        kernel = fwd_kernel<T, CONVEX, GATE, VEC>;
     if (!allow_smem(kernel, smem, allowed)) return MI_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cdiv(a.D, CB) * a.cs, a.batch);
@@ -480,7 +611,7 @@ static int launch(const Args& a, cudaStream_t s) {
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int n = 0;
-    if (CLUSTER) {
+    if (a.cs > 1) {
         attr[n].id = cudaLaunchAttributeClusterDimension;
         attr[n].val.clusterDim.x = a.cs;
         attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
@@ -501,22 +632,24 @@ static int launch(const Args& a, cudaStream_t s) {
 }
 
 template <typename T, bool BWD>
-static int dispatch(const Args& a, bool convex, cudaStream_t s) {
-#define MI_REC(CONVEX, GATE) \
-    return a.cs > 1 ? launch<T, CONVEX, GATE, true, BWD>(a, s) : launch<T, CONVEX, GATE, false, BWD>(a, s)
+static int dispatch(Args& a, bool convex, bool vec, cudaStream_t s) {
+    a.cs = cluster_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS);
+#define MI_REC(CONVEX, GATE) return vec ? launch<T, CONVEX, GATE, true, BWD>(a, s) : launch<T, CONVEX, GATE, false, BWD>(a, s)
     if (convex) {
-        if (a.z.p) MI_REC(true, true);
+        if (a.in[Z].p) MI_REC(true, true);
         MI_REC(true, false);
     }
-    if (a.z.p) MI_REC(false, true);
+    if (a.in[Z].p) MI_REC(false, true);
     MI_REC(false, false);
 #undef MI_REC
 }
 
 static inline int elem_size(int dtype) { return dtype == MI_DT_F32 ? 4 : 2; }
-static inline bool rows_vec(const Seq& s, int dtype) {
+static inline bool rows_vec(const Args& a, int D, int dtype) {
     const int k = 16 / elem_size(dtype);
-    return !s.p || (s.sb % k == 0 && s.sl % k == 0 && aligned16(s.p));
+    for (const Seq& s : a.in)
+        if (s.p && (s.sb % k != 0 || s.sl % k != 0 || !aligned16(s.p))) return false;
+    return D % k == 0;
 }
 
 }  // namespace rec
@@ -541,8 +674,8 @@ extern "C" int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row
                                    const float* h0, const int32_t* lengths, void* y, float* h_out, float* checkpoints,
                                    int batch, int L, int D, int convex, int dtype, void* stream) {
     mi::rec::Args a = {};
-    a.x = {x, x_batch, x_row}, a.f = {f, f_batch, f_row}, a.z = {z, z_batch, z_row};
-    const int rc = mi_rec_check(a.x, a.f, a.z, batch, L, D, dtype);
+    a.in[mi::rec::X] = {x, x_batch, x_row}, a.in[mi::rec::F] = {f, f_batch, f_row}, a.in[mi::rec::Z] = {z, z_batch, z_row};
+    const int rc = mi_rec_check(a.in[0], a.in[1], a.in[2], batch, L, D, dtype);
     if (rc != MI_OK) return rc;
     if (!y) return MI_ERR_INVALID;
     if (batch == 0) return MI_OK;
@@ -550,12 +683,8 @@ extern "C" int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row
     a.batch = batch, a.L = L, a.D = D;
     const int e = mi::rec::elem_size(dtype);
     a.ovec = D % 2 == 0 && reinterpret_cast<uintptr_t>(y) % (2 * e) == 0;
-    a.vec = D % (16 / e) == 0 && mi::rec::rows_vec(a.x, dtype) && mi::rec::rows_vec(a.f, dtype) &&
-            mi::rec::rows_vec(a.z, dtype);
-    MI_DISPATCH_DTYPE(dtype, T, {
-        a.cs = mi::rec::cluster_of(batch, L, D, mi::rec::SUB_FWD<T> * mi::rec::WARPS);
-        return (mi::rec::dispatch<T, false>(a, convex, (cudaStream_t)stream));
-    });
+    const bool vec = mi::rec::rows_vec(a, D, dtype);
+    MI_DISPATCH_DTYPE(dtype, T, return (mi::rec::dispatch<T, false>(a, convex, vec, (cudaStream_t)stream)););
 }
 
 extern "C" int64_t mi_gated_recurrence_backward_workspace(int batch, int L, int D) {
@@ -570,8 +699,9 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
                                             float* dbias, float* dh0, void* workspace, int batch, int L, int D, int convex,
                                             int dtype, void* stream) {
     mi::rec::Args a = {};
-    a.x = {x, x_batch, x_row}, a.f = {f, f_batch, f_row}, a.z = {z, z_batch, z_row}, a.dy = {dy, dy_batch, dy_row};
-    const int rc = mi_rec_check(a.x, a.f, a.z, batch, L, D, dtype);
+    a.in[mi::rec::X] = {x, x_batch, x_row}, a.in[mi::rec::F] = {f, f_batch, f_row}, a.in[mi::rec::Z] = {z, z_batch, z_row};
+    a.in[mi::rec::DY] = {dy, dy_batch, dy_row};
+    const int rc = mi_rec_check(a.in[0], a.in[1], a.in[2], batch, L, D, dtype);
     if (rc != MI_OK) return rc;
     if (!dy || dy_batch < 0 || dy_row < 0 || !checkpoints || !dx || !df || (z && !dz) || (dbias && !workspace))
         return MI_ERR_INVALID;
@@ -586,11 +716,9 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
     const int e = mi::rec::elem_size(dtype);
     a.ovec = D % 2 == 0;
     for (const void* p : {dx, df, z ? dz : nullptr}) a.ovec = a.ovec && reinterpret_cast<uintptr_t>(p) % (2 * e) == 0;
-    a.vec = D % (16 / e) == 0 && mi::rec::rows_vec(a.x, dtype) && mi::rec::rows_vec(a.f, dtype) &&
-            mi::rec::rows_vec(a.z, dtype) && mi::rec::rows_vec(a.dy, dtype);
-    a.cs = mi::rec::cluster_of(batch, L, D, mi::rec::CK * mi::rec::WARPS);
+    const bool vec = mi::rec::rows_vec(a, D, dtype);
     int rc2 = MI_ERR_INVALID;
-    MI_DISPATCH_DTYPE(dtype, T, (rc2 = mi::rec::dispatch<T, true>(a, convex, s)););
+    MI_DISPATCH_DTYPE(dtype, T, (rc2 = mi::rec::dispatch<T, true>(a, convex, vec, s)););
     if (rc2 != MI_OK || !dbias) return rc2;
     mi::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, s>>>(a.part, dbias, batch * a.cs, D);
     MI_CHECK_LAUNCH();
