@@ -7,20 +7,26 @@
 //   those, w_i >= min_p.  The token is the first index whose running sum of the
 //   kept w, in index order, exceeds u times their total.
 //
-// Every filter keeps a first part of one order, so all of them end in one
-// number: a token's rank is key = (order-preserving bits of l, mask - index),
-// which no two tokens share, and the kept ones are those with key >= cut.
+// Every filter keeps a first part of one order, that of the keys
+// (order-preserving bits of l, mask - index), which no two tokens share.
 //
 // Borders between tokens are sharp, so masses are whole numbers: w in units of
-// 2^-44 from a 64-bit evaluation (2^-42 relative), which add up exactly and in
+// 2^-44 from a 64-bit evaluation (7e-12 relative), which add up exactly and in
 // any order.  fp32 weights would move the borders of a flat distribution over
 // 32768 tokens by 1e-8 each, one row in some ten thousand.
 //
-// A row lies in the shared memory of one CTA or of a cluster of up to 8, read
-// once.  A border is found by a histogram over 1024 bins of equal width between
-// the maximum and where the weights end, which leaves a bin of few tokens; these
-// are listed and ranked against one another, or, where they are many (equal or
-// nearly equal logits), divided again by the bits of their keys.
+// What bounds it: the logits come from HBM once and from L2 after that; a
+// 64-bit weight is 16 operations of half rate, so a pass over all weights costs as
+// much as the first read, and the filters are arranged to need few of them.  A
+// row's 512 groups of tokens (a thread's, or those of some threads of a cluster)
+// have a maximum each: the k-th largest of these is below no k tokens, and where
+// the largest of them hold p of the total mass, the smallest of those is below all
+// that top-p keeps.  What lies above such a bound, a few tokens more than are kept, is
+// listed, and the rest is done on the list.  Lists that would be too long (large k,
+// flat distributions) go by histograms over bins of equal width below the maximum
+// instead, then by the leading bits of the keys, until the border's bin is a list.
+//
+// A row belongs to one CTA, or to a cluster of up to 8 where rows are few.
 #include <cooperative_groups.h>
 
 #include "mi_elem.cuh"
@@ -31,7 +37,7 @@ namespace sample {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 1024, LIST = 256, MAX_CLUSTER = 8, MAX_SEG = 32768;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = THREADS, MAX_CLUSTER = 8, MAX_V = 262144, MAX_SEG = 131072;
 constexpr int SCALE = 44;                      // weights are whole numbers of 2^-44
 constexpr uint32_t LOWEST = 0x00800000u;       // key of -FLT_MAX
 constexpr uint32_t INF = 0xff800000u;          // key of +inf; NaN above it
@@ -48,7 +54,7 @@ struct Args {
     int top_k1;
     int64_t* token;
     float* prob;  // may be NULL
-    int V, cs, seg, vec;
+    int V, cs, seg;
 };
 
 __device__ __forceinline__ uint32_t key_of(float v) {  // of a v without -0
@@ -64,26 +70,28 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 struct Weights {
     double most, scale;  // log2(e) / temperature
     __device__ __forceinline__ double power(float v) const { return ((double)v - most) * scale; }
-    // 2^x times 2^SCALE: x = n + f, |f| <= 1/2; the power series of 2^f, ended behind (f ln 2)^10 / 10!,
-    // leaves 2.2e-13.  Not rounded to a whole number; 0 where less than half of one is left.
-    __device__ __forceinline__ static double scaled(double x) {
-        if (!(x > -(SCALE + 1))) return 0.0;
-        const double n = __dsub_rn(__dadd_rn(x, 6755399441055744.0), 6755399441055744.0), f = __dsub_rn(x, n);
-        const double g = f * 0.693147180559945309417;
-        double p = 1.0 / 3628800;
-        p = __fma_rn(p, g, 1.0 / 362880);
-        p = __fma_rn(p, g, 1.0 / 40320);
-        p = __fma_rn(p, g, 1.0 / 5040);
-        p = __fma_rn(p, g, 1.0 / 720);
-        p = __fma_rn(p, g, 1.0 / 120);
-        p = __fma_rn(p, g, 1.0 / 24);
-        p = __fma_rn(p, g, 1.0 / 6);
-        p = __fma_rn(p, g, 0.5);
-        p = __fma_rn(p, g, 1.0);
-        p = __fma_rn(p, g, 1.0);
-        return p * __hiloint2double((1023 + SCALE + (int)n) << 20, 0);
+    // 2^x in units of 2^-SCALE, rounded to a whole one; 0 where less than half of one is left.  x = n + f with
+    // |f| <= 1/2; the power series of 2^f, ended behind (f ln 2)^9 / 9!, leaves 7e-12.
+    // Adding 1.5 2^52 rounds to a whole number, which the sum's low bits hold.
+    __device__ __forceinline__ static u64 mass(double x) {
+        constexpr double ROUND = 6755399441055744.0, L = 0.693147180559945309417;
+        constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4, C5 = C4 * L / 5, C6 = C5 * L / 6, C7 = C6 * L / 7,
+                         C8 = C7 * L / 8, C9 = C8 * L / 9;
+        if (!(x > -(SCALE + 1))) return 0;
+        const double r = __dadd_rn(x, ROUND), f = __dsub_rn(x, __dsub_rn(r, ROUND));
+        double p = __fma_rn(C9, f, C8);
+        p = __fma_rn(p, f, C7);
+        p = __fma_rn(p, f, C6);
+        p = __fma_rn(p, f, C5);
+        p = __fma_rn(p, f, C4);
+        p = __fma_rn(p, f, C3);
+        p = __fma_rn(p, f, C2);
+        p = __fma_rn(p, f, L);
+        p = __fma_rn(p, f, 1.0);
+        p = __fma_rn(p, __hiloint2double((1023 + SCALE + __double2loint(r)) << 20, 0), ROUND);
+        return (u64)(__double_as_longlong(p) - __double_as_longlong(ROUND));
     }
-    __device__ __forceinline__ u64 mass(float v) const { return __double2ull_rn(scaled(power(v))); }
+    __device__ __forceinline__ u64 mass(float v) const { return mass(power(v)); }
 };
 
 // Bins of equal width downwards from the maximum; falls monotonically as v rises.
@@ -95,25 +103,25 @@ struct Bins {
     }
 };
 
-struct Row {  // what the CTAs of a row tell one another
-    uint32_t most[MAX_CLUSTER], at[MAX_CLUSTER], least[MAX_CLUSTER];
-    u64 sums[MAX_CLUSTER][WARPS];
-};
 struct Entry {
     u64 key, mass;
 };
 struct Shared {
-    u64 mass[2][BINS];
-    Entry own[LIST], all[LIST];
-    Row row;
-    uint32_t count[2][BINS];
+    // what the CTAs of a row tell one another
+    uint32_t most[MAX_CLUSTER][WARPS], at[MAX_CLUSTER][WARPS], listed_by[MAX_CLUSTER];
+    u64 sums[MAX_CLUSTER][WARPS];
+    uint32_t maxima[THREADS];
+    Entry all[LIST];
+    // this CTA's own
+    Entry own[LIST];
+    u64 swap[2][THREADS];
+    uint32_t count[2][BINS], limb[2][3][BINS];  // limbs of 15 bits, which MAX_SEG tokens do not overflow
     u64 warp_mass[WARPS];
-    uint32_t warp_count[WARPS], warp_low[WARPS];
-    uint32_t listed;
+    uint32_t warp_count[WARPS];
+    uint32_t listed, bound;
     // a border's bin: what lies above it, what it holds
-    u64 above_mass, in_mass, target;
+    u64 above_mass, in_mass, target, cut;
     uint32_t above_count, in_count, bin, edge[2];
-    u64 cut, floor;
 };
 
 // The smallest key in (lo, hi] for which pred holds; it holds for hi, and from some key on.  By a whole warp.
@@ -149,20 +157,39 @@ __device__ __forceinline__ V warp_scan(V v) {  // inclusive
     return v;
 }
 
+// share of `total`, as the smallest whole number that is not below it, from 1 to total
+__device__ __forceinline__ u64 part_of(u64 total, double share) {
+    const double t = ceil(share * (double)total);
+    return t >= (double)total ? total : t < 1.0 ? 1 : (u64)t;
+}
+// the number that a running sum has to exceed
+__device__ __forceinline__ u64 target_of(u64 total, float u) {
+    const double t = floor((double)u * (double)total);
+    return !(t > 0.0) ? 0 : t >= (double)total ? total - 1 : (u64)t < total ? (u64)t : total - 1;
+}
+
 template <typename T>
 struct Chooser {
+    static constexpr int K = 16 / sizeof(T);
     const Args& a;
     Shared& sh;
-    float* vals;
-    int n, first, rank;  // this CTA's tokens: first .. first + n - 1
-    int cs, bits;        // bits of an index
+    const T* from;            // this CTA's tokens: first .. first + n - 1 of the row
+    int n, first, rank, cs, part;  // part: neighbouring tokens of a warp
+    int tid, warp, lane;
+    int bits;                 // of an index
     Weights weights;
     Bins bins;
     uint32_t kmax;
-    int level = 0;  // of the histograms, which alternate
+    int level = 0;            // of the histograms, which alternate
 
     __device__ __forceinline__ u64 full_key(float v, int e) const {
         return (u64)key_of(v) << bits | (u64)((1u << bits) - 1 - (uint32_t)(first + e));
+    }
+    __device__ __forceinline__ float value(u64 key) const { return value_of((uint32_t)(key >> bits)); }
+    __device__ __forceinline__ int index(u64 key) const { return (int)((1u << bits) - 1 - ((uint32_t)key & ((1u << bits) - 1))); }
+    // v is at or above the cut, of which only equal values need the index
+    __device__ __forceinline__ bool kept(float v, int e, float vcut, u64 cut) const {
+        return v > vcut || (v == vcut && full_key(v, e) >= cut);
     }
     __device__ __forceinline__ void sync() {
         if (cs > 1)
@@ -170,31 +197,174 @@ struct Chooser {
         else
             __syncthreads();
     }
+    __device__ __forceinline__ Shared& of(int r) { return cs > 1 ? *cg::this_cluster().map_shared_rank(&sh, r) : sh; }
+
+    // f(v, e) for this warp's tokens, by blocks of 16 bytes, U of them a lane in flight; beside the tokens a block may
+    // hold others' places, for which v is -infinity.
+    template <int U, typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int begin = warp * part, end = min(begin + part, n);
+        const int off = (int)((reinterpret_cast<uintptr_t>(from + begin) & 15) / sizeof(T));
+        for (int e0 = begin - off + lane * K; e0 < end; e0 += U * 32 * K) {
+            Pack<T, K> v[U];
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                const int e = e0 + j * 32 * K;
+                if (e >= begin && e + K <= end) {
+                    v[j] = *reinterpret_cast<const Pack<T, K>*>(from + e);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K; i++)
+                        v[j].v[i] = e + i >= begin && e + i < end ? from[e + i] : from_f<T>(-__int_as_float(0x7f800000));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; j++)
+#pragma unroll
+                for (int i = 0; i < K; i++)  // no -0: it is as good as 0
+                    f(__fadd_rn(to_f(v[j].v[i]), 0.0f), e0 + j * 32 * K + i);
+        }
+    }
+
+    // The warps' sums to all CTAs; the row's total.
+    __device__ __forceinline__ u64 exchange_sums(u64 sum) {
+        sum = warp_sum(sum);
+        if (lane < cs) of(lane).sums[rank][warp] = sum;
+        sync();
+        const u64* sums = &sh.sums[0][0];
+        u64 own = 0;
+        for (int i = lane; i < cs * WARPS; i += 32) own += sums[i];
+        return warp_sum(own);
+    }
+
+    // The sum over the CTA's threads before this one, and over all.
+    __device__ __forceinline__ u64 block_before(u64 v, u64& all) {
+        u64 upto = warp_scan(v);
+        __syncthreads();  // the last sums were read
+        if (lane == 31) sh.warp_mass[warp] = upto;
+        __syncthreads();
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) {
+            if (i == warp) upto += all;
+            all += sh.warp_mass[i];
+        }
+        return upto - v;
+    }
+
+    // Sorts `size` values (a power of 2 from 32 to THREADS), one a thread, into falling order.
+    template <typename V>
+    __device__ __forceinline__ V sorted(V v, int size) {
+        V(*swap)[THREADS] = reinterpret_cast<V(*)[THREADS]>(sh.swap);
+        int set = 0;
+        for (int k = 2; k <= size; k <<= 1) {
+            for (int j = k >> 1; j; j >>= 1) {
+                V o;
+                if (j >= 32) {
+                    swap[set][tid] = v;
+                    __syncthreads();
+                    o = swap[set][tid ^ j];
+                    set ^= 1;
+                } else {
+                    o = __shfl_xor_sync(0xffffffffu, v, j);
+                }
+                const bool larger = ((tid & k) == 0) == ((tid & j) == 0);
+                v = larger == (v > o) ? v : o;
+            }
+        }
+        return v;
+    }
+
+    // Lists the row's tokens from `bound` on in CTA 0's sh.all.  Their number, or -1 if they are too many.
+    __device__ __forceinline__ int list(float bound) {
+        each<2>([&](float v, int e) {
+            if (v >= bound) {
+                const uint32_t i = atomicAdd(&sh.listed, 1u);
+                if (i < LIST) sh.own[i].key = full_key(v, e);
+            }
+        });
+        __syncthreads();
+        const int mine = min(sh.listed, (uint32_t)LIST + 1);
+        if (tid < cs) of(tid).listed_by[rank] = mine;
+        sync();
+        int all = 0, before = 0;
+        for (int r = 0; r < cs; r++) {
+            if (r == rank) before = all;
+            all += sh.listed_by[r];
+        }
+        if (all > LIST) return -1;
+        if (tid < mine) of(0).all[before + tid].key = sh.own[tid].key;
+        sync();
+        return all;
+    }
+
+    // The filters and the choice on the listed tokens, which hold all that are kept.  By CTA 0.
+    __device__ __forceinline__ void choose_listed(int m, bool by_k, int k, bool by_p, double p, u64 total, double least_power,
+                                                  float u, int64_t row) {
+        int size = 32;
+        while (size < m) size *= 2;
+        u64 q = sorted(tid < m ? sh.all[tid].key : 0, size);
+        const bool some = tid < m;
+        const float v = value(q);
+        u64 mass = some ? weights.mass(v) : 0;
+        bool keep = some && (!by_k || tid < k);
+        if (by_p) {
+            u64 all;
+            const u64 before = block_before(keep ? mass : 0, all);
+            keep = keep && (before < part_of(by_k ? all : total, p) || tid == 0);
+        }
+        if (keep && !(weights.power(v) >= least_power)) keep = false;
+        __syncthreads();  // the sort before is over for all
+        // now by index: the lowest comes first
+        q = sorted(keep ? (u64)(0xffffffffu - index(q)) << 32 | key_of(v) : 0, size);
+        const float chosen = value_of((uint32_t)q);
+        mass = q ? weights.mass(chosen) : 0;
+        const u64 before = block_before(mass, total), target = target_of(total, u);
+        if (mass && before <= target && target < before + mass) {
+            a.token[row] = 0xffffffffu - (uint32_t)(q >> 32);
+            if (a.prob) a.prob[row] = (float)(exp2(weights.power(chosen) + SCALE) / (double)total);
+        }
+    }
+
+    // ----- by histograms -----
+    __device__ __forceinline__ void clear(int set) {
+        for (int i = tid; i < BINS; i += THREADS) {
+            sh.count[set][i] = 0;
+#pragma unroll
+            for (int j = 0; j < 3; j++) sh.limb[set][j][i] = 0;
+        }
+    }
+    template <bool MASS>
+    __device__ __forceinline__ void add(int at, float v) {
+        atomicAdd(&sh.count[level & 1][at], 1u);
+        if (MASS) {
+            const u64 w = weights.mass(v);
+#pragma unroll
+            for (int j = 0; j < 3; j++) atomicAdd(&sh.limb[level & 1][j][at], (uint32_t)(w >> (15 * j)) & 0x7fffu);
+        }
+    }
 
     // Adds up the row's histograms and finds the bin of the border: by count, the bin of the target-th
     // token; by mass, the bin in which the mass reaches the target, `share` of all if `share` is given.
     // false: there are no more than target tokens.
     template <bool MASS>
-    __device__ __forceinline__ bool border(uint64_t target, const double* share) {
-        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, k = level & 1;
-        constexpr int PER = BINS / THREADS;
+    __device__ __forceinline__ bool border(u64 target, const double* share) {
+        const int k = level & 1;
+        static_assert(BINS == THREADS, "a bin a thread");
         sync();
-        uint32_t c[PER] = {}, ctot = 0;
-        u64 m[PER] = {}, mtot = 0;
+        uint32_t c = 0;
+        u64 m = 0;
         for (int r = 0; r < cs; r++) {
-            const Shared& from = cs > 1 ? *cg::this_cluster().map_shared_rank(&sh, r) : sh;
+            const Shared& with = of(r);
+            c += with.count[k][tid];
+            if (MASS) {
 #pragma unroll
-            for (int i = 0; i < PER; i++) {
-                c[i] += from.count[k][tid * PER + i];
-                if (MASS) m[i] += from.mass[k][tid * PER + i];
+                for (int j = 0; j < 3; j++) m += (u64)with.limb[k][j][tid] << (15 * j);
             }
         }
-#pragma unroll
-        for (int i = 0; i < PER; i++) ctot += c[i], mtot += m[i];
-        // the other set was last read before this barrier
-        for (int i = tid; i < BINS; i += THREADS) sh.count[k ^ 1][i] = 0, sh.mass[k ^ 1][i] = 0;
-        uint32_t cup = warp_scan(ctot);
-        u64 mup = MASS ? warp_scan(mtot) : 0;
+        clear(k ^ 1);  // last read before this barrier
+        uint32_t cup = warp_scan(c);
+        u64 mup = MASS ? warp_scan(m) : 0;
         if (lane == 31) sh.warp_count[warp] = cup, sh.warp_mass[warp] = mup;
         if (tid == 0) sh.listed = 0;
         __syncthreads();
@@ -205,22 +375,14 @@ struct Chooser {
             call += sh.warp_count[i];
             mall += sh.warp_mass[i];
         }
-        if (MASS && share) {
-            const double t = ceil(*share * (double)mall);
-            target = t >= (double)mall ? mall : t < 1.0 ? 1 : (u64)t;
-        }
+        if (MASS && share) target = part_of(mall, *share);
         level++;
         if (!MASS && call <= target) return false;
-        uint32_t cb = cup - ctot;
-        u64 mb = mup - mtot;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const bool here = MASS ? mb < target && target <= mb + m[i] : cb < target && target <= cb + c[i];
-            if (here) {
-                sh.bin = tid * PER + i;
-                sh.above_count = cb, sh.above_mass = mb, sh.in_count = c[i], sh.in_mass = m[i], sh.target = target;
-            }
-            cb += c[i], mb += m[i];
+        const uint32_t cb = cup - c;
+        const u64 mb = mup - m;
+        if (MASS ? mb < target && target <= mup : cb < target && target <= cup) {
+            sh.bin = tid;
+            sh.above_count = cb, sh.above_mass = mb, sh.in_count = c, sh.in_mass = m, sh.target = target;
         }
         __syncthreads();
         return true;
@@ -230,24 +392,20 @@ struct Chooser {
     // which the mass reaches `share` of all that is kept.
     template <bool MASS>
     __device__ __forceinline__ void descend(uint32_t k, double share, u64& cut) {
-        const int tid = threadIdx.x, warp = tid >> 5;
-        const float vcut = value_of((uint32_t)(cut >> bits));
-        for (int e = tid; e < n; e += THREADS) {
-            const float v = vals[e];
-            if (!(v >= vcut) || full_key(v, e) < cut) continue;
-            const int at = bins(v);
-            atomicAdd(&sh.count[level & 1][at], 1u);
-            if (MASS) atomicAdd(&sh.mass[level & 1][at], weights.mass(v));
-        }
+        const float vcut = value(cut);
+        each<1>([&](float v, int e) {
+            if (kept(v, e, vcut, cut)) add<MASS>(bins(v), v);
+        });
         if (!border<MASS>(k, &share)) return;
         // the keys of the bin
         const int b = sh.bin;
         if (warp < 2) {
             const int last = b - warp;
             const uint32_t edge = last < 0 ? kmax + 1
-                                  : last == BINS - 1 ? LOWEST
-                                                     : first_key(LOWEST - 1, kmax, [&](uint32_t q) { return bins(value_of(q)) <= last; });
-            if ((tid & 31) == 0) sh.edge[warp] = edge;
+                                  : last == BINS - 1
+                                      ? LOWEST
+                                      : first_key(LOWEST - 1, kmax, [&](uint32_t q) { return bins(value_of(q)) <= last; });
+            if (lane == 0) sh.edge[warp] = edge;
         }
         __syncthreads();
         u64 lo = (u64)sh.edge[0] << bits, hi = ((u64)sh.edge[1] << bits) - 1;
@@ -260,22 +418,21 @@ struct Chooser {
                 __syncthreads();
                 return;
             }
-            const float vlo = value_of((uint32_t)(lo >> bits)), vhi = value_of((uint32_t)(hi >> bits));
+            const float vlo = value(lo), vhi = value(hi);
             if (sh.in_count <= LIST) {
-                for (int e = tid; e < n; e += THREADS) {
-                    const float v = vals[e];
-                    if (!(v >= vlo && v <= vhi)) continue;
+                each<1>([&](float v, int e) {
+                    if (!(v >= vlo && v <= vhi)) return;
                     const u64 q = full_key(v, e);
-                    if (q < lo || q > hi) continue;
+                    if (q < lo || q > hi) return;
                     const uint32_t i = atomicAdd(&sh.listed, 1u);
                     if (i < LIST) sh.own[i] = {q, MASS ? weights.mass(v) : 1ull};
-                }
+                });
                 sync();
                 uint32_t m = 0;
                 for (int r = 0; r < cs; r++) {
-                    const Shared& from = cs > 1 ? *cg::this_cluster().map_shared_rank(&sh, r) : sh;
-                    const uint32_t some = from.listed;
-                    for (uint32_t i = tid; i < some && m + i < LIST; i += THREADS) sh.all[m + i] = from.own[i];
+                    const Shared& with = of(r);
+                    const uint32_t some = with.listed;
+                    if (tid < some && m + tid < LIST) sh.all[m + tid] = with.own[tid];
                     m += some;
                 }
                 if (m > LIST) m = LIST;
@@ -294,62 +451,50 @@ struct Chooser {
             int shift = 0;
             while (((hi - lo) >> shift) >= BINS) shift++;
             const u64 in_lo = lo, in_hi = hi;
-            const u64 next = left;
-            for (int e = tid; e < n; e += THREADS) {
-                const float v = vals[e];
-                if (!(v >= vlo && v <= vhi)) continue;
+            each<1>([&](float v, int e) {
+                if (!(v >= vlo && v <= vhi)) return;
                 const u64 q = full_key(v, e);
-                if (q < in_lo || q > in_hi) continue;
-                const int at = (int)((in_hi - q) >> shift);
-                atomicAdd(&sh.count[level & 1][at], 1u);
-                if (MASS) atomicAdd(&sh.mass[level & 1][at], weights.mass(v));
-            }
-            border<MASS>(next, nullptr);
-            const u64 b2 = sh.bin;
-            hi = in_hi - (b2 << shift);
+                if (q >= in_lo && q <= in_hi) add<MASS>((int)((in_hi - q) >> shift), v);
+            });
+            border<MASS>(left, nullptr);
+            hi = in_hi - ((u64)sh.bin << shift);
             const u64 span = ((u64)1 << shift) - 1;
             lo = hi - in_lo > span ? hi - span : in_lo;
             target = sh.target;
         }
     }
 
-    // Tokens of a warp are neighbours: the sums by warp are in the order of the indices.
+    // The choice among the tokens from the cut on.  Tokens of a warp are neighbours: the sums by warp are in the
+    // order of the indices.
     __device__ __forceinline__ void choose(float u, u64 cut, int64_t row) {
-        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-        const int part = cdiv(cdiv(n, WARPS), 32) * 32;  // tokens a warp
-        const float vcut = value_of((uint32_t)(cut >> bits));
+        const float vcut = value(cut);
         u64 sum = 0;
-        for (int e = warp * part + lane; e < (warp + 1) * part && e < n; e += 32) {
-            const float v = vals[e];
-            if (v >= vcut && full_key(v, e) >= cut) sum += weights.mass(v);
-        }
+        each<1>([&](float v, int e) {
+            if (kept(v, e, vcut, cut)) sum += weights.mass(v);
+        });
         sum = warp_sum(sum);
-        if (lane < cs) {
-            Row& to = cs > 1 ? *cg::this_cluster().map_shared_rank(&sh.row, lane) : sh.row;
-            to.sums[rank][warp] = sum;
-        }
+        if (lane < cs) of(lane).sums[rank][warp] = sum;
         sync();
         // every warp adds up all of them, some neighbouring ones a lane
-        const u64* sums = &sh.row.sums[0][0];
+        const u64* sums = &sh.sums[0][0];
         const int all = cs * WARPS, some = cdiv(all, 32);
         u64 own = 0;
         for (int i = lane * some; i < (lane + 1) * some && i < all; i++) own += sums[i];
-        u64 to_lane = warp_scan(own);
-        const u64 total = __shfl_sync(0xffffffffu, to_lane, 31);
-        // the token whose sum is the first above `target`
-        const double t = floor((double)u * (double)total);
-        const u64 target = !(t > 0.0) ? 0 : t >= (double)total ? total - 1 : (u64)t < total ? (u64)t : total - 1;
+        const u64 to_lane = warp_scan(own), total = __shfl_sync(0xffffffffu, to_lane, 31);
+        const u64 target = target_of(total, u);
         const int in = __ffs(__ballot_sync(0xffffffffu, to_lane > target)) - 1;
         u64 before = __shfl_sync(0xffffffffu, to_lane - own, in);
         int owner = in * some;
         for (; before + sums[owner] <= target; owner++) before += sums[owner];
         if (owner / WARPS != rank) return;
+        // its tokens, some neighbouring ones a thread
         const int begin = owner % WARPS * part, end = min(begin + part, n);
-        const int each = cdiv(part, THREADS), e0 = begin + tid * each;
+        const int per = cdiv(part, THREADS), e0 = begin + tid * per;
+        auto at = [&](int e) { return __fadd_rn(to_f(from[e]), 0.0f); };
         u64 mine = 0;
-        for (int e = e0; e < e0 + each && e < end; e++) {
-            const float v = vals[e];
-            if (v >= vcut && full_key(v, e) >= cut) mine += weights.mass(v);
+        for (int e = e0; e < e0 + per && e < end; e++) {
+            const float v = at(e);
+            if (kept(v, e, vcut, cut)) mine += weights.mass(v);
         }
         u64 upto = warp_scan(mine);
         if (lane == 31) sh.warp_mass[warp] = upto;
@@ -357,128 +502,143 @@ struct Chooser {
         for (int i = 0; i < warp; i++) upto += sh.warp_mass[i];
         upto += before;
         if (upto - mine <= target && target < upto) {
-            u64 at = upto - mine;
-            for (int e = e0; e < e0 + each && e < end; e++) {
-                const float v = vals[e];
-                if (!(v >= vcut) || full_key(v, e) < cut) continue;
+            u64 sum = upto - mine;
+            for (int e = e0; e < e0 + per && e < end; e++) {
+                const float v = at(e);
+                if (!kept(v, e, vcut, cut)) continue;
                 const u64 w = weights.mass(v);
-                if (at + w > target) {
+                if (sum + w > target) {
                     a.token[row] = first + e;
-                    if (a.prob) a.prob[row] = (float)(Weights::scaled(weights.power(v)) / (double)total);
+                    if (a.prob) a.prob[row] = (float)(exp2(weights.power(v) + SCALE) / (double)total);
                     break;
                 }
-                at += w;
+                sum += w;
             }
         }
     }
 };
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) sample_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) unsigned char smem[];
     Shared& sh = *reinterpret_cast<Shared*>(smem);
-    float* vals = reinterpret_cast<float*>(smem + sizeof(Shared));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cs = a.cs, rank = blockIdx.x % cs;
     const int64_t row = blockIdx.x / cs;
-    const int first = rank * a.seg, n = max(0, min(a.seg, a.V - first));
-    const T* from = static_cast<const T*>(a.logits) + row * a.ld + first;
+    Chooser<T> c = {a, sh};
+    c.first = rank * a.seg, c.n = max(0, min(a.seg, a.V - c.first));
+    c.rank = rank, c.cs = cs, c.tid = tid, c.warp = warp, c.lane = lane;
+    c.part = cdiv(cdiv(c.n, WARPS), 32) * 32;
+    c.from = static_cast<const T*>(a.logits) + row * a.ld + c.first;
+    c.bits = 32 - __clz(a.V - 1 | 1);
+    if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this CTA has started
     grid_dependency_sync();
-    for (int i = tid; i < 2 * BINS; i += THREADS) sh.count[0][i] = 0, sh.mass[0][i] = 0;
-    // the row's part into shared memory; its first maximum (NaN above all) and its least finite value
-    uint32_t most = 0, at = 0xffffffffu, least = 0xffffffffu;
-    auto take = [&](float v, int e) {
-        v = __fadd_rn(v, 0.0f);  // no -0: it is as good as 0
-        vals[e] = v;
-        const uint32_t q = key_of(v);
-        if (q > most) most = q, at = first + e;
-        if (q >= LOWEST && q < least) least = q;
-    };
-    constexpr int K = 16 / sizeof(T);
-    if (a.vec) {
-        int e = tid * K;
-#pragma unroll 4
-        for (; e + K <= n; e += THREADS * K) {
-            const Pack<T, K> p = *reinterpret_cast<const Pack<T, K>*>(from + e);
-#pragma unroll
-            for (int i = 0; i < K; i++) take(to_f(p.v[i]), e + i);
-        }
-        for (int i = n / K * K + tid; i < n; i += THREADS) take(to_f(from[i]), i);
-    } else {
-#pragma unroll 4
-        for (int e = tid; e < n; e += THREADS) take(to_f(from[e]), e);
-    }
-    {
-        const uint32_t m = __reduce_max_sync(0xffffffffu, most);
-        at = __reduce_min_sync(0xffffffffu, most == m ? at : 0xffffffffu);
-        least = __reduce_min_sync(0xffffffffu, least);
-        if (lane == 0) sh.warp_count[warp] = m, sh.warp_low[warp] = least, sh.edge[0] = 0, sh.warp_mass[warp] = at;
-    }
-    if (cs > 1)
-        cg::this_cluster().sync();  // the others have started
-    else
-        __syncthreads();
-    if (warp == 0) {
-        most = lane < WARPS ? sh.warp_count[lane] : 0;
-        at = lane < WARPS ? (uint32_t)sh.warp_mass[lane] : 0xffffffffu;
-        least = lane < WARPS ? sh.warp_low[lane] : 0xffffffffu;
-        const uint32_t m = __reduce_max_sync(0xffffffffu, most);
-        at = __reduce_min_sync(0xffffffffu, most == m ? at : 0xffffffffu);
-        least = __reduce_min_sync(0xffffffffu, least);
-        if (lane < cs) {
-            Row& to = cs > 1 ? *cg::this_cluster().map_shared_rank(&sh.row, lane) : sh.row;
-            to.most[rank] = m, to.at[rank] = at, to.least[rank] = least;
-        }
-    }
-    if (cs > 1)
-        cg::this_cluster().sync();
-    else
-        __syncthreads();
-    most = 0, at = 0xffffffffu, least = 0xffffffffu;
-    for (int i = 0; i < cs; i++) {
-        const uint32_t m = sh.row.most[i];
-        if (m > most) most = m, at = sh.row.at[i];
-        if (sh.row.least[i] < least) least = sh.row.least[i];
-    }
     const float temperature = a.temperature ? a.temperature[row] : a.temperature1;
+    const int k = a.top_k ? a.top_k[row] : a.top_k1;
+    const float p = a.top_p ? a.top_p[row] : a.top_p1, min_p = a.min_p ? a.min_p[row] : a.min_p1;
+    const bool greedy = !(temperature > 0.0f), by_k = k > 0 && k < a.V, by_p = p < 1.0f, by_m = min_p > 0.0f;
+    if (tid == 0) sh.listed = 0;
+    float top = -__int_as_float(0x7f800000);
+    c.each<4>([&](float v, int) { top = max_nan(top, v); });
+    {
+        const uint32_t q = key_of(top), m = __reduce_max_sync(0xffffffffu, q);
+        if (cs > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
+        if (lane < cs) c.of(lane).most[rank][warp] = m;
+        if (by_k || by_p) {
+            uint32_t g = q;
+            for (int i = 1; i < cs; i <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, i));
+            // cs neighbouring threads are a group, and each tells one CTA
+            c.of(lane % cs).maxima[(rank * THREADS + tid) / cs] = g;
+        }
+    }
+    c.sync();
+    uint32_t most = 0;
+    for (int i = lane; i < cs * WARPS; i += 32) most = max(most, (&sh.most[0][0])[i]);
+    most = __reduce_max_sync(0xffffffffu, most);
     // greedy rows, and those whose maximum leaves no distribution: infinite, NaN, or nothing but -infinity
-    if (!(temperature > 0.0f) || most >= INF || most < LOWEST) {
-        if (rank == 0 && tid == 0) {
+    if (greedy || most >= INF || most < LOWEST) {
+        uint32_t at = 0xffffffffu;
+        c.each<1>([&](float v, int e) {
+            if (key_of(v) == most) at = min(at, (uint32_t)(c.first + e));
+        });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) c.of(0).at[rank][warp] = at;
+        c.sync();
+        if (rank || warp) return;
+        at = 0xffffffffu;
+        for (int i = lane; i < cs * WARPS; i += 32) at = min(at, (&sh.at[0][0])[i]);
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) {
             a.token[row] = at;
             if (a.prob) a.prob[row] = 1.0f;
         }
         return;
     }
-    const int k = a.top_k ? a.top_k[row] : a.top_k1;
-    const float p = a.top_p ? a.top_p[row] : a.top_p1, min_p = a.min_p ? a.min_p[row] : a.min_p1;
-    Chooser<T> c = {a, sh, vals, n, first, rank, cs, 32 - __clz(a.V - 1 | 1)};
     c.kmax = most;
     c.weights.most = (double)value_of(most);
     c.weights.scale = 1.4426950408889634 / (double)temperature;
-    c.bins.most = value_of(most);
-    // the weights end SCALE powers of 2 below the maximum; the row may end before
-    const float range = fminf(__fsub_rn(c.bins.most, value_of(least)), __fmul_rn((SCALE + 2) * 0.6931472f, temperature));
-    const float scale = __fdiv_rn((float)BINS, range);
-    c.bins.scale = scale < 3.0e38f ? scale : 0.0f;  // rows of one value
-    u64 cut = (u64)LOWEST << c.bits;
-    if (k > 0 && k < a.V) c.template descend<false>(k, 0.0, cut);
-    if (p < 1.0f) c.template descend<true>(0, (double)p, cut);
-    if (min_p > 0.0f) {
-        if (warp == 0) {
-            const double least_power = min_p < 1.0f ? log2((double)min_p) : 0.0;
-            const uint32_t q = first_key(LOWEST - 1, most, [&](uint32_t q) { return c.weights.power(value_of(q)) >= least_power; });
-            if (lane == 0) sh.floor = (u64)q << c.bits;
+    const double least_power = !by_m ? -1e300 : min_p < 1.0f ? log2((double)min_p) : 0.0;
+    u64 total = 0;
+    if (by_p && !by_k) {  // top-p of all tokens
+        u64 sum = 0;
+        c.each<1>([&](float v, int) { sum += c.weights.mass(v); });
+        total = c.exchange_sums(sum);
+    }
+    // a bound that all kept tokens reach
+    bool bounded = (by_m && !(by_k && by_p)) || (a.V <= LIST && (by_k || by_p || by_m));
+    float bound = -3.402823466e38f;
+    if (by_m && !(by_k && by_p))  // the power falls by 1e-9 of itself below the least: rounded down, all that reach it are above
+        bound = fmaxf(bound, __double2float_rd(c.weights.most + least_power * (1.0 + 1e-9) / c.weights.scale));
+    if (a.V > LIST && (by_k ? k <= THREADS : by_p)) {
+        const uint32_t q = c.sorted(sh.maxima[tid], THREADS);
+        if (tid == 0) sh.bound = 0;
+        __syncthreads();
+        if (by_k) {
+            if (tid == k - 1) sh.bound = q;
+        } else {
+            const u64 w = q >= LOWEST ? c.weights.mass(value_of(q)) : 0;
+            u64 all;
+            const u64 before = c.block_before(w, all), want = part_of(total, (double)p);
+            if (before < want && want <= before + w) sh.bound = q;
         }
         __syncthreads();
-        if (sh.floor > cut) cut = sh.floor;
+        if (sh.bound >= LOWEST) bounded = true, bound = fmaxf(bound, value_of(sh.bound));
+    }
+    if (bounded) {
+        const int m = c.list(bound);
+        if (m >= 0) {
+            if (rank == 0) c.choose_listed(m, by_k, k, by_p, (double)p, total, least_power, a.u[row], row);
+            return;
+        }
+    }
+    u64 cut = (u64)LOWEST << c.bits;
+    if (by_k || by_p) {
+        // the weights end SCALE powers of 2 below the maximum
+        const float scale = __fdiv_rn((float)BINS, __fmul_rn((SCALE + 2) * 0.6931472f, temperature));
+        c.bins.most = value_of(most);
+        c.bins.scale = scale < 3.0e38f ? scale : 0.0f;
+        c.clear(0);
+        c.clear(1);
+        __syncthreads();
+        if (by_k) c.template descend<false>(k, 0.0, cut);
+        if (by_p) c.template descend<true>(0, (double)p, cut);
+    }
+    if (by_m) {
+        __syncthreads();
+        if (warp == 0) {
+            const uint32_t q = first_key(LOWEST - 1, most, [&](uint32_t q) { return c.weights.power(value_of(q)) >= least_power; });
+            if (lane == 0) sh.bound = q;
+        }
+        __syncthreads();
+        if (((u64)sh.bound << c.bits) > cut) cut = (u64)sh.bound << c.bits;
     }
     c.choose(a.u[row], cut, row);
 }
 
-// CTAs of a row: as many as its shared memory needs, and more where the rows leave SMs idle, down to 4096 tokens a CTA.
+// CTAs of a row: doubled where rows leave SMs idle, down to 4096 tokens a CTA.
 static inline int cluster_of(int rows, int V) {
     int cs = 1;
-    while (cs < MAX_CLUSTER && ((int64_t)cs * MAX_SEG < V || ((int64_t)rows * cs * 2 <= 148 * 2 && V > cs * 4096))) cs *= 2;
+    while (cs < MAX_CLUSTER && (V > cs * MAX_SEG || ((int64_t)rows * cs * 2 <= 148 * 4 && V > cs * 4096))) cs *= 2;
     return cs;
 }
 
@@ -490,25 +650,22 @@ extern "C" int mi_sample_rows(const void* logits, int64_t ld, const float* u, co
                               float top_p1, float min_p1, int64_t* token, float* prob, int rows, int V, int dtype,
                               void* stream) {
     if (!logits || !u || !token || rows < 0 || V <= 0 || ld < 0) return MI_ERR_INVALID;
-    if (V > mi::sample::MAX_CLUSTER * mi::sample::MAX_SEG) return MI_ERR_UNSUPPORTED;
-    if (rows > 1 << 27) return MI_ERR_UNSUPPORTED;
+    if (V > mi::sample::MAX_V || rows > 1 << 27) return MI_ERR_UNSUPPORTED;
     mi::sample::Args a = {};
     a.logits = logits, a.ld = ld, a.u = u, a.temperature = temperature, a.top_k = top_k, a.top_p = top_p, a.min_p = min_p;
     a.temperature1 = temperature1, a.top_k1 = top_k1, a.top_p1 = top_p1, a.min_p1 = min_p1;
     a.token = token, a.prob = prob, a.V = V;
     a.cs = mi::sample::cluster_of(rows, V);
     a.seg = mi::cdiv(mi::cdiv(V, a.cs), 8) * 8;
-    const size_t smem = sizeof(mi::sample::Shared) + sizeof(float) * a.seg;
     MI_DISPATCH_DTYPE(dtype, T, {
-        a.vec = mi::aligned16(logits) && ld % (16 / sizeof(T)) == 0;
         if (rows == 0) return MI_OK;
         static std::atomic<uint64_t> allowed{0};
         auto kernel = mi::sample::sample_kernel<T>;
-        if (!mi::allow_smem(kernel, sizeof(mi::sample::Shared) + sizeof(float) * mi::sample::MAX_SEG, allowed)) return MI_ERR_CUDA;
+        if (!mi::allow_smem(kernel, sizeof(mi::sample::Shared), allowed)) return MI_ERR_CUDA;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(rows * a.cs);
         cfg.blockDim = dim3(mi::sample::THREADS);
-        cfg.dynamicSmemBytes = smem;
+        cfg.dynamicSmemBytes = sizeof(mi::sample::Shared);
         cfg.stream = (cudaStream_t)stream;
         cudaLaunchAttribute attr[2];
         int m = 0;

@@ -391,7 +391,7 @@ def kernels(cuda_dev):
     return kernels
 
 
-# masses are whole numbers of 2^-44 from powers right to 2^-42: sums of up to 2^17 of them are off by less than 2^-30 of
+# masses are whole numbers of 2^-44 from powers right to 2^-37: sums of up to 2^17 of them are off by less than 2^-30 of
 # the total, and a border that lies nearer than that to the number asked for may be taken from either side
 NEAR = 2.0 ** -30
 
