@@ -37,7 +37,8 @@ namespace sample {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = THREADS, MAX_CLUSTER = 8, MAX_V = 262144, MAX_SEG = 131072;
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = THREADS, FINE = 4096, MAX_CLUSTER = 8,
+              MAX_V = 262144, MAX_SEG = 131072;
 constexpr int SCALE = 44;                      // weights are whole numbers of 2^-44
 constexpr uint32_t LOWEST = 0x00800000u;       // key of -FLT_MAX
 constexpr uint32_t INF = 0xff800000u;          // key of +inf; NaN above it
@@ -67,39 +68,53 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // What the row's weights depend on.
+constexpr int ROOTS = 32;
 struct Weights {
-    double most, scale;  // log2(e) / temperature
-    __device__ __forceinline__ double power(float v) const { return ((double)v - most) * scale; }
-    // 2^x in units of 2^-SCALE, rounded to a whole one; 0 where less than half of one is left.  x = n + f with
-    // |f| <= 1/2; the power series of 2^f, ended behind (f ln 2)^9 / 9!, leaves 7e-12.
-    // Adding 1.5 2^52 rounds to a whole number, which the sum's low bits hold.
-    __device__ __forceinline__ static u64 mass(double x) {
-        constexpr double ROUND = 6755399441055744.0, L = 0.693147180559945309417;
-        constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4, C5 = C4 * L / 5, C6 = C5 * L / 6, C7 = C6 * L / 7,
-                         C8 = C7 * L / 8, C9 = C8 * L / 9;
-        if (!(x > -(SCALE + 1))) return 0;
-        const double r = __dadd_rn(x, ROUND), f = __dsub_rn(x, __dsub_rn(r, ROUND));
-        double p = __fma_rn(C9, f, C8);
-        p = __fma_rn(p, f, C7);
-        p = __fma_rn(p, f, C6);
-        p = __fma_rn(p, f, C5);
-        p = __fma_rn(p, f, C4);
-        p = __fma_rn(p, f, C3);
+    double most, scale;   // ROOTS log2(e) / temperature
+    const double* roots;  // 2^(i / ROOTS + SCALE), in shared memory
+    float end;            // there are no weights below it
+    __device__ __forceinline__ Weights() {}
+    __device__ __forceinline__ Weights(float m, float temperature, const double* r)
+        : most(m), scale(ROOTS * 1.4426950408889634 / (double)temperature), roots(r) {
+        // 2^-(SCALE + 1) is half a unit; in front of -infinity even if the weights do not end
+        end = fmaxf(-3.402823466e38f, __double2float_rd(most - (SCALE + 1) * ROOTS / scale));
+    }
+    __device__ __forceinline__ double power(float v) const { return ((double)v - most) * scale; }  // of the ROOTS-th root of 2
+    // 2^(y / ROOTS) in units of 2^-SCALE, rounded to a whole one.  y = n + f with |f| <= 1/2: a root, a shift of the
+    // exponent, and the power series of 2^(f / ROOTS) up to the fourth power, which leaves 1.3e-12.  Adding 1.5 2^52
+    // rounds to a whole number, which the sum's low bits hold.
+    __device__ __forceinline__ u64 mass(float v) const {
+        constexpr double ROUND = 6755399441055744.0, L = 0.693147180559945309417 / ROOTS;
+        constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4;
+        if (!(v >= end)) return 0;
+        const double y = power(v), r = __dadd_rn(y, ROUND), f = __dsub_rn(y, __dsub_rn(r, ROUND));
+        double p = __fma_rn(C4, f, C3);
         p = __fma_rn(p, f, C2);
         p = __fma_rn(p, f, L);
         p = __fma_rn(p, f, 1.0);
-        p = __fma_rn(p, __hiloint2double((1023 + SCALE + __double2loint(r)) << 20, 0), ROUND);
+        const int n = __double2loint(r);
+        const double root = roots[n & (ROOTS - 1)];
+        p = __fma_rn(p, __hiloint2double(__double2hiint(root) + ((n >> 5) << 20), __double2loint(root)), ROUND);
         return (u64)(__double_as_longlong(p) - __double_as_longlong(ROUND));
     }
-    __device__ __forceinline__ u64 mass(float v) const { return mass(power(v)); }
+    __device__ __forceinline__ float share(float v, u64 total) const {
+        return (float)(exp2(power(v) * (1.0 / ROOTS) + SCALE) / (double)total);
+    }
 };
+static_assert(ROOTS == 32, "the shift of n");
 
 // Bins of equal width downwards from the maximum; falls monotonically as v rises.
+template <int N>
 struct Bins {
     float most, scale;
+    // over the least of `range` and what the weights reach (they end SCALE powers of 2 below the maximum)
+    __device__ __forceinline__ Bins(float most, float temperature, float range) : most(most) {
+        scale = __fdiv_rn((float)N, fminf(range, __fmul_rn((SCALE + 2) * 0.6931472f, temperature)));
+        if (!(scale < 3.0e38f)) scale = 0.0f;  // a row of one value
+    }
     __device__ __forceinline__ int operator()(float v) const {
         const float at = __fmul_rn(__fsub_rn(most, v), scale);
-        return at < (float)(BINS - 1) ? (int)at : BINS - 1;
+        return at < (float)(N - 1) ? (int)at : N - 1;
     }
 };
 
@@ -109,19 +124,26 @@ struct Entry {
 struct Shared {
     // what the CTAs of a row tell one another
     uint32_t most[MAX_CLUSTER][WARPS], at[MAX_CLUSTER][WARPS], listed_by[MAX_CLUSTER];
-    u64 sums[MAX_CLUSTER][WARPS];
+    u64 sums[MAX_CLUSTER][WARPS], above[MAX_CLUSTER][WARPS];
     uint32_t maxima[THREADS];
     Entry all[LIST];
     // this CTA's own
     Entry own[LIST];
     u64 swap[2][THREADS];
-    uint32_t count[2][BINS], limb[2][3][BINS];  // limbs of 15 bits, which MAX_SEG tokens do not overflow
+    union {
+        struct {
+            uint32_t count[2][BINS], limb[2][3][BINS];  // limbs of 15 bits, which MAX_SEG tokens do not overflow
+        };
+        uint32_t fine[FINE];
+    };
+    double roots[ROOTS];
+    u64 warp_low[WARPS];
     u64 warp_mass[WARPS];
     uint32_t warp_count[WARPS];
     uint32_t listed, bound;
     // a border's bin: what lies above it, what it holds
     u64 above_mass, in_mass, target, cut;
-    uint32_t above_count, in_count, bin, edge[2];
+    uint32_t above_count, in_count, bin, edge[2], upto[2];
 };
 
 // The smallest key in (lo, hi] for which pred holds; it holds for hi, and from some key on.  By a whole warp.
@@ -178,7 +200,7 @@ struct Chooser {
     int tid, warp, lane;
     int bits;                 // of an index
     Weights weights;
-    Bins bins;
+    float temperature;
     uint32_t kmax;
     int level = 0;            // of the histograms, which alternate
 
@@ -199,25 +221,33 @@ struct Chooser {
     }
     __device__ __forceinline__ Shared& of(int r) { return cs > 1 ? *cg::this_cluster().map_shared_rank(&sh, r) : sh; }
 
-    // f(v, e) for this warp's tokens, by blocks of 16 bytes, U of them a lane in flight; beside the tokens a block may
-    // hold others' places, for which v is -infinity.
+    // f(v, e) for this warp's tokens, by blocks of 16 bytes, U of them a lane at a time and the next U on their way;
+    // beside the tokens a block may hold others' places, for which v is -infinity.
     template <int U, typename F>
     __device__ __forceinline__ void each(F f) const {
         const int begin = warp * part, end = min(begin + part, n);
         const int off = (int)((reinterpret_cast<uintptr_t>(from + begin) & 15) / sizeof(T));
-        for (int e0 = begin - off + lane * K; e0 < end; e0 += U * 32 * K) {
-            Pack<T, K> v[U];
+        constexpr int STEP = U * 32 * K;
+        Pack<T, K> v[U], next[U];
+        auto load = [&](int e0) {
 #pragma unroll
             for (int j = 0; j < U; j++) {
                 const int e = e0 + j * 32 * K;
                 if (e >= begin && e + K <= end) {
-                    v[j] = *reinterpret_cast<const Pack<T, K>*>(from + e);
+                    next[j] = *reinterpret_cast<const Pack<T, K>*>(from + e);
                 } else {
 #pragma unroll
                     for (int i = 0; i < K; i++)
-                        v[j].v[i] = e + i >= begin && e + i < end ? from[e + i] : from_f<T>(-__int_as_float(0x7f800000));
+                        next[j].v[i] = e + i >= begin && e + i < end ? from[e + i] : from_f<T>(-__int_as_float(0x7f800000));
                 }
             }
+        };
+        int e0 = begin - off + lane * K;
+        if (e0 < end) load(e0);
+        for (; e0 < end; e0 += STEP) {
+#pragma unroll
+            for (int j = 0; j < U; j++) v[j] = next[j];
+            if (e0 + STEP < end) load(e0 + STEP);
 #pragma unroll
             for (int j = 0; j < U; j++)
 #pragma unroll
@@ -275,14 +305,12 @@ struct Chooser {
         return v;
     }
 
-    // Lists the row's tokens from `bound` on in CTA 0's sh.all.  Their number, or -1 if they are too many.
-    __device__ __forceinline__ int list(float bound) {
-        each<2>([&](float v, int e) {
-            if (v >= bound) {
-                const uint32_t i = atomicAdd(&sh.listed, 1u);
-                if (i < LIST) sh.own[i].key = full_key(v, e);
-            }
-        });
+    __device__ __forceinline__ void list_one(float v, int e) {
+        const uint32_t i = atomicAdd(&sh.listed, 1u);
+        if (i < LIST) sh.own[i].key = full_key(v, e);
+    }
+    // Brings the CTAs' listed tokens to CTA 0's sh.all.  Their number, or -1 if they are too many.
+    __device__ __forceinline__ int gather() {
         __syncthreads();
         const int mine = min(sh.listed, (uint32_t)LIST + 1);
         if (tid < cs) of(tid).listed_by[rank] = mine;
@@ -297,12 +325,63 @@ struct Chooser {
         sync();
         return all;
     }
+    __device__ __forceinline__ int size_of(int m) const {
+        int size = 32;
+        while (size < m) size *= 2;
+        return size;
+    }
+
+    __device__ __forceinline__ int part_of_cta(int r) const {
+        return cdiv(cdiv(max(0, min(a.seg, a.V - r * a.seg)), WARPS), 32) * 32;
+    }
+
+    // The choice, from the sums of the kept masses by the row's warps, in the order of the indices.  By the CTA whose
+    // token it is, or by this one.
+    template <typename F>
+    __device__ __forceinline__ void finish(const u64* sums, float u, int64_t row, F kept, bool here) {
+        // every warp adds up all of them, some neighbouring ones a lane
+        const int all = cs * WARPS, some = cdiv(all, 32);
+        u64 own = 0;
+        for (int i = lane * some; i < (lane + 1) * some && i < all; i++) own += sums[i];
+        const u64 to_lane = warp_scan(own), total = __shfl_sync(0xffffffffu, to_lane, 31);
+        const u64 target = target_of(total, u);
+        const int in = __ffs(__ballot_sync(0xffffffffu, to_lane > target)) - 1;
+        u64 before = __shfl_sync(0xffffffffu, to_lane - own, in);
+        int owner = in * some;
+        for (; before + sums[owner] <= target; owner++) before += sums[owner];
+        const int r = owner / WARPS, part = part_of_cta(r);
+        if (!here && r != rank) return;
+        // its tokens, some neighbouring ones a thread; e counts from this CTA's first on
+        const int begin = (r - rank) * a.seg + owner % WARPS * part;
+        const int end = min(begin + part, min((r + 1) * a.seg, a.V) - first);
+        const int per = cdiv(part, THREADS), e0 = begin + tid * per;
+        auto at = [&](int e) { return __fadd_rn(to_f(from[e]), 0.0f); };
+        u64 mine = 0;
+        for (int e = e0; e < e0 + per && e < end; e++) {
+            const float v = at(e);
+            if (kept(v, e)) mine += weights.mass(v);
+        }
+        u64 block;
+        u64 sum = before + block_before(mine, block);
+        if (sum <= target && target < sum + mine) {
+            for (int e = e0; e < e0 + per && e < end; e++) {
+                const float v = at(e);
+                if (!kept(v, e)) continue;
+                const u64 w = weights.mass(v);
+                if (sum + w > target) {
+                    a.token[row] = first + e;
+                    if (a.prob) a.prob[row] = weights.share(v, total);
+                    break;
+                }
+                sum += w;
+            }
+        }
+    }
 
     // The filters and the choice on the listed tokens, which hold all that are kept.  By CTA 0.
     __device__ __forceinline__ void choose_listed(int m, bool by_k, int k, bool by_p, double p, u64 total, double least_power,
                                                   float u, int64_t row) {
-        int size = 32;
-        while (size < m) size *= 2;
+        const int size = size_of(m);
         u64 q = sorted(tid < m ? sh.all[tid].key : 0, size);
         const bool some = tid < m;
         const float v = value(q);
@@ -322,8 +401,141 @@ struct Chooser {
         const u64 before = block_before(mass, total), target = target_of(total, u);
         if (mass && before <= target && target < before + mass) {
             a.token[row] = 0xffffffffu - (uint32_t)(q >> 32);
-            if (a.prob) a.prob[row] = (float)(exp2(weights.power(chosen) + SCALE) / (double)total);
+            if (a.prob) a.prob[row] = weights.share(chosen, total);
         }
+    }
+
+    // The border of top-k, or of top-p of all tokens, by counts in fine bins, and the choice.  The counts give the bin of the
+    // k-th token, or bound the masses up to each bin from both sides, and so the bins in which top-p's border can lie.
+    // One pass over the weights then adds up what lies above those bins, by warps, and lists the tokens in them (or all
+    // down to them, if they are few).  CTA 0 finds the border among these and has the sums of what is kept.  `least`: the
+    // row's least finite value; `floor`: the least that min-p keeps.  False: too many tokens lie in those bins.
+    __device__ __forceinline__ bool choose_by_bins(bool by_k, int k, double p, float least, float floor, double least_power, float u,
+                                                   int64_t row) {
+        const Bins<FINE> bins(value_of(kmax), temperature, __fsub_rn(value_of(kmax), least));
+        for (int i = tid; i < FINE; i += THREADS) sh.fine[i] = 0;
+        __syncthreads();
+        // what has no weight is never chosen, but counts for top-k
+        const float end = by_k ? -3.402823466e38f : weights.end;
+        each<2>([&](float v, int) {
+            if (v >= end) atomicAdd(&sh.fine[bins(v)], 1u);
+        });
+        sync();
+        if (cs > 1) {  // each CTA adds up a part of the bins for all
+            for (int i = rank * (FINE / cs) + tid; i < (rank + 1) * (FINE / cs); i += THREADS) {
+                uint32_t all = 0;
+                for (int r = 0; r < cs; r++) all += of(r).fine[i];
+                for (int r = 0; r < cs; r++) of(r).fine[i] = all;
+            }
+            sync();
+        }
+        constexpr int PER = FINE / THREADS;
+        uint32_t c[PER], counts = 0;
+#pragma unroll
+        for (int i = 0; i < PER; i++) c[i] = sh.fine[tid * PER + i];
+        // a bin's weights lie between those of its edges, in units of 2^-30; 3e-5 for their rounding and that of
+        // (most - v) * scale.  Whole numbers again, so that every thread of every CTA has the same sums.
+        // A single bin and the last one have no lower edge.
+        u64 low[PER], high[PER], lows = 0, highs = 0;
+        const bool one = !(bins.scale > 0.0f);
+        const float width = one ? 0.0f : (float)(weights.scale * (1.0 / ROOTS) / (double)bins.scale);
+        float edge = exp2f(-(float)(tid * PER) * width) * 1073741824.0f;
+        const float ratio = exp2f(-width);
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const float next = one || tid * PER + i == FINE - 1 ? 0.0f : edge * ratio;
+            high[i] = (u64)c[i] * ((uint32_t)(edge * (1 + 3e-5f)) + 1);
+            low[i] = (u64)c[i] * (uint32_t)(next * (1 - 3e-5f));
+            edge = next;
+            lows += low[i], highs += high[i], counts += c[i];
+        }
+        u64 lup = warp_scan(lows), hup = warp_scan(highs);
+        uint32_t cup = warp_scan(counts);
+        if (lane == 31) sh.warp_low[warp] = lup, sh.warp_mass[warp] = hup, sh.warp_count[warp] = cup;
+        __syncthreads();
+        u64 lall = 0, hall = 0;
+        for (int i = 0; i < WARPS; i++) {
+            if (i == warp) lup += lall, hup += hall;
+            if (i < warp) cup += sh.warp_count[i];
+            lall += sh.warp_low[i], hall += sh.warp_mass[i];
+        }
+        lup -= lows, hup -= highs, cup -= counts;
+        if (by_k) {
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (cup < k && (k <= cup + c[i] || tid * PER + i == FINE - 1))
+                    sh.edge[0] = sh.edge[1] = tid * PER + i, sh.upto[0] = cup, sh.upto[1] = cup + c[i];
+                cup += c[i];
+            }
+        } else {
+            // the first bin whose upper sum reaches the least that is wanted, and the first whose lower sum reaches the most
+            const u64 want_low = (u64)fmax(p * (double)lall * (1 - 1e-9), 0.0);
+            const u64 want_high = (u64)(fmax(p, 0.0) * (double)hall * (1 + 1e-9)) + 1;
+            bool below_low = tid == 0 || hup < want_low, below_high = tid == 0 || lup < want_high;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                hup += high[i], lup += low[i];
+                if (below_low && hup >= want_low) sh.edge[0] = tid * PER + i, sh.upto[0] = cup;
+                cup += c[i];
+                if (below_high && (lup >= want_high || tid * PER + i == FINE - 1)) sh.edge[1] = tid * PER + i, sh.upto[1] = cup;
+                below_low = hup < want_low, below_high = lup < want_high;
+            }
+        }
+        __syncthreads();
+        const int b0 = sh.edge[0], b1 = sh.edge[1], counted = sh.upto[0];
+        const bool whole = sh.upto[1] <= LIST;
+        if (!whole && sh.upto[1] - counted > LIST) return false;
+        u64 sum = 0, above = 0;
+        each<1>([&](float v, int e) {
+            if (!(v >= end)) return;
+            const int b = bins(v);
+            if (by_k && b > b1) return;
+            const u64 w = weights.mass(v);
+            sum += w;
+            if (b < b0 && v >= floor) above += w;
+            if (b <= b1 && (whole || b >= b0)) list_one(v, e);
+        });
+        above = warp_sum(above);
+        if (lane == 0) of(0).above[rank][warp] = above;
+        const u64 total = exchange_sums(sum);
+        const int m = gather();
+        if (m < 0) return false;
+        if (rank) return true;
+        if (whole) {
+            choose_listed(m, by_k, k, !by_k, p, total, least_power, u, row);
+            return true;
+        }
+        u64* sums = &sh.above[0][0];
+        u64 over = 0;
+        for (int i = lane; i < cs * WARPS; i += 32) over += sums[i];
+        over = warp_sum(over);
+        const u64 q = sorted(tid < m ? sh.all[tid].key : 0, size_of(m));
+        const float v = value(q);
+        const u64 w = tid < m ? weights.mass(v) : 0;
+        u64 all;
+        const u64 before = block_before(w, all);  // behind its barriers `sums` is read by all
+        bool keep = tid < m && v >= floor && weights.power(v) >= least_power;
+        // min-p's floor only lowers `over` where the border lies below it, and then nothing listed is kept
+        keep = keep && (by_k ? tid < k - counted : over + before < part_of(total, p));
+        if (tid == 0) sh.cut = ~0ull;
+        if (tid < cs * WARPS)
+            for (int j = 0; j < 3; j++) sh.limb[0][j][tid] = 0;
+        __syncthreads();
+        if (keep) {
+            const int at = index(q), r = at / a.seg, part = part_of_cta(r);
+#pragma unroll
+            for (int j = 0; j < 3; j++)
+                atomicAdd(&sh.limb[0][j][r * WARPS + (at - r * a.seg) / part], (uint32_t)(w >> (15 * j)) & 0x7fffu);
+        }
+        const uint32_t some = __ballot_sync(0xffffffffu, keep);
+        if (some && lane == 31 - __clz(some)) atomicMin(&sh.cut, q);  // the warp's last in the order
+        __syncthreads();
+        if (tid < cs * WARPS)
+            for (int j = 0; j < 3; j++) sums[tid] += (u64)sh.limb[0][j][tid] << (15 * j);
+        const u64 cut = sh.cut;
+        __syncthreads();
+        finish(sums, u, row, [&](float v, int e) { return v >= floor && (bins(v) < b0 || full_key(v, e) >= cut); }, true);
+        return true;
     }
 
     // ----- by histograms -----
@@ -393,6 +605,7 @@ struct Chooser {
     template <bool MASS>
     __device__ __forceinline__ void descend(uint32_t k, double share, u64& cut) {
         const float vcut = value(cut);
+        const Bins<BINS> bins(value_of(kmax), temperature, __int_as_float(0x7f800000));
         each<1>([&](float v, int e) {
             if (kept(v, e, vcut, cut)) add<MASS>(bins(v), v);
         });
@@ -475,46 +688,7 @@ struct Chooser {
         sum = warp_sum(sum);
         if (lane < cs) of(lane).sums[rank][warp] = sum;
         sync();
-        // every warp adds up all of them, some neighbouring ones a lane
-        const u64* sums = &sh.sums[0][0];
-        const int all = cs * WARPS, some = cdiv(all, 32);
-        u64 own = 0;
-        for (int i = lane * some; i < (lane + 1) * some && i < all; i++) own += sums[i];
-        const u64 to_lane = warp_scan(own), total = __shfl_sync(0xffffffffu, to_lane, 31);
-        const u64 target = target_of(total, u);
-        const int in = __ffs(__ballot_sync(0xffffffffu, to_lane > target)) - 1;
-        u64 before = __shfl_sync(0xffffffffu, to_lane - own, in);
-        int owner = in * some;
-        for (; before + sums[owner] <= target; owner++) before += sums[owner];
-        if (owner / WARPS != rank) return;
-        // its tokens, some neighbouring ones a thread
-        const int begin = owner % WARPS * part, end = min(begin + part, n);
-        const int per = cdiv(part, THREADS), e0 = begin + tid * per;
-        auto at = [&](int e) { return __fadd_rn(to_f(from[e]), 0.0f); };
-        u64 mine = 0;
-        for (int e = e0; e < e0 + per && e < end; e++) {
-            const float v = at(e);
-            if (kept(v, e, vcut, cut)) mine += weights.mass(v);
-        }
-        u64 upto = warp_scan(mine);
-        if (lane == 31) sh.warp_mass[warp] = upto;
-        __syncthreads();
-        for (int i = 0; i < warp; i++) upto += sh.warp_mass[i];
-        upto += before;
-        if (upto - mine <= target && target < upto) {
-            u64 sum = upto - mine;
-            for (int e = e0; e < e0 + per && e < end; e++) {
-                const float v = at(e);
-                if (!kept(v, e, vcut, cut)) continue;
-                const u64 w = weights.mass(v);
-                if (sum + w > target) {
-                    a.token[row] = first + e;
-                    if (a.prob) a.prob[row] = (float)(exp2(weights.power(v) + SCALE) / (double)total);
-                    break;
-                }
-                sum += w;
-            }
-        }
+        finish(&sh.sums[0][0], u, row, [&](float v, int e) { return kept(v, e, vcut, cut); }, false);
     }
 };
 
@@ -528,9 +702,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     Chooser<T> c = {a, sh};
     c.first = rank * a.seg, c.n = max(0, min(a.seg, a.V - c.first));
     c.rank = rank, c.cs = cs, c.tid = tid, c.warp = warp, c.lane = lane;
-    c.part = cdiv(cdiv(c.n, WARPS), 32) * 32;
     c.from = static_cast<const T*>(a.logits) + row * a.ld + c.first;
     c.bits = 32 - __clz(a.V - 1 | 1);
+    c.part = c.part_of_cta(rank);
     if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");  // this CTA has started
     grid_dependency_sync();
     const float temperature = a.temperature ? a.temperature[row] : a.temperature1;
@@ -538,13 +712,19 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     const float p = a.top_p ? a.top_p[row] : a.top_p1, min_p = a.min_p ? a.min_p[row] : a.min_p1;
     const bool greedy = !(temperature > 0.0f), by_k = k > 0 && k < a.V, by_p = p < 1.0f, by_m = min_p > 0.0f;
     if (tid == 0) sh.listed = 0;
-    float top = -__int_as_float(0x7f800000);
-    c.each<4>([&](float v, int) { top = max_nan(top, v); });
+    if (tid < ROOTS) sh.roots[tid] = exp2((double)tid / ROOTS + SCALE);
+    const bool wide = a.V > LIST && by_k != by_p;  // bins down to the least value are likely
+    float top = -__int_as_float(0x7f800000), low = __int_as_float(0x7f800000);
+    c.each<2>([&](float v, int) {
+        top = max_nan(top, v);
+        if (wide && v > -__int_as_float(0x7f800000)) low = fminf(low, v);
+    });
     {
         const uint32_t q = key_of(top), m = __reduce_max_sync(0xffffffffu, q);
         if (cs > 1) asm volatile("barrier.cluster.wait;" ::: "memory");
-        if (lane < cs) c.of(lane).most[rank][warp] = m;
-        if (by_k || by_p) {
+        const uint32_t l = __reduce_min_sync(0xffffffffu, key_of(low));
+        if (lane < cs) c.of(lane).most[rank][warp] = m, c.of(lane).at[rank][warp] = l;
+        if (by_k) {
             uint32_t g = q;
             for (int i = 1; i < cs; i <<= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, i));
             // cs neighbouring threads are a group, and each tells one CTA
@@ -552,9 +732,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         }
     }
     c.sync();
-    uint32_t most = 0;
-    for (int i = lane; i < cs * WARPS; i += 32) most = max(most, (&sh.most[0][0])[i]);
+    uint32_t most = 0, least = 0xffffffffu;
+    for (int i = lane; i < cs * WARPS; i += 32)
+        most = max(most, (&sh.most[0][0])[i]), least = min(least, (&sh.at[0][0])[i]);
     most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
     // greedy rows, and those whose maximum leaves no distribution: infinite, NaN, or nothing but -infinity
     if (greedy || most >= INF || most < LOWEST) {
         uint32_t at = 0xffffffffu;
@@ -562,6 +744,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
             if (key_of(v) == most) at = min(at, (uint32_t)(c.first + e));
         });
         at = __reduce_min_sync(0xffffffffu, at);
+        c.sync();  // all have read the least values there
         if (lane == 0) c.of(0).at[rank][warp] = at;
         c.sync();
         if (rank || warp) return;
@@ -575,70 +758,66 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         return;
     }
     c.kmax = most;
-    c.weights.most = (double)value_of(most);
-    c.weights.scale = 1.4426950408889634 / (double)temperature;
-    const double least_power = !by_m ? -1e300 : min_p < 1.0f ? log2((double)min_p) : 0.0;
-    u64 total = 0;
-    if (by_p && !by_k) {  // top-p of all tokens
-        u64 sum = 0;
-        c.each<1>([&](float v, int) { sum += c.weights.mass(v); });
-        total = c.exchange_sums(sum);
-    }
-    // a bound that all kept tokens reach
-    bool bounded = (by_m && !(by_k && by_p)) || (a.V <= LIST && (by_k || by_p || by_m));
-    float bound = -3.402823466e38f;
-    if (by_m && !(by_k && by_p))  // the power falls by 1e-9 of itself below the least: rounded down, all that reach it are above
-        bound = fmaxf(bound, __double2float_rd(c.weights.most + least_power * (1.0 + 1e-9) / c.weights.scale));
-    if (a.V > LIST && (by_k ? k <= THREADS : by_p)) {
-        const uint32_t q = c.sorted(sh.maxima[tid], THREADS);
-        if (tid == 0) sh.bound = 0;
-        __syncthreads();
-        if (by_k) {
-            if (tid == k - 1) sh.bound = q;
-        } else {
-            const u64 w = q >= LOWEST ? c.weights.mass(value_of(q)) : 0;
-            u64 all;
-            const u64 before = c.block_before(w, all), want = part_of(total, (double)p);
-            if (before < want && want <= before + w) sh.bound = q;
-        }
-        __syncthreads();
-        if (sh.bound >= LOWEST) bounded = true, bound = fmaxf(bound, value_of(sh.bound));
-    }
-    if (bounded) {
-        const int m = c.list(bound);
-        if (m >= 0) {
-            if (rank == 0) c.choose_listed(m, by_k, k, by_p, (double)p, total, least_power, a.u[row], row);
-            return;
-        }
-    }
-    u64 cut = (u64)LOWEST << c.bits;
-    if (by_k || by_p) {
-        // the weights end SCALE powers of 2 below the maximum
-        const float scale = __fdiv_rn((float)BINS, __fmul_rn((SCALE + 2) * 0.6931472f, temperature));
-        c.bins.most = value_of(most);
-        c.bins.scale = scale < 3.0e38f ? scale : 0.0f;
-        c.clear(0);
-        c.clear(1);
-        __syncthreads();
-        if (by_k) c.template descend<false>(k, 0.0, cut);
-        if (by_p) c.template descend<true>(0, (double)p, cut);
-    }
+    c.temperature = temperature;
+    c.weights = Weights(value_of(most), temperature, sh.roots);
+    // min-p as the power that a token has to reach, and as the least value that does
+    const double least_power = !by_m ? -1e300 : min_p < 1.0f ? ROOTS * log2((double)min_p) : 0.0;
+    float floor = -3.402823466e38f;
     if (by_m) {
-        __syncthreads();
         if (warp == 0) {
             const uint32_t q = first_key(LOWEST - 1, most, [&](uint32_t q) { return c.weights.power(value_of(q)) >= least_power; });
             if (lane == 0) sh.bound = q;
         }
         __syncthreads();
-        if (((u64)sh.bound << c.bits) > cut) cut = (u64)sh.bound << c.bits;
+        floor = value_of(sh.bound);
+        __syncthreads();
     }
+    // a bound that all kept tokens reach
+    bool bounded = (by_m && !(by_k && by_p)) || (a.V <= LIST && (by_k || by_p || by_m));
+    float bound = by_m && !(by_k && by_p) ? floor : -3.402823466e38f;
+    if (a.V > LIST && by_k && k <= THREADS) {
+        const uint32_t q = c.sorted(sh.maxima[tid], THREADS);
+        if (tid == k - 1) sh.bound = q;
+        __syncthreads();
+        if (sh.bound >= LOWEST) bounded = true, bound = fmaxf(bound, value_of(sh.bound));
+    }
+    if (bounded && (by_k || !by_p || a.V <= LIST)) {
+        c.template each<2>([&](float v, int e) {
+            if (v >= bound) c.list_one(v, e);
+        });
+        u64 total = 0;
+        if (by_p && !by_k) {  // of a row as short as a list
+            u64 sum = 0;
+            c.template each<1>([&](float v, int) { sum += c.weights.mass(v); });
+            total = c.exchange_sums(sum);
+        }
+        const int m = c.gather();
+        if (m >= 0) {
+            if (rank == 0) c.choose_listed(m, by_k, k, by_p, (double)p, total, least_power, a.u[row], row);
+            return;
+        }
+        __syncthreads();
+        if (tid == 0) sh.listed = 0;
+    }
+    if (wide && c.choose_by_bins(by_k, k, (double)p, value_of(least), floor, least_power, a.u[row], row)) return;
+    u64 cut = (u64)LOWEST << c.bits;
+    if (by_k || by_p) {
+        c.sync();  // all have read what lies in the histograms' place
+        c.clear(0);
+        c.clear(1);
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+        if (by_k) c.template descend<false>(k, 0.0, cut);
+        if (by_p) c.template descend<true>(0, (double)p, cut);
+    }
+    if (((u64)key_of(floor) << c.bits) > cut) cut = (u64)key_of(floor) << c.bits;
     c.choose(a.u[row], cut, row);
 }
 
 // CTAs of a row: doubled where rows leave SMs idle, down to 4096 tokens a CTA.
 static inline int cluster_of(int rows, int V) {
     int cs = 1;
-    while (cs < MAX_CLUSTER && (V > cs * MAX_SEG || ((int64_t)rows * cs * 2 <= 148 * 4 && V > cs * 4096))) cs *= 2;
+    while (cs < MAX_CLUSTER && (V > cs * MAX_SEG || ((int64_t)rows * cs * 2 <= 148 && V > cs * 4096))) cs *= 2;
     return cs;
 }
 

@@ -450,6 +450,18 @@ def test_sample_rows_with_settings_of_their_own(kernels, cuda_dev, v, dtype):
     check_sample(kernels, cuda_dev, sample_logits(rows, v, seed=v, dtype=dtype), uniform(rows, v), t, k, p, m)
 
 
+@pytest.mark.parametrize("v", [600, 5000, 32768, 100003])
+@pytest.mark.parametrize("spread", [0.01, 0.3, 1.0, 8.0])
+def test_sample_nuclei_of_flat_and_steep_rows(kernels, cuda_dev, v, spread):
+    """Top-p (and large k) that keep a few tokens, some thousands, and nearly all."""
+    logits = torch.cat([spread * torch.randn(4, v, generator=torch.Generator().manual_seed(v)), sample_logits(4, v)])
+    p = [0.05, 0.5, 0.9, 0.999, 0.3, 0.8, 0.99, 0.9999]
+    check_sample(kernels, cuda_dev, logits, uniform(8, v), 1.0, 0, p, 0.0)
+    check_sample(kernels, cuda_dev, logits, uniform(8, v + 1), 0.6, 0, p, [0.0, 0.01, 0.2, 0.0, 1e-4, 0.5, 0.0, 1e-6])
+    check_sample(kernels, cuda_dev, logits, uniform(8, v + 2), 2.0, v // 3, p[::-1], 0.0)
+    check_sample(kernels, cuda_dev, logits.repeat(40, 1), uniform(320, v + 3), 1.0, 0, p * 40, 0.0)
+
+
 @pytest.mark.parametrize("v", [999, 32768, 70000])
 def test_sample_equal_logits(kernels, cuda_dev, v):
     """Ties go to the lower index: rows of one value, of few values, and of values that differ in their last bits."""
