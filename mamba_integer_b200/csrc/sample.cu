@@ -86,8 +86,8 @@ struct Weights {
     __device__ __forceinline__ u64 mass(float v) const {
         constexpr double ROUND = 6755399441055744.0, L = 0.693147180559945309417 / ROOTS;
         constexpr double C2 = L * L / 2, C3 = C2 * L / 3, C4 = C3 * L / 4;
-        if (!(v >= end)) return 0;
-        const double y = power(v), r = __dadd_rn(y, ROUND), f = __dsub_rn(y, __dsub_rn(r, ROUND));
+        const bool some = v >= end;  // no branch: neighbouring tokens' chains run side by side
+        const double y = power(some ? v : end), r = __dadd_rn(y, ROUND), f = __dsub_rn(y, __dsub_rn(r, ROUND));
         double p = __fma_rn(C4, f, C3);
         p = __fma_rn(p, f, C2);
         p = __fma_rn(p, f, L);
@@ -95,7 +95,7 @@ struct Weights {
         const int n = __double2loint(r);
         const double root = roots[n & (ROOTS - 1)];
         p = __fma_rn(p, __hiloint2double(__double2hiint(root) + ((n >> 5) << 20), __double2loint(root)), ROUND);
-        return (u64)(__double_as_longlong(p) - __double_as_longlong(ROUND));
+        return some ? (u64)(__double_as_longlong(p) - __double_as_longlong(ROUND)) : 0;
     }
     __device__ __forceinline__ float share(float v, u64 total) const {
         return (float)(exp2(power(v) * (1.0 / ROOTS) + SCALE) / (double)total);
@@ -221,8 +221,8 @@ struct Chooser {
     }
     __device__ __forceinline__ Shared& of(int r) { return cs > 1 ? *cg::this_cluster().map_shared_rank(&sh, r) : sh; }
 
-    // f(v, e) for this warp's tokens, by blocks of 16 bytes, U of them a lane at a time and the next U on their way;
-    // beside the tokens a block may hold others' places, for which v is -infinity.
+    // f(v, e) for this warp's tokens e .. e + K - 1, by blocks of 16 bytes, U of them a lane at a time and the next U on
+    // their way; beside the tokens a block may hold others' places, for which v is -infinity.
     template <int U, typename F>
     __device__ __forceinline__ void each(F f) const {
         const int begin = warp * part, end = min(begin + part, n);
@@ -249,10 +249,12 @@ struct Chooser {
             for (int j = 0; j < U; j++) v[j] = next[j];
             if (e0 + STEP < end) load(e0 + STEP);
 #pragma unroll
-            for (int j = 0; j < U; j++)
+            for (int j = 0; j < U; j++) {
+                float x[K];
 #pragma unroll
-                for (int i = 0; i < K; i++)  // no -0: it is as good as 0
-                    f(__fadd_rn(to_f(v[j].v[i]), 0.0f), e0 + j * 32 * K + i);
+                for (int i = 0; i < K; i++) x[i] = __fadd_rn(to_f(v[j].v[i]), 0.0f);  // no -0: it is as good as 0
+                f(x, e0 + j * 32 * K);
+            }
         }
     }
 
@@ -417,8 +419,13 @@ struct Chooser {
         __syncthreads();
         // what has no weight is never chosen, but counts for top-k
         const float end = by_k ? -3.402823466e38f : weights.end;
-        each<2>([&](float v, int) {
-            if (v >= end) atomicAdd(&sh.fine[bins(v)], 1u);
+        each<2>([&](const float (&v)[K], int) {
+            int b[K];
+#pragma unroll
+            for (int i = 0; i < K; i++) b[i] = bins(v[i]);
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (v[i] >= end) atomicAdd(&sh.fine[b[i]], 1u);
         });
         sync();
         if (cs > 1) {  // each CTA adds up a part of the bins for all
@@ -486,14 +493,24 @@ struct Chooser {
         const bool whole = sh.upto[1] <= LIST;
         if (!whole && sh.upto[1] - counted > LIST) return false;
         u64 sum = 0, above = 0;
-        each<1>([&](float v, int e) {
-            if (!(v >= end)) return;
-            const int b = bins(v);
-            if (by_k && b > b1) return;
-            const u64 w = weights.mass(v);
-            sum += w;
-            if (b < b0 && v >= floor) above += w;
-            if (b <= b1 && (whole || b >= b0)) list_one(v, e);
+        const int from_bin = whole ? 0 : b0;
+        each<1>([&](const float (&v)[K], int e) {
+            bool any = !by_k;
+            int b[K];
+#pragma unroll
+            for (int i = 0; i < K; i++) b[i] = bins(v[i]), any = any || b[i] <= b1;
+            if (!any) return;  // of top-k only what may be kept has to be weighed
+            u64 w[K];
+#pragma unroll
+            for (int i = 0; i < K; i++) w[i] = weights.mass(v[i]);
+#pragma unroll
+            for (int i = 0; i < K; i++) {
+                sum += w[i];
+                above += b[i] < b0 && v[i] >= floor ? w[i] : 0;
+            }
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (b[i] <= b1 && b[i] >= from_bin && v[i] >= end) list_one(v[i], e + i);
         });
         above = warp_sum(above);
         if (lane == 0) of(0).above[rank][warp] = above;
@@ -606,8 +623,10 @@ struct Chooser {
     __device__ __forceinline__ void descend(uint32_t k, double share, u64& cut) {
         const float vcut = value(cut);
         const Bins<BINS> bins(value_of(kmax), temperature, __int_as_float(0x7f800000));
-        each<1>([&](float v, int e) {
-            if (kept(v, e, vcut, cut)) add<MASS>(bins(v), v);
+        each<1>([&](const float (&v)[K], int e) {
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (kept(v[i], e + i, vcut, cut)) add<MASS>(bins(v[i]), v[i]);
         });
         if (!border<MASS>(k, &share)) return;
         // the keys of the bin
@@ -633,12 +652,15 @@ struct Chooser {
             }
             const float vlo = value(lo), vhi = value(hi);
             if (sh.in_count <= LIST) {
-                each<1>([&](float v, int e) {
-                    if (!(v >= vlo && v <= vhi)) return;
-                    const u64 q = full_key(v, e);
-                    if (q < lo || q > hi) return;
-                    const uint32_t i = atomicAdd(&sh.listed, 1u);
-                    if (i < LIST) sh.own[i] = {q, MASS ? weights.mass(v) : 1ull};
+                each<1>([&](const float (&v)[K], int e) {
+#pragma unroll
+                    for (int j = 0; j < K; j++) {
+                        if (!(v[j] >= vlo && v[j] <= vhi)) continue;
+                        const u64 q = full_key(v[j], e + j);
+                        if (q < lo || q > hi) continue;
+                        const uint32_t i = atomicAdd(&sh.listed, 1u);
+                        if (i < LIST) sh.own[i] = {q, MASS ? weights.mass(v[j]) : 1ull};
+                    }
                 });
                 sync();
                 uint32_t m = 0;
@@ -664,10 +686,13 @@ struct Chooser {
             int shift = 0;
             while (((hi - lo) >> shift) >= BINS) shift++;
             const u64 in_lo = lo, in_hi = hi;
-            each<1>([&](float v, int e) {
-                if (!(v >= vlo && v <= vhi)) return;
-                const u64 q = full_key(v, e);
-                if (q >= in_lo && q <= in_hi) add<MASS>((int)((in_hi - q) >> shift), v);
+            each<1>([&](const float (&v)[K], int e) {
+#pragma unroll
+                for (int i = 0; i < K; i++) {
+                    if (!(v[i] >= vlo && v[i] <= vhi)) continue;
+                    const u64 q = full_key(v[i], e + i);
+                    if (q >= in_lo && q <= in_hi) add<MASS>((int)((in_hi - q) >> shift), v[i]);
+                }
             });
             border<MASS>(left, nullptr);
             hi = in_hi - ((u64)sh.bin << shift);
@@ -682,8 +707,16 @@ struct Chooser {
     __device__ __forceinline__ void choose(float u, u64 cut, int64_t row) {
         const float vcut = value(cut);
         u64 sum = 0;
-        each<1>([&](float v, int e) {
-            if (kept(v, e, vcut, cut)) sum += weights.mass(v);
+        each<1>([&](const float (&v)[K], int e) {
+            bool in[K], any = false;
+#pragma unroll
+            for (int i = 0; i < K; i++) in[i] = kept(v[i], e + i, vcut, cut), any = any || in[i];
+            if (!any) return;
+            u64 w[K];
+#pragma unroll
+            for (int i = 0; i < K; i++) w[i] = weights.mass(v[i]);
+#pragma unroll
+            for (int i = 0; i < K; i++) sum += in[i] ? w[i] : 0;
         });
         sum = warp_sum(sum);
         if (lane < cs) of(lane).sums[rank][warp] = sum;
@@ -715,9 +748,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     if (tid < ROOTS) sh.roots[tid] = exp2((double)tid / ROOTS + SCALE);
     const bool wide = a.V > LIST && by_k != by_p;  // bins down to the least value are likely
     float top = -__int_as_float(0x7f800000), low = __int_as_float(0x7f800000);
-    c.each<2>([&](float v, int) {
-        top = max_nan(top, v);
-        if (wide && v > -__int_as_float(0x7f800000)) low = fminf(low, v);
+    constexpr int K = Chooser<T>::K;
+    c.template each<2>([&](const float (&v)[K], int) {
+#pragma unroll
+        for (int i = 0; i < K; i++) {
+            top = max_nan(top, v[i]);
+            if (wide && v[i] > -__int_as_float(0x7f800000)) low = fminf(low, v[i]);
+        }
     });
     {
         const uint32_t q = key_of(top), m = __reduce_max_sync(0xffffffffu, q);
@@ -740,8 +777,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     // greedy rows, and those whose maximum leaves no distribution: infinite, NaN, or nothing but -infinity
     if (greedy || most >= INF || most < LOWEST) {
         uint32_t at = 0xffffffffu;
-        c.each<1>([&](float v, int e) {
-            if (key_of(v) == most) at = min(at, (uint32_t)(c.first + e));
+        c.template each<2>([&](const float (&v)[K], int e) {
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (key_of(v[i]) == most) at = min(at, (uint32_t)(c.first + e + i));
         });
         at = __reduce_min_sync(0xffffffffu, at);
         c.sync();  // all have read the least values there
@@ -782,13 +821,18 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
         if (sh.bound >= LOWEST) bounded = true, bound = fmaxf(bound, value_of(sh.bound));
     }
     if (bounded && (by_k || !by_p || a.V <= LIST)) {
-        c.template each<2>([&](float v, int e) {
-            if (v >= bound) c.list_one(v, e);
+        c.template each<2>([&](const float (&v)[K], int e) {
+#pragma unroll
+            for (int i = 0; i < K; i++)
+                if (v[i] >= bound) c.list_one(v[i], e + i);
         });
         u64 total = 0;
         if (by_p && !by_k) {  // of a row as short as a list
             u64 sum = 0;
-            c.template each<1>([&](float v, int) { sum += c.weights.mass(v); });
+            c.template each<1>([&](const float (&v)[K], int) {
+#pragma unroll
+                for (int i = 0; i < K; i++) sum += c.weights.mass(v[i]);
+            });
             total = c.exchange_sums(sum);
         }
         const int m = c.gather();
