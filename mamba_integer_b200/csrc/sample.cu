@@ -37,7 +37,7 @@ namespace sample {
 namespace cg = cooperative_groups;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = THREADS, FINE = 4096, MAX_CLUSTER = 8,
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 512, LIST = THREADS, FINE = 2048, MAX_CLUSTER = 8,
               MAX_V = 262144, MAX_SEG = 131072;
 constexpr int SCALE = 44;                      // weights are whole numbers of 2^-44
 constexpr uint32_t LOWEST = 0x00800000u;       // key of -FLT_MAX
@@ -112,9 +112,10 @@ struct Bins {
         scale = __fdiv_rn((float)N, fminf(range, __fmul_rn((SCALE + 2) * 0.6931472f, temperature)));
         if (!(scale < 3.0e38f)) scale = 0.0f;  // a row of one value
     }
+    __device__ __forceinline__ float at(float v) const { return __fmul_rn(__fsub_rn(most, v), scale); }
     __device__ __forceinline__ int operator()(float v) const {
-        const float at = __fmul_rn(__fsub_rn(most, v), scale);
-        return at < (float)(N - 1) ? (int)at : N - 1;
+        const float x = at(v);
+        return x < (float)(N - 1) ? (int)x : N - 1;
     }
 };
 
@@ -134,7 +135,9 @@ struct Shared {
         struct {
             uint32_t count[2][BINS], limb[2][3][BINS];  // limbs of 15 bits, which MAX_SEG tokens do not overflow
         };
-        uint32_t fine[FINE];
+        struct {
+            uint32_t fine[FINE], depth[FINE];  // tokens of a bin, and the sum of how far they lie in it, in 256ths
+        };
     };
     double roots[ROOTS];
     u64 warp_low[WARPS];
@@ -408,31 +411,39 @@ struct Chooser {
     }
 
     // The border of top-k, or of top-p of all tokens, by counts in fine bins, and the choice.  The counts give the bin of the
-    // k-th token, or bound the masses up to each bin from both sides, and so the bins in which top-p's border can lie.
+    // k-th token.  The mass of a bin's c tokens, which lie t_i into it (0 to 1) where weights fall by r, is the sum of
+    // r^t_i: at least c r^mean(t), as r^t is convex, and at most c - (1 - r) sum(t), the chord's.  That bounds the masses
+    // up to each bin from both sides, to 1e-4, and so the bins in which top-p's border can lie.
     // One pass over the weights then adds up what lies above those bins, by warps, and lists the tokens in them (or all
     // down to them, if they are few).  CTA 0 finds the border among these and has the sums of what is kept.  `least`: the
     // row's least finite value; `floor`: the least that min-p keeps.  False: too many tokens lie in those bins.
     __device__ __forceinline__ bool choose_by_bins(bool by_k, int k, double p, float least, float floor, double least_power, float u,
                                                    int64_t row) {
         const Bins<FINE> bins(value_of(kmax), temperature, __fsub_rn(value_of(kmax), least));
-        for (int i = tid; i < FINE; i += THREADS) sh.fine[i] = 0;
+        for (int i = tid; i < FINE; i += THREADS) sh.fine[i] = sh.depth[i] = 0;
         __syncthreads();
         // what has no weight is never chosen, but counts for top-k
         const float end = by_k ? -3.402823466e38f : weights.end;
         each<2>([&](const float (&v)[K], int) {
-            int b[K];
+            int b[K], t[K];
 #pragma unroll
-            for (int i = 0; i < K; i++) b[i] = bins(v[i]);
+            for (int i = 0; i < K; i++) {
+                b[i] = bins(v[i]);
+                t[i] = (int)((bins.at(v[i]) - (float)b[i]) * 256.0f);
+            }
 #pragma unroll
             for (int i = 0; i < K; i++)
-                if (v[i] >= end) atomicAdd(&sh.fine[b[i]], 1u);
+                if (v[i] >= end) {
+                    atomicAdd(&sh.fine[b[i]], 1u);
+                    if (!by_k) atomicAdd(&sh.depth[b[i]], (uint32_t)min(t[i], 255));
+                }
         });
         sync();
         if (cs > 1) {  // each CTA adds up a part of the bins for all
             for (int i = rank * (FINE / cs) + tid; i < (rank + 1) * (FINE / cs); i += THREADS) {
-                uint32_t all = 0;
-                for (int r = 0; r < cs; r++) all += of(r).fine[i];
-                for (int r = 0; r < cs; r++) of(r).fine[i] = all;
+                uint32_t all = 0, deep = 0;
+                for (int r = 0; r < cs; r++) all += of(r).fine[i], deep += of(r).depth[i];
+                for (int r = 0; r < cs; r++) of(r).fine[i] = all, of(r).depth[i] = deep;
             }
             sync();
         }
@@ -440,20 +451,19 @@ struct Chooser {
         uint32_t c[PER], counts = 0;
 #pragma unroll
         for (int i = 0; i < PER; i++) c[i] = sh.fine[tid * PER + i];
-        // a bin's weights lie between those of its edges, in units of 2^-30; 3e-5 for their rounding and that of
-        // (most - v) * scale.  Whole numbers again, so that every thread of every CTA has the same sums.
-        // A single bin and the last one have no lower edge.
+        // in units of 2^-30; 3e-5 for the rounding of the weights and of (most - v) * scale.  Whole numbers again, so that
+        // every thread of every CTA has the same sums.  A single bin and the last one are open downwards.
         u64 low[PER], high[PER], lows = 0, highs = 0;
         const bool one = !(bins.scale > 0.0f);
         const float width = one ? 0.0f : (float)(weights.scale * (1.0 / ROOTS) / (double)bins.scale);
-        float edge = exp2f(-(float)(tid * PER) * width) * 1073741824.0f;
-        const float ratio = exp2f(-width);
+        const float fall = 1.0f - exp2f(-width);
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            const float next = one || tid * PER + i == FINE - 1 ? 0.0f : edge * ratio;
-            high[i] = (u64)c[i] * ((uint32_t)(edge * (1 + 3e-5f)) + 1);
-            low[i] = (u64)c[i] * (uint32_t)(next * (1 - 3e-5f));
-            edge = next;
+            const int b = tid * PER + i;
+            const float n = (float)c[i], t = (float)sh.depth[b] * (1.0f / 256.0f), edge = exp2f(30.0f - (float)b * width);
+            const bool open = one || b == FINE - 1;
+            high[i] = (u64)(edge * (open ? n : n - fall * t) * (1 + 3e-5f)) + (c[i] > 0);
+            low[i] = open || !c[i] ? 0 : (u64)(edge * n * exp2f(-width * (t / n + 1.0f / 256.0f)) * (1 - 3e-5f));
             lows += low[i], highs += high[i], counts += c[i];
         }
         u64 lup = warp_scan(lows), hup = warp_scan(highs);
@@ -814,7 +824,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     // a bound that all kept tokens reach
     bool bounded = (by_m && !(by_k && by_p)) || (a.V <= LIST && (by_k || by_p || by_m));
     float bound = by_m && !(by_k && by_p) ? floor : -3.402823466e38f;
-    if (a.V > LIST && by_k && k <= THREADS) {
+    if (a.V > LIST && by_k && k <= (by_p ? THREADS : THREADS * 5 / 8)) {  // beyond, the list is likely to be too long
         const uint32_t q = c.sorted(sh.maxima[tid], THREADS);
         if (tid == k - 1) sh.bound = q;
         __syncthreads();
@@ -858,10 +868,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const __grid_constan
     c.choose(a.u[row], cut, row);
 }
 
-// CTAs of a row: doubled where rows leave SMs idle, down to 4096 tokens a CTA.
+// CTAs of a row: doubled where rows leave SMs idle, down to 8192 tokens a CTA.
 static inline int cluster_of(int rows, int V) {
     int cs = 1;
-    while (cs < MAX_CLUSTER && (V > cs * MAX_SEG || ((int64_t)rows * cs * 2 <= 148 && V > cs * 4096))) cs *= 2;
+    while (cs < MAX_CLUSTER && (V > cs * MAX_SEG || ((int64_t)rows * cs * 2 <= 148 && V > cs * 8192))) cs *= 2;
     return cs;
 }
 
