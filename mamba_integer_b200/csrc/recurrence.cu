@@ -40,7 +40,7 @@ namespace rec {
 
 constexpr int WARPS = 8, THREADS = WARPS * 32, CB = 64;  // channels a CTA
 constexpr int CK = 8;          // positions between the states kept for the backward pass
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 16;
 
 struct Seq {  // a [batch, L, D] operand with unit last stride
     const void* p;
@@ -76,7 +76,9 @@ __device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
 
 // sigmoid(v) and sigmoid(-v), neither taken from 1 minus the other, for |v| up
 // to 87 (beyond it counts as 87; a NaN stays one).  The product with log2(e) is
-// carried on in two parts, which keeps the power to 2 ulp where |v| is large.
+// carried on in two parts, which keeps the power to 2 ulp where |v| is large, and
+// a Newton step makes the reciprocal right to its last bit: where a is near 1, a
+// state has its error as often as its memory is long.
 __device__ __forceinline__ void sigmoids(float2 v, float2& up, float2& down) {
     v.x = max_nan(min_nan(v.x, 87.0f), -87.0f);
     v.y = max_nan(min_nan(v.y, 87.0f), -87.0f);
@@ -84,15 +86,26 @@ __device__ __forceinline__ void sigmoids(float2 v, float2& up, float2& down) {
     const float2 r = __ffma2_rn(v, dup(1.92596299e-8f), __ffma2_rn(v, dup(LOG2E), t));  // t is too large by this
     float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
     e = __ffma2_rn(__fmul2_rn(e, dup(-LN2)), r, e);
-    const float2 d = __fadd2_rn(e, dup(1.0f));
-    up = make_float2(rcp_fast(d.x), rcp_fast(d.y));
+    const float2 d = __ffma2_rn(e, dup(-1.0f), dup(-1.0f));  // -(1 + e)
+    const float2 q = make_float2(rcp_fast(-d.x), rcp_fast(-d.y));
+    up = __ffma2_rn(q, __ffma2_rn(d, q, dup(1.0f)), q);
     down = __fmul2_rn(e, up);
 }
 
-// z sigmoid(z) and its derivative
+// z sigmoid(z), and its derivative.  In 16 bits without the care above: |z| 2^-24
+// of the power is far below half a step.
+template <typename T>
 __device__ __forceinline__ float2 silu(float2 z, float2& slope) {
     float2 s, n;
-    sigmoids(z, s, n);
+    if constexpr (sizeof(T) == 4) {
+        sigmoids(z, s, n);
+    } else {
+        const float2 t = __fmul2_rn(z, dup(-LOG2E));
+        const float2 e = make_float2(exp2_fast(min_nan(t.x, 126.0f)), exp2_fast(min_nan(t.y, 126.0f)));
+        const float2 d = __fadd2_rn(e, dup(1.0f));
+        s = make_float2(rcp_fast(d.x), rcp_fast(d.y));
+        n = __fmul2_rn(e, s);
+    }
     const float2 zs = __fmul2_rn(z, s);
     slope = __ffma2_rn(zs, n, s);
     return zs;
@@ -101,8 +114,8 @@ template <typename T>
 __device__ __forceinline__ float2 silu(float2 z) {
     if constexpr (sizeof(T) == 4) {
         float2 slope;
-        return silu(z, slope);
-    } else {  // |z| 2^-24 of the power is far below half a step of 16 bits
+        return silu<T>(z, slope);
+    } else {
         const float2 t = __fmul2_rn(z, dup(-LOG2E));
         const float2 d = __fadd2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), dup(1.0f));
         return __fmul2_rn(z, make_float2(rcp_fast(d.x), rcp_fast(d.y)));
@@ -263,15 +276,16 @@ __device__ __forceinline__ uint32_t off16(const Seq& s, int b, int t, int c0) {
 // writes to one has seen the other's round end, which all read the first before.
 struct Exchange {
     Fold warp[2][WARPS][32];
-    Fold cta[2][MAX_CLUSTER][32];
     uint64_t arrived[2];
 };
+constexpr size_t CTA_FOLDS = sizeof(Fold) * 2 * 32;  // bytes for each CTA of a cluster, [2][cluster][32] behind the rows
 
 // Slots a warp: as many as leave room for two CTAs an SM.
 template <typename R>
-constexpr int STAGES = sizeof(R) * WARPS * 2 + sizeof(Exchange) <= 113 * 1024 ? 2 : 1;
+constexpr int STAGES = sizeof(R) * WARPS * 2 + sizeof(Exchange) + 8 * CTA_FOLDS <= 113 * 1024 ? 2 : 1;
 
-__device__ __forceinline__ float2 exchange(Exchange& ex, int round, int cs, int rank, Fold mine, float2& s) {
+__device__ __forceinline__ float2 exchange(Exchange& ex, Fold* folds, int round, int cs, int rank, Fold mine,
+                                           float2& s) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = round & 1;
     mine.p = some(mine.p);
     ex.warp[k][warp][lane] = mine;
@@ -286,21 +300,23 @@ __device__ __forceinline__ float2 exchange(Exchange& ex, int round, int cs, int 
         }
         return from;
     }
-    if (warp < cs) {  // warp i tells CTA i
+    if (warp < cs) {  // warp i tells CTA i (and i + 8)
         Fold all = ex.warp[k][0][lane];
 #pragma unroll
         for (int i = 1; i < WARPS; i++) all = join(all, ex.warp[k][i][lane]);
-        uint32_t to, bar;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&ex.cta[k][rank][lane])), "r"(warp));
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&ex.arrived[k])), "r"(warp));
-        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
-                     "f"(all.p.x), "f"(all.p.y), "f"(all.q.x), "f"(all.q.y), "r"(bar)
-                     : "memory");
+        for (int i = warp; i < cs; i += WARPS) {
+            uint32_t to, bar;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&folds[(k * cs + rank) * 32 + lane])), "r"(i));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&ex.arrived[k])), "r"(i));
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+                         "f"(all.p.x), "f"(all.p.y), "f"(all.q.x), "f"(all.q.y), "r"(bar)
+                         : "memory");
+        }
     }
     bar_wait(&ex.arrived[k], (round >> 1) & 1);
     for (int i = 0; i < cs; i++) {
         if (i == rank) from = s;
-        s = fold(s, ex.cta[k][i][lane]);
+        s = fold(s, folds[(k * cs + i) * 32 + lane]);
     }
     for (int i = 0; i < warp; i++) from = fold(from, ex.warp[k][i][lane]);
     return from;
@@ -326,6 +342,7 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
     extern __shared__ __align__(16) unsigned char smem[];
     Exchange& ex = *reinterpret_cast<Exchange*>(smem);
     R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
+    Fold* folds = reinterpret_cast<Fold*>(smem + sizeof(Exchange) + sizeof(R) * ST * WARPS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
     const int c = c0 + 2 * lane, valid = a.D - c;
@@ -382,7 +399,7 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
                 mine.q = __ffma2_rn(av[i], mine.q, uv[i]);
             }
         }
-        float2 h = exchange(ex, round, cs, rank, mine, s);
+        float2 h = exchange(ex, folds, round, cs, rank, mine, s);
         if (n > 0) {
             T* y = static_cast<T*>(a.y) + ((int64_t)b * a.L + t0) * a.D + c;
             float* ck = a.ckpt ? a.ckpt + ((int64_t)b * cdiv(a.L, CK) + t0 / CK) * a.D + c : nullptr;
@@ -422,6 +439,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
     extern __shared__ __align__(16) unsigned char smem[];
     Exchange& ex = *reinterpret_cast<Exchange*>(smem);
     R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
+    Fold* folds = reinterpret_cast<Fold*>(smem + sizeof(Exchange) + sizeof(R) * ST * WARPS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
     const int c = c0 + 2 * lane, valid = a.D - c;
@@ -479,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
                     h = __ffma2_rn(av[i], h, CONVEX ? __fmul2_rn(wv[i], x) : x);
                     if (GATE) {
                         float2 slope;
-                        const float2 gate = silu(pair<VEC>(rows.v[N - 1][i], off16<VEC, T>(a.in[Z], b, t0 + i, c0)), slope);
+                        const float2 gate = silu<T>(pair<VEC>(rows.v[N - 1][i], off16<VEC, T>(a.in[Z], b, t0 + i, c0)), slope);
                         if (FAST || i < n)
                             put<FAST>(static_cast<T*>(a.dz) + at + (int64_t)i * a.D, __fmul2_rn(__fmul2_rn(dv[i], h), slope),
                                       valid, a.ovec);
@@ -502,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
                 mine.q = __fmul2_rn(av[i], __fadd2_rn(dv[i], mine.q));
             }
         }
-        float2 G = exchange(ex, round, cs, rank, mine, s);
+        float2 G = exchange(ex, folds, round, cs, rank, mine, s);
         if (n > 0) {
             auto leave = [&](auto quick) {
                 constexpr bool FAST = decltype(quick)::value;
@@ -592,22 +610,49 @@ static inline int cluster_of(int batch, int L, int D, int tile) {
     return cs;
 }
 
+// Clusters of more than 8 CTAs are not portable: whether this device takes them, asked once (by two bits a device).
+static bool allow_wide_clusters(void (*kernel)(const Args), size_t smem, std::atomic<uint64_t>& known) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 32) return false;
+    const uint64_t have = known.load(std::memory_order_relaxed) >> (2 * dev) & 3;
+    if (have) return have == 3;
+    bool yes = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess;
+    if (yes) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(MAX_CLUSTER);
+        cfg.blockDim = dim3(THREADS);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = MAX_CLUSTER;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int fit = 0;
+        yes = cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) == cudaSuccess && fit > 0;
+    }
+    cudaGetLastError();
+    known.fetch_or((uint64_t)(yes ? 3 : 1) << (2 * dev), std::memory_order_relaxed);
+    return yes;
+}
+
 template <typename T, bool CONVEX, bool GATE, bool VEC, bool BWD>
-static int launch(const Args& a, cudaStream_t s) {
+static int launch(Args& a, cudaStream_t s) {
     constexpr int N = (GATE ? 3 : 2) + BWD, SUB = BWD ? CK : SUB_FWD<T>;
     using R = Rows<T, N, SUB, VEC>;
-    constexpr size_t smem = sizeof(R) * STAGES<R> * WARPS + sizeof(Exchange);
-    static std::atomic<uint64_t> allowed{0};
+    constexpr size_t alone = sizeof(R) * STAGES<R> * WARPS + sizeof(Exchange);
+    static std::atomic<uint64_t> allowed{0}, wide{0};
     void (*kernel)(const Args);
     if constexpr (BWD)
         kernel = bwd_kernel<T, CONVEX, GATE, VEC>;
     else
         kernel = fwd_kernel<T, CONVEX, GATE, VEC>;
-    if (!allow_smem(kernel, smem, allowed)) return MI_ERR_CUDA;
+    if (!allow_smem(kernel, alone + MAX_CLUSTER * CTA_FOLDS, allowed)) return MI_ERR_CUDA;
+    if (a.cs > 8 && !allow_wide_clusters(kernel, alone + MAX_CLUSTER * CTA_FOLDS, wide)) a.cs = 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cdiv(a.D, CB) * a.cs, a.batch);
     cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = alone + (a.cs > 1 ? a.cs * CTA_FOLDS : 0);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     int n = 0;
