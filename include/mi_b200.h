@@ -447,26 +447,27 @@ int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const 
  *   y[t] = h[t] * z sigmoid(z) (h[t] with z NULL)
  * x, f, z, y [batch, L, D]; bias [D]; h0, h_out [batch, D]; z, bias, h0,
  * lengths, h_out may be NULL.  checkpoints (NULL without a backward pass):
- * mi_gated_recurrence_checkpoints() floats.  L >= 1.  Gates never reach 0 (e^-|f|
- * is 2^-126 at least): infinite states stay infinite.
+ * mi_gated_recurrence_checkpoints() floats.  workspace (NULL if 0):
+ * mi_gated_recurrence_workspace(.., 0, dtype) bytes.  L >= 1.  Gate logits count as
+ * at most 87 from 0, so that gates never reach 0: infinite states stay infinite.
  */
 int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,
                         const void* z, int64_t z_batch, int64_t z_row, const float* bias, const float* h0,
-                        const int32_t* lengths, void* y, float* h_out, float* checkpoints, int batch, int L, int D,
-                        int convex, int dtype, void* stream);
+                        const int32_t* lengths, void* y, float* h_out, float* checkpoints, void* workspace, int batch, int L,
+                        int D, int convex, int dtype, void* stream);
 int64_t mi_gated_recurrence_checkpoints(int batch, int L, int D);
+int64_t mi_gated_recurrence_workspace(int batch, int L, int D, int backward, int dtype);
 
 /* Its gradients, from dy [batch, L, D] and dh_out (NULL: 0): dx, df, dz [batch,
  * L, D] (dz with z); dbias [D] and dh0 [batch, D], which may be NULL.
- * workspace (for dbias): mi_gated_recurrence_backward_workspace() bytes.  The
- * same inputs give the same bits. */
+ * workspace (NULL if 0): mi_gated_recurrence_workspace(.., 1, dtype) bytes.  The same
+ * inputs give the same bits. */
 int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const float* dh_out, const void* x,
                                  int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,
                                  const void* z, int64_t z_batch, int64_t z_row, const float* bias,
                                  const int32_t* lengths, const float* checkpoints, void* dx, void* df, void* dz,
                                  float* dbias, float* dh0, void* workspace, int batch, int L, int D, int convex,
                                  int dtype, void* stream);
-int64_t mi_gated_recurrence_backward_workspace(int batch, int L, int D);
 
 /* One new token a stream: x, f, z, y [batch, D]; h [batch, D] is advanced in
  * place. */

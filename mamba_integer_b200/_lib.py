@@ -67,10 +67,10 @@ SIGNATURES = {
     "mi_causal_conv1d_backward": [*_s, _p, *_s, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _p],
     "mi_causal_conv1d_backward_workspace": [_i, _i, _i, _i],
     "mi_causal_conv1d_step": [_p, _i64, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p],
-    "mi_gated_recurrence": [_p, _i64, _i64] * 3 + [_p] * 6 + [_i] * 5 + [_p],
+    "mi_gated_recurrence": [_p, _i64, _i64] * 3 + [_p] * 7 + [_i] * 5 + [_p],
     "mi_gated_recurrence_checkpoints": [_i, _i, _i],
     "mi_gated_recurrence_backward": [_p, _i64, _i64, _p] + [_p, _i64, _i64] * 3 + [_p] * 9 + [_i] * 5 + [_p],
-    "mi_gated_recurrence_backward_workspace": [_i, _i, _i],
+    "mi_gated_recurrence_workspace": [_i, _i, _i, _i, _i],
     "mi_gated_recurrence_step": [_p, _i64] * 3 + [_p] * 3 + [_i] * 4 + [_p],
     "mi_rms_norm": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
     "mi_rms_norm_quant": [_p, _i64, _p, _i64, _p, _p, _p, _p, _i, _i, _f, _i, _i, _p],
@@ -85,7 +85,7 @@ _RESTYPE = {"mi_status_string": ctypes.c_char_p, "mi_selective_scan_checkpoints"
             "mi_selective_scan_workspace": _i64, "mi_causal_conv1d_backward_workspace": _i64,
             "mi_rms_norm_backward_workspace": _i64, "mi_gated_recurrence_checkpoints": _i64,
             "mi_layer_norm_backward_workspace": _i64,
-            "mi_gated_recurrence_backward_workspace": _i64}
+            "mi_gated_recurrence_workspace": _i64}
 
 _lib = None
 

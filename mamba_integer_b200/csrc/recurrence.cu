@@ -12,8 +12,11 @@
 //
 // A position and channel move 3 elements forward (4 with z) and meet 2 (4)
 // special-function results, so HBM bounds it as long as enough loads are in
-// flight and the instructions are few: at 45 of them a channel and position
-// (8 x 2048 x 1536 bf16 71 us, 3.2 TB/s) issue slots did.
+// flight and the instructions are few (30 a channel and position with z, of
+// which 4 are special functions).  32 x 512 x 1536 bf16 with z: forward 50 us
+// (201 MB, 4.0 TB/s), 36 without the arithmetic; backward 84 (352 MB, 4.2 TB/s),
+// 78 without: what is left is two CTAs of 128 registers a thread an SM, whose
+// warps load, wait for the fold and store by turns.
 //
 // Layout: a CTA has 64 channels, two a lane in f32x2 arithmetic, and walks the
 // sequence in tiles; a warp has SUB neighbouring positions of a tile, whose rows
@@ -21,9 +24,10 @@
 // positions acts on the state as h -> P h + H; the warps fold theirs through
 // shared memory, once a tile, and then run their own positions again from the
 // state they start from, with a and c x still in registers.  Where the channels
-// leave SMs idle, a cluster of up to 8 CTAs shares the tiles of a round: each
+// leave SMs idle, a cluster of up to 16 CTAs shares the tiles of a round: each
 // sends its fold to the others' shared memory, counted by their mbarriers;
-// nothing is read twice.
+// nothing is read twice.  Long sequences of few channels are cut into chunks,
+// whose folds a pass in front takes.
 //
 // Gates and folds never reach 0: gate logits count as at most 87 from 0, and a
 // stretch's P is at least 2^-126, so that an infinite state stays infinite and an
@@ -60,10 +64,12 @@ struct Args {
     float* ckpt;         // [batch, cdiv(L, CK), D] or NULL
     void *dx, *df, *dz;
     float* dh0;          // [batch, D] or NULL
-    float* part;         // [batch * cluster, D]: the CTAs' sums of df, or NULL
+    float* part;         // [batch * chunks * cluster, D]: the CTAs' sums of df, or NULL
+    float* folds;        // with chunks > 1: [batch, chunks, 2, D], what each chunk does to the state
     int batch, L, D;
     int ovec;            // outputs' rows start on a lane's two elements' alignment
     int cs;              // CTAs of a cluster
+    int chunks, span;    // chunks of a sequence, positions of a chunk
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) {
@@ -331,6 +337,38 @@ __device__ __forceinline__ void begin(Exchange& ex, int cs) {
         __syncthreads();
 }
 
+// A chunk's place in its sequence of `len` positions.
+struct Chunk {
+    int b, ch, org, end;  // its positions: org .. end - 1 (those that exist)
+    __device__ __forceinline__ Chunk(const Args& a, int y) {
+        b = a.chunks == 1 ? y : y / a.chunks, ch = a.chunks == 1 ? 0 : y - b * a.chunks;
+        org = ch * a.span;
+        end = min(length_of(a, b), a.L - org > a.span ? org + a.span : a.L);
+    }
+};
+
+// The state in front of a chunk (behind it, backwards): `s` from the sequence's end on through the other chunks between.
+// The warps fold some each.
+template <bool BWD>
+__device__ __forceinline__ float2 through_chunks(const Args& a, const Chunk& k, int c, int valid, Fold (*slots)[32], float2 s) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = BWD ? a.chunks - 1 - k.ch : k.ch;
+    if (n == 0) return s;
+    const int each = cdiv(n, WARPS), to = min((warp + 1) * each, n);
+    Fold mine = {dup(1.0f), dup(0.0f)};
+#pragma unroll 4
+    for (int i = warp * each; i < to; i++) {
+        const float* p = a.folds + ((int64_t)k.b * a.chunks + (BWD ? a.chunks - 1 - i : i)) * 2 * a.D + c;
+        mine = join(mine, {load2(p, valid), load2(p + a.D, valid)});
+    }
+    slots[warp][lane] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) s = fold(s, slots[i][lane]);
+    __syncthreads();
+    return s;
+}
+
 template <typename T>
 constexpr int SUB_FWD = sizeof(T) == 2 ? 16 : 8;
 
@@ -344,12 +382,13 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
     R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
     Fold* folds = reinterpret_cast<Fold*>(smem + sizeof(Exchange) + sizeof(R) * ST * WARPS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
+    const int cs = a.cs, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
     const int c = c0 + 2 * lane, valid = a.D - c;
     begin(ex, cs);
     grid_dependency_sync();
-    const int len = length_of(a, b);
-    const int rounds = cdiv(len, TT * cs);
+    const Chunk chunk(a, blockIdx.y);
+    const int b = chunk.b, len = chunk.end;
+    const int rounds = len > chunk.org ? cdiv(len - chunk.org, TT * cs) : 0;
     const float2 bias = a.bias ? load2(a.bias + c, valid) : dup(0.0f);
     float2 s = a.h0 ? load2(a.h0 + (int64_t)b * a.D + c, valid) : dup(0.0f);
     Fetch<T, N, SUB, VEC> fetch;
@@ -357,7 +396,7 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
         fetch.init(a, b, c0, X, F, Z);
     else
         fetch.init(a, b, c0, X, F);
-    auto start = [&](int round) { return (round * cs + rank) * TT + warp * SUB; };
+    auto start = [&](int round) { return chunk.org + (round * cs + rank) * TT + warp * SUB; };
     auto load = [&](int round) {
         const int t0 = start(round);
         if (round < rounds && t0 < len) {
@@ -370,6 +409,7 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
     };
 #pragma unroll
     for (int i = 0; i < ST; i++) load(i);
+    if (a.chunks > 1) s = through_chunks<false>(a, chunk, c, valid, ex.warp[0], s);
     for (int round = 0; round < rounds; round++) {
         const int t0 = start(round), k = round % ST;
         const int n = len - t0;  // positions of this stretch that exist
@@ -423,8 +463,9 @@ __global__ void __launch_bounds__(THREADS, 2) fwd_kernel(const __grid_constant__
         load(round + ST);
     }
     cp_async_wait();
-    if (a.hT && rank == 0 && warp == 0) store2(a.hT + (int64_t)b * a.D + c, s, valid);
-    for (int t = len + rank * WARPS + warp; t < a.L; t += cs * WARPS)
+    if (a.hT && rank == 0 && warp == 0 && chunk.ch == a.chunks - 1) store2(a.hT + (int64_t)b * a.D + c, s, valid);
+    const int last = min(a.L - chunk.org, a.span) + chunk.org;
+    for (int t = max(len, chunk.org) + rank * WARPS + warp; t < last; t += cs * WARPS)
         put<false>(static_cast<T*>(a.y) + ((int64_t)b * a.L + t) * a.D + c, dup(0.0f), valid, a.ovec);
     if (cs > 1) cooperative_groups::this_cluster().sync();  // none leaves before the others are done with its memory
 }
@@ -441,11 +482,12 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
     R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem + sizeof(Exchange));
     Fold* folds = reinterpret_cast<Fold*>(smem + sizeof(Exchange) + sizeof(R) * ST * WARPS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int cs = a.cs, b = blockIdx.y, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
+    const int cs = a.cs, c0 = blockIdx.x / cs * CB, rank = blockIdx.x % cs;
     const int c = c0 + 2 * lane, valid = a.D - c;
     begin(ex, cs);
-    const int len = length_of(a, b);
-    const int stretches = cdiv(len, SUB), rounds = cdiv(stretches, WARPS * cs);
+    const Chunk chunk(a, blockIdx.y);
+    const int b = chunk.b, len = chunk.end;
+    const int stretches = len > chunk.org ? cdiv(len - chunk.org, SUB) : 0, rounds = cdiv(stretches, WARPS * cs);
     const float2 bias = a.bias ? load2(a.bias + c, valid) : dup(0.0f);
     float2 s = a.dhT ? load2(a.dhT + (int64_t)b * a.D + c, valid) : dup(0.0f);
     float2 dbias = dup(0.0f), next_h = dup(0.0f);
@@ -458,22 +500,24 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
     auto load = [&](int round) {
         const int j = stretch(round);
         if (j >= 0) {
+            const int t0 = chunk.org + j * SUB;
             if constexpr (GATE)
-                fetch.start(a, slots[round % ST][warp], j * SUB, len - j * SUB, X, F, DY, Z);
+                fetch.start(a, slots[round % ST][warp], t0, len - t0, X, F, DY, Z);
             else
-                fetch.start(a, slots[round % ST][warp], j * SUB, len - j * SUB, X, F, DY);
+                fetch.start(a, slots[round % ST][warp], t0, len - t0, X, F, DY);
         }
         cp_async_commit();
     };
     auto load_h = [&](int round) {
         const int j = stretch(round);
-        if (j >= 0) next_h = load2(a.ckpt + ((int64_t)b * cdiv(a.L, CK) + j) * a.D + c, valid);
+        if (j >= 0) next_h = load2(a.ckpt + ((int64_t)b * cdiv(a.L, CK) + chunk.org / CK + j) * a.D + c, valid);
     };
 #pragma unroll
     for (int i = 0; i < ST; i++) load(i);
     load_h(0);
+    if (a.chunks > 1) s = through_chunks<true>(a, chunk, c, valid, ex.warp[0], s);
     for (int round = 0; round < rounds; round++) {
-        const int j = stretch(round), t0 = j * SUB, k = round % ST;
+        const int j = stretch(round), t0 = chunk.org + j * SUB, k = round % ST;
         const int n = j >= 0 ? len - t0 : 0;
         const int64_t at = ((int64_t)b * a.L + t0) * a.D + c;
         const bool fast = a.ovec && n >= SUB && c0 + CB <= a.D;
@@ -545,8 +589,9 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
         load(round + ST);
     }
     cp_async_wait();
-    if (a.dh0 && rank == 0 && warp == 0) store2(a.dh0 + (int64_t)b * a.D + c, s, valid);
-    for (int t = len + rank * WARPS + warp; t < a.L; t += cs * WARPS) {
+    if (a.dh0 && rank == 0 && warp == 0 && chunk.ch == 0) store2(a.dh0 + (int64_t)b * a.D + c, s, valid);
+    const int last = min(a.L - chunk.org, a.span) + chunk.org;
+    for (int t = max(len, chunk.org) + rank * WARPS + warp; t < last; t += cs * WARPS) {
         const int64_t at = ((int64_t)b * a.L + t) * a.D + c;
         put<false>(static_cast<T*>(a.dx) + at, dup(0.0f), valid, a.ovec);
         put<false>(static_cast<T*>(a.df) + at, dup(0.0f), valid, a.ovec);
@@ -560,10 +605,88 @@ __global__ void __launch_bounds__(THREADS, 2) bwd_kernel(const __grid_constant__
         if (warp == 0) {
 #pragma unroll
             for (int i = 1; i < WARPS; i++) dbias = __fadd2_rn(dbias, sums[i][lane]);
-            store2(a.part + ((int64_t)b * cs + rank) * a.D + c, dbias, valid);
+            store2(a.part + ((int64_t)blockIdx.y * cs + rank) * a.D + c, dbias, valid);
         }
     }
     if (cs > 1) cooperative_groups::this_cluster().sync();
+}
+
+// What a chunk does to the state (backwards: to its gradient), for long sequences
+// of few channels.  Each warp walks positions of its own, without a barrier.
+template <typename T, bool CONVEX, bool GATE, bool VEC, bool BWD>
+__global__ void __launch_bounds__(THREADS, 2) chunk_kernel(const __grid_constant__ Args a) {
+    constexpr int SUB = BWD ? CK : SUB_FWD<T>, N = BWD && GATE ? 3 : 2, ST = 2;
+    using R = Rows<T, N, SUB, VEC>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    R(*slots)[WARPS] = reinterpret_cast<R(*)[WARPS]>(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c0 = blockIdx.x * CB, c = c0 + 2 * lane, valid = a.D - c;
+    grid_dependency_sync();
+    const Chunk chunk(a, blockIdx.y);
+    if (chunk.ch == (BWD ? 0 : a.chunks - 1)) return;  // nothing lies behind it
+    const int b = chunk.b;
+    const float2 bias = a.bias ? load2(a.bias + c, valid) : dup(0.0f);
+    Fetch<T, N, SUB, VEC> fetch;
+    // a warp's stretches, in the order in which they are passed
+    const int part = a.span / WARPS, first = chunk.org + warp * part, end = min(first + part, chunk.end);
+    const int stretches = end > first ? cdiv(end - first, SUB) : 0;
+    auto start = [&](int i) { return first + (BWD ? stretches - 1 - i : i) * SUB; };
+    auto load = [&](int i) {
+        if (i < stretches) {
+            const int t0 = start(i);
+            if constexpr (BWD && GATE)
+                fetch.start(a, slots[i % ST][warp], t0, end - t0, F, DY, Z);
+            else if constexpr (BWD)
+                fetch.start(a, slots[i % ST][warp], t0, end - t0, F, DY);
+            else
+                fetch.start(a, slots[i % ST][warp], t0, end - t0, F, X);
+        }
+        cp_async_commit();
+    };
+    if constexpr (BWD && GATE)
+        fetch.init(a, b, c0, F, DY, Z);
+    else if constexpr (BWD)
+        fetch.init(a, b, c0, F, DY);
+    else
+        fetch.init(a, b, c0, F, X);
+    load(0), load(1);
+    Fold all = {dup(1.0f), dup(0.0f)};
+    for (int k = 0; k < stretches; k++) {
+        const int t0 = start(k), n = end - t0;
+        R& rows = slots[k % ST][warp];
+        cp_async_wait<ST - 1>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < SUB; j++) {
+            const int i = BWD ? SUB - 1 - j : j;
+            const float2 f = __fadd2_rn(pair<VEC>(rows.v[0][i], off16<VEC, T>(a.in[F], b, t0 + i, c0)), bias);
+            float2 in = pair<VEC>(rows.v[1][i], off16<VEC, T>(a.in[BWD ? DY : X], b, t0 + i, c0));
+            float2 up, down;
+            sigmoids(f, up, down);
+            if (BWD && GATE) in = __fmul2_rn(in, silu<T>(pair<VEC>(rows.v[N - 1][i], off16<VEC, T>(a.in[Z], b, t0 + i, c0))));
+            if (!BWD && CONVEX) in = __fmul2_rn(down, in);
+            if (i < n) {
+                all.p = __fmul2_rn(all.p, up);
+                all.q = BWD ? __fmul2_rn(up, __fadd2_rn(in, all.q)) : __ffma2_rn(up, all.q, in);
+            }
+        }
+        all.p = some(all.p);
+        __syncwarp();
+        load(k + ST);
+    }
+    cp_async_wait();
+    Fold(*sums)[32] = reinterpret_cast<Fold(*)[32]>(smem);
+    __syncthreads();
+    sums[warp][lane] = all;
+    __syncthreads();
+    if (warp == 0) {
+        Fold f = sums[BWD ? WARPS - 1 : 0][lane];
+#pragma unroll
+        for (int i = 1; i < WARPS; i++) f = join(f, sums[BWD ? WARPS - 1 - i : i][lane]);
+        float* to = a.folds + (int64_t)blockIdx.y * 2 * a.D + c;
+        store2(to, f.p, valid);
+        store2(to + a.D, f.q, valid);
+    }
 }
 
 // One position: 4 channels a thread.
@@ -597,17 +720,34 @@ __global__ void __launch_bounds__(128) step_kernel(const T* __restrict__ x, int6
     store_pack<4>(y + b * D + c, o, valid, vec);
 }
 
-// CTAs of a cluster: doubled as long as SMs are left without a CTA, and further,
-// up to 800 CTAs, where each still has 4 tiles.
-// us forward and backward in bf16 (fp16) by CTAs of a cluster, 1, 2, 4, 8:
-// 1 x 2048 x 1536 37 22 12.5 12.2, 62 40 25 22; 6 x 777 x 2048 ragged
-// 23 24 28 43, 38 37 44 60; 8 x 2048 x 1536 64 54 57 68, 105 110 99 117;
-// 32 x 512 x 1536 48 55 72 145, 85 99 117 162.
-static inline int cluster_of(int batch, int L, int D, int tile) {
+// How a call's positions are shared out.
+// Few channels and a long sequence: chunks of at least 4 tiles, two CTAs an SM,
+// with a pass for each chunk's fold in front (which reads 2 operands, 3
+// backwards, a first time).  Else CTAs of a cluster: doubled as long as SMs are
+// left without a CTA, and further, up to 800 CTAs, where each still has 4 tiles.
+// us forward and backward in bf16, in clusters and in chunks:
+// 1 x 32768 x 512 (no gate) 64 40, 112 59; 1 x 32768 x 64 53 18, 94 21;
+// 1 x 8192 x 1024 45 31, 62 46; 2 x 8192 x 256 30 28, 38 29; but
+// 1 x 4096 x 256 8.7 17, 16 18; 4 x 4096 x 1024 47 53, 73 81.
+// By CTAs of a cluster, 1, 2, 4, 8: 1 x 2048 x 1536 37 22 12.5 12.2, 62 40 25 22;
+// 6 x 777 x 2048 ragged (fp16) 23 24 28 43, 38 37 44 60; 8 x 2048 x 1536
+// 64 54 57 68, 105 110 99 117; 32 x 512 x 1536 48 55 72 145, 85 99 117 162.
+struct Plan {
+    int cs, chunks, span;
+};
+static inline Plan plan_of(int batch, int L, int D, int tile) {
     const int64_t base = (int64_t)batch * cdiv(D, CB);
-    int cs = 1;
-    while (cs < MAX_CLUSTER && cs * tile < L && base * cs * 2 <= 800 && (base * cs < 148 || L >= (int64_t)cs * 8 * tile)) cs *= 2;
-    return cs;
+    Plan p = {1, 1, L};
+    if (base <= 37 && L / 64 >= tile) {
+        const int64_t room = 148 * 2 / base, most = L / (4 * tile);
+        p.span = cdiv(cdiv(L, (int)(room < most ? room : most)), tile) * tile;
+        p.chunks = cdiv(L, p.span);
+        return p;
+    }
+    while (p.cs < MAX_CLUSTER && p.cs * tile < L && base * p.cs * 2 <= 800 &&
+           (base * p.cs < 148 || L >= (int64_t)p.cs * 8 * tile))
+        p.cs *= 2;
+    return p;
 }
 
 // Clusters of more than 8 CTAs are not portable: whether this device takes them, asked once (by two bits a device).
@@ -648,9 +788,21 @@ static int launch(Args& a, cudaStream_t s) {
     else
         kernel = fwd_kernel<T, CONVEX, GATE, VEC>;
     if (!allow_smem(kernel, alone + MAX_CLUSTER * CTA_FOLDS, allowed)) return MI_ERR_CUDA;
+    if (a.chunks > 1) {
+        constexpr size_t bytes = sizeof(Rows<T, BWD && GATE ? 3 : 2, SUB, VEC>) * 2 * WARPS;
+        static std::atomic<uint64_t> let{0};
+        if (!allow_smem(chunk_kernel<T, CONVEX, GATE, VEC, BWD>, bytes, let)) return MI_ERR_CUDA;
+        const dim3 grid(cdiv(a.D, CB), a.batch * a.chunks);
+        if (BWD) {
+            chunk_kernel<T, CONVEX, GATE, VEC, BWD><<<grid, THREADS, bytes, s>>>(a);
+            MI_CHECK_LAUNCH();
+        } else {
+            MI_LAUNCH_DEPENDENT(chunk_kernel<T, CONVEX, GATE, VEC, BWD>, grid, THREADS, bytes, s, a);
+        }
+    }
     if (a.cs > 8 && !allow_wide_clusters(kernel, alone + MAX_CLUSTER * CTA_FOLDS, wide)) a.cs = 8;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cdiv(a.D, CB) * a.cs, a.batch);
+    cfg.gridDim = dim3(cdiv(a.D, CB) * a.cs, a.batch * a.chunks);
     cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = alone + (a.cs > 1 ? a.cs * CTA_FOLDS : 0);
     cfg.stream = s;
@@ -678,7 +830,9 @@ static int launch(Args& a, cudaStream_t s) {
 
 template <typename T, bool BWD>
 static int dispatch(Args& a, bool convex, bool vec, cudaStream_t s) {
-    a.cs = cluster_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS);
+    const Plan p = plan_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS);
+    a.cs = p.cs, a.chunks = p.chunks, a.span = p.span;
+    if (a.chunks > 1 && !a.folds) return MI_ERR_INVALID;
 #define MI_REC(CONVEX, GATE) return vec ? launch<T, CONVEX, GATE, true, BWD>(a, s) : launch<T, CONVEX, GATE, false, BWD>(a, s)
     if (convex) {
         if (a.in[Z].p) MI_REC(true, true);
@@ -714,10 +868,25 @@ extern "C" int64_t mi_gated_recurrence_checkpoints(int batch, int L, int D) {
     return (int64_t)batch * mi::cdiv(L, mi::rec::CK) * D;
 }
 
+namespace mi {
+namespace rec {
+static inline int64_t fold_bytes(const Plan& p, int batch, int D) {
+    return p.chunks > 1 ? (int64_t)sizeof(float) * batch * p.chunks * 2 * D : 0;
+}
+}  // namespace rec
+}  // namespace mi
+
+extern "C" int64_t mi_gated_recurrence_workspace(int batch, int L, int D, int backward, int dtype) {
+    if (batch <= 0 || L <= 0 || D <= 0 || dtype < 0 || dtype > 2) return 0;
+    const int sub = backward ? mi::rec::CK : dtype == MI_DT_F32 ? mi::rec::SUB_FWD<float> : mi::rec::SUB_FWD<__half>;
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, sub * mi::rec::WARPS);
+    return mi::rec::fold_bytes(p, batch, D) + (backward ? (int64_t)sizeof(float) * batch * p.chunks * p.cs * D : 0);
+}
+
 extern "C" int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch,
                                    int64_t f_row, const void* z, int64_t z_batch, int64_t z_row, const float* bias,
                                    const float* h0, const int32_t* lengths, void* y, float* h_out, float* checkpoints,
-                                   int batch, int L, int D, int convex, int dtype, void* stream) {
+                                   void* workspace, int batch, int L, int D, int convex, int dtype, void* stream) {
     mi::rec::Args a = {};
     a.in[mi::rec::X] = {x, x_batch, x_row}, a.in[mi::rec::F] = {f, f_batch, f_row}, a.in[mi::rec::Z] = {z, z_batch, z_row};
     const int rc = mi_rec_check(a.in[0], a.in[1], a.in[2], batch, L, D, dtype);
@@ -725,16 +894,12 @@ extern "C" int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row
     if (!y) return MI_ERR_INVALID;
     if (batch == 0) return MI_OK;
     a.bias = bias, a.h0 = h0, a.lengths = lengths, a.y = y, a.hT = h_out, a.ckpt = checkpoints;
+    a.folds = static_cast<float*>(workspace);
     a.batch = batch, a.L = L, a.D = D;
     const int e = mi::rec::elem_size(dtype);
     a.ovec = D % 2 == 0 && reinterpret_cast<uintptr_t>(y) % (2 * e) == 0;
     const bool vec = mi::rec::rows_vec(a, D, dtype);
     MI_DISPATCH_DTYPE(dtype, T, return (mi::rec::dispatch<T, false>(a, convex, vec, (cudaStream_t)stream)););
-}
-
-extern "C" int64_t mi_gated_recurrence_backward_workspace(int batch, int L, int D) {
-    if (batch <= 0 || L <= 0 || D <= 0) return 0;
-    return (int64_t)sizeof(float) * batch * D * mi::rec::cluster_of(batch, L, D, mi::rec::CK * mi::rec::WARPS);
 }
 
 extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, int64_t dy_row, const float* dh_out,
@@ -756,8 +921,11 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
         return MI_OK;
     }
     a.bias = bias, a.dhT = dh_out, a.lengths = lengths, a.ckpt = const_cast<float*>(checkpoints);
-    a.dx = dx, a.df = df, a.dz = dz, a.dh0 = dh0, a.part = dbias ? static_cast<float*>(workspace) : nullptr;
+    a.dx = dx, a.df = df, a.dz = dz, a.dh0 = dh0;
     a.batch = batch, a.L = L, a.D = D;
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, mi::rec::CK * mi::rec::WARPS);
+    a.folds = static_cast<float*>(workspace);
+    if (dbias) a.part = a.folds + mi::rec::fold_bytes(p, batch, D) / (int64_t)sizeof(float);
     const int e = mi::rec::elem_size(dtype);
     a.ovec = D % 2 == 0;
     for (const void* p : {dx, df, z ? dz : nullptr}) a.ovec = a.ovec && reinterpret_cast<uintptr_t>(p) % (2 * e) == 0;
@@ -765,7 +933,7 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
     int rc2 = MI_ERR_INVALID;
     MI_DISPATCH_DTYPE(dtype, T, (rc2 = mi::rec::dispatch<T, true>(a, convex, vec, s)););
     if (rc2 != MI_OK || !dbias) return rc2;
-    mi::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, s>>>(a.part, dbias, batch * a.cs, D);
+    mi::column_sum_kernel<<<mi::cdiv(D, 32), 1024, 0, s>>>(a.part, dbias, batch * a.chunks * a.cs, D);
     MI_CHECK_LAUNCH();
     return MI_OK;
 }

@@ -36,7 +36,7 @@ using OptTensor = std::optional<Tensor>;
     X(mi_causal_conv1d_backward_workspace) X(mi_causal_conv1d_step) X(mi_rms_norm) X(mi_rms_norm_quant)      \
     X(mi_rms_norm_backward) X(mi_rms_norm_backward_workspace) X(mi_gated_recurrence)                         \
     X(mi_gated_recurrence_checkpoints) X(mi_gated_recurrence_backward)                                       \
-    X(mi_gated_recurrence_backward_workspace) X(mi_gated_recurrence_step) X(mi_layer_norm)                   \
+    X(mi_gated_recurrence_workspace) X(mi_gated_recurrence_step) X(mi_layer_norm)                   \
     X(mi_layer_norm_backward) X(mi_layer_norm_backward_workspace) X(mi_sample_rows)
 
 struct Entries {
@@ -485,9 +485,10 @@ std::tuple<Tensor, Tensor, Tensor> rec_forward(const Tensor& x, const Tensor& f,
     Place place(x);
     Tensor y = at::empty({batch, L, d}, x.options()), h = floats({batch, d}, x), ckpt;
     if (keep) ckpt = floats({mi.mi_gated_recurrence_checkpoints(batch, L, d)}, x);
+    Tensor ws = workspace(mi.mi_gated_recurrence_workspace(batch, L, d, 0, dtype_code(x)), x);
     check(mi.mi_gated_recurrence(ptr(x), st(x, 0), st(x, 1), ptr(f), st(f, 0), st(f, 1), ptr(z), st(z, 0), st(z, 1),
                                  fptr(bias), fptr(h0), static_cast<int32_t*>(ptr(lengths)), ptr(y), fptr(h), fptr(ckpt),
-                                 batch, L, d, convex, dtype_code(x), place.stream),
+                                 ptr(ws), batch, L, d, convex, dtype_code(x), place.stream),
           "mi_gated_recurrence");
     return {y, h, ckpt};
 }
@@ -517,8 +518,8 @@ struct GatedRecurrence : torch::autograd::Function<GatedRecurrence> {
         const Tensor dy = g[0].defined() ? unit(g[0]) : at::zeros({batch, L, d}, x.options());
         const Tensor dh = g[1].defined() ? aligned(g[1]) : Tensor();
         Tensor dx = empty_as(x), df = empty_as(f), dz = empty_as(z), dbias = empty_as(bias, need & 1);
-        Tensor dh0 = need & 2 ? floats({batch, d}, x) : Tensor(), ws;
-        if (need & 1) ws = workspace(mi.mi_gated_recurrence_backward_workspace(batch, L, d), x);
+        Tensor dh0 = need & 2 ? floats({batch, d}, x) : Tensor();
+        Tensor ws = workspace(mi.mi_gated_recurrence_workspace(batch, L, d, 1, dtype_code(x)), x);
         check(mi.mi_gated_recurrence_backward(
                   ptr(dy), st(dy, 0), st(dy, 1), fptr(dh), ptr(x), st(x, 0), st(x, 1), ptr(f), st(f, 0), st(f, 1), ptr(z),
                   st(z, 0), st(z, 1), fptr(bias), static_cast<int32_t*>(ptr(lengths)), fptr(ckpt), ptr(dx), ptr(df),

@@ -94,6 +94,23 @@ def test_recurrence_options(sel, cuda_dev, n, convex, z, bias, h0):
     check_rec_grads(got, a, None, dh)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("d", [66, 72])
+def test_recurrence_long_sequences(sel, cuda_dev, dtype, d):
+    """Few channels and many positions, which are shared out in chunks; lengths that end at a chunk's border, inside one, in
+    front of all."""
+    n, lens = 4500, [4500, 1024, 1027, 0, 3333]
+    a = rec_inputs(cuda_dev, dtype, 5, n, d, h0=True, lengths=lens)
+    a["bias"] += 3  # memories long enough to reach through chunks
+    dy, dh = torch.randn(5, n, d, device=cuda_dev).to(dtype), torch.randn(5, d, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+    with torch.no_grad():
+        again = call_rec(sel, a)
+    assert torch.equal(again[0], y) and torch.equal(again[1], h)
+
+
 @pytest.mark.parametrize("n", [37, 260])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_recurrence_lengths(sel, cuda_dev, n, dtype):

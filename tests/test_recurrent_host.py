@@ -122,7 +122,7 @@ def test_entry_points_refuse_on_the_host():
     p, s, none = 256, (256, 512, 64), (None, 0, 0)
 
     def fwd(x=s, f=s, z=none, y=p, batch=2, L=8, D=64, dtype=0):
-        return lib.mi_gated_recurrence(*x, *f, *z, None, None, None, y, p, None, batch, L, D, 1, dtype, None)
+        return lib.mi_gated_recurrence(*x, *f, *z, None, None, None, y, p, None, None, batch, L, D, 1, dtype, None)
     assert fwd(x=none) == -1 and fwd(f=none) == -1 and fwd(y=None) == -1
     assert fwd(L=0) == -1 and fwd(L=-1) == -1 and fwd(D=0) == -1 and fwd(batch=-1) == -1
     assert fwd(dtype=3) == -1 and fwd(dtype=-1) == -1 and fwd(z=(256, -1, 64)) == -1
@@ -147,7 +147,9 @@ def test_entry_points_refuse_on_the_host():
     assert pick(x=None) == -1 and pick(u=None) == -1 and pick(token=None) == -1 and pick(rows=-1) == -1 and pick(V=0) == -1
     assert pick(ld=-1) == -1 and pick(dtype=3) == -1 and pick(V=262145) == -2 and pick(rows=0) == 0
     assert lib.mi_gated_recurrence_checkpoints(2, 17, 5) == 2 * 3 * 5
-    assert lib.mi_gated_recurrence_backward_workspace(1, 64, 64) == 4 * 64
+    assert lib.mi_gated_recurrence_workspace(1, 64, 64, 1, 1) == 4 * 64
+    assert lib.mi_gated_recurrence_workspace(1, 64, 64, 0, 1) == 0
+    assert lib.mi_gated_recurrence_workspace(1, 65536, 64, 0, 1) > 0 and fwd(batch=1, L=65536) == -1  # it wants the workspace
 
 
 def slopes(value, leaves, got, prefix="d"):
