@@ -11,22 +11,27 @@
 // (order-preserving bits of l, mask - index), which no two tokens share.
 //
 // Borders between tokens are sharp, so masses are whole numbers: w in units of
-// 2^-44 from a 64-bit evaluation (7e-12 relative), which add up exactly and in
+// 2^-44 from a 64-bit evaluation (1.3e-12 relative), which add up exactly and in
 // any order.  fp32 weights would move the borders of a flat distribution over
 // 32768 tokens by 1e-8 each, one row in some ten thousand.
 //
-// What bounds it: the logits come from HBM once and from L2 after that; a
-// 64-bit weight is 16 operations of half rate, so a pass over all weights costs as
-// much as the first read, and the filters are arranged to need few of them.  A
-// row's 512 groups of tokens (a thread's, or those of some threads of a cluster)
-// have a maximum each: the k-th largest of these is below no k tokens, and where
-// the largest of them hold p of the total mass, the smallest of those is below all
-// that top-p keeps.  What lies above such a bound, a few tokens more than are kept, is
-// listed, and the rest is done on the list.  Lists that would be too long (large k,
-// flat distributions) go by histograms over bins of equal width below the maximum
-// instead, then by the leading bits of the keys, until the border's bin is a list.
+// What bounds it: the logits come from HBM once and from L2 after that; a weight
+// is 10 operations of 64 bits and 20 around them, so issue slots bound a pass over
+// all weights (256 x 32768: 10 us against 5 for the first read), and the filters
+// are arranged to need few of them.
+//   A row's 512 groups of tokens (a thread's, or those of some threads of a
+// cluster) have a maximum each: no fewer than k tokens lie at or above the k-th
+// largest of these.  What does, a few tokens more than are kept, is listed, sorted
+// and chosen from (256 x 32768 fp32, k = 50: 18 us).
+//   Top-p, and top-k whose list would be too long, go by counts in 2048 bins of equal
+// width below the maximum, which leave some bins in which the border can lie, and
+// one pass over the weights (p = 0.9: 52 us).
+//   What is left, top-p of a large top-k and rows of equal logits, goes by
+// histograms of the masses and then by the leading bits of the keys.
 //
-// A row belongs to one CTA, or to a cluster of up to 8 where rows are few.
+// A row belongs to one CTA, or to a cluster of up to 8 where rows are few (a
+// barrier of a cluster costs about 0.5 us: 256 x 32768 with k = 50 17 us in one CTA
+// a row, 28 in two; 4 x 32768 with p = 0.9 in one 54, in four 18).
 #include <cooperative_groups.h>
 
 #include "mi_elem.cuh"

@@ -686,3 +686,21 @@ def test_prompt_steps_and_choices_of_all(sel, kernels, cuda_dev):
                 assert near < 1e-6 or int(tok[b]) == want  # 0.8 and 0.95 as fp32 numbers move a border by 1e-7
             seq = torch.cat([seq, tok[:, None]], 1)
             logits, states = net.forward(Ours(sel, step=True), tok, states)
+
+
+def test_integration_example(sel, kernels, cuda_dev):
+    """The recurrent layer's calls of INTEGRATION.md as they are written there."""
+    import os
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")) as f:
+        code = f.read().split("## 1b.")[1].split("```python\n")[2].split("```")[0]
+    b, n, d, width = 3, 10, 64, 32
+    r = lambda *s: torch.randn(*s, device=cuda_dev)  # noqa: E731
+    v = dict(torch=torch, selective=sel, kernels=kernels, d=d, x=r(b, n, width), residual=r(b, n, width), ln_w=r(width),
+             ln_b=r(width), w_in=r(3 * d, width), gate_b=r(d) + 2, rows1=r(b, 3 * d), logits=r(b, 500), u=torch.rand(b, device=cuda_dev),
+             lengths=torch.tensor([10, 4, 0], dtype=torch.int32, device=cuda_dev))
+    exec(code, v)
+    for i, e in enumerate((10, 4, 0)):  # the tokens go on from each sequence's own length
+        rows = torch.cat([v["rows"][i:i + 1, :e], v["rows1"][i:i + 1, None]], 1)
+        want = ref.recurrence(dict(x=rows[..., :d], f=rows[..., d:2 * d], z=rows[..., 2 * d:], bias=v["gate_b"]))
+        ref.check(v["s1"][i], tuple(t[0, -1] for t in want["y"]), "s1")
+    assert v["tok"].tolist() == [ref.sample(v["logits"][i], float(v["u"][i]), float(torch.tensor(0.8)), 50, 1.0, 0.0)[0] for i in range(b)]
