@@ -55,6 +55,7 @@ class Sampling:
             raise ValueError(f"temperature must be 0 (greedy) or more and finite, got {self.temperature}")
         if not 0 <= int(self.top_k) < 2 ** 31 or int(self.top_k) != self.top_k:
             raise ValueError(f"top_k must be a whole number from 0 (off) on, got {self.top_k}")
+        object.__setattr__(self, "top_k", int(self.top_k))
         if not 0 <= self.top_p <= 1:
             raise ValueError(f"top_p must be from 0 to 1, got {self.top_p}")
         if not 0 <= self.min_p <= 1:
