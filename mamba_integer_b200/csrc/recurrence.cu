@@ -12,8 +12,8 @@
 //
 // A position and channel move 3 elements forward (4 with z) and meet 2 (4)
 // special-function results, so HBM bounds it as long as enough loads are in
-// flight and the instructions are few (30 a channel and position with z, of
-// which 4 are special functions).  32 x 512 x 1536 bf16 with z: forward 50 us
+// flight and the instructions are few (33 a channel and position with z, of
+// which 4 are special functions; 57 backward).  32 x 512 x 1536 bf16 with z: forward 50 us
 // (201 MB, 4.0 TB/s), 36 without the arithmetic; backward 84 (352 MB, 4.2 TB/s),
 // 78 without: what is left is two CTAs of 128 registers a thread an SM, whose
 // warps load, wait for the fold and store by turns.

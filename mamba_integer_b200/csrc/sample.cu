@@ -31,7 +31,7 @@
 //
 // A row belongs to one CTA, or to a cluster of up to 8 where rows are few (a
 // barrier of a cluster costs about 0.5 us: 256 x 32768 with k = 50 17 us in one CTA
-// a row, 28 in two; 4 x 32768 with p = 0.9 in one 54, in four 18).
+// a row, 28 in two; 4 x 32768 with p = 0.9 in one 54, in four 19).
 #include <cooperative_groups.h>
 
 #include "mi_elem.cuh"
