@@ -423,13 +423,23 @@ __global__ void __launch_bounds__(MAX_BLOCK, 1) bwd_kernel(const Args a) {
         float* to = rows > 1 ? sh + group * a.D : part + which * a.D;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int j = 0; j < NV; j++) {
+            if (VEC) {  // 16 bytes a store; with 4 the call took 60.0 us instead of 54.9 (4096 x 4096 bf16, fp32 residual)
+                if (!cols.any(j)) continue;
+#pragma unroll
+                for (int i = 0; i < K; i += 4) {
+                    const float2 u = which ? db[j][i / 2] : dw[j][i / 2], v = which ? db[j][i / 2 + 1] : dw[j][i / 2 + 1];
+                    *reinterpret_cast<float4*>(to + cols.at(j) + i) = make_float4(u.x, u.y, v.x, v.y);
+                }
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < K / 2; i++) {
                 const float2 v = which ? db[j][i] : dw[j][i];
                 if (cols.has(j, 2 * i)) to[cols.at(j, 2 * i)] = v.x;
                 if (cols.has(j, 2 * i + 1)) to[cols.at(j, 2 * i + 1)] = v.y;
             }
+        }
         if (rows == 1) continue;
         __syncthreads();
         for (int c = tid; c < a.D; c += block) {
@@ -633,7 +643,7 @@ extern "C" int mi_layer_norm_backward(const void* dy, const void* dsum, const vo
     a.part = sums ? static_cast<float*>(workspace) : nullptr;
     a.T = T, a.D = D;
     const bool vec = D % 8 == 0 && lds % 8 == 0 && mi::aligned16(dy) && mi::aligned16(s) && mi::aligned16(weight) &&
-                     (!dsum || mi::aligned16(dsum)) &&
+                     (!dsum || mi::aligned16(dsum)) && (!sums || mi::aligned16(workspace)) &&
                      (!dx || mi::aligned16(dx)) && (!dresidual || mi::aligned16(dresidual));
     const mi::ln::Plan p = mi::ln::backward_plan(T, D);
     const int rc2 = mi::ln::dispatch<true>(a, p, vec, dtype, rdtype, st);
