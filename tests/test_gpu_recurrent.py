@@ -1,5 +1,6 @@
 """The float recurrent layer's operators against their 64-bit formulas (tests/recurrent_ref.py, where the tolerances are
 derived)."""
+import numpy as np
 import pytest
 import torch
 
@@ -211,6 +212,82 @@ def test_recurrence_step(sel, cuda_dev, dtype, size, convex, z, bias):
             ys.append(sel.gated_recurrence_step(h, a["x"][:, t], a["f"][:, t], z=None if a["z"] is None else a["z"][:, t],
                                                 gate_bias=a["bias"], convex=convex))
     check_rec(torch.stack(ys, 1), h, a)
+
+
+# Output gates over the types' whole range.  sigmoid reaches 0 within 110 of 0, where z sigmoid(z) and its slope are 0 too.
+GATES = [-85.0, -87.5, -89.0, -95.0, -110.0, -1e4, -1e30, -1e34, -1e37, "lowest", 60.0, 86.0, 88.0, 100.0, 1e3]
+
+
+def gate_rows(dtype, dev, b, n, d):
+    """A z of each of GATES at every channel, between ordinary ones."""
+    z = torch.randn(b, n, d, generator=torch.Generator().manual_seed(9))
+    low = torch.finfo(dtype).min
+    for i, v in enumerate(GATES):
+        z[:, 1 + 2 * i] = low if v == "lowest" else max(v, low)
+    return z.to(dtype).to(dev)
+
+
+def check_gated(got, want, error, name):
+    """`error`: absolute, before the result's own rounding (half a step, or half the smallest subnormal)."""
+    dtype = got.dtype
+    tol = error + torch.finfo(dtype).eps / 2 * (want.abs() + error) + torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2
+    off = (got.detach().cpu().double() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), (name, bad.nonzero()[:6].tolist(), got.cpu()[bad][:6], want[bad][:6])
+
+
+def check_output_gate(a, y, dz=None, dy=None):
+    """y and dz from the states' own errors (the formula without a gate) and the gate's.
+
+    sigmoid(z) and sigmoid(-z) are off by 10 units and 3 |z| more of the smaller one (tests/recurrent_ref.py).  One below
+    e^-87 (fp32) or 2^-126 (16 bits) counts as 0; with the roundings of z and of the power, up to 1.0001 times that."""
+    z = ref.d64(a["z"])
+    plain, mags = dict(a, z=None), dict(a, z=None, x=a["x"].abs(), h0=None if a["h0"] is None else a["h0"].abs())
+    want = ref.recurrence(plain)
+    h, e_h = want["y"]
+    m_h = ref.recurrence(mags)["y"][0]
+    s, n = torch.sigmoid(z), torch.sigmoid(-z)
+    r_s, r_n = (torch.where(q > 0.5, 10.0, 9 + 3 * z.abs()) for q in (s, n))
+    U, least = 2.0 ** -24, 1.0001 * (np.exp(-87.0) if y.dtype == F32 else 2.0 ** -126)
+    lost = lambda q: torch.where(q < least, q, 0.0)  # noqa: E731
+    gate, slope, m_slope = z * s, s + z * s * n, s + z.abs() * s * n
+    e_gate = U * (r_s + 2) * gate.abs() + z.abs() * lost(s)
+    e_slope = U * ((r_s + 2) * s + (r_s + r_n + 4) * z.abs() * s * n) + lost(s) * (1 + z.abs() * n) + lost(n) * z.abs() * s
+    check_gated(y, h * gate, U * e_h * gate.abs() + m_h * e_gate + 2.0 ** -149, "y")
+    if dz is not None:
+        g = ref.d64(dy).abs()
+        error = g * (U * e_h * m_slope + m_h * (e_slope + 2 * U * m_slope)) + 2.0 ** -149 * (1 + g)
+        check_gated(dz, ref.d64(dy) * h * slope, error, "dz")
+
+
+@pytest.mark.parametrize("d", [40, 41])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_output_gate_over_its_whole_range(sel, cuda_dev, dtype, d):
+    n = 37
+    a = rec_inputs(cuda_dev, dtype, 2, n, d, h0=True)
+    a["z"] = gate_rows(dtype, cuda_dev, 2, n, d)
+    dy, dh = torch.randn(2, n, d, device=cuda_dev).to(dtype), torch.randn(2, d, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_output_gate(a, y, got["z"], dy)
+    check_rec_grads({k: t for k, t in got.items() if k != "z"}, a, dy, dh)  # a gate of 0 passes nothing on
+    with torch.no_grad():
+        assert torch.equal(call_rec(sel, a)[0], y)
+    for v in (float("-inf"), float("nan")):  # 0 times an infinity, as in the formula
+        a["z"][:, 5] = v
+        assert call_rec(sel, a)[0][:, 5].isnan().all() and not call_rec(sel, a)[0][:, 6].isnan().any()
+
+
+@pytest.mark.parametrize("d", [40, 41])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_step_output_gate_over_its_whole_range(sel, cuda_dev, dtype, d):
+    n = 37
+    a = rec_inputs(cuda_dev, dtype, 2, n, d, h0=True)
+    a["z"] = gate_rows(dtype, cuda_dev, 2, n, d)
+    h, ys = a["h0"].clone(), []
+    for t in range(n):
+        with torch.no_grad():
+            ys.append(sel.gated_recurrence_step(h, a["x"][:, t], a["f"][:, t], z=a["z"][:, t], gate_bias=a["bias"]))
+    check_output_gate(a, torch.stack(ys, 1))
 
 
 def test_recurrence_same_bits_and_streams(sel, cuda_dev):
