@@ -159,6 +159,10 @@ __device__ __forceinline__ void row_sync(int tpr) {
     else
         __syncwarp();
 }
+// Behind a reduction, before the row's window is filled again by all of its threads:
+// every one has read it.  Rows of several warps have met at the reduction's barrier;
+// the shuffles of those within a warp put no order on shared memory.
+__device__ __forceinline__ void window_read() { __syncwarp(); }
 template <typename T>
 __device__ __forceinline__ float2 two(const Pack<T, K>& p, int i) {
     return make_float2(to_f(p.v[2 * i]), to_f(p.v[2 * i + 1]));
@@ -233,7 +237,10 @@ __global__ void __launch_bounds__(BLOCK, BLOCK > 256 ? 1 : 2) fwd_kernel(const A
         if (VEC) fetch(t + ST * step, k);
         float sum[1] = {__fadd_rn(acc.x, acc.y)};
         reduce(sum);
-        if (!VEC) fetch(t + ST * step, k);  // behind the reduction all of the row's threads have read the window
+        if (!VEC) {
+            window_read();
+            fetch(t + ST * step, k);
+        }
         k = k + 1 == ST ? 0 : k + 1;
         const float mean = __fdiv_rn(sum[0], n);
         acc = dup(0.0f);
@@ -389,7 +396,10 @@ __global__ void __launch_bounds__(MAX_BLOCK, 1) bwd_kernel(const Args a) {
         }
         if (VEC) fetch(t0 + ST * AT * step, k);
         reduce(sums);
-        if (!VEC) fetch(t0 + ST * AT * step, k);
+        if (!VEC) {
+            window_read();
+            fetch(t0 + ST * AT * step, k);
+        }
         k = k + 1 == ST ? 0 : k + 1;
         if (!a.dx && !a.dr) continue;
 #pragma unroll

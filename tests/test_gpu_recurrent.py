@@ -393,6 +393,22 @@ def test_layer_norm_many_rows(sel, cuda_dev, t, d):
     check_norm(sel, norm_inputs(cuda_dev, BF16, t, d, rdtype=BF16))
 
 
+@pytest.mark.parametrize("d", [3, 31, 33, 65, 129, 255])
+@pytest.mark.parametrize("dtype,rdtype", [(F32, F32), (BF16, BF16), (F16, F32)])
+def test_layer_norm_many_narrow_odd_rows(sel, cuda_dev, dtype, rdtype, d):
+    """Rows of 4 to 32 threads whose windows are filled many times over by other lanes, the sum's gradient among them; the
+    same bits in every run."""
+    t = 20011
+    a = norm_inputs(cuda_dev, dtype, t, d, rdtype=rdtype)
+    check_norm(sel, a)
+    leaves = {k: a[k].detach().clone().requires_grad_(True) for k in ("x", "w", "b", "r")}
+    runs = []
+    for _ in range(5):
+        y, s = sel.layer_norm(leaves["x"], leaves["w"], leaves["b"], eps=EPS, residual=leaves["r"])
+        runs.append([y.detach(), s.detach(), *torch.autograd.grad([y, s], list(leaves.values()), [a["dy"], a["dsum"]])])
+    assert all(torch.equal(p, q) for run in runs[1:] for p, q in zip(runs[0], run))
+
+
 def test_layer_norm_rows_far_from_zero(sel, cuda_dev):
     """A mean a thousand times the spread, rows that are constant, and rows of zeros."""
     a = norm_inputs(cuda_dev, F32, 40, 700, offset=1000.0)
