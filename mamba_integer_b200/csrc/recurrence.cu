@@ -167,30 +167,12 @@ __device__ __forceinline__ Fold join(const Fold& a, const Fold& b) {  // a, then
     return {some(__fmul2_rn(a.p, b.p)), __ffma2_rn(b.p, a.q, b.q)};
 }
 
-// ---------------------------------------------------------------------------
-// barriers in shared memory
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void bar_init(uint64_t* bar) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_at(bar)) : "memory");
-}
-__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok)
-                 : "r"(smem_at(bar)), "r"(parity)
-                 : "memory");
-    return ok != 0;
-}
 // Bounded: after about 2 s the device's error word is set and the wait given up.
 __device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity) {
-    if (bar_try(bar, parity)) return;
+    if (mbar_try(smem_u32(bar), parity)) return;
     const long long t0 = clock64();
-    while (!bar_try(bar, parity)) {
-        if (clock64() - t0 > 4000000000LL) {
+    while (!mbar_try(smem_u32(bar), parity)) {
+        if (clock64() - t0 > WAIT_CYCLES) {
             raise_dev_error(MI_DEV_TIMEOUT);
             return;
         }
@@ -302,7 +284,7 @@ __device__ __forceinline__ float2 exchange(Exchange& ex, Fold* folds, int round,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = round & 1;
     mine.p = some(mine.p);
     ex.warp[k][warp][lane] = mine;
-    if (cs > 1 && threadIdx.x == 0) bar_expect(&ex.arrived[k], cs * 32 * sizeof(Fold));
+    if (cs > 1 && threadIdx.x == 0) mbar_expect_tx(smem_u32(&ex.arrived[k]), cs * 32 * sizeof(Fold));
     __syncthreads();
     float2 from = s;
     if (cs == 1) {
@@ -319,8 +301,8 @@ __device__ __forceinline__ float2 exchange(Exchange& ex, Fold* folds, int round,
         for (int i = 1; i < WARPS; i++) all = join(all, ex.warp[k][i][lane]);
         for (int i = warp; i < cs; i += WARPS) {
             uint32_t to, bar;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_at(&folds[(k * cs + rank) * 32 + lane])), "r"(i));
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_at(&ex.arrived[k])), "r"(i));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&folds[(k * cs + rank) * 32 + lane])), "r"(i));
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&ex.arrived[k])), "r"(i));
             asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
                          "f"(all.p.x), "f"(all.p.y), "f"(all.q.x), "f"(all.q.y), "r"(bar)
                          : "memory");
@@ -336,7 +318,7 @@ __device__ __forceinline__ float2 exchange(Exchange& ex, Fold* folds, int round,
 }
 
 __device__ __forceinline__ void begin(Exchange& ex, int cs) {
-    if (threadIdx.x < 2) bar_init(&ex.arrived[threadIdx.x]);
+    if (threadIdx.x < 2) mbar_init(smem_u32(&ex.arrived[threadIdx.x]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (cs > 1)
         cooperative_groups::this_cluster().sync();
