@@ -451,6 +451,7 @@ int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const 
  * mi_gated_recurrence_workspace(.., 0, dtype) bytes.  L >= 1.  Gate logits count as
  * at most 87 from 0, so that gates never reach 0: infinite states stay infinite.
  * z has no such bound: sigmoid(z) below e^-87 (2^-126 in 16 bits) counts as 0.
+ * A wait between CTAs that runs out (MI_DEV_TIMEOUT) leaves NaN in what follows.
  */
 int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,
                         const void* z, int64_t z_batch, int64_t z_row, const float* bias, const float* h0,

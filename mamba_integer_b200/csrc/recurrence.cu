@@ -33,18 +33,16 @@
 // stretch's P is at least 2^-126, so that an infinite state stays infinite and an
 // infinite input reaches it, whether or not a stretch is folded.  (A state of
 // 1e38 leaves up to 1 of itself behind a stretch that forgets it.)
-#include <cooperative_groups.h>
-
 #include <type_traits>
 
 #include "mi_elem.cuh"
+#include "mi_folds.cuh"
 
 namespace mi {
 namespace rec {
 
-constexpr int WARPS = 8, THREADS = WARPS * 32, CB = 64;  // channels a CTA
+constexpr int CB = 64;         // channels a CTA
 constexpr int CK = 8;          // positions between the states kept for the backward pass
-constexpr int MAX_CLUSTER = 16;
 
 struct Seq {  // a [batch, L, D] operand with unit last stride
     const void* p;
@@ -77,8 +75,6 @@ __device__ __forceinline__ int length_of(const Args& a, int b) {
     const int n = a.lengths[b];
     return n < 0 ? 0 : (n < a.L ? n : a.L);
 }
-
-__device__ __forceinline__ float2 dup(float v) { return make_float2(v, v); }
 
 // sigmoid(v) and sigmoid(-v), neither taken from 1 minus the other, for |v| up
 // to 87 (beyond it counts as 87; a NaN stays one).  The product with log2(e) is
@@ -152,30 +148,6 @@ __device__ __forceinline__ void put(T* p, float2 v, int valid, bool vec) {
     } else {
         const float o[2] = {v.x, v.y};
         store_pack<2>(p, o, valid, vec);
-    }
-}
-
-// what a stretch of positions does to the state of two channels: s -> p s + q
-struct Fold {
-    float2 p, q;
-};
-__device__ __forceinline__ float2 fold(float2 s, const Fold& f) { return __ffma2_rn(f.p, s, f.q); }
-__device__ __forceinline__ float2 some(float2 p) {
-    return make_float2(max_nan(p.x, 1.17549435e-38f), max_nan(p.y, 1.17549435e-38f));
-}
-__device__ __forceinline__ Fold join(const Fold& a, const Fold& b) {  // a, then b
-    return {some(__fmul2_rn(a.p, b.p)), __ffma2_rn(b.p, a.q, b.q)};
-}
-
-// Bounded: after about 2 s the device's error word is set and the wait given up.
-__device__ __forceinline__ void bar_wait(uint64_t* bar, uint32_t parity) {
-    if (mbar_try(smem_u32(bar), parity)) return;
-    const long long t0 = clock64();
-    while (!mbar_try(smem_u32(bar), parity)) {
-        if (clock64() - t0 > WAIT_CYCLES) {
-            raise_dev_error(MI_DEV_TIMEOUT);
-            return;
-        }
     }
 }
 
@@ -265,66 +237,9 @@ __device__ __forceinline__ uint32_t off16(const Seq& s, int b, int t, int c0) {
                       (16 / sizeof(T)));
 }
 
-// The folds of a round, in order: `mine` is this warp's, `s` the state that the
-// round starts from.  Returns the state that this warp starts from; s becomes
-// the state after the round.  Rounds alternate between two sets of slots: whoever
-// writes to one has seen the other's round end, which all read the first before.
-struct Exchange {
-    Fold warp[2][WARPS][32];
-    uint64_t arrived[2];
-};
-constexpr size_t CTA_FOLDS = sizeof(Fold) * 2 * 32;  // bytes for each CTA of a cluster, [2][cluster][32] behind the rows
-
 // Slots a warp: as many as leave room for two CTAs an SM.
 template <typename R>
 constexpr int STAGES = sizeof(R) * WARPS * 2 + sizeof(Exchange) + 8 * CTA_FOLDS <= 113 * 1024 ? 2 : 1;
-
-__device__ __forceinline__ float2 exchange(Exchange& ex, Fold* folds, int round, int cs, int rank, Fold mine,
-                                           float2& s) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, k = round & 1;
-    mine.p = some(mine.p);
-    ex.warp[k][warp][lane] = mine;
-    if (cs > 1 && threadIdx.x == 0) mbar_expect_tx(smem_u32(&ex.arrived[k]), cs * 32 * sizeof(Fold));
-    __syncthreads();
-    float2 from = s;
-    if (cs == 1) {
-#pragma unroll
-        for (int i = 0; i < WARPS; i++) {
-            if (i == warp) from = s;
-            s = fold(s, ex.warp[k][i][lane]);
-        }
-        return from;
-    }
-    if (warp < cs) {  // warp i tells CTA i (and i + 8)
-        Fold all = ex.warp[k][0][lane];
-#pragma unroll
-        for (int i = 1; i < WARPS; i++) all = join(all, ex.warp[k][i][lane]);
-        for (int i = warp; i < cs; i += WARPS) {
-            uint32_t to, bar;
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&folds[(k * cs + rank) * 32 + lane])), "r"(i));
-            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&ex.arrived[k])), "r"(i));
-            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
-                         "f"(all.p.x), "f"(all.p.y), "f"(all.q.x), "f"(all.q.y), "r"(bar)
-                         : "memory");
-        }
-    }
-    bar_wait(&ex.arrived[k], (round >> 1) & 1);
-    for (int i = 0; i < cs; i++) {
-        if (i == rank) from = s;
-        s = fold(s, folds[(k * cs + i) * 32 + lane]);
-    }
-    for (int i = 0; i < warp; i++) from = fold(from, ex.warp[k][i][lane]);
-    return from;
-}
-
-__device__ __forceinline__ void begin(Exchange& ex, int cs) {
-    if (threadIdx.x < 2) mbar_init(smem_u32(&ex.arrived[threadIdx.x]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (cs > 1)
-        cooperative_groups::this_cluster().sync();
-    else
-        __syncthreads();
-}
 
 // A chunk's place in its sequence of `len` positions.
 struct Chunk {
