@@ -447,7 +447,7 @@ int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const 
  *   y[t] = h[t] * z sigmoid(z) (h[t] with z NULL)
  * x, f, z, y [batch, L, D]; bias [D]; h0, h_out [batch, D]; z, bias, h0,
  * lengths, h_out may be NULL.  checkpoints (NULL without a backward pass):
- * mi_gated_recurrence_checkpoints() floats.  workspace (NULL if 0):
+ * mi_gated_recurrence_checkpoints() floats, 8-byte aligned.  workspace (NULL if 0):
  * mi_gated_recurrence_workspace(.., 0, dtype) bytes.  L >= 1.  Gate logits count as
  * at most 87 from 0, so that gates never reach 0: infinite states stay infinite.
  * z has no such bound: sigmoid(z) below e^-87 (2^-126 in 16 bits) counts as 0.

@@ -615,6 +615,7 @@ extern "C" int mi_layer_norm(const void* x, int64_t ldx, const void* residual, i
                              const float* bias, void* y, void* sum, float* stats, int T, int D, float eps, int dtype,
                              int rdtype, void* stream) {
     if (!x || !weight || !y || (residual && !sum) || ldx < 0 || (residual && ldr < 0)) return MI_ERR_INVALID;
+    if (reinterpret_cast<uintptr_t>(stats) & 7) return MI_ERR_INVALID;
     const int rc = mi_ln_check(T, D);
     if (rc != MI_OK) return rc;
     if (T == 0) return MI_OK;

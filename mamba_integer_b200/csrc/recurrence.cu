@@ -795,7 +795,7 @@ extern "C" int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row
     a.in[mi::rec::X] = {x, x_batch, x_row}, a.in[mi::rec::F] = {f, f_batch, f_row}, a.in[mi::rec::Z] = {z, z_batch, z_row};
     const int rc = mi_rec_check(a.in[0], a.in[1], a.in[2], batch, L, D, dtype);
     if (rc != MI_OK) return rc;
-    if (!y) return MI_ERR_INVALID;
+    if (!y || (reinterpret_cast<uintptr_t>(checkpoints) & 7)) return MI_ERR_INVALID;
     if (batch == 0) return MI_OK;
     a.bias = bias, a.h0 = h0, a.lengths = lengths, a.y = y, a.hT = h_out, a.ckpt = checkpoints;
     a.folds = static_cast<float*>(workspace);

@@ -152,6 +152,19 @@ def test_entry_points_refuse_on_the_host():
     assert lib.mi_gated_recurrence_workspace(1, 65536, 64, 0, 1) > 0 and fwd(batch=1, L=65536) == -1  # it wants the workspace
 
 
+def test_entry_points_refuse_buffers_off_their_pairs():
+    """What the kernels store two floats at a time: the states kept for the backward pass, the norm's mean and rstd."""
+    lib = _lib.load()
+    p, s = 256, (256, 512, 64)
+    for off in (4, 12, 1):
+        assert lib.mi_gated_recurrence(*s, *s, None, 0, 0, None, None, None, p, p, p + off, None, 2, 8, 64, 1, 0, None) == -1
+        assert lib.mi_layer_norm(p, 64, None, 0, p, None, p, None, p + off, 4, 64, 1e-5, 0, 0, None) == -1
+        assert lib.mi_layer_norm_backward(p, None, p, 64, p, p + off, p, None, None, None, None, 4, 64, 0, 0, None) == -1
+    # on the boundary the call goes on (nothing to do)
+    assert lib.mi_gated_recurrence(*s, *s, None, 0, 0, None, None, None, p, p, p + 8, None, 0, 8, 64, 1, 0, None) == 0
+    assert lib.mi_layer_norm(p, 64, None, 0, p, None, p, None, p + 8, 0, 64, 1e-5, 0, 0, None) == 0
+
+
 def slopes(value, leaves, got, prefix="d"):
     """Central differences of 1e-6 in 64 bits: 1e-12 of curvature and 1e-10 of rounding next to values of order 10."""
     g = torch.Generator().manual_seed(77)
