@@ -25,7 +25,8 @@ top-k, top-p and min-p (``Sampling``; kernels.sample_rows on the step's logits).
 
 Streams are independent, so multi-GPU decoding shards them across ranks
 (``mamba_integer_b200.distributed.shard_range``) with no collective until the
-generated ids are gathered.
+generated ids are gathered; ranks that sample tell ``generate`` which streams
+theirs are.
 """
 from __future__ import annotations
 
@@ -245,16 +246,24 @@ class DecodeEngine:
         """argmax of the logits of the last step (int64 [batch])."""
         return self.ws.next_ids
 
-    def generate(self, prompt_ids: torch.Tensor, n_new: int, sampling: Optional[Sampling] = None) -> torch.Tensor:
+    def generate(self, prompt_ids: torch.Tensor, n_new: int, sampling: Optional[Sampling] = None, first: int = 0,
+                 total: Optional[int] = None) -> torch.Tensor:
         """Continuation int64 [batch, n_new]: greedy, or sampled where ``sampling`` is given (each stream and position has
-        a number of its own; the same seed, batch and length give the same tokens)."""
+        a number of its own; the same seed, batch and length give the same tokens).  A rank that has streams ``first`` to
+        ``first + batch - 1`` of ``total`` (distributed.shard_range) says so, and its streams are those of one call over
+        all of them, whatever the number of ranks."""
+        if total is None and first == 0:
+            total = prompt_ids.shape[0]
+        if total is None or first < 0 or first + prompt_ids.shape[0] > total:
+            raise ValueError(f"streams {first} to {first + prompt_ids.shape[0] - 1} of {total}: first and total are those of "
+                             "all ranks' streams")
         logits = self.start(prompt_ids)
         batch = prompt_ids.shape[0]
         out = torch.empty(batch, n_new, dtype=torch.int64, device=self.pre.dev)
         if n_new == 0:
             return out
         s = sampling if sampling is not None and sampling.temperature > 0 else None
-        u = None if s is None else s.numbers(n_new, batch).to(self.pre.dev)
+        u = None if s is None else s.numbers(n_new, total)[:, first:first + batch].contiguous().to(self.pre.dev)
         kernels.argmax_rows(logits, out=self.ws.next_ids)
         for t in range(n_new):
             if s is not None:  # in the place of the argmax

@@ -98,3 +98,77 @@ def test_shard_counts():
     assert shard_range(64, 4, 3) == (48, 64)
     with pytest.raises(ValueError):
         shard_counts(4, 0)
+
+
+def toy_engine():
+    """DecodeEngine.generate over logits of a toy rule, the choice by the 64-bit formula."""
+    from types import SimpleNamespace
+
+    import recurrent_ref as ref
+    from mamba_integer_b200 import decode, kernels
+
+    kernels.argmax_rows = lambda x, V=None, out=None: torch.argmax(x, -1) if out is None else out.copy_(torch.argmax(x, -1))
+
+    class Toy(decode.DecodeEngine):
+        def __init__(self):
+            self.pre = SimpleNamespace(dev=torch.device("cpu"))
+
+        def start(self, prompt_ids):
+            self.ws = SimpleNamespace(next_ids=torch.zeros(prompt_ids.shape[0], dtype=torch.int64))
+            return self.step(prompt_ids.sum(1))
+
+        def step(self, ids):
+            return torch.cos(torch.arange(60.0)[None] * (1 + ids[:, None].float() % 7))
+
+        @staticmethod
+        def sample(logits, u, temperature, top_k, top_p, min_p, out=None):
+            got = [ref.sample(row, float(v), temperature, top_k, top_p, min_p)[0] for row, v in zip(logits, u)]
+            return out.copy_(torch.tensor(got))
+    return Toy()
+
+
+def _sampling_worker(rank, world, port, prompts, n_new, kw, q):
+    for path in (ROOT, os.path.join(ROOT, "tests")):
+        sys.path.insert(0, path)
+    from mamba_integer_b200 import distributed as mdist
+    from mamba_integer_b200.decode import Sampling
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    mdist.init_from_env("gloo", timeout_s=30)
+    torch.manual_seed(21)  # as a program that seeds every rank alike
+    ids, total = torch.tensor(prompts), len(prompts)
+    lo, hi = mdist.shard_range(total, world, rank)
+    mine = toy_engine().generate(ids[lo:hi], n_new, sampling=Sampling(**kw), first=lo, total=total)
+    q.put((rank, mdist.gather_ids(mine, total).tolist()))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("kw", [dict(temperature=1.0, seed=3), dict(temperature=0.8, top_k=20, top_p=0.9)])
+def test_sampled_streams_do_not_depend_on_the_number_of_ranks(kw):
+    from mamba_integer_b200 import kernels
+    from mamba_integer_b200.decode import Sampling
+
+    prompts, n_new = [[5, 9, 2]] * 7, 9
+    keep = kernels.argmax_rows
+    try:
+        eng = toy_engine()
+        torch.manual_seed(21)
+        want = eng.generate(torch.tensor(prompts), n_new, sampling=Sampling(**kw)).tolist()
+        assert len({tuple(t) for t in want}) == 7  # equal prompts, numbers of their own
+        for first, total in ((1, None), (5, 7), (-1, 9), (0, 2)):
+            with pytest.raises(ValueError):
+                eng.generate(torch.tensor(prompts)[:3], n_new, sampling=Sampling(**kw), first=first, total=total)
+    finally:
+        kernels.argmax_rows = keep
+    ctx = mp.get_context("spawn")
+    for world in (2, 3):
+        q, port = ctx.Queue(), _free_port()
+        procs = [ctx.Process(target=_sampling_worker, args=(r, world, port, prompts, n_new, kw, q)) for r in range(world)]
+        for p in procs:
+            p.start()
+        res = [q.get(timeout=120) for _ in procs]
+        for p in procs:
+            p.join(timeout=60)
+            assert p.exitcode == 0
+        assert all(ids == want for _, ids in res), world
