@@ -67,6 +67,38 @@ class Sampling:
         g = None if self.seed is None else torch.Generator().manual_seed(self.seed)
         return torch.rand(*shape, generator=g)
 
+    def one_by_one(self, n: int, block: int = 4096) -> "Numbers":
+        """numbers(n), for one who takes them one after the other."""
+        return Numbers(self, n, block)
+
+
+class Numbers:
+    """The numbers of one stream, in order of their index, drawn a block at a time: what a request may ask for at most is
+    not held, nor drawn if its tokens end before.  Without a seed torch's default generator has moved past all of them
+    once this is made, as after ``Sampling.numbers``."""
+
+    def __init__(self, sampling: Sampling, n: int, block: int):
+        self.n, self.block, self.at, self.now = n, block, 0, []
+        if n <= block:
+            self.now = sampling.numbers(n).tolist()
+            return
+        self.generator = torch.Generator()
+        if sampling.seed is not None:
+            self.generator.manual_seed(sampling.seed)
+        else:
+            self.generator.set_state(torch.get_rng_state())
+            for left in range(n, 0, -(1 << 20)):
+                torch.rand(min(left, 1 << 20))
+
+    def __getitem__(self, i: int) -> float:
+        """Indices may only rise."""
+        if not self.at <= i < self.n:
+            raise IndexError(i)
+        while i >= self.at + len(self.now):
+            self.at += len(self.now)
+            self.now = torch.rand(min(self.block, self.n - self.at), generator=self.generator).tolist()
+        return self.now[i - self.at]
+
 
 class StreamStates:
     """Per-layer recurrent state of `batch` streams: conv windows

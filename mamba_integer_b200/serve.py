@@ -37,7 +37,7 @@ from typing import Dict, List, Optional, Sequence
 
 import torch
 
-from .decode import DecodeEngine, Sampling
+from .decode import DecodeEngine, Numbers, Sampling
 
 
 @dataclass
@@ -47,7 +47,7 @@ class Request:
     max_new_tokens: int
     tokens: List[int] = field(default_factory=list)
     sampling: Optional[Sampling] = None
-    numbers: Optional[List[float]] = None  # one for each token, with sampling
+    numbers: Optional[Numbers] = None      # one for each token, with sampling
     issued: int = 0                        # tokens that were launched, credited or not
 
 
@@ -85,7 +85,7 @@ class DecodeServer:
         self._next_rid += 1
         r = Request(rid, [int(t) for t in prompt], int(max_new_tokens))
         if sampling is not None and sampling.temperature > 0:
-            r.sampling, r.numbers = sampling, sampling.numbers(r.max_new_tokens).tolist()
+            r.sampling, r.numbers = sampling, sampling.one_by_one(r.max_new_tokens)
         self.queue.append(r)
         return rid
 

@@ -2,6 +2,7 @@
 "model" is a toy rule: the first token of a prompt is sum(prompt) % V and
 every next token is (previous + 1) % V.  Checks admission (equal-length
 grouping, queueing beyond the slots), per-slot inputs, retirement and EOS."""
+import pytest
 import torch
 
 from mamba_integer_b200.serve import DecodeServer
@@ -145,3 +146,38 @@ def test_sampling_whole_top_k_of_any_number_type():
         assert s.top_k == 5 and type(s.top_k) is int
     with pytest.raises(ValueError):
         Sampling(top_k=5.5)
+
+
+def test_a_sampled_request_with_a_large_cap_holds_few_numbers():
+    """Its numbers are those of Sampling.numbers, the default generator's too, but not all at once."""
+    import tracemalloc
+
+    from mamba_integer_b200.decode import Sampling
+    eng, cap = SamplingEngine(), 3_000_000
+    srv = DecodeServer(None, slots=2, eos_id=12, engine=eng)
+    for kw in (dict(seed=6), dict()):
+        torch.manual_seed(8)
+        want = Sampling(1.0, **kw).numbers(cap)
+        after = torch.rand(3)
+        torch.manual_seed(8)
+        tracemalloc.start()
+        rid = srv.submit([4, 5], cap, Sampling(1.0, **kw))
+        peak = tracemalloc.get_traced_memory()[1]
+        tracemalloc.stop()
+        assert peak < 1 << 20
+        if not kw:
+            assert torch.equal(after, torch.rand(3))
+        r = srv.queue[-1]
+        spots = [0, 1, 4095, 4096, 10000, 10000, 10001, 2_500_000, cap - 1]
+        assert [r.numbers[i] for i in spots] == want[spots].tolist()
+        with pytest.raises(IndexError):
+            r.numbers[cap]
+        srv.queue.remove(r)
+    # served to its end token
+    s = Sampling(1.0, seed=6)
+    rid = srv.submit([4, 5], 20000, s)
+    want = sampled_alone([4, 5], 20000, s, eos=12)
+    assert srv.run()[rid] == want and want[-1] == 12 and len(want) < 20000
+    for n in (1, 2, 4095, 4096, 4097, 9000):
+        got = s.one_by_one(n)
+        assert [got[i] for i in range(n)] == s.numbers(n).tolist()
