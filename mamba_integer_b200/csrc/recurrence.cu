@@ -624,33 +624,60 @@ __global__ void __launch_bounds__(128) step_kernel(const T* __restrict__ x, int6
     store_pack<4>(y + b * D + c, o, valid, vec);
 }
 
-// How a call's positions are shared out.
-// Few channels and a long sequence: chunks of at least 4 tiles, two CTAs an SM,
-// with a pass for each chunk's fold in front (which reads 2 operands, 3
-// backwards, a first time).  Else CTAs of a cluster: doubled as long as SMs are
-// left without a CTA, and further, up to 800 CTAs, where each still has 4 tiles.
-// us forward and backward in bf16, in clusters and in chunks:
-// 1 x 32768 x 512 (no gate) 64 40, 112 59; 1 x 32768 x 64 53 18, 94 21;
-// 1 x 8192 x 1024 45 31, 62 46; 2 x 8192 x 256 30 28, 38 29; but
-// 1 x 4096 x 256 8.7 17, 16 18; 4 x 4096 x 1024 47 53, 73 81.
-// By CTAs of a cluster, 1, 2, 4, 8: 1 x 2048 x 1536 37 22 12.5 12.2, 62 40 25 22;
-// 6 x 777 x 2048 ragged (fp16) 23 24 28 43, 38 37 44 60; 8 x 2048 x 1536
-// 64 54 57 68, 105 110 99 117; 32 x 512 x 1536 48 55 72 145, 85 99 117 162.
+// How a call's positions are shared out: CTAs of a cluster, or, for long sequences of
+// few channels, chunks, with a pass for each chunk's fold in front (which reads 2
+// operands, 3 backwards, a first time).  By an estimate of the time, in tiles that a
+// CTA passes one after the other (and 0.84 for its start, 1.83 for the chunks' pass):
+//   cost     of a tile by CTAs of a cluster, whose folds go through the cluster, and
+//            of a chunk's tile, whose operands are read twice
+//   waves    so many CTAs run at once, or alone on an SM, where one takes 0.7 of the
+//            time (backward 0.85).  Clusters of 4 and more do not find places on
+//            every SM: above 33, 15, 7 of 4, 8, 16 CTAs they share SMs, and above
+//            66, 33, 14 they take turns.
+// Fitted to 1405 sizes (1 to 400 CTAs without sharing, 100 to 32768 positions, bf16 and
+// fp32, both directions), where it takes 0.5 % more than the best plan on average and
+// up to 20 % (fp32 1 x 300 x 2112, 7.1 5.9).  us of a gated call, 1 x L x 64 base, in clusters of
+// 16 (8 from base 16 on) and in chunks:
+//             L =   4096         6144         8192         16384
+//   base 2, bf16     8.1 10.2    11.1 10.8    14.0 10.8    26 16
+//     backward       16 18       22 18        27 18        50 21
+//   base 4, bf16     8.3 10.5    11.2 13.9    14.2 16.0    27 20
+//     fp32           12.1 13.4   17.6 18.7    22.6 20.1    43 23
+//   base 16, bf16    20 19       28 25        37 30        70 52
+//     backward       35 28       49 36        63 45        120 77
+//   base 33, bf16    24 30       34 41        43 52        82 94
+//   base 34, bf16    32 30       44 41        58 52        110 94
+// By CTAs of a cluster, 1, 2, 4, 8, forward and backward in bf16: 8 x 2048 x 1536 63
+// 55 58 71, 104 113 97 115; 4 x 2048 x 1536 39 37 30 38, 70 59 60 61; 8 x 2048 x 2048
+// 62 72 77 92, 105 117 127 150; 1 x 2048 x 512 of 8 and 16: 7.3 9.9, 14.3 12.7.
 struct Plan {
     int cs, chunks, span;
 };
-static inline Plan plan_of(int batch, int L, int D, int tile) {
+static inline Plan plan_of(int batch, int L, int D, int tile, bool backward) {
     const int64_t base = (int64_t)batch * cdiv(D, CB);
+    static constexpr struct {
+        int alone, at_once;
+        double cost;
+    } SHAPES[] = {{148, 296, 1}, {148, 296, 1.07}, {132, 264, 1.12}, {120, 264, 1.21}, {112, 224, 1.57}};
+    const auto waves = [&](int64_t ctas, int log_cs) {
+        const int64_t rest = ctas % SHAPES[log_cs].at_once;
+        return (double)(ctas / SHAPES[log_cs].at_once) +
+               (rest == 0 ? 0.0 : rest > SHAPES[log_cs].alone ? 1.0 : backward ? 0.85 : 0.7);
+    };
     Plan p = {1, 1, L};
-    if (base <= 37 && L / 64 >= tile) {
-        const int64_t room = 148 * 2 / base, most = L / (4 * tile);
-        p.span = cdiv(cdiv(L, (int)(room < most ? room : most)), tile) * tile;
-        p.chunks = cdiv(L, p.span);
-        return p;
+    double least = 0;
+    for (int i = 0; i < 5; i++) {
+        const int cs = 1 << i;
+        const double time = (cdiv(L, cs * tile) + 0.84) * SHAPES[i].cost * waves(base * cs, i);
+        if (i == 0 || time < least) least = time, p.cs = cs;
+        if (cs * tile >= L) break;
     }
-    while (p.cs < MAX_CLUSTER && p.cs * tile < L && base * p.cs * 2 <= 800 &&
-           (base * p.cs < 148 || L >= (int64_t)p.cs * 8 * tile))
-        p.cs *= 2;
+    if (L >= 2048 && base <= 49) {  // chunks of at least 256 positions, at least 6 of them where the length allows
+        const int64_t room = 148 * 2 / base, most = L / 256;
+        const int span = cdiv(cdiv(L, (int)(room < most ? room : most)), tile) * tile, chunks = cdiv(L, span);
+        const double time = (span / tile + 0.84) * (backward ? 1.35 : 1.36) * waves(base * chunks, 0) + 1.83;
+        if (chunks > 1 && time < least) p = {1, chunks, span};
+    }
     return p;
 }
 
@@ -734,7 +761,7 @@ static int launch(Args& a, cudaStream_t s) {
 
 template <typename T, bool BWD>
 static int dispatch(Args& a, bool convex, bool vec, cudaStream_t s) {
-    const Plan p = plan_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS);
+    const Plan p = plan_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS, BWD);
     a.cs = p.cs, a.chunks = p.chunks, a.span = p.span;
     if (a.chunks > 1 && !a.folds) return MI_ERR_INVALID;
 #define MI_REC(CONVEX, GATE) return vec ? launch<T, CONVEX, GATE, true, BWD>(a, s) : launch<T, CONVEX, GATE, false, BWD>(a, s)
@@ -783,7 +810,7 @@ static inline int64_t fold_bytes(const Plan& p, int batch, int D) {
 extern "C" int64_t mi_gated_recurrence_workspace(int batch, int L, int D, int backward, int dtype) {
     if (batch <= 0 || L <= 0 || D <= 0 || dtype < 0 || dtype > 2) return 0;
     const int sub = backward ? mi::rec::CK : dtype == MI_DT_F32 ? mi::rec::SUB_FWD<float> : mi::rec::SUB_FWD<__half>;
-    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, sub * mi::rec::WARPS);
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, sub * mi::rec::WARPS, backward);
     return mi::rec::fold_bytes(p, batch, D) + (backward ? (int64_t)sizeof(float) * batch * p.chunks * p.cs * D : 0);
 }
 
@@ -827,7 +854,7 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
     a.bias = bias, a.dhT = dh_out, a.lengths = lengths, a.ckpt = const_cast<float*>(checkpoints);
     a.dx = dx, a.df = df, a.dz = dz, a.dh0 = dh0;
     a.batch = batch, a.L = L, a.D = D;
-    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, mi::rec::CK * mi::rec::WARPS);
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, mi::rec::CK * mi::rec::WARPS, true);
     a.folds = static_cast<float*>(workspace);
     if (dbias) a.part = a.folds + mi::rec::fold_bytes(p, batch, D) / (int64_t)sizeof(float);
     const int e = mi::rec::elem_size(dtype);

@@ -165,6 +165,24 @@ def test_entry_points_refuse_buffers_off_their_pairs():
     assert lib.mi_layer_norm(p, 64, None, 0, p, None, p, None, p + 8, 0, 64, 1e-5, 0, 0, None) == 0
 
 
+@pytest.mark.parametrize("size,forward16,forward32,backward", [
+    # chunks (> 0 bytes of folds) where they were measured to be faster than clusters, None where the two are alike
+    ((1, 4096, 128), False, False, False), ((1, 4096, 256), False, False, False), ((1, 4096, 1024), True, True, True),
+    ((1, 6144, 256), False, None, True), ((1, 8192, 256), None, True, True), ((1, 16384, 256), True, True, True),
+    ((2, 4096, 1024), False, False, False), ((4, 8192, 512), False, False, False), ((1, 32768, 512), True, True, True),
+    ((1, 2048, 1536), False, False, False), ((8, 2048, 1536), False, False, False), ((1, 100, 64), False, False, False),
+    ((1, 4096, 2176), True, True, True), ((1, 4096, 2112), False, False, False),
+])
+def test_chunks_are_taken_where_they_are_faster(size, forward16, forward32, backward):
+    lib = _lib.load()
+    b, n, d = size
+    for dtype, want in ((0, forward32), (1, forward16), (2, forward16)):
+        assert want is None or (lib.mi_gated_recurrence_workspace(b, n, d, 0, dtype) > 0) == want, dtype
+    # backward: the folds of chunks, and a row of sums for each CTA of a block of channels
+    rows = lib.mi_gated_recurrence_workspace(b, n, d, 1, 1) / (4 * b * d)
+    assert (rows == int(rows) and rows % 3 == 0) if backward else rows in (1, 2, 4, 8, 16)
+
+
 def slopes(value, leaves, got, prefix="d"):
     """Central differences of 1e-6 in 64 bits: 1e-12 of curvature and 1e-10 of rounding next to values of order 10."""
     g = torch.Generator().manual_seed(77)
