@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import recurrent_ref as ref
+from mamba_integer_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -290,6 +291,75 @@ def test_recurrence_step_output_gate_over_its_whole_range(sel, cuda_dev, dtype, 
     check_output_gate(a, torch.stack(ys, 1))
 
 
+# Sequences of 8229 positions of few channels go in chunks, both ways and in every type: for 6 of them spans of 384
+# forward in 16 bits, of 320 else (of 33 channels) or 384 (of 72).
+CHUNK_LENGTHS = [8229, 1920, 1921, 639, 0, 5000]  # all; at a border of each, behind it, in front of one; none; inside
+
+
+@pytest.mark.parametrize("d", [72, 33])
+@pytest.mark.parametrize("z,bias,convex", [(True, True, True), (False, True, True), (True, False, False), (False, False, False)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_in_chunks(sel, cuda_dev, dtype, z, bias, convex, d):
+    b, n = len(CHUNK_LENGTHS), 8229
+    a = rec_inputs(cuda_dev, dtype, b, n, d, z=z, bias=bias, h0=True, convex=convex, lengths=CHUNK_LENGTHS)
+    if bias:
+        a["bias"] += 3  # memories that reach through chunks
+    if z:
+        a["z"][0, 100::1000] = torch.finfo(dtype).min  # closed output gates
+    dy, dh = torch.randn(b, n, d, device=cuda_dev).to(dtype), torch.randn(b, d, device=cuda_dev)
+    lib = _lib.load()
+    for backward in (0, 1):  # (a row of sums a cluster's CTA, or three a chunk)
+        assert lib.mi_gated_recurrence_workspace(b, n, d, backward, {F32: 0, BF16: 1, F16: 2}[dtype]) > 4 * b * d * 16 * backward
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+    if z:
+        assert not y[0, 100::1000].any() and not got["z"][0, 100::1000].any()
+    with torch.no_grad():
+        again = call_rec(sel, a)
+    assert torch.equal(again[0], y) and torch.equal(again[1], h)
+
+
+@pytest.mark.parametrize("n", [8192, 20000])
+def test_recurrence_one_long_sequence(sel, cuda_dev, n):
+    a = rec_inputs(cuda_dev, BF16, 1, n, 24, z=False)
+    a["bias"] += 4
+    dy = torch.randn(1, n, 24, device=cuda_dev).to(BF16)
+    y, h, got = rec_grads(sel, a, dy, None)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, None)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_extreme_values_in_chunks(sel, cuda_dev, dtype):
+    """Gates that keep and that drop the state, and infinite and NaN inputs, states and gradients, through chunks that they
+    do not lie in."""
+    n, d = 8300, 64
+    a = rec_inputs(cuda_dev, dtype, 1, n, d, h0=True, bias=False, z=False)
+    a["f"][0, ::3], a["f"][0, 1::7] = 60.0, -60.0
+    dy, dh = torch.randn(1, n, d, device=cuda_dev).to(dtype), torch.randn(1, d, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+    inf, nan = float("inf"), float("nan")
+    a["x"][0, 3000, :32] = inf
+    a["h0"][0, 40] = -inf
+    a["x"][0, 6000, 50] = nan
+    dy[0, 7000, 33], dh[0, 34] = nan, inf
+    y, h, got = rec_grads(sel, a, dy, dh)
+    assert (y[0, 3000:, :32] == inf).all() and torch.isfinite(y[0, :3000, :32]).all() and (h[0, :32] == inf).all()
+    assert (y[0, :, 40] == -inf).all() and h[0, 40] == -inf
+    assert torch.isfinite(y[0, :6000, 50]).all() and y[0, 6000:, 50].isnan().all() and h[0, 50].isnan()
+    rest = [i for i in range(32, 64) if i not in (40, 50)]
+    assert torch.isfinite(y[..., rest]).all() and torch.isfinite(h[..., rest]).all()
+    dx = got["x"]
+    assert dx[0, :7001, 33].isnan().all() and torch.isfinite(dx[0, 7001:, 33]).all() and got["h0"][0, 33].isnan()
+    # 1 - a is e^-60 at the least, so an infinite gradient reaches every input
+    assert (dx[0, :, 34] == inf).all() and got["h0"][0, 34] == inf
+    rest = [i for i in range(64) if i not in (33, 34)]
+    assert torch.isfinite(dx[..., rest]).all() and torch.isfinite(got["h0"][..., rest]).all()
+
+
 def test_recurrence_same_bits_and_streams(sel, cuda_dev):
     """The same inputs give the same bits, on another stream and captured in a graph that is replayed."""
     a = rec_inputs(cuda_dev, BF16, 2, 700, 192, h0=True)
@@ -545,6 +615,28 @@ SETTINGS = [(1.0, 0, 1.0, 0.0), (0.7, 50, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.3, 0
 @pytest.mark.parametrize("rows,v", [(1, 1), (3, 2), (5, 64), (7, 1000), (4, 4096), (9, 32768), (2, 50021), (1, 131072)])
 def test_sample(kernels, cuda_dev, rows, v, setting):
     check_sample(kernels, cuda_dev, sample_logits(rows, v, seed=v), uniform(rows, v), *setting)
+
+
+# More than 131072 tokens take clusters whatever the number of rows.
+@pytest.mark.parametrize("setting", SETTINGS)
+@pytest.mark.parametrize("rows,v", [(2, 131073), (3, 200003), (2, 262144)])
+def test_sample_large_vocabularies(kernels, cuda_dev, rows, v, setting):
+    check_sample(kernels, cuda_dev, sample_logits(rows, v, seed=v), uniform(rows, v), *setting)
+
+
+@pytest.mark.parametrize("v", [131073, 262144])
+def test_sample_many_rows_of_large_vocabularies(kernels, cuda_dev, v):
+    rows = 160
+    g = torch.Generator().manual_seed(v)
+    r = lambda: torch.rand(rows, generator=g)  # noqa: E731
+    t = torch.where(r() < 0.1, 0.0, 0.3 + 1.5 * r()).tolist()
+    k = torch.where(r() < 0.5, 0, (r() * 2000).int() + 1).int().tolist()
+    p = torch.where(r() < 0.4, 1.0, r()).tolist()
+    m = torch.where(r() < 0.5, 0.0, 0.3 * r()).tolist()
+    logits = sample_logits(rows, v, seed=v, dtype=BF16)
+    logits[3] = 0.0  # ties all over
+    logits[4, : v - 5] = -float("inf")
+    check_sample(kernels, cuda_dev, logits, uniform(rows, v), t, k, p, m)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
