@@ -1,4 +1,4 @@
-// torch_ops.cpp -- the float Mamba operators' calls from torch: checks of the
+// torch_ops.cpp -- the float operators' calls from torch: checks of the
 // arguments, outputs and workspaces, the launch on the tensors' device and
 // current stream, and the autograd nodes.
 //
@@ -142,7 +142,7 @@ bool any_requires_grad(const Ts&... ts) {
 template <typename... Ts>
 void no_grad_needed(const Ts&... ts) {
     TORCH_CHECK(!at::GradMode::is_enabled() || !any_requires_grad(ts...),
-                "the single-token and quantised forms have no backward pass: call them under torch.no_grad()");
+                "this call has no backward pass: make it under torch.no_grad()");
 }
 
 // No formulas for tangents: forward-mode differentiation would lose them.
@@ -151,7 +151,7 @@ void no_tangents(const Ts&... ts) {
     TORCH_CHECK_NOT_IMPLEMENTED(
         !((ts.defined() && ts._fw_grad(/*level=*/0).defined()) || ...) ||
             !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
-        "the float Mamba operators have no forward-mode derivative: an argument is a dual tensor");
+        "the float operators have no forward-mode derivative: an argument is a dual tensor");
 }
 
 // A training call that is being captured.  Where an earlier autograd graph is
@@ -224,7 +224,7 @@ Tensor empty_as(const Tensor& t, bool want = true) {
 variable_list once(variable_list grads, bool create, const variable_list& saved, const variable_list& incoming) {
     using namespace torch::autograd;
     if (!create || !(any_variable_requires_grad(saved) || any_variable_requires_grad(incoming))) return grads;
-    const auto refusal = std::make_shared<Error>("the float Mamba operators have gradients of first order only",
+    const auto refusal = std::make_shared<Error>("the float operators have gradients of first order only",
                                                  collect_next_edges(saved, incoming));
     for (auto& t : grads) {
         if (!t.defined()) continue;
@@ -792,7 +792,10 @@ struct Setting {
 std::tuple<Tensor, OptTensor> sample_rows(const Tensor& logits, const Tensor& u_, const std::variant<Tensor, double>& t_,
                                           const std::variant<Tensor, int64_t>& k_, const std::variant<Tensor, double>& p_,
                                           const std::variant<Tensor, double>& m_, const OptTensor& out, bool return_prob) {
-    no_grad_needed(logits);
+    const auto rows_of = [](const auto& s) { return std::holds_alternative<Tensor>(s) ? std::get<Tensor>(s) : Tensor(); };
+    const Tensor ts = rows_of(t_), ps = rows_of(p_), ms = rows_of(m_);
+    no_tangents(logits, u_, ts, ps, ms);
+    no_grad_needed(logits, u_, ts, ps, ms);
     activation(logits, "logits");
     TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1 && logits.size(1) <= 262144,
                       "logits must be [rows, 1 to 262144 tokens], got ", logits.sizes());

@@ -375,7 +375,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     total; with ``return_prob`` also its share w / total (fp32 [rows]).  Temperature 0 is argmax_rows, with share 1; so
     is a row whose maximum is infinite or NaN, or that is all -inf.  Every setting is a number or a tensor of one value a
     row (fp32, top_k int32), whose values are not checked: a temperature below 0 counts as 0, and the filters of values
-    beyond their range as off or as their nearest end.  Up to 262144 tokens.  The same inputs give the same bits."""
+    beyond their range as off or as their nearest end.  Up to 262144 tokens.  The same inputs give the same bits.  No derivatives: an
+    argument that requires them raises RuntimeError, a dual tensor NotImplementedError."""
     from . import selective
     token, prob = (selective._ops or selective._load()).sample_rows(logits, u, temperature, top_k, top_p, min_p, out,
                                                                     return_prob)

@@ -105,6 +105,20 @@ def test_sample_refuses(change, error):
         kernels.sample_rows(**{**dict(logits=_t(4, 9), u=_t(4)), **change})
 
 
+def test_sample_refuses_to_lose_derivatives():
+    """Of a setting or the numbers as of the logits: prob would come without them."""
+    from torch.autograd import forward_ad
+
+    args = lambda: dict(logits=_t(4, 9), u=_t(4), temperature=torch.ones(4), top_p=torch.ones(4), min_p=_t(4))  # noqa: E731
+    for name in args():
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            kernels.sample_rows(**{**args(), name: args()[name].requires_grad_(True)})
+        with torch.no_grad(), pytest.raises(ValueError, match="must be a CUDA tensor"):
+            kernels.sample_rows(**{**args(), name: args()[name].requires_grad_(True)})
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            kernels.sample_rows(**{**args(), name: forward_ad.make_dual(args()[name], torch.ones_like(args()[name]))})
+
+
 def test_sizes_past_the_counters_are_refused():
     """Expanded views: no such memory is there."""
     for shape, what in (((1, (1 << 30) + 1, 1), "too long"), ((65536, 1, 1), "at most 65535"),
