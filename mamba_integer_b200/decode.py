@@ -54,7 +54,7 @@ class Sampling:
     def __post_init__(self):
         if not 0 <= self.temperature <= 3.4e38:
             raise ValueError(f"temperature must be 0 (greedy) or more and finite, got {self.temperature}")
-        if not 0 <= int(self.top_k) < 2 ** 31 or int(self.top_k) != self.top_k:
+        if not 0 <= self.top_k < 2 ** 31 or int(self.top_k) != self.top_k:
             raise ValueError(f"top_k must be a whole number from 0 (off) on, got {self.top_k}")
         object.__setattr__(self, "top_k", int(self.top_k))
         if not 0 <= self.top_p <= 1:

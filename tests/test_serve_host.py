@@ -181,3 +181,11 @@ def test_a_sampled_request_with_a_large_cap_holds_few_numbers():
     for n in (1, 2, 4095, 4096, 4097, 9000):
         got = s.one_by_one(n)
         assert [got[i] for i in range(n)] == s.numbers(n).tolist()
+
+
+def test_sampling_refuses_top_k_that_is_no_number_by_the_same_error():
+    from mamba_integer_b200.decode import Sampling
+    for k in (float("inf"), float("nan"), -float("inf"), 2.0 ** 31, -0.5):
+        with pytest.raises(ValueError, match="top_k"):
+            Sampling(top_k=k)
+    assert Sampling(top_k=2 ** 31 - 1).top_k == 2 ** 31 - 1
