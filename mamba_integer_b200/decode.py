@@ -1,4 +1,4 @@
-"""Decode executor: greedy generation for a batch of independent streams.
+"""Decode executor: generation for a batch of independent streams, greedy or sampled.
 
 The prompt runs through the prefill kernels, which leave behind, per layer,
 the last three conv inputs of every stream (the conv window) and the final
@@ -142,7 +142,7 @@ class _StepWorkspace:
 
 
 class DecodeEngine:
-    """Greedy decoding over the sm_100a kernels (prompt prefill, then one step
+    """Decoding over the sm_100a kernels, greedy or sampled (prompt prefill, then one step
     per token).  ``use_graph`` replays each step from a CUDA graph captured on
     the first step (the step launches no allocation and no host sync)."""
 
@@ -275,7 +275,7 @@ class DecodeEngine:
         return kernels.sample_rows(logits, u, temperature, top_k, top_p, min_p, out=out)
 
     def next_ids(self) -> torch.Tensor:
-        """argmax of the logits of the last step (int64 [batch])."""
+        """argmax of the logits of the last step (int64 [batch]); who samples writes its choice there."""
         return self.ws.next_ids
 
     def generate(self, prompt_ids: torch.Tensor, n_new: int, sampling: Optional[Sampling] = None, first: int = 0,

@@ -136,8 +136,10 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, z: Optional[torch.Tens
 
     Without ``convex`` the input is not weighed: h[t] = a[t] h[t-1] + x[t].
     x, gate, z [batch, L, channels]; gate_bias [channels]; h0 [batch,
-    channels].  Returns y, or (y, final state) with ``return_state``.  A gate is
-    at least 2^-127, so that an infinite state stays one."""
+    channels].  Returns y, or (y, final state) with ``return_state``.  The gate's
+    logits count as at most 87 from 0, so that an infinite state stays one: a and
+    1 - a are at least e^-87 (1.6e-38), which states and inputs of 1e30 and more
+    show.  The output gate z has no such bound and reaches 0."""
     y, h = (_ops or _load()).gated_recurrence(x, gate, z, gate_bias, convex, h0, lengths)
     return (y, h) if return_state else y
 
