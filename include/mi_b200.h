@@ -449,8 +449,9 @@ int mi_causal_conv1d_step(const void* x, int64_t x_batch, const float* w, const 
  * lengths, h_out may be NULL.  checkpoints (NULL without a backward pass):
  * mi_gated_recurrence_checkpoints() floats, 8-byte aligned.  workspace (NULL if 0):
  * mi_gated_recurrence_workspace(.., 0, dtype) bytes.  L >= 1.  Gate logits count as
- * at most 87 from 0, so that gates never reach 0: infinite states stay infinite.
- * z has no such bound: sigmoid(z) below e^-87 (2^-126 in 16 bits) counts as 0.
+ * at least -87, so that a never reaches 0: infinite states stay infinite.  The
+ * others do: 1 - a below 2^-126 counts as 0, and sigmoid(z) below e^-87 (2^-126 in
+ * 16 bits).
  * A wait between CTAs that runs out (MI_DEV_TIMEOUT) leaves NaN in what follows.
  */
 int mi_gated_recurrence(const void* x, int64_t x_batch, int64_t x_row, const void* f, int64_t f_batch, int64_t f_row,

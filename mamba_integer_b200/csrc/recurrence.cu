@@ -29,10 +29,11 @@
 // nothing is read twice.  Long sequences of few channels are cut into chunks,
 // whose folds a pass in front takes.
 //
-// Gates and folds never reach 0: gate logits count as at most 87 from 0, and a
-// stretch's P is at least 2^-126, so that an infinite state stays infinite and an
-// infinite input reaches it, whether or not a stretch is folded.  (A state of
-// 1e38 leaves up to 1 of itself behind a stretch that forgets it.)
+// Gates and folds never reach 0: gate logits count as at least -87, and a stretch's
+// P is at least 2^-126, so that an infinite state stays infinite, whether or not a
+// stretch is folded.  (A state of 1e38 leaves up to 1 of itself behind a stretch that
+// forgets it.)  An input's weight does reach 0, where it would be below 2^-126: what a
+// gate keeps out counts for nothing, the type's lowest value included.
 #include <type_traits>
 
 #include "mi_elem.cuh"
@@ -76,14 +77,14 @@ __device__ __forceinline__ int length_of(const Args& a, int b) {
     return n < 0 ? 0 : (n < a.L ? n : a.L);
 }
 
-// sigmoid(v) and sigmoid(-v), neither taken from 1 minus the other, for |v| up
-// to 87 (beyond it counts as 87; a NaN stays one).  The product with log2(e) is
+// sigmoid(v), at least e^-87, and sigmoid(-v), 0 from v = 87.4 on, neither taken from
+// 1 minus the other (a NaN stays one).  The product with log2(e) is
 // carried on in two parts, which keeps the power to 2 ulp where |v| is large, and
 // a Newton step makes the reciprocal right to its last bit: where a is near 1, a
 // state has its error as often as its memory is long.
 __device__ __forceinline__ void sigmoids(float2 v, float2& up, float2& down) {
-    v.x = max_nan(min_nan(v.x, 87.0f), -87.0f);
-    v.y = max_nan(min_nan(v.y, 87.0f), -87.0f);
+    v.x = max_nan(min_nan(v.x, 127.0f), -87.0f);
+    v.y = max_nan(min_nan(v.y, 127.0f), -87.0f);
     const float2 t = __fmul2_rn(v, dup(-LOG2E));
     const float2 r = __ffma2_rn(v, dup(1.92596299e-8f), __ffma2_rn(v, dup(LOG2E), t));  // t is too large by this
     float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));
@@ -105,7 +106,6 @@ __device__ __forceinline__ float2 silu(float2 z, float2& slope) {
     if constexpr (sizeof(T) == 4) {
         sigmoids(z, s, n);
         s = make_float2(z.x < -87.0f ? 0.0f : s.x, z.y < -87.0f ? 0.0f : s.y);
-        n = make_float2(z.x > 87.0f ? 0.0f : n.x, z.y > 87.0f ? 0.0f : n.y);
     } else {
         const float2 t = __fmul2_rn(z, dup(-LOG2E));
         const float2 e = make_float2(exp2_fast(t.x), exp2_fast(t.y));

@@ -137,9 +137,9 @@ def gated_recurrence(x: torch.Tensor, gate: torch.Tensor, z: Optional[torch.Tens
     Without ``convex`` the input is not weighed: h[t] = a[t] h[t-1] + x[t].
     x, gate, z [batch, L, channels]; gate_bias [channels]; h0 [batch,
     channels].  Returns y, or (y, final state) with ``return_state``.  The gate's
-    logits count as at most 87 from 0, so that an infinite state stays one: a and
-    1 - a are at least e^-87 (1.6e-38), which states and inputs of 1e30 and more
-    show.  The output gate z has no such bound and reaches 0."""
+    logits count as at least -87, so that an infinite state stays one (a state of
+    1e38 leaves up to 2 of itself).  An input's weight and the output gate have no
+    such bound: 1 - a below 2^-126 counts as 0, and so does sigmoid(z) below e^-87."""
     y, h = (_ops or _load()).gated_recurrence(x, gate, z, gate_bias, convex, h0, lengths)
     return (y, h) if return_state else y
 

@@ -291,6 +291,28 @@ def test_recurrence_step_output_gate_over_its_whole_range(sel, cuda_dev, dtype, 
     check_output_gate(a, torch.stack(ys, 1))
 
 
+@pytest.mark.parametrize("n,d", [(37, 40), (37, 41), (8300, 24)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_recurrence_inputs_of_weight_zero(sel, cuda_dev, dtype, n, d):
+    """Where the gate keeps the whole state, an input counts for nothing, the type's lowest value included."""
+    a = rec_inputs(cuda_dev, dtype, 1, n, d, h0=True, bias=False)
+    most = torch.finfo(dtype).max
+    for i, (f, x) in enumerate([(200.0, -most), (1e4, most), (most, -most), (most, -1e4), (200.0, -min(most, 1e30)), (1e30, most)]):
+        a["f"][0, 2 + 5 * i], a["x"][0, 2 + 5 * i] = min(f, most), x
+    dy, dh = torch.randn(1, n, d, device=cuda_dev).to(dtype), torch.randn(1, d, device=cuda_dev)
+    y, h, got = rec_grads(sel, a, dy, dh)
+    check_rec(y, h, a)
+    check_rec_grads(got, a, dy, dh)
+    assert not got["x"][0, 2:30:5].any() and not got["f"][0, 2:30:5].any()
+    s, ys = a["h0"].clone(), []
+    for t in range(min(n, 37)):
+        with torch.no_grad():
+            ys.append(sel.gated_recurrence_step(s, a["x"][:, t], a["f"][:, t], z=a["z"][:, t]))
+    check_rec(torch.stack(ys, 1), s, {k: v[:, :37] if k in ("x", "f", "z") else v for k, v in a.items()})
+    a["f"][0, 2:30:5] = float("inf")
+    assert torch.equal(call_rec(sel, a)[0], y)
+
+
 # Sequences of 8229 positions of few channels go in chunks, both ways and in every type: for 6 of them spans of 384
 # forward in 16 bits, of 320 else (of 33 channels) or 384 (of 72).
 CHUNK_LENGTHS = [8229, 1920, 1921, 639, 0, 5000]  # all; at a border of each, behind it, in front of one; none; inside
