@@ -627,17 +627,18 @@ __global__ void __launch_bounds__(128) step_kernel(const T* __restrict__ x, int6
 // How a call's positions are shared out: CTAs of a cluster, or, for long sequences of
 // few channels, chunks, with a pass for each chunk's fold in front (which reads 2
 // operands, 3 backwards, a first time).  By an estimate of the time, in tiles that a
-// CTA passes one after the other (and 0.84 for its start, 1.83 for the chunks' pass):
-//   cost     of a tile by CTAs of a cluster, whose folds go through the cluster, and
-//            of a chunk's tile, whose operands are read twice
-//   waves    so many CTAs run at once, or alone on an SM, where one takes 0.7 of the
-//            time (backward 0.85).  Clusters of 4 and more do not find places on
-//            every SM: above 33, 15, 7 of 4, 8, 16 CTAs they share SMs, and above
-//            66, 33, 14 they take turns.
-// Fitted to 1405 sizes (1 to 400 CTAs without sharing, 100 to 32768 positions, bf16 and
-// fp32, both directions), where it takes 0.5 % more than the best plan on average and
-// up to 20 % (fp32 1 x 300 x 2112, 7.1 5.9).  us of a gated call, 1 x L x 64 base, in clusters of
-// 16 (8 from base 16 on) and in chunks:
+// CTA passes one after the other (and `start` for its first, `pass` for the chunks'):
+//   tile     what one costs by CTAs of a cluster, whose folds go through the cluster;
+//            `twice` in a chunk, whose operands are read twice
+//   waves    so many CTAs run at once, or alone on an SM, where one takes `alone` of
+//            the time.  Clusters of 4 and more do not find places on every SM: above
+//            33, 15, 7 of 4, 8, 16 CTAs they share SMs, and above 66, 33, 14 they take
+//            turns.
+// Widths off 16 bytes, whose tiles cost more, have figures of their own.  Fitted to
+// 1405 sizes each (1 to 400 CTAs without sharing, 100 to 32768 positions, bf16 and fp32,
+// both directions), where the choice takes 0.5 % (0.3 %) more than the best plan on
+// average and up to 20 % (fp32 1 x 300 x 2112, 7.1 us for 5.9).  us of a gated call,
+// 1 x L x 64 base, in clusters of 16 (8 from base 16 on) and in chunks:
 //             L =   4096         6144         8192         16384
 //   base 2, bf16     8.1 10.2    11.1 10.8    14.0 10.8    26 16
 //     backward       16 18       22 18        27 18        50 21
@@ -650,32 +651,38 @@ __global__ void __launch_bounds__(128) step_kernel(const T* __restrict__ x, int6
 // By CTAs of a cluster, 1, 2, 4, 8, forward and backward in bf16: 8 x 2048 x 1536 63
 // 55 58 71, 104 113 97 115; 4 x 2048 x 1536 39 37 30 38, 70 59 60 61; 8 x 2048 x 2048
 // 62 72 77 92, 105 117 127 150; 1 x 2048 x 512 of 8 and 16: 7.3 9.9, 14.3 12.7.
+// By CTAs of a cluster, off 16 bytes, forward: 8 x 2048 x 1531 bf16 114 104 96 106,
+// 1 x 2048 x 763 of 8 and 16 13.1 9.9.
 struct Plan {
     int cs, chunks, span;
 };
-static inline Plan plan_of(int batch, int L, int D, int tile, bool backward) {
+struct Costs {
+    double alone, start, tile[5], twice, pass;
+};
+static inline Plan plan_of(int batch, int L, int D, int tile, bool backward, bool off16) {
+    static constexpr Costs COSTS[2][2] = {{{0.7, 0.84, {1, 1.07, 1.12, 1.21, 1.57}, 1.36, 1.83},
+                                           {0.85, 0.84, {1, 1.07, 1.12, 1.21, 1.57}, 1.35, 1.83}},
+                                          {{0.9, 0.55, {1, 1.08, 1.1, 1.17, 1.27}, 1.66, 1.29},
+                                           {0.82, 0.55, {1, 1.08, 1.1, 1.17, 1.27}, 1.46, 1.29}}};
+    static constexpr int APART[5] = {148, 148, 132, 120, 112}, AT_ONCE[5] = {296, 296, 264, 264, 224};
+    const Costs& cost = COSTS[off16][backward];
     const int64_t base = (int64_t)batch * cdiv(D, CB);
-    static constexpr struct {
-        int alone, at_once;
-        double cost;
-    } SHAPES[] = {{148, 296, 1}, {148, 296, 1.07}, {132, 264, 1.12}, {120, 264, 1.21}, {112, 224, 1.57}};
     const auto waves = [&](int64_t ctas, int log_cs) {
-        const int64_t rest = ctas % SHAPES[log_cs].at_once;
-        return (double)(ctas / SHAPES[log_cs].at_once) +
-               (rest == 0 ? 0.0 : rest > SHAPES[log_cs].alone ? 1.0 : backward ? 0.85 : 0.7);
+        const int64_t rest = ctas % AT_ONCE[log_cs];
+        return (double)(ctas / AT_ONCE[log_cs]) + (rest == 0 ? 0.0 : rest > APART[log_cs] ? 1.0 : cost.alone);
     };
     Plan p = {1, 1, L};
     double least = 0;
     for (int i = 0; i < 5; i++) {
         const int cs = 1 << i;
-        const double time = (cdiv(L, cs * tile) + 0.84) * SHAPES[i].cost * waves(base * cs, i);
+        const double time = (cdiv(L, cs * tile) + cost.start) * cost.tile[i] * waves(base * cs, i);
         if (i == 0 || time < least) least = time, p.cs = cs;
         if (cs * tile >= L) break;
     }
     if (L >= 2048 && base <= 49) {  // chunks of at least 256 positions, at least 6 of them where the length allows
         const int64_t room = 148 * 2 / base, most = L / 256;
         const int span = cdiv(cdiv(L, (int)(room < most ? room : most)), tile) * tile, chunks = cdiv(L, span);
-        const double time = (span / tile + 0.84) * (backward ? 1.35 : 1.36) * waves(base * chunks, 0) + 1.83;
+        const double time = (span / tile + cost.start) * cost.twice * waves(base * chunks, 0) + cost.pass;
         if (chunks > 1 && time < least) p = {1, chunks, span};
     }
     return p;
@@ -761,7 +768,7 @@ static int launch(Args& a, cudaStream_t s) {
 
 template <typename T, bool BWD>
 static int dispatch(Args& a, bool convex, bool vec, cudaStream_t s) {
-    const Plan p = plan_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS, BWD);
+    const Plan p = plan_of(a.batch, a.L, a.D, (BWD ? CK : SUB_FWD<T>)*WARPS, BWD, (int64_t)a.D * sizeof(T) % 16 != 0);
     a.cs = p.cs, a.chunks = p.chunks, a.span = p.span;
     if (a.chunks > 1 && !a.folds) return MI_ERR_INVALID;
 #define MI_REC(CONVEX, GATE) return vec ? launch<T, CONVEX, GATE, true, BWD>(a, s) : launch<T, CONVEX, GATE, false, BWD>(a, s)
@@ -775,6 +782,7 @@ static int dispatch(Args& a, bool convex, bool vec, cudaStream_t s) {
 }
 
 static inline int elem_size(int dtype) { return dtype == MI_DT_F32 ? 4 : 2; }
+static inline bool width_off16(int D, int dtype) { return (int64_t)D * elem_size(dtype) % 16 != 0; }
 static inline bool rows_vec(const Args& a, int D, int dtype) {
     const int k = 16 / elem_size(dtype);
     for (const Seq& s : a.in)
@@ -810,7 +818,7 @@ static inline int64_t fold_bytes(const Plan& p, int batch, int D) {
 extern "C" int64_t mi_gated_recurrence_workspace(int batch, int L, int D, int backward, int dtype) {
     if (batch <= 0 || L <= 0 || D <= 0 || dtype < 0 || dtype > 2) return 0;
     const int sub = backward ? mi::rec::CK : dtype == MI_DT_F32 ? mi::rec::SUB_FWD<float> : mi::rec::SUB_FWD<__half>;
-    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, sub * mi::rec::WARPS, backward);
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, sub * mi::rec::WARPS, backward, mi::rec::width_off16(D, dtype));
     return mi::rec::fold_bytes(p, batch, D) + (backward ? (int64_t)sizeof(float) * batch * p.chunks * p.cs * D : 0);
 }
 
@@ -854,7 +862,7 @@ extern "C" int mi_gated_recurrence_backward(const void* dy, int64_t dy_batch, in
     a.bias = bias, a.dhT = dh_out, a.lengths = lengths, a.ckpt = const_cast<float*>(checkpoints);
     a.dx = dx, a.df = df, a.dz = dz, a.dh0 = dh0;
     a.batch = batch, a.L = L, a.D = D;
-    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, mi::rec::CK * mi::rec::WARPS, true);
+    const mi::rec::Plan p = mi::rec::plan_of(batch, L, D, mi::rec::CK * mi::rec::WARPS, true, mi::rec::width_off16(D, dtype));
     a.folds = static_cast<float*>(workspace);
     if (dbias) a.part = a.folds + mi::rec::fold_bytes(p, batch, D) / (int64_t)sizeof(float);
     const int e = mi::rec::elem_size(dtype);

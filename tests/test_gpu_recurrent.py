@@ -313,17 +313,17 @@ def test_recurrence_inputs_of_weight_zero(sel, cuda_dev, dtype, n, d):
     assert torch.equal(call_rec(sel, a)[0], y)
 
 
-# Sequences of 8229 positions of few channels go in chunks, both ways and in every type: for 6 of them spans of 384
-# forward in 16 bits, of 320 else (of 33 channels) or 384 (of 72).
-CHUNK_LENGTHS = [8229, 1920, 1921, 639, 0, 5000]  # all; at a border of each, behind it, in front of one; none; inside
+# Sequences of 8229 positions of few channels go in chunks (of 384), both ways and in every type; with rows off 16 bytes those
+# of 16421.
+CHUNK_LENGTHS = [30000, 5376, 5377, 2687, 0, 5000]  # all; at a border of each, behind it, in front of it; none; inside
 
 
 @pytest.mark.parametrize("d", [72, 33])
 @pytest.mark.parametrize("z,bias,convex", [(True, True, True), (False, True, True), (True, False, False), (False, False, False)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_recurrence_in_chunks(sel, cuda_dev, dtype, z, bias, convex, d):
-    b, n = len(CHUNK_LENGTHS), 8229
-    a = rec_inputs(cuda_dev, dtype, b, n, d, z=z, bias=bias, h0=True, convex=convex, lengths=CHUNK_LENGTHS)
+    b, n = len(CHUNK_LENGTHS), 8229 if d == 72 else 16421
+    a = rec_inputs(cuda_dev, dtype, b, n, d, z=z, bias=bias, h0=True, convex=convex, lengths=[min(v, n) for v in CHUNK_LENGTHS])
     if bias:
         a["bias"] += 3  # memories that reach through chunks
     if z:
