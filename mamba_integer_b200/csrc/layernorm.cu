@@ -434,20 +434,20 @@ __global__ void __launch_bounds__(MAX_BLOCK, 1) bwd_kernel(const Args a) {
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < NV; j++) {
-            if (VEC) {  // 16 bytes a store; with 4 the call took 60.0 us instead of 54.9 (4096 x 4096 bf16, fp32 residual)
+            if constexpr (VEC) {  // 16 bytes a store; with 4 the call took 60.0 us instead of 54.9 (4096 x 4096 bf16, fp32 residual)
                 if (!cols.any(j)) continue;
 #pragma unroll
                 for (int i = 0; i < K; i += 4) {
                     const float2 u = which ? db[j][i / 2] : dw[j][i / 2], v = which ? db[j][i / 2 + 1] : dw[j][i / 2 + 1];
                     *reinterpret_cast<float4*>(to + cols.at(j) + i) = make_float4(u.x, u.y, v.x, v.y);
                 }
-                continue;
-            }
+            } else {
 #pragma unroll
-            for (int i = 0; i < K / 2; i++) {
-                const float2 v = which ? db[j][i] : dw[j][i];
-                if (cols.has(j, 2 * i)) to[cols.at(j, 2 * i)] = v.x;
-                if (cols.has(j, 2 * i + 1)) to[cols.at(j, 2 * i + 1)] = v.y;
+                for (int i = 0; i < K / 2; i++) {
+                    const float2 v = which ? db[j][i] : dw[j][i];
+                    if (cols.has(j, 2 * i)) to[cols.at(j, 2 * i)] = v.x;
+                    if (cols.has(j, 2 * i + 1)) to[cols.at(j, 2 * i + 1)] = v.y;
+                }
             }
         }
         if (rows == 1) continue;
