@@ -13,8 +13,8 @@
 // A position and channel move 3 elements forward (4 with z) and meet 2 (4)
 // special-function results, so HBM bounds it as long as enough loads are in
 // flight and the instructions are few (33 a channel and position with z, of
-// which 4 are special functions; 57 backward).  32 x 512 x 1536 bf16 with z: forward 50 us
-// (201 MB, 4.0 TB/s), 36 without the arithmetic; backward 84 (352 MB, 4.2 TB/s),
+// which 4 are special functions; 57 backward).  32 x 512 x 1536 bf16 with z: forward 47 us
+// (201 MB, 4.3 TB/s), 36 without the arithmetic; backward 82 (352 MB, 4.3 TB/s),
 // 78 without: what is left is two CTAs of 128 registers a thread an SM, whose
 // warps load, wait for the fold and store by turns.
 //
@@ -98,8 +98,8 @@ __device__ __forceinline__ void sigmoids(float2 v, float2& up, float2& down) {
 // z sigmoid(z), and its derivative.  Unlike a state's gate an output gate reaches 0:
 // a sigmoid below e^-87 counts as 0 (2^-126 in 16 bits), so that at the types' lowest
 // values both are 0 and not the smallest gate times z.  In 16 bits without
-// sigmoids()' care: |z| 2^-24 of the power is far below half a step.  fp32 forward at
-// 8 x 2048 x 1536 84 us; with sigmoids that fall on below e^-87 it took 87.
+// sigmoids()' care: |z| 2^-24 of the power is far below half a step.  Sigmoids that
+// fall on below e^-87 in fp32 cost 3 us of 78 (forward, 8 x 2048 x 1536).
 template <typename T>
 __device__ __forceinline__ float2 silu(float2 z, float2& slope) {
     float2 s, n;
